@@ -176,6 +176,14 @@ SIGNATURES = {
     "hx_emulate_tree_solve_units": (C.c_int, [C.c_int, C.c_int, _I, _D, _D, _D, C.c_double, _D, _D, _D, C.c_int,
                                               _I, _I]),
     "hx_get_replay_kernel_time": (C.c_int, [_P, _D, C.POINTER(C.c_longlong)]),
+    # the readout operators' argument records, packed by heliox_amd.readout
+    "hx_linear_attention_workspace": (C.c_int64, [C.c_char_p, C.c_int]),
+    "hx_linear_attention": (C.c_int, [C.c_char_p]),
+    "hx_linear_attention_grad": (C.c_int, [C.c_char_p]),
+    "hx_linear_attention_step": (C.c_int, [C.c_char_p]),
+    "hx_distill_loss": (C.c_int, [C.c_char_p]),
+    "hx_sample": (C.c_int, [C.c_char_p]),
+    "hx_readout_error": (C.c_char_p, []),
 }
 
 

@@ -495,6 +495,110 @@ int hx_simulate_and_replay_dw_dx_streaming_into(
 int hx_set_replay_timing(hx_sim* sim, int enable);
 int hx_get_replay_kernel_time(hx_sim* sim, double* ms, long long* launches);
 
+/* ---- Readout operators (no counterpart in the reference, which leaves what turns captured
+ *      output voltages into answers, and their loss, to its caller): linear attention with a
+ *      decay for each head, the loss against a teacher's top logits, the drawing of an answer.
+ *      They need no model.  Every pointer is device memory of the current device; work is
+ *      queued on `stream` (a hipStream_t, NULL: the default stream) and nothing is allocated,
+ *      copied to the host or waited for, so calls may be captured into a graph.  Sizes and
+ *      strides are in elements; the last dimension of every array is contiguous.  0 on
+ *      success; -1 with a text in hx_readout_error() (of the calling thread) if the arguments
+ *      are refused or a launch fails, in which case nothing was queued after it. ---- */
+enum { HX_F32 = 0, HX_F16 = 1, HX_BF16 = 2 };
+
+/* S_t = e^g S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, for t < length; S_{-1} is the initial
+ * state (NULL: zero), end_state is S_{length-1} (the initial state where length is 0); outputs
+ * past a sequence's length are zero, whatever its inputs hold there.  Head h reads head
+ * h q_heads / heads of q, and so on: q_heads, k_heads and v_heads each divide heads.
+ * g = log_decay[h] is at most 0 (-inf: no memory).  States are (batch, heads, dk, dv) fp32,
+ * contiguous.  dk and dv are at most 256. */
+typedef struct hx_attention_args {
+    int64_t type, batch, time, heads, q_heads, k_heads, v_heads, dk, dv;
+    const void *q, *k, *v;                                /* (batch, time, heads of each, d) */
+    int64_t q_stride[3], k_stride[3], v_stride[3];        /* batch, time, head */
+    const float* log_decay;                               /* (heads) */
+    const float* initial_state;                           /* or NULL */
+    const int32_t* lengths;                               /* (batch), 0..time; NULL: all of time */
+    double scale;
+    void* o;                                              /* (batch, time, heads, dv), type */
+    int64_t o_stride[3];
+    float* end_state;                                     /* or NULL */
+    /* gradient: grad_o in; grad_q, grad_k, grad_v out, contiguous, of the shapes of q, k, v */
+    const void* grad_o;
+    int64_t grad_o_stride[3];
+    const float* grad_end;                                /* or NULL: zero */
+    void *grad_q, *grad_k, *grad_v;
+    float* grad_initial;                                  /* or NULL */
+    /* single step: time is 1; the state of row i is slot slots[i] of state (n_slots, heads, dk,
+     * dv), updated in place; a slot outside 0..n_slots-1 leaves its row out (o is zero); the
+     * slots of one call are distinct.  slots NULL: slot i for row i. */
+    float* state;
+    const int32_t* slots;
+    int64_t n_slots;
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} hx_attention_args;
+
+/* Bytes of workspace that the call with these sizes needs (grad: hx_linear_attention_grad);
+ * -1 if the sizes are refused.  The pointers are not looked at. */
+int64_t hx_linear_attention_workspace(const hx_attention_args* args, int grad);
+int hx_linear_attention(const hx_attention_args* args);
+int hx_linear_attention_grad(const hx_attention_args* args);
+int hx_linear_attention_step(const hx_attention_args* args);
+
+/* loss_i = t^2 [ sum_k p_k (log p_k - log q_k) + p_r (log p_r - log q_r) ] of row i, with
+ * q = softmax(logits / t), the teacher's entries k at vocabulary places index[i, k] (one
+ * outside 0..vocab-1 is absent; entries at one place add up), and
+ *   teacher_lse NULL: p = softmax of teacher / t over the row's entries, no p_r term;
+ *   else:  p_k = exp(teacher_k / t - teacher_lse_i), p_r = max(0, 1 - sum_k p_k) and q_r the
+ *          student's mass of all other places (no such term where p_r or q_r is 0).
+ * A row without entries has loss 0 and gradient 0.  grad (NULL: not made) receives
+ * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself. */
+typedef struct hx_distill_args {
+    int64_t type, teacher_type, index_bits;               /* index_bits 32 or 64 */
+    int64_t rows, vocab, top;                             /* vocab <= 2^20, top <= 2048 */
+    const void* logits;
+    int64_t logits_stride;
+    const void* index;
+    int64_t index_stride;
+    const void* teacher;
+    int64_t teacher_stride;
+    const float *teacher_lse, *weight;                    /* (rows) each, or NULL */
+    double temperature;
+    float* loss;                                          /* (rows) */
+    void* grad;
+    int64_t grad_stride;
+    void* stream;
+} hx_distill_args;
+int hx_distill_loss(const hx_distill_args* args);
+
+/* One answer a row from given random numbers u in [0, 1).  With t the row's temperature, place
+ * j has the whole-number mass floor(2^40 exp((x_j - max x) / t)), so that sums of masses do not
+ * depend on their order.  Of the places ranked by x (ties: the lowest index first) the first
+ * top_k stay (<= 0: all), of those the ones with less than top_p of their mass before them
+ * (>= 1: all; the first always), of those the ones with exp((x_j - max x) / t) >= min_p (at
+ * most 1).  The token is the first place, by index, whose running sum of the masses that stay
+ * is over floor(u times their sum); logprob is log of its share of that sum (fp32).  t <= 0
+ * takes the largest logit.  NaN counts as -inf; a row of nothing but -inf gives token -1 and
+ * logprob -inf.  Each setting is an array (rows) or, where that is NULL, one value. */
+typedef struct hx_sample_args {
+    int64_t type, rows, vocab;
+    const void* logits;
+    int64_t logits_stride;
+    const float* u;
+    const float* temperature;
+    const int32_t* top_k;
+    const float *top_p, *min_p;
+    double temperature_value, top_p_value, min_p_value;
+    int64_t top_k_value;
+    int64_t* token;                                       /* (rows) */
+    float* logprob;                                       /* (rows) */
+    void* stream;
+} hx_sample_args;
+int hx_sample(const hx_sample_args* args);
+const char* hx_readout_error(void);
+
 /* Host emulation of the device tree solve (no counterpart in the reference;
  * a diagnostic for CPU-only checks of the solver schedule): capacitance and
  * axial assembly, elimination and back substitution over the same chunk

@@ -1,0 +1,245 @@
+"""Linear attention with decays on the GPU against the recurrence in 64 bits: outputs, end
+states, every gradient and the single step, over types, head layouts, lengths, strides and
+decays."""
+import pytest
+import torch
+
+import readout_util as ref
+from heliox_amd import readout
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+# Bounds on the 2-norm of the error, relative.  Outputs of 16 bits: the result, the masked
+# products and the state as it enters a product are each rounded once, at most one unit of the
+# type each.  fp32 results (and states, whatever the inputs): sums of up to 2^17 terms whose
+# roundings are independent, sqrt(2^17) units.
+def bound(dtype):
+    return 3 * ref.UNIT[dtype] if dtype != torch.float32 else 2 ** 8.5 * ref.UNIT[torch.float32]
+
+
+def make(seed, dtype, batch, time, heads, qh, kh, vh, dk, dv, layout="packed"):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    if layout == "packed":
+        one = r(batch, time, qh * dk + kh * dk + vh * dv).to(dtype).cuda()
+        q, k, v = (x.unflatten(-1, (n, -1)) for x, n in zip(one.split([qh * dk, kh * dk, vh * dv], -1), (qh, kh, vh)))
+    elif layout == "heads_first":
+        q, k, v = (r(batch, n, time, d).to(dtype).cuda().transpose(1, 2) for n, d in ((qh, dk), (kh, dk), (vh, dv)))
+    elif layout == "odd":        # one element past an aligned address, rows of an odd stride
+        q, k, v = (r(batch, time, n, d + 3).to(dtype).cuda()[..., 1:d + 1] for n, d in ((qh, dk), (kh, dk), (vh, dv)))
+    elif layout == "channels_apart":
+        q, k, v = (r(batch, time, d, n).to(dtype).cuda().transpose(2, 3) for n, d in ((qh, dk), (kh, dk), (vh, dv)))
+    elif layout == "broadcast":
+        q, k, v = (r(1, time, n, d).to(dtype).cuda().expand(batch, -1, -1, -1)
+                   for n, d in ((qh, dk), (kh, dk), (vh, dv)))
+    # decays from none at all to no memory
+    g = torch.tensor([0.0, -0.002, -0.05, -0.4, -3.0, -float("inf"), -0.01, -1e-5])[torch.arange(heads) % 8].cuda()
+    state = r(batch, heads, dk, dv).cuda()
+    do = r(batch, time, heads, dv).to(dtype).cuda()
+    dend = r(batch, heads, dk, dv).cuda()
+    return q, k, v, g, state, do, dend
+
+
+def check(dtype, shape, layout="packed", with_state=True, lengths=None, scale=None, seed=0):
+    batch, time, heads, qh, kh, vh, dk, dv = shape
+    q, k, v, g, state, do, dend = make(seed, dtype, *shape, layout=layout)
+    print(f"case attention {dtype} {shape} {layout} state={with_state} lengths={lengths}", flush=True)
+    if lengths is not None:
+        for i, n in enumerate(lengths):     # what lies past a length is never looked at
+            if layout != "broadcast":
+                for x in (q, k, v, do):
+                    x[i, n:] = float("nan")
+        lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    if not with_state:
+        state = dend = None
+    o, end = readout.linear_attention(q, k, v, g, scale=scale, initial_state=state, lengths=lengths)
+    got = readout.linear_attention_grad(q, k, v, g, do, scale=scale, initial_state=state, lengths=lengths, dstate=dend)
+    torch.cuda.synchronize()
+    want = ref.attention(q, k, v, g, dk ** -0.5 if scale is None else scale, state, lengths, do, dend)
+    assert o.dtype == dtype and end.dtype == torch.float32
+    assert ref.rel(o, want[0]) <= bound(dtype)
+    assert ref.rel(end, want[1]) <= bound(torch.float32)
+    for x, w, like in zip(got[:3], want[2:5], (q, k, v)):
+        assert x.dtype == dtype and x.shape == like.shape
+        assert ref.rel(x, w) <= bound(dtype)
+    if with_state:
+        assert ref.rel(got[3], want[5]) <= bound(torch.float32)
+    else:
+        assert got[3] is None
+    if lengths is not None:
+        for i, n in enumerate(lengths.tolist()):
+            assert not o[i, n:].any() and not any(x[i, n:].any() for x in got[:3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("time", [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 200])
+def test_lengths(dtype, time):
+    check(dtype, (2, time, 2, 2, 2, 2, 32, 32), seed=time)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dk,dv", [(1, 1), (1, 40), (7, 5), (16, 16), (64, 64), (40, 80), (80, 40), (96, 96), (128, 128),
+                                   (129, 17), (200, 130), (160, 256), (256, 256)])
+def test_head_sizes(dtype, dk, dv):
+    check(dtype, (1, 150, 3, 3, 3, 3, dk, dv), seed=dk + dv)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [(4, 4, 1, 4), (4, 4, 2, 2), (6, 2, 3, 1), (8, 1, 1, 8), (12, 12, 4, 12), (5, 5, 5, 1)])
+def test_shared_heads(dtype, heads):
+    check(dtype, (2, 90, *heads, 24, 40), seed=sum(heads))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["heads_first", "odd", "channels_apart", "broadcast"])
+def test_strides(dtype, layout):
+    check(dtype, (3, 77, 2, 2, 1, 2, 33, 48), layout=layout, seed=5)
+    check(dtype, (2, 130, 2, 2, 2, 2, 64, 64), layout=layout, seed=6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("with_state", [True, False])
+def test_ragged(dtype, with_state):
+    check(dtype, (7, 140, 3, 3, 3, 3, 48, 20), with_state=with_state, lengths=[140, 0, 1, 64, 65, 128, 99], seed=7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_and_few(dtype):
+    """One sequence, one head: the time axis is what fills the chip."""
+    check(dtype, (1, 5000, 1, 1, 1, 1, 64, 48), seed=8)
+    check(dtype, (2, 3001, 2, 2, 1, 2, 20, 36), lengths=[3001, 1500], seed=9)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scale_and_no_state(dtype):
+    check(dtype, (2, 70, 8, 8, 8, 8, 32, 64), with_state=False, scale=0.37, seed=10)
+
+
+def test_empty():
+    for batch, time in ((0, 5), (3, 0)):
+        q, k, v, g, state, do, dend = make(1, torch.float32, batch, time, 2, 2, 2, 2, 8, 8)
+        o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+        got = readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)
+        assert o.shape == v.shape and torch.equal(end, state) and torch.equal(got[3], dend)
+        _, end = readout.linear_attention(q, k, v, g)
+        assert not end.any()
+
+
+def test_large_values_stay_finite():
+    """fp16 inputs whose products and states pass fp16's largest number."""
+    q, k, v, g, *_ = make(3, torch.float16, 1, 130, 2, 2, 2, 2, 64, 64)
+    g = torch.full((2,), -0.003, device="cuda")
+    k, q = k * 60, q * 60
+    o, end = readout.linear_attention(q, k, v, g, scale=1e-4)
+    want = ref.attention(q, k, v, g, 1e-4)
+    assert float(want[1].abs().max()) > 400
+    assert float((q[0, 0, 0].double() @ k[0, 0, 0].double()).abs()) >= 0
+    assert ref.rel(o, want[0]) <= bound(torch.float16) and ref.rel(end, want[1]) <= bound(torch.float32)
+    k2 = k * 100
+    _, end = readout.linear_attention(q, k2, v * 20, g, scale=1e-9)
+    want = ref.attention(q, k2, v * 20, g, 1e-9)
+    assert float(want[1].abs().max()) > 65504
+    o, _ = readout.linear_attention(q, k2, v * 20, g, scale=1e-7)
+    assert ref.rel(end, want[1]) <= bound(torch.float32)
+    assert ref.rel(o, want[0] * 100) <= bound(torch.float16)
+
+
+def test_gradient_against_differences():
+    """The loss is linear in each of q, k, v and the initial state, so central differences have
+    no error of their own: what is left is the rounding of two losses, each a sum of 2^13
+    products good to 2^8.5 units, over the step."""
+    shape = (2, 70, 2, 2, 1, 2, 24, 16)
+    q, k, v, g, state, do, dend = make(11, torch.float32, *shape)
+    g = torch.tensor([-0.02, -0.3], device="cuda")
+
+    def loss(q, k, v, state):
+        o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+        return (o.double() * do.double()).sum() + (end.double() * dend.double()).sum(), \
+            (o.double() * do.double()).norm() + (end.double() * dend.double()).norm()
+
+    grads = readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)
+    args = [q, k, v, state]
+    for n, grad in enumerate(grads):
+        way = torch.randn(args[n].shape, generator=torch.Generator().manual_seed(n)).cuda()
+        step = 0.5
+        up, down = list(args), list(args)
+        up[n], down[n] = args[n] + step * way, args[n] - step * way
+        (a, na), (b, nb) = loss(*up), loss(*down)
+        diff = float(a - b) / (2 * step)
+        exact = float((grad.double() * way.double()).sum())
+        assert abs(diff - exact) <= 2 ** 8.5 * ref.UNIT[torch.float32] * float(na + nb) / step
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 1, 1), (3, 4, 4, 4, 4, 64, 64), (5, 6, 6, 2, 3, 40, 33),
+                                   (2, 3, 1, 1, 3, 128, 128), (4, 2, 2, 2, 2, 7, 256), (2, 2, 2, 2, 2, 256, 200)])
+def test_step(dtype, shape):
+    batch, heads, qh, kh, vh, dk, dv = shape
+    q, k, v, g, *_ = make(13, dtype, batch, 3, heads, qh, kh, vh, dk, dv)
+    pool = torch.randn(batch + 4, heads, dk, dv, generator=torch.Generator().manual_seed(3)).cuda()
+    slots = torch.randperm(batch + 4, generator=torch.Generator().manual_seed(4))[:batch].to(torch.int32)
+    if batch > 2:
+        slots[1], slots[2] = -1, batch + 4      # neither is a slot
+    before = pool.clone()
+    run = [i for i in range(batch) if 0 <= slots[i] < batch + 4]
+    at = slots[run].long().cuda()
+    outs = [readout.linear_attention_step(q[:, t], k[:, t], v[:, t], g, pool, slots=slots.cuda()) for t in range(3)]
+    o = torch.stack(outs, 1)
+    want, end = ref.attention(q[run], k[run], v[run], g, dk ** -0.5, before[at])
+    assert o.dtype == dtype and ref.rel(o[run], want) <= bound(dtype)
+    assert ref.rel(pool[at], end) <= bound(torch.float32)
+    others = torch.ones(batch + 4, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert torch.equal(pool[others], before[others])
+    assert not o[[i for i in range(batch) if i not in run]].any()
+
+
+def test_step_goes_on_from_a_recording():
+    """Steps after a chunked pass give what the chunked pass over all of it gives."""
+    q, k, v, g, *_ = make(17, torch.float32, 2, 101, 3, 3, 3, 3, 32, 48)
+    whole, end = readout.linear_attention(q, k, v, g)
+    _, state = readout.linear_attention(q[:, :90], k[:, :90], v[:, :90], g)
+    for t in range(90, 101):
+        o = readout.linear_attention_step(q[:, t], k[:, t], v[:, t], g, state)
+        assert ref.rel(o, whole[:, t].cpu().double()) <= 2 * bound(torch.float32)
+    assert ref.rel(state, end.cpu().double()) <= 2 * bound(torch.float32)
+
+
+def test_same_bits_every_time_and_on_another_stream():
+    q, k, v, g, state, do, dend = make(19, torch.bfloat16, 2, 700, 4, 4, 2, 1, 64, 64)
+    one = [*readout.linear_attention(q, k, v, g, initial_state=state),
+           *readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        two = [*readout.linear_attention(q, k, v, g, initial_state=state),
+               *readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)]
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+def test_captured_into_a_graph():
+    q, k, v, g, state, *_ = make(23, torch.bfloat16, 2, 300, 2, 2, 2, 2, 64, 64)
+    pool = state.clone()
+
+    def work():
+        o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+        return o, end, readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, pool)
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for n in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(n)).to(q.dtype))
+        pool.copy_(state)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [x.clone() for x in got]
+        pool.copy_(state)
+        want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, want)), n

@@ -1,0 +1,112 @@
+"""Refusals of the readout operators, in Python and at the C entry points (no GPU)."""
+import pytest
+import torch
+
+from heliox_amd import lib, readout
+
+GOOD = dict(type=2, batch=2, time=5, heads=4, q_heads=4, k_heads=2, v_heads=1, dk=16, dv=24)
+
+
+def attention(scale=1.0, n_slots=0, **sizes):
+    s = {**GOOD, **sizes}
+    return readout._ATTENTION.pack(*(s[n] for n in GOOD), 0, 0, 0, *[0] * 9, 0, 0, 0, scale, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                                   0, 0, 0, 0, 0, 0, n_slots, 0, 0, 0)
+
+
+def error():
+    return lib().hx_readout_error().decode()
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"type": 3}, "type"), ({"batch": -1}, "negative"), ({"time": -1}, "negative"), ({"heads": 0}, "heads"),
+    ({"k_heads": 3}, "multiple"), ({"q_heads": 0}, "multiple"), ({"v_heads": 8}, "multiple"), ({"dk": 0}, "dk"),
+    ({"dk": 257}, "dk"), ({"dv": 300}, "dv"), ({"scale": float("nan")}, "scale"), ({"batch": 2 ** 24}, "2^24"),
+    ({"batch": 2 ** 62}, "2^24"), ({"time": 2 ** 40}, "2^30")])
+@pytest.mark.parametrize("call", ["hx_linear_attention", "hx_linear_attention_grad", "hx_linear_attention_step"])
+def test_attention_sizes_are_refused(call, change, text):
+    assert getattr(lib(), call)(attention(**change)) == -1
+    assert call in error() and text in error()
+
+
+@pytest.mark.parametrize("call", ["hx_linear_attention", "hx_linear_attention_grad"])
+def test_attention_missing_pointers_are_refused(call):
+    assert getattr(lib(), call)(attention()) == -1
+    assert "missing" in error()
+    assert getattr(lib(), call)(None) == -1
+    assert getattr(lib(), call)(attention(batch=0)) == 0
+
+
+def test_step_is_refused():
+    L = lib()
+    assert L.hx_linear_attention_step(attention(time=5)) == -1 and "time" in error()
+    assert L.hx_linear_attention_step(attention(time=1, n_slots=1)) == -1 and "states" in error()
+    assert L.hx_linear_attention_step(attention(time=1, n_slots=2)) == -1 and "missing" in error()
+    assert L.hx_linear_attention_step(attention(time=1, batch=0)) == 0
+
+
+def test_workspace_grows_with_the_problem():
+    L = lib()
+    assert L.hx_linear_attention_workspace(attention(dk=999), 0) == -1
+    small, large = (L.hx_linear_attention_workspace(attention(time=t), 1) for t in (5, 5000))
+    assert 0 <= small <= large
+
+
+def distill(type=0, teacher_type=0, bits=32, rows=2, vocab=9, top=3, temperature=1.0):
+    return readout._DISTILL.pack(type, teacher_type, bits, rows, vocab, top, 0, 0, 0, 0, 0, 0, 0, 0, temperature, 0, 0,
+                                 0, 0)
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"type": 7}, "type"), ({"teacher_type": -1}, "type"), ({"bits": 16}, "bits"), ({"rows": -1}, "rows"),
+    ({"vocab": 0}, "vocab"), ({"vocab": 2 ** 20 + 1}, "vocab"), ({"top": 2049}, "top"), ({"top": -1}, "top"),
+    ({"temperature": 0.0}, "temperature"), ({"temperature": float("inf")}, "temperature"),
+    ({"temperature": float("nan")}, "temperature"), ({}, "missing")])
+def test_distill_is_refused(change, text):
+    assert lib().hx_distill_loss(distill(**change)) == -1
+    assert text in error()
+
+
+@pytest.mark.parametrize("sizes,text", [((9, 1, 5), "type"), ((0, -1, 5), "rows"), ((0, 1, 0), "vocab"),
+                                        ((0, 1, 2 ** 22 + 1), "vocab"), ((0, 1, 5), "missing")])
+def test_sample_is_refused(sizes, text):
+    record = readout._SAMPLE.pack(*sizes, 0, 0, 0, 0, 0, 0, 0, 1.0, 1.0, 0.0, 0, 0, 0, 0)
+    assert lib().hx_sample(record) == -1
+    assert text in error()
+
+
+def test_empty_problems_need_no_gpu():
+    assert lib().hx_distill_loss(distill(rows=0)) == 0
+    assert lib().hx_sample(readout._SAMPLE.pack(0, 0, 5, 0, 0, 0, 0, 0, 0, 0, 1.0, 1.0, 0.0, 0, 0, 0, 0)) == 0
+
+
+def test_python_refuses_tensors_off_the_gpu():
+    x = torch.zeros(2, 3, 4, 8)
+    with pytest.raises(ValueError, match="GPU"):
+        readout.linear_attention(x, x, x, torch.zeros(4))
+    with pytest.raises(ValueError, match="GPU"):
+        readout.linear_attention_grad(x, x, x, torch.zeros(4), x)
+    with pytest.raises(ValueError, match="GPU"):
+        readout.linear_attention_step(x[:, 0], x[:, 0], x[:, 0], torch.zeros(4), torch.zeros(2, 4, 8, 8))
+    with pytest.raises(ValueError, match="GPU"):
+        readout.sample(x[0, 0], torch.zeros(4))
+    with pytest.raises(ValueError, match="GPU"):
+        readout.distill_loss_grad(x[0, 0], torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, 1))
+    with pytest.raises(TypeError, match="tensor"):
+        readout.sample([[1.0]], torch.zeros(1))
+
+
+def test_records_are_as_long_as_the_header_says(tmp_path):
+    import os
+    import shutil
+    import subprocess
+
+    cc = shutil.which("g++") or shutil.which("c++")
+    if cc is None:
+        pytest.skip("no host compiler")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "s.cpp").write_text('#include "heliox.h"\n#include <cstdio>\nint main() { printf("%zu %zu %zu", '
+                                    "sizeof(hx_attention_args), sizeof(hx_distill_args), sizeof(hx_sample_args)); }\n")
+    subprocess.run([cc, "-I", os.path.join(root, "include"), str(tmp_path / "s.cpp"), "-o", str(tmp_path / "s")],
+                   check=True)
+    got = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout
+    assert got.split() == [str(r.size) for r in (readout._ATTENTION, readout._DISTILL, readout._SAMPLE)]
