@@ -7,6 +7,7 @@
 //   o:  a, b, c = q, k, v   forward, state k v^T        dq: a, b, c = do, v, k  forward, state v k^T
 //   dk: a, b, c = v, do, q  reverse, state do q^T       dv: a, b, c = k, q, do  reverse, state q do^T
 #include <algorithm>
+#include <type_traits>
 
 #include "readout.h"
 
@@ -20,7 +21,7 @@ constexpr int kParts = kThreads / kCols;      // lanes that share a column's row
 struct ScanArgs {
     const void *a, *b, *c;
     long long a_stride[3], b_stride[3], c_stride[3];
-    int a_heads, b_heads, c_heads, heads, da, dc, time, ncol;
+    int a_heads, b_heads, c_heads, heads, da, dc, time;
     bool reverse;
     float scale_in, scale_out;       // of what enters the state, and of y
     const float* log_decay;
@@ -28,66 +29,427 @@ struct ScanArgs {
     const float* state_in;
     float* state_out;
     int row_stride, col_stride;      // of a state's da and dc
-    const int32_t* slots;            // states by slot instead of by sequence
-    long long n_slots;
-    bool by_slot;
     void* y;
     long long y_stride[3];
-    int y_heads;
 };
 
-// One workgroup per (sequence, head, 16 state columns), one step after another: a column's
-// rows lie over 16 lanes, so that y is one shuffled sum.
-template <class T, class Y>
-__global__ void __launch_bounds__(kThreads) k_scan(ScanArgs S) {
-    const int col = blockIdx.x % S.ncol * kCols + threadIdx.x / kParts;
-    const int bh = blockIdx.x / S.ncol;
+// ------------------------------------------------------------------- one step
+// One workgroup per (sequence, head, 16 state columns): a column's rows lie over 16 lanes, so
+// that o is one shuffled sum.
+template <class T>
+__global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, const int32_t* slots, long long n_slots,
+                                                   int ncol) {
+    const int col = blockIdx.x % ncol * kCols + threadIdx.x / kParts;
+    const int bh = blockIdx.x / ncol;
     const int batch = bh / S.heads, h = bh - batch * S.heads;
     const int part = threadIdx.x % kParts;
-    const bool mine = col < S.dc;
-    const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
+    const long long slot = slots ? slots[batch] : batch;
+    const bool run = slot >= 0 && slot < n_slots && col < S.dc;
     const float decay = expf(S.log_decay[h]);
-    long long slot = batch;
-    if (S.by_slot && S.slots) slot = S.slots[batch];
-    const bool run = !S.by_slot || (slot >= 0 && slot < S.n_slots);
-    const long long at = (slot * S.heads + h) * static_cast<long long>(S.da) * S.dc +
-                         static_cast<long long>(col) * S.col_stride;
+    float* s = states + (slot * S.heads + h) * static_cast<long long>(S.da) * S.dc + col;
     const T* a = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
     const T* b = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
     const T* c = static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2];
-    Y* y = static_cast<Y*>(S.y) + batch * S.y_stride[0] + h * S.y_stride[2];
-    float s[kAttnMaxDim / kParts];
-#pragma unroll
-    for (int i = 0; i < kAttnMaxDim / kParts; ++i) {
-        const int row = i * kParts + part;
-        s[i] = run && mine && row < S.da && S.state_in ? S.state_in[at + static_cast<long long>(row) * S.row_stride] : 0.f;
+    float sum = 0.f;
+    if (run) {
+        const float ct = to_f32(c[col]);
+        for (int row = part; row < S.da; row += kParts) {
+            float* at = s + static_cast<long long>(row) * S.dc;
+            const float x = fmaf(to_f32(b[row]), ct, *at * decay);
+            *at = x;
+            sum = fmaf(to_f32(a[row]), x, sum);
+        }
     }
-    for (int i = 0; i < S.time; ++i) {
-        const int t = S.reverse && i < len ? len - 1 - i : i;
-        float sum = 0.f;
-        if (run && i < len && mine) {
-            const float ct = to_f32(c[t * S.c_stride[1] + col]) * S.scale_in;
-            // a state that enters in reverse has not decayed before the last step
-            const float keep = S.reverse && i == 0 ? 1.f : decay;
+    for (int m = kParts / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+    if (col < S.dc && part == 0)
+        static_cast<T*>(S.y)[batch * S.y_stride[0] + h * S.y_stride[2] + col] = from_f32<T>(sum * S.scale_out);
+}
+
+// ------------------------------------------------------------------- whole sequences
+// Chunks of kC steps.  With i, j counted inside a chunk of n steps, X the state that enters it
+// and off 1 (forward) or 0 (reverse, where a state has not decayed before its first step):
+//   P_ij = scale_in e^{g (i - j)} (a_i . b_j) for j <= i
+//   y_i  = scale_out (sum_j P_ij c_j + e^{g (i + off)} X^T a_i)
+//   X'   = e^{g n} X + sum_j b_j (scale_in e^{g (n - off - j)} c_j)^T
+// are products of matrices.  A workgroup walks through the chunks of one (sequence, head,
+// slice of c's columns, segment of the steps); each wave keeps X^T's rows for its own columns
+// in accumulator registers, whose layout (lane: one column, four rows) is at the same time
+// that of an operand, so X enters y's product without leaving the registers.  y and P are made
+// transposed for the same reason: P goes to LDS, and y to memory, four neighbours a lane.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// Operand fragments are taken 16 reduction indices at a time, four consecutive ones a lane
+// (lane: index 4 (lane / 16) .. + 3 of row lane % 16).
+//
+// bf16 inputs: 32 indices an instruction.  Products of inputs are exact in fp32; P and the
+// state as it enters y are rounded to bf16 once, as y is afterwards.  The state itself stays
+// fp32: its weighted c enters as three bf16 terms (24 bits).
+struct MathBf16 {
+    using Elem = __bf16;
+    using Frag = bf16x4;
+    static constexpr int kC = 64, kPiece = 8, kTerms = 3;
+    static constexpr int kRowPad = 8, kColPad = 16;     // LDS rows: 4 / 8 banks on, read by rows / by columns
+    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Frag a0, Frag a1, Frag b0, Frag b1) {
+        const bf16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+        const bf16x8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Frag frag(f32x4 x) { return __builtin_convertvector(x, Frag); }
+    static __device__ __forceinline__ f32x4 wide(Frag x) { return __builtin_convertvector(x, f32x4); }
+    // Column `lane % 16` of the 16 x 16 block at p, rows 4 (lane / 16) .. + 3: the transposing read
+    // takes four neighbours of row (lane % 16) / 4 from each lane.
+    static __device__ __forceinline__ Frag column(const Elem* p, int stride, int lane) {
+        const Elem* at = p + (4 * (lane / 16) + lane % 16 / 4) * stride + 4 * (lane % 4);
+        return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) Frag*)at);
+    }
+};
+
+// fp32 and fp16 inputs, in fp32 throughout (fp16's range would not hold P or the states).
+struct MathF32 {
+    using Elem = float;
+    using Frag = f32x4;
+    static constexpr int kC = 32, kPiece = 4, kTerms = 1;
+    static constexpr int kRowPad = 4, kColPad = 4;
+    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Frag a0, Frag a1, Frag b0, Frag b1) {
 #pragma unroll
-            for (int r = 0; r < kAttnMaxDim / kParts; ++r) {
-                const int row = r * kParts + part;
-                if (row < S.da) {
-                    s[r] = fmaf(to_f32(b[t * S.b_stride[1] + row]), ct, s[r] * keep);
-                    sum = fmaf(to_f32(a[t * S.a_stride[1] + row]), s[r], sum);
+        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[i], b0[i], acc, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[i], b1[i], acc, 0, 0, 0);
+        return acc;
+    }
+    static __device__ __forceinline__ Frag frag(f32x4 x) { return x; }
+    static __device__ __forceinline__ f32x4 wide(Frag x) { return x; }
+    static __device__ __forceinline__ Frag column(const Elem* p, int stride, int lane) {
+        const Elem* at = p + 4 * (lane / 16) * stride + lane % 16;
+        return Frag{at[0], at[stride], at[2 * stride], at[3 * stride]};
+    }
+};
+
+template <class T> struct InputOf;      // math, and a piece of a row as it is loaded
+template <> struct InputOf<float> { using Math = MathF32; using Elem = float; using Raw = f32x4; };
+template <> struct InputOf<__half> { using Math = MathF32; using Elem = _Float16; using Raw = f16x4; };
+template <> struct InputOf<__hip_bfloat16> { using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; };
+
+// Rows [0, n) of a chunk into registers, kD columns padded with zeros; row(i) is where a row
+// starts.  `wide` says that whole pieces may be loaded.
+template <class T, int kD, int kT>
+struct Tile {
+    using In = InputOf<T>;
+    using Math = typename In::Math;
+    static constexpr int kP = Math::kPiece, kRowPieces = kD / kP, kN = Math::kC * kRowPieces / kT;
+    static_assert(kN * kT == Math::kC * kRowPieces, "whole rounds of pieces");
+    typename In::Raw raw[kN];
+
+    __device__ __forceinline__ void load(const void* base, long long first, long long step, int n, int d, bool wide) {
+#pragma unroll
+        for (int p = 0; p < kN; ++p) {
+            const int e = p * kT + threadIdx.x, i = e / kRowPieces, col = e % kRowPieces * kP;
+            typename In::Raw x = {};
+            if (i < n && col < d) {
+                const typename In::Elem* at = static_cast<const typename In::Elem*>(base) + first + i * step + col;
+                if (wide) {
+                    x = *reinterpret_cast<const typename In::Raw*>(at);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kP; ++k)
+                        if (col + k < d) x[k] = at[k];
+                }
+            }
+            raw[p] = x;
+        }
+    }
+    __device__ __forceinline__ void store(typename Math::Elem* lds, int stride) const {
+        typedef typename Math::Elem Out __attribute__((ext_vector_type(kP)));
+#pragma unroll
+        for (int p = 0; p < kN; ++p) {
+            const int e = p * kT + threadIdx.x, i = e / kRowPieces, col = e % kRowPieces * kP;
+            *reinterpret_cast<Out*>(lds + i * stride + col) = __builtin_convertvector(raw[p], Out);
+        }
+    }
+};
+
+struct ChunkArgs {
+    ScanArgs s;
+    int nslice, nseg, seg_steps;       // seg_steps a multiple of the chunk
+    float* states;                     // of the segments, registers of each thread side by side
+    bool wide_a, wide_b, wide_c, wide_y, y_f32;
+};
+
+// kDA: rows of the state (a's and b's columns) padded; kW waves of kCT 16-column tiles each.
+// kStates: only each segment's own state, from zero.
+template <class T, int kDA, int kW, int kCT, bool kStates>
+__global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
+    using In = InputOf<T>;
+    using M = typename In::Math;
+    using Elem = typename M::Elem;
+    using Frag = typename M::Frag;
+    constexpr int kC = M::kC, kB = kC / 16, kT = kW * 64, kDC = kW * kCT * 16, kRT = kDA / 16;
+    constexpr int kSA = kDA + M::kRowPad, kSB = kDA + M::kColPad, kSC = kDC + M::kColPad, kSP = kC + M::kRowPad;
+    __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kC * kSA], lb[kC * kSB], lc[kC * kSC],
+        lp[kStates ? 1 : kC * kSP];
+    const ScanArgs& S = A.s;
+    const int lane = threadIdx.x % 64, r = lane % 16, g4 = lane / 16 * 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int slice = blockIdx.x % A.nslice;
+    const int unit = blockIdx.x / A.nslice;
+    const int nseg = kStates ? A.nseg - 1 : A.nseg;
+    const int seg = unit % nseg, bh = unit / nseg;
+    const int batch = bh / S.heads, h = bh - batch * S.heads;
+    const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
+    const int col0 = slice * kDC;                          // of the slice
+    const int mine = wave * kCT * 16;                      // of the wave, in the slice
+    const float lg = S.log_decay[h] * 1.44269504f;
+    const float g = lg < -1e4f ? -1e4f : lg;               // -inf: e^{g 0} stays 1
+    const int off = S.reverse ? 0 : 1;
+    const long long dir = S.reverse ? -1 : 1;
+    const int dc_here = min(S.dc - col0, kDC);
+
+    const long long a0 = batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
+    const long long b0 = batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
+    const long long c0 = batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2] + col0;
+    const int begin = seg * A.seg_steps, end = min(begin + A.seg_steps, S.time);
+
+    Tile<T, kDA, kT> ta, tb;
+    Tile<T, kDC, kT> tc;
+    auto fetch = [&](int i0) {
+        const int n = min(kC, len - i0);
+        const long long t0 = S.reverse ? len - 1 - i0 : i0;
+        if constexpr (!kStates) ta.load(S.a, a0 + t0 * S.a_stride[1], dir * S.a_stride[1], n, S.da, A.wide_a);
+        tb.load(S.b, b0 + t0 * S.b_stride[1], dir * S.b_stride[1], n, S.da, A.wide_b);
+        tc.load(S.c, c0 + t0 * S.c_stride[1], dir * S.c_stride[1], n, dc_here, A.wide_c);
+    };
+    fetch(begin);
+
+    // The state that enters: what came before the sequence, and the segments before this one.
+    f32x4 X[kRT][kCT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+        for (int ct = 0; ct < kCT; ++ct) X[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const long long state0 = static_cast<long long>(bh) * S.da * S.dc;
+    if constexpr (!kStates) {
+        if (S.state_in) {
+            const float left = exp2f(g * static_cast<float>(min(begin, len)));
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
+                        if (row < S.da && col < S.dc)
+                            X[rt][ct][i] = left * S.state_in[state0 + static_cast<long long>(row) * S.row_stride +
+                                                             static_cast<long long>(col) * S.col_stride];
+                    }
+        }
+        if (seg > 0) {
+            const f32x4* w = reinterpret_cast<const f32x4*>(A.states) +
+                             ((static_cast<long long>(bh) * (A.nseg - 1) + seg - 1) * A.nslice + slice) * (kRT * kCT * kT);
+#pragma unroll
+            for (int k = 0; k < kRT * kCT; ++k) X[k / kCT][k % kCT] += w[k * kT + threadIdx.x];
+        }
+    }
+    // e^{g (n - off - j)} of a whole chunk, for the four steps of each 16 that the lane holds
+    f32x4 left[kB];
+    auto weights = [&](int n) {
+#pragma unroll
+        for (int sb = 0; sb < kB; ++sb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = sb * 16 + g4 + i;
+                left[sb][i] = j < n ? S.scale_in * exp2f(g * static_cast<float>(n - off - j)) : 0.f;
+            }
+    };
+    weights(kC);
+
+    for (int i0 = begin; i0 < end; i0 += kC) {
+        const int n = min(kC, len - i0);
+        if (n <= 0) break;
+        if (n < kC) weights(n);
+        __syncthreads();                       // the chunk before is done with
+        if constexpr (!kStates) ta.store(la, kSA);
+        tb.store(lb, kSB);
+        tc.store(lc, kSC);
+        __syncthreads();
+        if (i0 + kC < end) fetch(i0 + kC);
+        f32x4 y[kB][kCT];
+        if constexpr (!kStates) {
+            // blocks on and under the diagonal, dealt out over the waves
+            int turn = 0;
+#pragma unroll
+            for (int tb_ = 0; tb_ < kB; ++tb_)
+#pragma unroll
+                for (int sb = 0; sb <= tb_; ++sb)
+                    if (turn++ % kW == wave) {
+                        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k = 0; k < kRT; k += 2) {
+                            const Elem* pa = la + (tb_ * 16 + r) * kSA + k * 16 + g4;
+                            const Elem* pb = lb + (sb * 16 + r) * kSB + k * 16 + g4;
+                            p = M::mma(p, *reinterpret_cast<const Frag*>(pb), *reinterpret_cast<const Frag*>(pb + 16),
+                                       *reinterpret_cast<const Frag*>(pa), *reinterpret_cast<const Frag*>(pa + 16));
+                        }
+                        // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int ago = (tb_ - sb) * 16 + r - g4 - i;
+                            p[i] = ago >= 0 ? p[i] * (S.scale_in * exp2f(g * static_cast<float>(ago))) : 0.f;
+                        }
+                        *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + sb * 16 + g4) = M::frag(p);
+                    }
+            // what the entering state adds
+#pragma unroll
+            for (int t = 0; t < kB; ++t)
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kRT; k += 2) {
+                Frag x0[kCT], x1[kCT];
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct) x0[ct] = M::frag(X[k][ct]), x1[ct] = M::frag(X[k + 1][ct]);
+#pragma unroll
+                for (int t = 0; t < kB; ++t) {
+                    const Elem* pa = la + (t * 16 + r) * kSA + k * 16 + g4;
+                    const Frag a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
+#pragma unroll
+                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], x0[ct], x1[ct], a_0, a_1);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < kB; ++t) {
+                const float since = exp2f(g * static_cast<float>(t * 16 + r + off));
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
+            }
+        }
+        Frag c[kB][kCT];
+#pragma unroll
+        for (int sb = 0; sb < kB; ++sb)
+#pragma unroll
+            for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::column(lc + sb * 16 * kSC + mine + ct * 16, kSC, lane);
+        if constexpr (!kStates) {
+            __syncthreads();                   // P is whole
+#pragma unroll
+            for (int t = 0; t < kB; ++t)
+#pragma unroll
+                for (int sb = 0; sb <= t; sb += 2) {
+                    const Elem* pp = lp + (t * 16 + r) * kSP + sb * 16 + g4;
+                    const Frag p0 = *reinterpret_cast<const Frag*>(pp);
+                    Frag p1 = {};
+                    if (sb + 1 <= t) p1 = *reinterpret_cast<const Frag*>(pp + 16);
+#pragma unroll
+                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], c[sb][ct], c[sb + 1][ct], p0, p1);
+                }
+            // lane: step t*16 + r, columns g4 .. + 3 of each tile
+#pragma unroll
+            for (int t = 0; t < kB; ++t) {
+                const int i = t * 16 + r;
+                if (i < n) {
+                    const long long step = S.reverse ? len - 1 - (i0 + i) : i0 + i;
+                    const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2];
+#pragma unroll
+                    for (int ct = 0; ct < kCT; ++ct) {
+                        const int col = col0 + mine + ct * 16 + g4;
+                        const f32x4 v = y[t][ct] * S.scale_out;
+                        if (A.y_f32) {
+                            float* o = static_cast<float*>(S.y) + at + col;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (col + k < S.dc) o[k] = v[k];
+                        } else {
+                            typedef typename In::Elem Out;
+                            typedef Out Out4 __attribute__((ext_vector_type(4)));
+                            Out* o = static_cast<Out*>(S.y) + at + col;
+                            const Out4 w = __builtin_convertvector(v, Out4);
+                            if (A.wide_y) {
+                                if (col < S.dc) *reinterpret_cast<Out4*>(o) = w;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (col + k < S.dc) o[k] = w[k];
+                            }
+                        }
+                    }
                 }
             }
         }
-        for (int m = kParts / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-        if (mine && part == 0) y[t * S.y_stride[1] + col] = from_f32<Y>(sum * S.scale_out);
-    }
-    if (S.state_out && run && mine) {
-        const float keep = S.reverse && len ? decay : 1.f;
+        // the state that leaves
+        const float keep = exp2f(g * static_cast<float>(n));
+        Frag wc[M::kTerms][kB][kCT];
 #pragma unroll
-        for (int r = 0; r < kAttnMaxDim / kParts; ++r) {
-            const int row = r * kParts + part;
-            if (row < S.da) S.state_out[at + static_cast<long long>(row) * S.row_stride] = s[r] * keep;
+        for (int sb = 0; sb < kB; ++sb)
+#pragma unroll
+            for (int ct = 0; ct < kCT; ++ct) {
+                f32x4 w = M::wide(c[sb][ct]) * left[sb];
+#pragma unroll
+                for (int k = 0; k < M::kTerms; ++k) {
+                    wc[k][sb][ct] = M::frag(w);
+                    w -= M::wide(wc[k][sb][ct]);
+                }
+            }
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+            Frag b[kB];
+#pragma unroll
+            for (int sb = 0; sb < kB; ++sb) b[sb] = M::column(lb + sb * 16 * kSB + rt * 16, kSB, lane);
+#pragma unroll
+            for (int ct = 0; ct < kCT; ++ct) {
+                f32x4 x = X[rt][ct] * keep;
+#pragma unroll
+                for (int sb = 0; sb < kB; sb += 2)
+#pragma unroll
+                    for (int k = 0; k < M::kTerms; ++k) x = M::mma(x, b[sb], b[sb + 1], wc[k][sb][ct], wc[k][sb + 1][ct]);
+                X[rt][ct] = x;
+            }
         }
+    }
+    if constexpr (kStates) {
+        f32x4* w = reinterpret_cast<f32x4*>(A.states) +
+                   ((static_cast<long long>(bh) * nseg + seg) * A.nslice + slice) * (kRT * kCT * kT);
+#pragma unroll
+        for (int k = 0; k < kRT * kCT; ++k) w[k * kT + threadIdx.x] = X[k / kCT][k % kCT];
+    } else {
+        // steps past the sequence's end
+        for (int i = max(begin, len) + wave; i < end; i += kW) {
+            const long long at = batch * S.y_stride[0] + i * S.y_stride[1] + h * S.y_stride[2];
+            for (int col = col0 + lane; col < col0 + dc_here; col += 64)
+                if (A.y_f32) static_cast<float*>(S.y)[at + col] = 0.f;
+                else static_cast<typename In::Elem*>(S.y)[at + col] = static_cast<typename In::Elem>(0.f);
+        }
+        if (S.state_out && seg == A.nseg - 1) {
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
+                        if (row < S.da && col < S.dc)
+                            S.state_out[state0 + static_cast<long long>(row) * S.row_stride +
+                                        static_cast<long long>(col) * S.col_stride] = X[rt][ct][i];
+                    }
+        }
+    }
+}
+
+// Segments' own states to the states that enter the segments after them, in place.
+__global__ void __launch_bounds__(kThreads) k_join(float* states, const float* log_decay, const int32_t* lengths,
+                                                   int heads, int time, int nseg, int seg_steps, int each) {
+    const int bh = blockIdx.y, batch = bh / heads, h = bh - batch * heads;
+    const int e = blockIdx.x * kThreads + threadIdx.x;
+    if (e >= each) return;
+    const int len = lengths ? min(max(lengths[batch], 0), time) : time;
+    const float lg = log_decay[h] * 1.44269504f;
+    const float g = lg < -1e4f ? -1e4f : lg;
+    f32x4* w = reinterpret_cast<f32x4*>(states) + static_cast<long long>(bh) * nseg * each + e;
+    f32x4 x = w[0];
+    for (int s = 1; s < nseg; ++s) {
+        const int n = min(max(len - s * seg_steps, 0), seg_steps);
+        x = x * exp2f(g * static_cast<float>(n)) + w[static_cast<long long>(s) * each];
+        w[static_cast<long long>(s) * each] = x;
     }
 }
 
@@ -109,17 +471,80 @@ __global__ void k_share(const float* part, T* out, long long n, int heads, int k
 
 hipStream_t stream_of(const hx_attention_args& A) { return static_cast<hipStream_t>(A.stream); }
 
-template <class T, class Y>
-hipError_t launch_scan(const ScanArgs& S, long long batch, hipStream_t st) {
-    k_scan<T, Y><<<static_cast<unsigned>(batch * S.heads * S.ncol), kThreads, 0, st>>>(S);
-    return hipGetLastError();
-}
-
 struct Operand {
     const void* p;
     const int64_t* stride;
     int64_t heads, d;
 };
+
+// How a call is cut: state rows padded, waves and their 16-column tiles, slices of c's
+// columns, segments of the steps.
+struct Cut {
+    int rows, waves, tiles, nslice, nseg, seg_steps;
+    size_t state_bytes;
+};
+
+Cut cut_of(int64_t type, int64_t batch, int64_t heads, int64_t time, int64_t da, int64_t dc) {
+    Cut c{};
+    c.rows = da <= 32 ? 32 : da <= 64 ? 64 : da <= 128 ? 128 : 256;
+    c.waves = dc <= 32 ? 2 : 4;
+    c.tiles = dc <= 64 || c.rows == 256 ? 1 : 2;
+    const int width = c.waves * c.tiles * 16, chunk = type == HX_BF16 ? MathBf16::kC : MathF32::kC;
+    c.nslice = static_cast<int>((dc + width - 1) / width);
+    const int64_t units = batch * heads * c.nslice, chunks = std::max<int64_t>(1, (time + chunk - 1) / chunk);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 4));
+    const int64_t each = (chunks + want - 1) / want;
+    c.seg_steps = static_cast<int>(each * chunk);
+    c.nseg = static_cast<int>((chunks + each - 1) / each);
+    c.state_bytes = sizeof(float) * (c.nseg - 1) * units * c.rows * width;
+    return c;
+}
+
+bool whole(const void* p, const long long* stride, int d, int piece, size_t size) {
+    return reinterpret_cast<uintptr_t>(p) % (piece * size) == 0 && d % piece == 0 && stride[0] % piece == 0 &&
+           stride[1] % piece == 0 && stride[2] % piece == 0;
+}
+
+template <class T, int kDA, int kW, int kCT>
+hipError_t launch_cut(const ChunkArgs& A, long long bh, hipStream_t st) {
+    if (A.nseg > 1) {
+        k_chunk<T, kDA, kW, kCT, true>
+            <<<static_cast<unsigned>(bh * (A.nseg - 1) * A.nslice), kW * 64, 0, st>>>(A);
+        const int each = A.nslice * (kDA / 16) * kCT * kW * 64;
+        k_join<<<dim3((each + kThreads - 1) / kThreads, static_cast<unsigned>(bh)), kThreads, 0, st>>>(
+            A.states, A.s.log_decay, A.s.lengths, A.s.heads, A.s.time, A.nseg - 1, A.seg_steps, each);
+    }
+    k_chunk<T, kDA, kW, kCT, false><<<static_cast<unsigned>(bh * A.nseg * A.nslice), kW * 64, 0, st>>>(A);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_chunks(const ScanArgs& S, int64_t type, long long batch, bool y_f32, void* states, hipStream_t st) {
+    const Cut c = cut_of(type, batch, S.heads, S.time, S.da, S.dc);
+    ChunkArgs A{};
+    A.s = S, A.nslice = c.nslice, A.nseg = c.nseg, A.seg_steps = c.seg_steps;
+    A.states = static_cast<float*>(states);
+    constexpr int kP = InputOf<T>::Math::kPiece;
+    A.wide_a = whole(S.a, S.a_stride, S.da, kP, sizeof(T));
+    A.wide_b = whole(S.b, S.b_stride, S.da, kP, sizeof(T));
+    A.wide_c = whole(S.c, S.c_stride, S.dc, kP, sizeof(T));
+    A.wide_y = whole(S.y, S.y_stride, S.dc, 4, sizeof(T));
+    A.y_f32 = y_f32;
+    const long long bh = batch * S.heads;
+    auto go = [&](auto rows) {
+        constexpr int kDA = decltype(rows)::value;
+        if (c.waves == 2) return launch_cut<T, kDA, 2, 1>(A, bh, st);
+        if constexpr (kDA < 256)
+            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2>(A, bh, st);
+        return launch_cut<T, kDA, 4, 1>(A, bh, st);
+    };
+    switch (c.rows) {
+        case 32: return go(std::integral_constant<int, 32>{});
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 128: return go(std::integral_constant<int, 128>{});
+        default: return go(std::integral_constant<int, 256>{});
+    }
+}
 
 ScanArgs scan_args(const hx_attention_args& A, const Operand& a, const Operand& b, const Operand& c, bool reverse) {
     ScanArgs S{};
@@ -127,7 +552,7 @@ ScanArgs scan_args(const hx_attention_args& A, const Operand& a, const Operand& 
     for (int i = 0; i < 3; ++i) S.a_stride[i] = a.stride[i], S.b_stride[i] = b.stride[i], S.c_stride[i] = c.stride[i];
     S.a_heads = static_cast<int>(a.heads), S.b_heads = static_cast<int>(b.heads), S.c_heads = static_cast<int>(c.heads);
     S.heads = static_cast<int>(A.heads), S.da = static_cast<int>(a.d), S.dc = static_cast<int>(c.d);
-    S.time = static_cast<int>(A.time), S.ncol = (S.dc + kCols - 1) / kCols;
+    S.time = static_cast<int>(A.time);
     S.reverse = reverse, S.scale_in = reverse ? static_cast<float>(A.scale) : 1.f;
     S.scale_out = reverse ? 1.f : static_cast<float>(A.scale);
     S.log_decay = A.log_decay, S.lengths = A.lengths;
@@ -139,6 +564,12 @@ void contiguous(long long* s, int64_t time, int64_t heads, int64_t d) {
     s[0] = time * heads * d, s[1] = heads * d, s[2] = d;
 }
 
+// Workspace: segments' states, then fp32 gradients by head where heads share an input.
+size_t state_part(const hx_attention_args& A, int64_t da, int64_t dc) {
+    const size_t n = cut_of(A.type, A.batch, A.heads, A.time, da, dc).state_bytes;
+    return (n + 255) / 256 * 256;
+}
+
 size_t shared_part(const hx_attention_args& A, int64_t heads, int64_t d) {
     return heads == A.heads ? 0 : sizeof(float) * A.batch * A.time * A.heads * d;
 }
@@ -146,8 +577,10 @@ size_t shared_part(const hx_attention_args& A, int64_t heads, int64_t d) {
 }  // namespace
 
 size_t attention_workspace(const hx_attention_args& A, bool grad) {
-    if (!grad) return 0;
-    return std::max({shared_part(A, A.q_heads, A.dk), shared_part(A, A.k_heads, A.dk), shared_part(A, A.v_heads, A.dv)});
+    const size_t there = state_part(A, A.dk, A.dv);
+    if (!grad) return there;
+    return std::max(there, state_part(A, A.dv, A.dk)) +
+           std::max({shared_part(A, A.q_heads, A.dk), shared_part(A, A.k_heads, A.dk), shared_part(A, A.v_heads, A.dv)});
 }
 
 hipError_t attention_forward(const hx_attention_args& A) {
@@ -157,43 +590,48 @@ hipError_t attention_forward(const hx_attention_args& A) {
     S.state_in = A.initial_state, S.state_out = A.end_state, S.row_stride = S.dc, S.col_stride = 1;
     S.y = A.o;
     for (int i = 0; i < 3; ++i) S.y_stride[i] = A.o_stride[i];
-    return with_type(A.type, [&](auto t) { return launch_scan<decltype(t), decltype(t)>(S, A.batch, stream_of(A)); });
+    return with_type(A.type, [&](auto t) {
+        return launch_chunks<decltype(t)>(S, A.type, A.batch, false, A.workspace, stream_of(A));
+    });
 }
 
 hipError_t attention_step(const hx_attention_args& A) {
     const Operand q{A.q, A.q_stride, A.q_heads, A.dk}, k{A.k, A.k_stride, A.k_heads, A.dk},
         v{A.v, A.v_stride, A.v_heads, A.dv};
     ScanArgs S = scan_args(A, q, k, v, false);
-    S.lengths = nullptr;
-    S.state_in = S.state_out = A.state, S.row_stride = S.dc, S.col_stride = 1;
-    S.by_slot = true, S.slots = A.slots, S.n_slots = A.n_slots;
     S.y = A.o;
     for (int i = 0; i < 3; ++i) S.y_stride[i] = A.o_stride[i];
-    return with_type(A.type, [&](auto t) { return launch_scan<decltype(t), decltype(t)>(S, A.batch, stream_of(A)); });
+    const int ncol = (S.dc + kCols - 1) / kCols;
+    return with_type(A.type, [&](auto t) {
+        k_step<decltype(t)><<<static_cast<unsigned>(A.batch * S.heads * ncol), kThreads, 0, stream_of(A)>>>(
+            S, A.state, A.slots, A.n_slots, ncol);
+        return hipGetLastError();
+    });
 }
 
 hipError_t attention_backward(const hx_attention_args& A) {
     const Operand q{A.q, A.q_stride, A.q_heads, A.dk}, k{A.k, A.k_stride, A.k_heads, A.dk},
         v{A.v, A.v_stride, A.v_heads, A.dv}, o{A.grad_o, A.grad_o_stride, A.heads, A.dv};
     const hipStream_t st = stream_of(A);
+    char* const space = static_cast<char*>(A.workspace);
+    float* const by_head = reinterpret_cast<float*>(
+        space + std::max(state_part(A, A.dk, A.dv), state_part(A, A.dv, A.dk)));
     auto one = [&](const Operand& a, const Operand& b, const Operand& c, bool reverse, bool transposed,
                    const float* in, float* out, void* y, int64_t kept) -> hipError_t {
         ScanArgs S = scan_args(A, a, b, c, reverse);
         S.state_in = in, S.state_out = out;
         S.row_stride = transposed ? 1 : S.dc, S.col_stride = transposed ? S.da : 1;
         const bool shared = kept != A.heads;
-        S.y = shared ? A.workspace : y;
+        S.y = shared ? by_head : y;
         contiguous(S.y_stride, A.time, A.heads, c.d);
         return with_type(A.type, [&](auto t) -> hipError_t {
             using T = decltype(t);
-            if (!shared) return launch_scan<T, T>(S, A.batch, st);
-            hipError_t e = launch_scan<T, float>(S, A.batch, st);
-            if (e != hipSuccess || !A.time) return e;
+            const hipError_t e = launch_chunks<T>(S, A.type, A.batch, shared, space, st);
+            if (e != hipSuccess || !A.time || !shared) return e;
             const long long n = A.batch * A.time;
             const long long blocks = std::min<long long>((n * kept * c.d + kThreads - 1) / kThreads, 1 << 16);
-            k_share<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(
-                static_cast<const float*>(A.workspace), static_cast<T*>(y), n, S.heads, static_cast<int>(kept),
-                static_cast<int>(c.d));
+            k_share<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(by_head, static_cast<T*>(y), n, S.heads,
+                                                                           static_cast<int>(kept), static_cast<int>(c.d));
             return hipGetLastError();
         });
     };
