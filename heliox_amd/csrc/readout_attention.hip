@@ -15,8 +15,6 @@ namespace hx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCols = 16;                     // state columns of one workgroup
-constexpr int kParts = kThreads / kCols;      // lanes that share a column's rows
 
 struct ScanArgs {
     const void *a, *b, *c;
@@ -34,35 +32,67 @@ struct ScanArgs {
 };
 
 // ------------------------------------------------------------------- one step
-// One workgroup per (sequence, head, 16 state columns): a column's rows lie over 16 lanes, so
-// that o is one shuffled sum.
-template <class T>
+// One workgroup per (sequence, head).  Lanes lie along a state's rows, kV columns each, so that
+// the state streams through as it lies in memory; k and q wait in LDS.  Bound by the state's
+// bytes, read and written once.
+template <class T, int kV>
 __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, const int32_t* slots, long long n_slots,
-                                                   int ncol) {
-    const int col = blockIdx.x % ncol * kCols + threadIdx.x / kParts;
-    const int bh = blockIdx.x / ncol;
-    const int batch = bh / S.heads, h = bh - batch * S.heads;
-    const int part = threadIdx.x % kParts;
+                                                   int lanes) {
+    typedef float Vec __attribute__((ext_vector_type(kV)));
+    constexpr int kBatch = 8;                  // rows in flight
+    __shared__ float lq[kAttnMaxDim], lk[kAttnMaxDim], part[kThreads * kV];
+    const int batch = blockIdx.x / S.heads, h = blockIdx.x - batch * S.heads;
+    const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = kThreads / lanes;
+    const int col = lane * kV;
     const long long slot = slots ? slots[batch] : batch;
-    const bool run = slot >= 0 && slot < n_slots && col < S.dc;
-    const float decay = expf(S.log_decay[h]);
+    const bool run = slot >= 0 && slot < n_slots, mine = run && col < S.dc;
+    T* o = static_cast<T*>(S.y) + batch * S.y_stride[0] + h * S.y_stride[2];
     float* s = states + (slot * S.heads + h) * static_cast<long long>(S.da) * S.dc + col;
+    Vec x[kBatch];
+    auto fetch = [&](int row0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int row = row0 + i * groups;
+            if (mine && row < S.da) x[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(s + row * S.dc));
+        }
+    };
+    fetch(group);
+    const float decay = expf(S.log_decay[h]);
     const T* a = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
     const T* b = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
     const T* c = static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2];
-    float sum = 0.f;
-    if (run) {
-        const float ct = to_f32(c[col]);
-        for (int row = part; row < S.da; row += kParts) {
-            float* at = s + static_cast<long long>(row) * S.dc;
-            const float x = fmaf(to_f32(b[row]), ct, *at * decay);
-            *at = x;
-            sum = fmaf(to_f32(a[row]), x, sum);
+    if (threadIdx.x < S.da) {
+        lq[threadIdx.x] = to_f32(a[threadIdx.x]);
+        lk[threadIdx.x] = to_f32(b[threadIdx.x]);
+    }
+    Vec v = {}, sum = {};
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) v[i] = to_f32(c[col + i]);
+    __syncthreads();
+    for (int row0 = group; row0 < S.da; row0 += kBatch * groups) {
+        if (row0 != group) fetch(row0);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int row = row0 + i * groups;
+            if (mine && row < S.da) {
+                const float kk = lk[row], qq = lq[row];
+#pragma unroll
+                for (int j = 0; j < kV; ++j) {
+                    x[i][j] = fmaf(kk, v[j], x[i][j] * decay);
+                    sum[j] = fmaf(qq, x[i][j], sum[j]);
+                }
+                __builtin_nontemporal_store(x[i], reinterpret_cast<Vec*>(s + row * S.dc));
+            }
         }
     }
-    for (int m = kParts / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-    if (col < S.dc && part == 0)
-        static_cast<T*>(S.y)[batch * S.y_stride[0] + h * S.y_stride[2] + col] = from_f32<T>(sum * S.scale_out);
+    *reinterpret_cast<Vec*>(part + threadIdx.x * kV) = sum;
+    __syncthreads();
+    if (threadIdx.x < S.dc) {
+        float y = 0.f;
+        for (int k = 0; k < groups; ++k) y += part[k * lanes * kV + threadIdx.x];
+        o[threadIdx.x] = from_f32<T>(run ? y * S.scale_out : 0.f);
+    }
 }
 
 // ------------------------------------------------------------------- whole sequences
@@ -601,10 +631,15 @@ hipError_t attention_step(const hx_attention_args& A) {
     ScanArgs S = scan_args(A, q, k, v, false);
     S.y = A.o;
     for (int i = 0; i < 3; ++i) S.y_stride[i] = A.o_stride[i];
-    const int ncol = (S.dc + kCols - 1) / kCols;
+    // four columns a lane where every row of a state starts at a whole 16 bytes
+    const bool wide = S.dc % 4 == 0 && reinterpret_cast<uintptr_t>(A.state) % 16 == 0;
+    int lanes = 1;
+    while (lanes * (wide ? 4 : 1) < S.dc) lanes *= 2;
+    const unsigned grid = static_cast<unsigned>(A.batch * S.heads);
     return with_type(A.type, [&](auto t) {
-        k_step<decltype(t)><<<static_cast<unsigned>(A.batch * S.heads * ncol), kThreads, 0, stream_of(A)>>>(
-            S, A.state, A.slots, A.n_slots, ncol);
+        using T = decltype(t);
+        if (wide) k_step<T, 4><<<grid, kThreads, 0, stream_of(A)>>>(S, A.state, A.slots, A.n_slots, lanes);
+        else k_step<T, 1><<<grid, kThreads, 0, stream_of(A)>>>(S, A.state, A.slots, A.n_slots, lanes);
         return hipGetLastError();
     });
 }
