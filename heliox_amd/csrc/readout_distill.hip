@@ -1,26 +1,27 @@
 // The loss against a teacher's top logits, and its gradient by the student's, one workgroup
 // per row.
+//
+// Two passes over a row: the running maximum and sums of a softmax, then the gradient, which
+// reads the row again from the cache.  Every place outside the teacher's entries has one factor
+// (w (P - p_r / q_r)); the few entries are written over afterwards.
 #include "readout.h"
+
+#include <algorithm>
 
 namespace hx {
 namespace {
 
-constexpr int kThreads = 256;
+template <class T> struct PieceOf;
+template <> struct PieceOf<float> { typedef float Vec __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct PieceOf<__half> { typedef _Float16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct PieceOf<__hip_bfloat16> { typedef __bf16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
 
-struct Pair {          // running maximum and the sum of e^{x - max}
-    float m, s;
-};
+// 2^x by the instruction: one unit off at most, 0 under 2^-126.
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ float exp_diff(float a, float b) { return a == b ? 1.f : expf(a - b); }
-
-__device__ __forceinline__ Pair join(Pair a, Pair b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s};
-    return {m, a.s * exp_diff(a.m, m) + b.s * exp_diff(b.m, m)};
-}
-
-template <class F>
-__device__ __forceinline__ float block_sum(float x, float* sh, F op) {
+// x reduced over the workgroup's waves; every thread gets the result.
+template <int kThreads, class F>
+__device__ __forceinline__ float block_reduce(float x, float* sh, F op) {
     for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
     __syncthreads();
     if (threadIdx.x % 64 == 0) sh[threadIdx.x / 64] = x;
@@ -36,82 +37,128 @@ __device__ __forceinline__ int entry(const void* index, long long at, int vocab)
     return j >= 0 && j < vocab ? static_cast<int>(j) : -1;
 }
 
-// LDS: places and teacher's shares of the row's entries, the student's logits there, and one
-// bit for each place of the vocabulary that holds an entry.
-template <class T, class U, class I>
-__global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A) {
+// LDS: places and teacher's shares of the row's entries, the student's logits there, and, where
+// the rest is one class, one bit for each place of the vocabulary that holds an entry.
+// Weights are 2^((x - max) cold), cold = log2 e / temperature: the difference comes first, so
+// that an error of the product is one of the small difference and not of the logit.
+template <class T, class U, class I, int kThreads, bool kRest>
+__global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float cold) {
+    using Vec = typename PieceOf<T>::Vec;
+    constexpr int kP = sizeof(Vec) / sizeof(T);
     extern __shared__ int lds[];
     __shared__ float red[kThreads / 64];
     const int top = static_cast<int>(A.top), vocab = static_cast<int>(A.vocab);
     int* place = lds;
     float* share = reinterpret_cast<float*>(lds + top);
-    float* logq = share + top;
-    unsigned* member = reinterpret_cast<unsigned*>(logq + top);
+    float* logit = share + top;
+    unsigned* member = reinterpret_cast<unsigned*>(logit + top);
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(A.logits) + row * A.logits_stride;
     const U* t = static_cast<const U*>(A.teacher) + row * A.teacher_stride;
-    const float cold = 1.f / static_cast<float>(A.temperature), tau = static_cast<float>(A.temperature);
-    const bool rest = A.teacher_lse != nullptr;
+    const float tau = static_cast<float>(A.temperature);
     auto add = [](float a, float b) { return a + b; };
     auto most = [](float a, float b) { return fmaxf(a, b); };
 
-    for (int w = threadIdx.x; w < (vocab + 31) / 32; w += kThreads) member[w] = 0;
-    __syncthreads();
+    if constexpr (kRest) {
+        for (int w = threadIdx.x; w < (vocab + 31) / 32; w += kThreads) member[w] = 0;
+        __syncthreads();
+    }
     float tmax = -INFINITY, some = 0.f;
     for (int k = threadIdx.x; k < top; k += kThreads) {
         const int j = entry<I>(A.index, row * A.index_stride + k, vocab);
         place[k] = j;
-        share[k] = j >= 0 ? to_f32(t[k]) * cold : -INFINITY;
-        logq[k] = j >= 0 ? to_f32(x[j]) * cold : 0.f;
+        share[k] = j >= 0 ? to_f32(t[k]) / tau : -INFINITY;
+        logit[k] = j >= 0 ? to_f32(x[j]) : 0.f;
         if (j >= 0) {
             some = 1.f;
             tmax = fmaxf(tmax, share[k]);
-            atomicOr(member + j / 32, 1u << (j % 32));
+            if constexpr (kRest) atomicOr(member + j / 32, 1u << (j % 32));
         }
     }
-    some = block_sum(some, red, most);
-    tmax = block_sum(tmax, red, most);
+    some = block_reduce<kThreads>(some, red, most);
+    if constexpr (!kRest) tmax = block_reduce<kThreads>(tmax, red, most);
 
     // the student's maximum and sums: all places, and those without an entry
-    Pair all{-INFINITY, 0.f};
-    float others = 0.f;
-    for (int j = threadIdx.x; j < vocab; j += kThreads) {
-        const float v = to_f32(x[j]) * cold;
-        const bool in = member[j / 32] >> (j % 32) & 1;
-        const float m = v != v ? v : fmaxf(all.m, v);
-        const float keep = all.m == m ? 1.f : expf(all.m - m), e = v == -INFINITY ? 0.f : exp_diff(v, m);
-        all = {m, all.s * keep + e};
-        others = others * keep + (in ? 0.f : e);
+    float m = -INFINITY, z = 0.f, others = 0.f;
+    const int pieces = vocab / kP;
+    auto take = [&](const float* v, int n, unsigned in) {
+        float c = v[0];
+#pragma unroll
+        for (int i = 1; i < kP; ++i)
+            if (i < n) c = fmaxf(c, v[i]);
+        if (c > m) {
+            const float keep = pow2((m - c) * cold);     // m = -inf: 0
+            z *= keep;
+            others *= keep;
+            m = c;
+        }
+        const float from = m == -INFINITY ? 0.f : m;     // nothing but -inf yet: its weights are 0, not NaN
+        float e[kP], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+            e[i] = i < n ? pow2((v[i] - from) * cold) : 0.f;
+            sum += e[i];
+        }
+        z += sum;
+        if constexpr (kRest) {
+            if (in) {
+                sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < kP; ++i) sum += in >> i & 1 ? 0.f : e[i];
+            }
+            others += sum;
+        }
+    };
+    const unsigned char* bits = reinterpret_cast<const unsigned char*>(member);
+    for (int p = threadIdx.x; p < pieces; p += kThreads) {
+        const Vec raw = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p) * kP);
+        float v[kP];
+#pragma unroll
+        for (int i = 0; i < kP; ++i) v[i] = static_cast<float>(raw[i]);
+        unsigned in = 0;
+        if constexpr (kRest) in = kP == 8 ? bits[p] : bits[p / 2] >> (p % 2 * 4) & 15;
+        take(v, kP, in);
     }
-    const float m = block_sum(all.m, red, most);
-    const float scale = all.m == -INFINITY ? 0.f : exp_diff(all.m, m);
-    const float z = block_sum(all.s * scale, red, add);
-    others = block_sum(others * scale, red, add);
-    const float lse = m + logf(z);
+    if (pieces * kP + static_cast<int>(threadIdx.x) < vocab) {       // fewer than a piece are left
+        const int j = pieces * kP + threadIdx.x;
+        float v[kP] = {to_f32(x[j])};
+        unsigned in = 0;
+        if constexpr (kRest) in = bits[j / 8] >> (j % 8) & 1;
+        take(v, 1, in);
+    }
+    const float mine = m;
+    m = block_reduce<kThreads>(m, red, most);
+    if (m == -INFINITY) m = 0.f;
+    const float scale = pow2((mine - m) * cold);
+    z = block_reduce<kThreads>(z * scale, red, add);
+    if constexpr (kRest) others = block_reduce<kThreads>(others * scale, red, add);
+    const float logz = logf(z);
 
     // the teacher's shares and the row's loss
-    float mass = 0.f;
-    if (!rest) {
+    float norm;
+    if constexpr (kRest) {
+        norm = A.teacher_lse[row];
+    } else {
+        float mass = 0.f;
         for (int k = threadIdx.x; k < top; k += kThreads)
-            if (share[k] > -INFINITY || share[k] != share[k]) mass += exp_diff(share[k], tmax);
-        mass = block_sum(mass, red, add);
+            if (share[k] != -INFINITY) mass += share[k] == tmax ? 1.f : expf(share[k] - tmax);
+        norm = tmax + logf(block_reduce<kThreads>(mass, red, add));
     }
-    const float norm = rest ? A.teacher_lse[row] : tmax + logf(mass);
     float loss = 0.f, psum = 0.f;
     for (int k = threadIdx.x; k < top; k += kThreads) {
         float p = 0.f;
-        if (place[k] >= 0) {
+        if (share[k] != -INFINITY) {
             const float logp = share[k] - norm;
-            p = share[k] == -INFINITY ? 0.f : expf(logp);
-            if (p != 0.f) loss += p * (logp - (logq[k] - lse));
+            p = expf(logp);
+            if (p != 0.f) loss += p * (logp - ((logit[k] - m) / tau - logz));
         }
         share[k] = p;
         psum += p;
     }
-    loss = block_sum(loss, red, add);
-    psum = block_sum(psum, red, add);
+    loss = block_reduce<kThreads>(loss, red, add);
+    psum = block_reduce<kThreads>(psum, red, add);
     float inside = psum, outside = psum;
-    if (rest) {
+    if constexpr (kRest) {
         const float pr = fmaxf(0.f, 1.f - psum), qr = others / z;
         if (pr > 0.f && qr > 0.f) {
             loss += pr * (logf(pr) - logf(qr));
@@ -122,10 +169,18 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A) {
     if (threadIdx.x == 0) A.loss[row] = some > 0.f ? loss * tau * tau : 0.f;
     if (!A.grad) return;
     T* g = static_cast<T*>(A.grad) + row * A.grad_stride;
-    const float w = tau * (A.weight ? A.weight[row] : 1.f);
-    for (int j = threadIdx.x; j < vocab; j += kThreads) {
-        const float v = to_f32(x[j]) * cold;
-        g[j] = from_f32<T>(some > 0.f ? w * outside * expf(v - lse) : 0.f);
+    const float w = some > 0.f ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
+    const float factor = w * outside / z;
+    auto slope = [&](float v) { return some > 0.f ? factor * pow2((v - m) * cold) : 0.f; };
+    for (int p = threadIdx.x; p < pieces; p += kThreads) {
+        Vec raw = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p) * kP);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) raw[i] = static_cast<decltype(raw[0] + raw[0])>(slope(static_cast<float>(raw[i])));
+        *reinterpret_cast<Vec*>(g + static_cast<long long>(p) * kP) = raw;
+    }
+    if (pieces * kP + static_cast<int>(threadIdx.x) < vocab) {
+        const int j = pieces * kP + threadIdx.x;
+        g[j] = from_f32<T>(slope(to_f32(x[j])));
     }
     __syncthreads();
     // entries: one of those at a place writes for all of them
@@ -139,29 +194,39 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A) {
                 p += share[i];
                 if (i < k) first = false;
             }
-        if (first) g[j] = from_f32<T>(w * (inside * expf(logq[k] - lse) - p));
+        if (first) g[j] = from_f32<T>(w * (inside / z * pow2((logit[k] - m) * cold) - p));
     }
+}
+
+template <class T, class U, class I, int kThreads, bool kRest>
+hipError_t launch(const hx_distill_args& A) {
+    const size_t lds = sizeof(int) * (3 * A.top + (kRest ? (A.vocab + 31) / 32 : 0));
+    auto kernel = k_distill<T, U, I, kThreads, kRest>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 163840 - 256);
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<static_cast<unsigned>(A.rows), kThreads, lds, static_cast<hipStream_t>(A.stream)>>>(
+        A, static_cast<float>(1.4426950408889634 / A.temperature));
+    return hipGetLastError();
+}
+
+template <class T, class U, class I>
+hipError_t pick(const hx_distill_args& A) {
+    const bool wide = A.vocab > 4096;
+    if (A.teacher_lse) return wide ? launch<T, U, I, 1024, true>(A) : launch<T, U, I, 256, true>(A);
+    return wide ? launch<T, U, I, 1024, false>(A) : launch<T, U, I, 256, false>(A);
 }
 
 }  // namespace
 
 hipError_t distill_launch(const hx_distill_args& A) {
-    const size_t lds = sizeof(int) * (3 * A.top + (A.vocab + 31) / 32);
-    const hipStream_t st = static_cast<hipStream_t>(A.stream);
     return with_type(A.type, [&](auto t) {
         return with_type(A.teacher_type, [&](auto u) {
-            auto go = [&](auto kernel) {
-                if (lds > 65536) {
-                    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                             hipFuncAttributeMaxDynamicSharedMemorySize, 163840 - 256);
-                    if (e != hipSuccess) return e;
-                }
-                kernel<<<static_cast<unsigned>(A.rows), kThreads, lds, st>>>(A);
-                return hipGetLastError();
-            };
             using T = decltype(t);
             using U = decltype(u);
-            return A.index_bits == 64 ? go(k_distill<T, U, int64_t>) : go(k_distill<T, U, int32_t>);
+            return A.index_bits == 64 ? pick<T, U, int64_t>(A) : pick<T, U, int32_t>(A);
         });
     });
 }
