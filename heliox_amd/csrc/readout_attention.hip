@@ -16,6 +16,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// 2^x by the instruction: one unit off at most, 0 under 2^-126.
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
 struct ScanArgs {
     const void *a, *b, *c;
     long long a_stride[3], b_stride[3], c_stride[3];
@@ -163,41 +166,60 @@ template <> struct InputOf<float> { using Math = MathF32; using Elem = float; us
 template <> struct InputOf<__half> { using Math = MathF32; using Elem = _Float16; using Raw = f16x4; };
 template <> struct InputOf<__hip_bfloat16> { using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; };
 
-// Rows [0, n) of a chunk into registers, kD columns padded with zeros; row(i) is where a row
-// starts.  `wide` says that whole pieces may be loaded.
-template <class T, int kD, int kT>
+// Rows [0, n) of a chunk into registers, kD columns padded with zeros, R rows a round of the
+// workgroup.  kWhole: d is a whole number of pieces and a round's rows are within 2 GiB, so that
+// a load is one instruction with a uniform address and the same 32-bit offset in every round
+// (64-bit addresses by lane, twelve a thread, went to scratch memory and were waited for one by
+// one).  The choice is the kernel's: a register that either of two loads may fill is waited for
+// at once.  Pieces start at any element: loads need no alignment.
+template <class T, int kD, int kT, bool kWhole>
 struct Tile {
     using In = InputOf<T>;
     using Math = typename In::Math;
-    static constexpr int kP = Math::kPiece, kRowPieces = kD / kP, kN = Math::kC * kRowPieces / kT;
-    static_assert(kN * kT == Math::kC * kRowPieces, "whole rounds of pieces");
-    typename In::Raw raw[kN];
+    static constexpr int kP = Math::kPiece, kRowPieces = kD / kP, kRows = kT / kRowPieces, kN = Math::kC / kRows;
+    static_assert(kRows * kRowPieces == kT && kN * kRows == Math::kC, "whole rounds of rows");
+    typedef typename In::Raw Raw;
+    typedef Raw Any __attribute__((aligned(sizeof(T))));
+    Raw raw[kN];
+    const T* base;          // row 0 of the sequence (reverse: row R - 1 of a round that starts there)
+    long long step;         // from row to row
+    int row, col, d;        // of this thread in a round
+    unsigned offset;        // bytes
 
-    __device__ __forceinline__ void load(const void* base, long long first, long long step, int n, int d, bool wide) {
+    __device__ __forceinline__ void start(const T* p, long long stride, bool reverse, int columns) {
+        row = threadIdx.x / kRowPieces, col = threadIdx.x % kRowPieces * kP, d = columns;
+        step = reverse ? -stride : stride;
+        if constexpr (kWhole) {
+            base = reverse ? p - (kRows - 1) * stride : p;
+            offset = static_cast<unsigned>(((reverse ? kRows - 1 - row : row) * stride + col) * sizeof(T));
+            if (col >= d) row = Math::kC;      // no row has these columns
+        } else {
+            base = p;
+        }
+    }
+    __device__ __forceinline__ void load(long long first, int n) {       // from row `first` (in memory order) on
 #pragma unroll
         for (int p = 0; p < kN; ++p) {
-            const int e = p * kT + threadIdx.x, i = e / kRowPieces, col = e % kRowPieces * kP;
-            typename In::Raw x = {};
-            if (i < n && col < d) {
-                const typename In::Elem* at = static_cast<const typename In::Elem*>(base) + first + i * step + col;
-                if (wide) {
-                    x = *reinterpret_cast<const typename In::Raw*>(at);
-                } else {
+            Raw x = {};
+            if constexpr (kWhole) {
+                const char* at = reinterpret_cast<const char*>(base + first + p * kRows * step);
+                if (row < n - p * kRows) x = *reinterpret_cast<const Any*>(at + offset);
+            } else if (row + p * kRows < n) {
+                const typename In::Elem* at =
+                    reinterpret_cast<const typename In::Elem*>(base) + first + (row + p * kRows) * step + col;
 #pragma unroll
-                    for (int k = 0; k < kP; ++k)
-                        if (col + k < d) x[k] = at[k];
-                }
+                for (int k = 0; k < kP; ++k)
+                    if (col + k < d) x[k] = at[k];
             }
             raw[p] = x;
         }
     }
     __device__ __forceinline__ void store(typename Math::Elem* lds, int stride) const {
         typedef typename Math::Elem Out __attribute__((ext_vector_type(kP)));
+        const int i = threadIdx.x / kRowPieces, j = threadIdx.x % kRowPieces * kP;
 #pragma unroll
-        for (int p = 0; p < kN; ++p) {
-            const int e = p * kT + threadIdx.x, i = e / kRowPieces, col = e % kRowPieces * kP;
-            *reinterpret_cast<Out*>(lds + i * stride + col) = __builtin_convertvector(raw[p], Out);
-        }
+        for (int p = 0; p < kN; ++p)
+            *reinterpret_cast<Out*>(lds + (i + p * kRows) * stride + j) = __builtin_convertvector(raw[p], Out);
     }
 };
 
@@ -205,13 +227,16 @@ struct ChunkArgs {
     ScanArgs s;
     int nslice, nseg, seg_steps;       // seg_steps a multiple of the chunk
     float* states;                     // of the segments, registers of each thread side by side
-    bool wide_a, wide_b, wide_c, wide_y, y_f32;
+    bool y_f32;
 };
+
+// Waves a SIMD that the registers have to leave room for.
+constexpr int waves_of(int) { return 2; }
 
 // kDA: rows of the state (a's and b's columns) padded; kW waves of kCT 16-column tiles each.
 // kStates: only each segment's own state, from zero.
-template <class T, int kDA, int kW, int kCT, bool kStates>
-__global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
+template <class T, int kDA, int kW, int kCT, bool kWhole, bool kStates>
+__global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     using In = InputOf<T>;
     using M = typename In::Math;
     using Elem = typename M::Elem;
@@ -234,22 +259,25 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
     const float lg = S.log_decay[h] * 1.44269504f;
     const float g = lg < -1e4f ? -1e4f : lg;               // -inf: e^{g 0} stays 1
     const int off = S.reverse ? 0 : 1;
-    const long long dir = S.reverse ? -1 : 1;
     const int dc_here = min(S.dc - col0, kDC);
 
-    const long long a0 = batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
-    const long long b0 = batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
-    const long long c0 = batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2] + col0;
+    const T* a0 = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
+    const T* b0 = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
+    const T* c0 =
+        static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2] + col0;
     const int begin = seg * A.seg_steps, end = min(begin + A.seg_steps, S.time);
 
-    Tile<T, kDA, kT> ta, tb;
-    Tile<T, kDC, kT> tc;
+    Tile<T, kDA, kT, kWhole> ta, tb;
+    Tile<T, kDC, kT, kWhole> tc;
+    if constexpr (!kStates) ta.start(a0, S.a_stride[1], S.reverse, S.da);
+    tb.start(b0, S.b_stride[1], S.reverse, S.da);
+    tc.start(c0, S.c_stride[1], S.reverse, dc_here);
     auto fetch = [&](int i0) {
         const int n = min(kC, len - i0);
         const long long t0 = S.reverse ? len - 1 - i0 : i0;
-        if constexpr (!kStates) ta.load(S.a, a0 + t0 * S.a_stride[1], dir * S.a_stride[1], n, S.da, A.wide_a);
-        tb.load(S.b, b0 + t0 * S.b_stride[1], dir * S.b_stride[1], n, S.da, A.wide_b);
-        tc.load(S.c, c0 + t0 * S.c_stride[1], dir * S.c_stride[1], n, dc_here, A.wide_c);
+        if constexpr (!kStates) ta.load(t0 * S.a_stride[1], n);
+        tb.load(t0 * S.b_stride[1], n);
+        tc.load(t0 * S.c_stride[1], n);
     };
     fetch(begin);
 
@@ -262,7 +290,7 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
     const long long state0 = static_cast<long long>(bh) * S.da * S.dc;
     if constexpr (!kStates) {
         if (S.state_in) {
-            const float left = exp2f(g * static_cast<float>(min(begin, len)));
+            const float left = pow2(g * static_cast<float>(min(begin, len)));
 #pragma unroll
             for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
@@ -282,23 +310,20 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
             for (int k = 0; k < kRT * kCT; ++k) X[k / kCT][k % kCT] += w[k * kT + threadIdx.x];
         }
     }
-    // e^{g (n - off - j)} of a whole chunk, for the four steps of each 16 that the lane holds
-    f32x4 left[kB];
-    auto weights = [&](int n) {
+    // scale_in e^{g (n - off - j)}: what is left at the chunk's end of what enters at step j
+    auto left = [&](int n, int sb) {
+        f32x4 w;
 #pragma unroll
-        for (int sb = 0; sb < kB; ++sb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = sb * 16 + g4 + i;
-                left[sb][i] = j < n ? S.scale_in * exp2f(g * static_cast<float>(n - off - j)) : 0.f;
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int ago = n - off - (sb * 16 + g4 + i);
+            w[i] = ago + off > 0 ? S.scale_in * pow2(g * static_cast<float>(ago)) : 0.f;
+        }
+        return w;
     };
-    weights(kC);
 
     for (int i0 = begin; i0 < end; i0 += kC) {
         const int n = min(kC, len - i0);
         if (n <= 0) break;
-        if (n < kC) weights(n);
         __syncthreads();                       // the chunk before is done with
         if constexpr (!kStates) ta.store(la, kSA);
         tb.store(lb, kSB);
@@ -326,7 +351,7 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int ago = (tb_ - sb) * 16 + r - g4 - i;
-                            p[i] = ago >= 0 ? p[i] * (S.scale_in * exp2f(g * static_cast<float>(ago))) : 0.f;
+                            p[i] = ago >= 0 ? p[i] * (S.scale_in * pow2(g * static_cast<float>(ago))) : 0.f;
                         }
                         *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + sb * 16 + g4) = M::frag(p);
                     }
@@ -350,7 +375,7 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
             }
 #pragma unroll
             for (int t = 0; t < kB; ++t) {
-                const float since = exp2f(g * static_cast<float>(t * 16 + r + off));
+                const float since = pow2(g * static_cast<float>(t * 16 + r + off));
 #pragma unroll
                 for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
             }
@@ -376,30 +401,38 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
             // lane: step t*16 + r, columns g4 .. + 3 of each tile
 #pragma unroll
             for (int t = 0; t < kB; ++t) {
-                const int i = t * 16 + r;
-                if (i < n) {
-                    const long long step = S.reverse ? len - 1 - (i0 + i) : i0 + i;
-                    const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2];
+                const long long step = S.reverse ? len - 1 - (i0 + t * 16) - 15 : i0 + t * 16;     // least of the 16
+                const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2] + col0 + mine;
+                const long long lane_at = (S.reverse ? 15 - r : r) * S.y_stride[1] + g4;
+                if (t * 16 + r < n) {
 #pragma unroll
                     for (int ct = 0; ct < kCT; ++ct) {
                         const int col = col0 + mine + ct * 16 + g4;
                         const f32x4 v = y[t][ct] * S.scale_out;
                         if (A.y_f32) {
-                            float* o = static_cast<float*>(S.y) + at + col;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (col + k < S.dc) o[k] = v[k];
-                        } else {
-                            typedef typename In::Elem Out;
-                            typedef Out Out4 __attribute__((ext_vector_type(4)));
-                            Out* o = static_cast<Out*>(S.y) + at + col;
-                            const Out4 w = __builtin_convertvector(v, Out4);
-                            if (A.wide_y) {
-                                if (col < S.dc) *reinterpret_cast<Out4*>(o) = w;
+                            float* o = static_cast<float*>(S.y) + at + ct * 16;
+                            if constexpr (kWhole) {
+                                typedef f32x4 Any __attribute__((aligned(4)));
+                                if (col < S.dc)
+                                    *reinterpret_cast<Any*>(o + static_cast<unsigned>(lane_at)) = v;
                             } else {
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
-                                    if (col + k < S.dc) o[k] = w[k];
+                                    if (col + k < S.dc) o[lane_at + k] = v[k];
+                            }
+                        } else {
+                            typedef typename In::Elem Out;
+                            typedef Out Out4 __attribute__((ext_vector_type(4)));
+                            Out* o = static_cast<Out*>(S.y) + at + ct * 16;
+                            const Out4 w = __builtin_convertvector(v, Out4);
+                            if constexpr (kWhole) {
+                                typedef Out4 Any __attribute__((aligned(sizeof(Out))));
+                                if (col < S.dc)
+                                    *reinterpret_cast<Any*>(o + static_cast<unsigned>(lane_at)) = w;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (col + k < S.dc) o[lane_at + k] = w[k];
                             }
                         }
                     }
@@ -407,32 +440,35 @@ __global__ void __launch_bounds__(kW * 64) k_chunk(ChunkArgs A) {
             }
         }
         // the state that leaves
-        const float keep = exp2f(g * static_cast<float>(n));
-        Frag wc[M::kTerms][kB][kCT];
+        const float keep = pow2(g * static_cast<float>(n));
 #pragma unroll
-        for (int sb = 0; sb < kB; ++sb)
+        for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
-            for (int ct = 0; ct < kCT; ++ct) {
-                f32x4 w = M::wide(c[sb][ct]) * left[sb];
+            for (int ct = 0; ct < kCT; ++ct) X[rt][ct] *= keep;
 #pragma unroll
-                for (int k = 0; k < M::kTerms; ++k) {
-                    wc[k][sb][ct] = M::frag(w);
-                    w -= M::wide(wc[k][sb][ct]);
+        for (int sb = 0; sb < kB; sb += 2) {
+            Frag wc[M::kTerms][2][kCT];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const f32x4 w0 = left(n, sb + e);
+#pragma unroll
+                for (int ct = 0; ct < kCT; ++ct) {
+                    f32x4 w = M::wide(c[sb + e][ct]) * w0;
+#pragma unroll
+                    for (int k = 0; k < M::kTerms; ++k) {
+                        wc[k][e][ct] = M::frag(w);
+                        w -= M::wide(wc[k][e][ct]);
+                    }
                 }
             }
 #pragma unroll
-        for (int rt = 0; rt < kRT; ++rt) {
-            Frag b[kB];
+            for (int rt = 0; rt < kRT; ++rt) {
+                const Frag b_0 = M::column(lb + sb * 16 * kSB + rt * 16, kSB, lane);
+                const Frag b_1 = M::column(lb + (sb + 1) * 16 * kSB + rt * 16, kSB, lane);
 #pragma unroll
-            for (int sb = 0; sb < kB; ++sb) b[sb] = M::column(lb + sb * 16 * kSB + rt * 16, kSB, lane);
+                for (int ct = 0; ct < kCT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < kCT; ++ct) {
-                f32x4 x = X[rt][ct] * keep;
-#pragma unroll
-                for (int sb = 0; sb < kB; sb += 2)
-#pragma unroll
-                    for (int k = 0; k < M::kTerms; ++k) x = M::mma(x, b[sb], b[sb + 1], wc[k][sb][ct], wc[k][sb + 1][ct]);
-                X[rt][ct] = x;
+                    for (int k = 0; k < M::kTerms; ++k) X[rt][ct] = M::mma(X[rt][ct], b_0, b_1, wc[k][0][ct], wc[k][1][ct]);
             }
         }
     }
@@ -478,7 +514,7 @@ __global__ void __launch_bounds__(kThreads) k_join(float* states, const float* l
     f32x4 x = w[0];
     for (int s = 1; s < nseg; ++s) {
         const int n = min(max(len - s * seg_steps, 0), seg_steps);
-        x = x * exp2f(g * static_cast<float>(n)) + w[static_cast<long long>(s) * each];
+        x = x * pow2(g * static_cast<float>(n)) + w[static_cast<long long>(s) * each];
         w[static_cast<long long>(s) * each] = x;
     }
 }
@@ -530,21 +566,16 @@ Cut cut_of(int64_t type, int64_t batch, int64_t heads, int64_t time, int64_t da,
     return c;
 }
 
-bool whole(const void* p, const long long* stride, int d, int piece, size_t size) {
-    return reinterpret_cast<uintptr_t>(p) % (piece * size) == 0 && d % piece == 0 && stride[0] % piece == 0 &&
-           stride[1] % piece == 0 && stride[2] % piece == 0;
-}
-
-template <class T, int kDA, int kW, int kCT>
+template <class T, int kDA, int kW, int kCT, bool kWhole>
 hipError_t launch_cut(const ChunkArgs& A, long long bh, hipStream_t st) {
     if (A.nseg > 1) {
-        k_chunk<T, kDA, kW, kCT, true>
+        k_chunk<T, kDA, kW, kCT, kWhole, true>
             <<<static_cast<unsigned>(bh * (A.nseg - 1) * A.nslice), kW * 64, 0, st>>>(A);
         const int each = A.nslice * (kDA / 16) * kCT * kW * 64;
         k_join<<<dim3((each + kThreads - 1) / kThreads, static_cast<unsigned>(bh)), kThreads, 0, st>>>(
             A.states, A.s.log_decay, A.s.lengths, A.s.heads, A.s.time, A.nseg - 1, A.seg_steps, each);
     }
-    k_chunk<T, kDA, kW, kCT, false><<<static_cast<unsigned>(bh * A.nseg * A.nslice), kW * 64, 0, st>>>(A);
+    k_chunk<T, kDA, kW, kCT, kWhole, false><<<static_cast<unsigned>(bh * A.nseg * A.nslice), kW * 64, 0, st>>>(A);
     return hipGetLastError();
 }
 
@@ -554,26 +585,29 @@ hipError_t launch_chunks(const ScanArgs& S, int64_t type, long long batch, bool 
     ChunkArgs A{};
     A.s = S, A.nslice = c.nslice, A.nseg = c.nseg, A.seg_steps = c.seg_steps;
     A.states = static_cast<float*>(states);
-    constexpr int kP = InputOf<T>::Math::kPiece;
-    A.wide_a = whole(S.a, S.a_stride, S.da, kP, sizeof(T));
-    A.wide_b = whole(S.b, S.b_stride, S.da, kP, sizeof(T));
-    A.wide_c = whole(S.c, S.c_stride, S.dc, kP, sizeof(T));
-    A.wide_y = whole(S.y, S.y_stride, S.dc, 4, sizeof(T));
     A.y_f32 = y_f32;
     const long long bh = batch * S.heads;
-    auto go = [&](auto rows) {
+    auto go = [&](auto rows, auto whole) {
         constexpr int kDA = decltype(rows)::value;
-        if (c.waves == 2) return launch_cut<T, kDA, 2, 1>(A, bh, st);
+        constexpr bool kWhole = decltype(whole)::value;
+        if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole>(A, bh, st);
         if constexpr (kDA < 256)
-            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2>(A, bh, st);
-        return launch_cut<T, kDA, 4, 1>(A, bh, st);
+            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole>(A, bh, st);
+        return launch_cut<T, kDA, 4, 1, kWhole>(A, bh, st);
     };
-    switch (c.rows) {
-        case 32: return go(std::integral_constant<int, 32>{});
-        case 64: return go(std::integral_constant<int, 64>{});
-        case 128: return go(std::integral_constant<int, 128>{});
-        default: return go(std::integral_constant<int, 256>{});
-    }
+    auto rows = [&](auto whole) {
+        switch (c.rows) {
+            case 32: return go(std::integral_constant<int, 32>{}, whole);
+            case 64: return go(std::integral_constant<int, 64>{}, whole);
+            case 128: return go(std::integral_constant<int, 128>{}, whole);
+            default: return go(std::integral_constant<int, 256>{}, whole);
+        }
+    };
+    constexpr int kP = InputOf<T>::Math::kPiece;
+    constexpr long long kFar = 1 << 23;          // elements from step to step: 64 of them in 32 bits of bytes
+    const bool whole = S.da % kP == 0 && S.dc % kP == 0 && S.a_stride[1] < kFar && S.b_stride[1] < kFar &&
+                       S.c_stride[1] < kFar && S.y_stride[1] < kFar;
+    return whole ? rows(std::true_type{}) : rows(std::false_type{});
 }
 
 ScanArgs scan_args(const hx_attention_args& A, const Operand& a, const Operand& b, const Operand& c, bool reverse) {
