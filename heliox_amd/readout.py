@@ -18,6 +18,7 @@ or TypeError; a failing library call raises HelioxError.
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Tuple, Union
 
@@ -34,19 +35,26 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _NO_STRIDE = (0, 0, 0)
 
 
+# A call's checks are most of a small call's time, so each goes the short way first (attributes
+# compared as they are, devices as numbers, 50-80 ns each) and finds out what is wrong only where
+# something is.
+
+
 def _type(x: torch.Tensor, what: str) -> int:
-    try:
-        return _TYPES[x.dtype]
-    except KeyError:
-        raise TypeError(f"{what}: {x.dtype} is not float32, float16 or bfloat16") from None
+    kind = _TYPES.get(x.dtype)
+    if kind is None:
+        raise TypeError(f"{what}: {x.dtype} is not float32, float16 or bfloat16")
+    return kind
 
 
-def _on_gpu(x: torch.Tensor, what: str) -> torch.device:
+def _on_gpu(x: torch.Tensor, what: str) -> int:
+    """The number of the GPU that x is on."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what} has to be a tensor, got {type(x).__name__}")
-    if not x.is_cuda:
+    device = x.get_device()
+    if device < 0:
         raise ValueError(f"{what} has to be on the GPU, it is on {x.device}")
-    return x.device
+    return device
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -54,61 +62,76 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
-def _array(x: Optional[torch.Tensor], what: str, dtype: torch.dtype, shape: tuple, device) -> Optional[torch.Tensor]:
+def _array(x: Optional[torch.Tensor], what: str, dtype: torch.dtype, shape: tuple,
+           device: int) -> Optional[torch.Tensor]:
     """An argument that is handed on as a contiguous array of one type."""
     if x is None:
         return None
-    if _on_gpu(x, what) != device:
-        raise ValueError(f"{what} is on {x.device}, not on {device}")
-    if x.dtype != dtype:
+    if not isinstance(x, torch.Tensor) or x.get_device() != device:
+        if _on_gpu(x, what) != device:
+            raise ValueError(f"{what} is on {x.device}, not on cuda:{device}")
+    if x.dtype is not dtype:
         raise TypeError(f"{what} is {x.dtype}, expected {dtype}")
     if x.shape != shape:
         raise ValueError(f"{what} has shape {tuple(x.shape)}, expected {tuple(shape)}")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _ptr(x: Optional[torch.Tensor]) -> int:
     return 0 if x is None else x.data_ptr()
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# torch's current stream on a device as the number that the library takes (torch.cuda's own
+# object for it takes 2 us to make).
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+_entries: dict = {}
 
 
-def _call(name: str, device, *args) -> int:
+def _call(name: str, device: int, *args) -> int:
     """The library's answer; on the device of the tensors."""
-    if torch.cuda.current_device() == device.index:
-        got = getattr(lib(), name)(*args)
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(lib(), name)
+    if torch.cuda.current_device() == device:
+        got = entry(*args)
     else:
         with torch.cuda.device(device):
-            got = getattr(lib(), name)(*args)
+            got = entry(*args)
     if got < 0:
         raise HelioxError(lib().hx_readout_error().decode())
     return got
 
 
+def _like(x: torch.Tensor, what: str, q: torch.Tensor, device: int) -> None:
+    if not isinstance(x, torch.Tensor) or x.get_device() != device:
+        if _on_gpu(x, what) != device:
+            raise ValueError(f"{what} is on {x.device}, q on cuda:{device}")
+    if x.dtype is not q.dtype:
+        raise TypeError(f"{what} is {x.dtype}, q is {q.dtype}")
+
+
 def _attention_inputs(q, k, v, log_decay, ndim: int):
     """q, k, v with contiguous last dimensions, and their sizes as the record takes them."""
     device = _on_gpu(q, "q")
-    for x, name in ((k, "k"), (v, "v")):
-        if _on_gpu(x, name) != device:
-            raise ValueError(f"{name} is on {x.device}, q on {device}")
-        if x.dtype != q.dtype:
-            raise TypeError(f"{name} is {x.dtype}, q is {q.dtype}")
+    _like(k, "k", q, device)
+    _like(v, "v", q, device)
     kind = _type(q, "q, k and v")
-    if not q.dim() == k.dim() == v.dim() == ndim:
+    sq, sk, sv = q.shape, k.shape, v.shape
+    if not len(sq) == len(sk) == len(sv) == ndim:
         want = "(batch, time, heads, d)" if ndim == 4 else "(batch, heads, d)"
-        raise ValueError(f"q, k and v have to be {want}, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if not q.shape[:-2] == k.shape[:-2] == v.shape[:-2]:
-        raise ValueError(f"q, k and v differ in batch or time: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"q has {q.shape[-1]} channels, k has {k.shape[-1]}")
+        raise ValueError(f"q, k and v have to be {want}, got {tuple(sq)}, {tuple(sk)}, {tuple(sv)}")
+    if not sq[:-2] == sk[:-2] == sv[:-2]:
+        raise ValueError(f"q, k and v differ in batch or time: {tuple(sq)}, {tuple(sk)}, {tuple(sv)}")
+    if sq[-1] != sk[-1]:
+        raise ValueError(f"q has {sq[-1]} channels, k has {sk[-1]}")
     heads = log_decay.shape[0] if isinstance(log_decay, torch.Tensor) and log_decay.dim() == 1 else -1
-    log_decay = _array(log_decay, "log_decay", torch.float32, (heads,), device)
     if log_decay is None:
         raise TypeError("log_decay has to be a tensor")
-    time = q.shape[1] if ndim == 4 else 1
-    sizes = (kind, q.shape[0], time, heads, q.shape[-2], k.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1])
+    log_decay = _array(log_decay, "log_decay", torch.float32, (heads,), device)
+    time = sq[1] if ndim == 4 else 1
+    sizes = (kind, sq[0], time, heads, sq[-2], sk[-2], sv[-2], sq[-1], sv[-1])
     return device, _rows(q), _rows(k), _rows(v), log_decay, sizes
 
 
@@ -142,8 +165,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     _, batch, time, heads, _, _, _, dk, dv = sizes
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, heads, dk, dv), device)
     lengths = _lengths(lengths, batch, device)
-    o = torch.empty((batch, time, heads, dv), dtype=q.dtype, device=device)
-    end = torch.empty((batch, heads, dk, dv), dtype=torch.float32, device=device)
+    o = torch.empty((batch, time, heads, dv), dtype=q.dtype, device=q.device)
+    end = torch.empty((batch, heads, dk, dv), dtype=torch.float32, device=q.device)
     head = (*sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay),
             _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, _ptr(o), *_strides(o),
             _ptr(end), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
@@ -151,9 +174,19 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     return o, end
 
 
-def _run_attention(name: str, device, head: tuple, grad: int) -> None:
-    need = _call("hx_linear_attention_workspace", device, _ATTENTION.pack(*head, 0, 0, 0), grad)
-    space = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+@functools.lru_cache(maxsize=1024)
+def _attention_space(sizes: tuple, grad: int) -> int:
+    """Bytes of workspace, by the sizes alone."""
+    record = _ATTENTION.pack(*sizes, *[0] * 15, 1.0, *[0] * 20)
+    need = lib().hx_linear_attention_workspace(record, grad)
+    if need < 0:
+        raise HelioxError(lib().hx_readout_error().decode())
+    return need
+
+
+def _run_attention(name: str, device: int, head: tuple, grad: int) -> None:
+    need = _attention_space(head[:9], grad)
+    space = torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}") if need else None
     _call(name, device, _ATTENTION.pack(*head, _ptr(space), need, _stream(device)))
 
 
@@ -168,17 +201,14 @@ def linear_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     for them."""
     device, q, k, v, log_decay, sizes = _attention_inputs(q, k, v, log_decay, 4)
     _, batch, time, heads, _, _, _, dk, dv = sizes
-    if _on_gpu(do, "do") != device:
-        raise ValueError(f"do is on {do.device}, q on {device}")
-    if do.dtype != q.dtype:
-        raise TypeError(f"do is {do.dtype}, q is {q.dtype}")
+    _like(do, "do", q, device)
     if do.shape != (batch, time, heads, dv):
         raise ValueError(f"do has shape {tuple(do.shape)}, expected {(batch, time, heads, dv)}")
     do = _rows(do)
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, heads, dk, dv), device)
     dstate = _array(dstate, "dstate", torch.float32, (batch, heads, dk, dv), device)
     lengths = _lengths(lengths, batch, device)
-    dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+    dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
     dinitial = None if initial_state is None else torch.empty_like(initial_state)
     head = (*sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay),
             _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, 0, *_NO_STRIDE, 0, _ptr(do),
@@ -197,11 +227,11 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     device, q, k, v, log_decay, sizes = _attention_inputs(q, k, v, log_decay, 3)
     _, batch, _, heads, _, _, _, dk, dv = sizes
     if _on_gpu(state, "state") != device or state.dtype != torch.float32 or not state.is_contiguous():
-        raise TypeError(f"state has to be a contiguous float32 tensor on {device}")
+        raise TypeError(f"state has to be a contiguous float32 tensor on {q.device}")
     if state.dim() != 4 or state.shape[1:] != (heads, dk, dv):
         raise ValueError(f"state has shape {tuple(state.shape)}, expected (n_slots, {heads}, {dk}, {dv})")
     slots = _array(slots, "slots", torch.int32, (batch,), device)
-    o = torch.empty((batch, heads, dv), dtype=q.dtype, device=device)
+    o = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
         *sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay), 0, 0,
         dk ** -0.5 if scale is None else scale, _ptr(o), *_strides(o), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, _ptr(state),
@@ -221,7 +251,7 @@ def _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, we
     rows, vocab = logits.shape
     for x, name in ((teacher_index, "teacher_index"), (teacher_logits, "teacher_logits")):
         if _on_gpu(x, name) != device:
-            raise ValueError(f"{name} is on {x.device}, logits on {device}")
+            raise ValueError(f"{name} is on {x.device}, logits on {logits.device}")
         if x.dim() != 2 or x.shape[0] != rows:
             raise ValueError(f"{name} has to be ({rows}, top), got shape {tuple(x.shape)}")
     if teacher_index.shape != teacher_logits.shape:
@@ -233,7 +263,7 @@ def _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, we
     teacher_index, teacher_logits = _rows(teacher_index), _rows(teacher_logits)
     teacher_lse = _array(teacher_lse, "teacher_lse", torch.float32, (rows,), device)
     weight = _array(weight, "weight", torch.float32, (rows,), device)
-    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     _call("hx_distill_loss", device, _DISTILL.pack(
         kind, teacher_kind, 32 if teacher_index.dtype == torch.int32 else 64, rows, vocab, teacher_index.shape[1],
         _ptr(logits), logits.stride(0), _ptr(teacher_index), teacher_index.stride(0), _ptr(teacher_logits),
@@ -263,7 +293,7 @@ def distill_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     if out is None:
         _on_gpu(logits, "logits")
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif (_on_gpu(out, "out") != logits.device or out.dtype != logits.dtype or out.shape != logits.shape
+    elif (_on_gpu(out, "out") != _on_gpu(logits, "logits") or out.dtype != logits.dtype or out.shape != logits.shape
           or (out.shape[-1] > 1 and out.stride(-1) != 1)):
         raise ValueError("out has to be like the logits, its last dimension contiguous")
     return _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, weight, out), out
@@ -301,8 +331,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
         else:
             pointers.append(None)
             values.append(x)
-    token = torch.empty(rows, dtype=torch.int64, device=device)
-    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    token = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
     _call("hx_sample", device, _SAMPLE.pack(
         kind, rows, vocab, _ptr(logits), logits.stride(0), _ptr(u), *map(_ptr, pointers), values[0], values[2],
         values[3], values[1], _ptr(token), _ptr(logprob), _stream(device)))
