@@ -162,9 +162,9 @@ struct MathF32 {
 };
 
 template <class T> struct InputOf;      // math, and a piece of a row as it is loaded
-template <> struct InputOf<float> { using Math = MathF32; using Elem = float; using Raw = f32x4; };
-template <> struct InputOf<__half> { using Math = MathF32; using Elem = _Float16; using Raw = f16x4; };
-template <> struct InputOf<__hip_bfloat16> { using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; };
+template <> struct InputOf<float> { using Math = MathF32; using Elem = float; using Raw = f32x4; using Four = f32x4; };
+template <> struct InputOf<__half> { using Math = MathF32; using Elem = _Float16; using Raw = f16x4; using Four = f16x4; };
+template <> struct InputOf<__hip_bfloat16> { using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; using Four = bf16x4; };
 
 // Rows [0, n) of a chunk into registers, kD columns padded with zeros, R rows a round of the
 // workgroup.  kWhole: d is a whole number of pieces and a round's rows are within 2 GiB, so that
@@ -198,6 +198,8 @@ struct Tile {
         }
     }
     __device__ __forceinline__ void load(long long first, int n) {       // from row `first` (in memory order) on
+        // new to the compiler in every chunk, or it keeps a running 64-bit address a load by lane
+        if constexpr (kWhole) asm volatile("" : "+v"(offset));
 #pragma unroll
         for (int p = 0; p < kN; ++p) {
             Raw x = {};
@@ -230,6 +232,20 @@ struct ChunkArgs {
     bool y_f32;
 };
 
+// Four neighbours of a row to base[at], of which `columns` are there.
+template <class Out, class Four, bool kWhole>
+__device__ __forceinline__ void put(Out* base, long long at, int columns, f32x4 v) {
+    const Four w = __builtin_convertvector(v, Four);
+    if constexpr (kWhole) {
+        typedef Four Any __attribute__((aligned(sizeof(Out))));
+        if (columns > 0) *reinterpret_cast<Any*>(base + static_cast<unsigned>(at)) = w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < columns) base[at + k] = w[k];
+    }
+}
+
 // Waves a SIMD that the registers have to leave room for.
 constexpr int waves_of(int) { return 2; }
 
@@ -257,8 +273,9 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     const int col0 = slice * kDC;                          // of the slice
     const int mine = wave * kCT * 16;                      // of the wave, in the slice
     const float lg = S.log_decay[h] * 1.44269504f;
-    const float g = lg < -1e4f ? -1e4f : lg;               // -inf: e^{g 0} stays 1
+    float g = lg < -1e4f ? -1e4f : lg;                     // -inf: e^{g 0} stays 1
     const int off = S.reverse ? 0 : 1;
+    const float scale = S.scale_in * S.scale_out;
     const int dc_here = min(S.dc - col0, kDC);
 
     const T* a0 = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
@@ -330,110 +347,92 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
         tc.store(lc, kSC);
         __syncthreads();
         if (i0 + kC < end) fetch(i0 + kC);
-        f32x4 y[kB][kCT];
+        asm volatile("" : "+v"(g));             // decays are made anew in every chunk: kept, they take 40 registers
+        Frag c[kB][kCT];
         if constexpr (!kStates) {
-            // blocks on and under the diagonal, dealt out over the waves
-            int turn = 0;
+            // P's blocks, as many for each wave (those over the diagonal come out as zero)
+            constexpr int kEach = kB * kB / kW;
+            f32x4 p[kEach];
 #pragma unroll
-            for (int tb_ = 0; tb_ < kB; ++tb_)
-#pragma unroll
-                for (int sb = 0; sb <= tb_; ++sb)
-                    if (turn++ % kW == wave) {
-                        f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int k = 0; k < kRT; k += 2) {
-                            const Elem* pa = la + (tb_ * 16 + r) * kSA + k * 16 + g4;
-                            const Elem* pb = lb + (sb * 16 + r) * kSB + k * 16 + g4;
-                            p = M::mma(p, *reinterpret_cast<const Frag*>(pb), *reinterpret_cast<const Frag*>(pb + 16),
-                                       *reinterpret_cast<const Frag*>(pa), *reinterpret_cast<const Frag*>(pa + 16));
-                        }
-                        // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int ago = (tb_ - sb) * 16 + r - g4 - i;
-                            p[i] = ago >= 0 ? p[i] * (S.scale_in * pow2(g * static_cast<float>(ago))) : 0.f;
-                        }
-                        *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + sb * 16 + g4) = M::frag(p);
-                    }
-            // what the entering state adds
-#pragma unroll
-            for (int t = 0; t < kB; ++t)
-#pragma unroll
-                for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < kEach; ++e) p[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int block0 = wave * kEach;
 #pragma unroll
             for (int k = 0; k < kRT; k += 2) {
-                Frag x0[kCT], x1[kCT];
+                Frag a_0, a_1;
 #pragma unroll
-                for (int ct = 0; ct < kCT; ++ct) x0[ct] = M::frag(X[k][ct]), x1[ct] = M::frag(X[k + 1][ct]);
-#pragma unroll
-                for (int t = 0; t < kB; ++t) {
-                    const Elem* pa = la + (t * 16 + r) * kSA + k * 16 + g4;
-                    const Frag a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
-#pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], x0[ct], x1[ct], a_0, a_1);
+                for (int e = 0; e < kEach; ++e) {
+                    const int sb = (block0 + e) % kB;
+                    if (e % kB == 0) {
+                        const Elem* pa = la + ((block0 + e) / kB * 16 + r) * kSA + k * 16 + g4;
+                        a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
+                    }
+                    const Elem* pb = lb + (sb * 16 + r) * kSB + k * 16 + g4;
+                    p[e] = M::mma(p[e], *reinterpret_cast<const Frag*>(pb), *reinterpret_cast<const Frag*>(pb + 16), a_0,
+                                  a_1);
                 }
             }
+            // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
 #pragma unroll
-            for (int t = 0; t < kB; ++t) {
-                const float since = pow2(g * static_cast<float>(t * 16 + r + off));
+            for (int e = 0; e < kEach; ++e) {
+                const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
 #pragma unroll
-                for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
+                for (int i = 0; i < 4; ++i) {
+                    const int ago = (tb_ - sb) * 16 + r - g4 - i;
+                    p[e][i] = ago >= 0 ? p[e][i] * (scale * pow2(g * static_cast<float>(ago))) : 0.f;
+                }
+                *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + sb * 16 + g4) = M::frag(p[e]);
             }
         }
-        Frag c[kB][kCT];
 #pragma unroll
         for (int sb = 0; sb < kB; ++sb)
 #pragma unroll
             for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::column(lc + sb * 16 * kSC + mine + ct * 16, kSC, lane);
         if constexpr (!kStates) {
             __syncthreads();                   // P is whole
+            // two blocks of steps at a time: what the entering state adds, then the chunk's own steps
 #pragma unroll
-            for (int t = 0; t < kB; ++t)
+            for (int t0 = 0; t0 < kB; t0 += 2) {
+                f32x4 y[2][kCT];
 #pragma unroll
-                for (int sb = 0; sb <= t; sb += 2) {
-                    const Elem* pp = lp + (t * 16 + r) * kSP + sb * 16 + g4;
-                    const Frag p0 = *reinterpret_cast<const Frag*>(pp);
-                    Frag p1 = {};
-                    if (sb + 1 <= t) p1 = *reinterpret_cast<const Frag*>(pp + 16);
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], c[sb][ct], c[sb + 1][ct], p0, p1);
+                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kRT; k += 2) {
+                    Frag x0[kCT], x1[kCT];
+#pragma unroll
+                    for (int ct = 0; ct < kCT; ++ct) x0[ct] = M::frag(X[k][ct]), x1[ct] = M::frag(X[k + 1][ct]);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const Elem* pa = la + ((t0 + t) * 16 + r) * kSA + k * 16 + g4;
+                        const Frag a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
+#pragma unroll
+                        for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], x0[ct], x1[ct], a_0, a_1);
+                    }
                 }
-            // lane: step t*16 + r, columns g4 .. + 3 of each tile
 #pragma unroll
-            for (int t = 0; t < kB; ++t) {
-                const long long step = S.reverse ? len - 1 - (i0 + t * 16) - 15 : i0 + t * 16;     // least of the 16
-                const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2] + col0 + mine;
-                const long long lane_at = (S.reverse ? 15 - r : r) * S.y_stride[1] + g4;
-                if (t * 16 + r < n) {
+                for (int t = 0; t < 2; ++t) {
+                    const float since = S.scale_out * pow2(g * static_cast<float>((t0 + t) * 16 + r + off));
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) {
-                        const int col = col0 + mine + ct * 16 + g4;
-                        const f32x4 v = y[t][ct] * S.scale_out;
-                        if (A.y_f32) {
-                            float* o = static_cast<float*>(S.y) + at + ct * 16;
-                            if constexpr (kWhole) {
-                                typedef f32x4 Any __attribute__((aligned(4)));
-                                if (col < S.dc)
-                                    *reinterpret_cast<Any*>(o + static_cast<unsigned>(lane_at)) = v;
-                            } else {
+                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    if (col + k < S.dc) o[lane_at + k] = v[k];
-                            }
-                        } else {
-                            typedef typename In::Elem Out;
-                            typedef Out Out4 __attribute__((ext_vector_type(4)));
-                            Out* o = static_cast<Out*>(S.y) + at + ct * 16;
-                            const Out4 w = __builtin_convertvector(v, Out4);
-                            if constexpr (kWhole) {
-                                typedef Out4 Any __attribute__((aligned(sizeof(Out))));
-                                if (col < S.dc)
-                                    *reinterpret_cast<Any*>(o + static_cast<unsigned>(lane_at)) = w;
-                            } else {
+                    for (int sb = 0; sb <= t0 + t; sb += 2) {
+                        const Elem* pp = lp + ((t0 + t) * 16 + r) * kSP + sb * 16 + g4;
+                        const Frag p0 = *reinterpret_cast<const Frag*>(pp), p1 = *reinterpret_cast<const Frag*>(pp + 16);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    if (col + k < S.dc) o[lane_at + k] = w[k];
-                            }
+                        for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], c[sb][ct], c[sb + 1][ct], p0, p1);
+                    }
+                    // lane: step (t0 + t)*16 + r, columns g4 .. + 3 of each tile
+                    const int i1 = i0 + (t0 + t) * 16;
+                    const long long step = S.reverse ? len - 1 - i1 - 15 : i1;         // least of the 16
+                    const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2] + col0 + mine;
+                    const long long lane_at = (S.reverse ? 15 - r : r) * S.y_stride[1] + g4;
+                    if (i1 + r < len) {
+#pragma unroll
+                        for (int ct = 0; ct < kCT; ++ct) {
+                            const int columns = S.dc - (col0 + mine + ct * 16 + g4);
+                            if (A.y_f32) put<float, f32x4, kWhole>(static_cast<float*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
+                            else put<typename In::Elem, typename In::Four, kWhole>(static_cast<typename In::Elem*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
                         }
                     }
                 }
@@ -511,11 +510,22 @@ __global__ void __launch_bounds__(kThreads) k_join(float* states, const float* l
     const float lg = log_decay[h] * 1.44269504f;
     const float g = lg < -1e4f ? -1e4f : lg;
     f32x4* w = reinterpret_cast<f32x4*>(states) + static_cast<long long>(bh) * nseg * each + e;
-    f32x4 x = w[0];
-    for (int s = 1; s < nseg; ++s) {
-        const int n = min(max(len - s * seg_steps, 0), seg_steps);
-        x = x * pow2(g * static_cast<float>(n)) + w[static_cast<long long>(s) * each];
-        w[static_cast<long long>(s) * each] = x;
+    // the segments' loads do not wait for each other
+    constexpr int kAhead = 8;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, next[kAhead];
+    for (int s0 = 0; s0 < nseg; s0 += kAhead) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (s0 + k < nseg) next[k] = w[static_cast<long long>(s0 + k) * each];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = s0 + k;
+            if (s < nseg) {
+                const int n = min(max(len - s * seg_steps, 0), seg_steps);
+                x = x * pow2(g * static_cast<float>(n)) + next[k];
+                w[static_cast<long long>(s) * each] = x;
+            }
+        }
     }
 }
 
