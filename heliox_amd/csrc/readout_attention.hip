@@ -30,8 +30,10 @@ struct ScanArgs {
     const float* state_in;
     float* state_out;
     int row_stride, col_stride;      // of a state's da and dc
+    float* states;                   // (batch, heads, segments - 1) states: what enters segment 1, 2, ...
     void* y;
     long long y_stride[3];
+    bool y_f32;                      // y is fp32 whatever the inputs are
 };
 
 // ------------------------------------------------------------------- one step
@@ -225,12 +227,19 @@ struct Tile {
     }
 };
 
+constexpr int kJobs = 3;               // sums of one launch: the gradients are three
 struct ChunkArgs {
-    ScanArgs s;
+    ScanArgs job[kJobs];
     int nslice, nseg, seg_steps;       // seg_steps a multiple of the chunk
-    float* states;                     // of the segments, registers of each thread side by side
-    bool y_f32;
 };
+
+// The block's job where it lies among the kernel's arguments (indexed as a value, the array
+// would be copied to every lane's scratch memory first: 157 -> 452 us).
+typedef const __attribute__((address_space(4))) ScanArgs JobArgs;
+__device__ __forceinline__ JobArgs& job_of(const ChunkArgs&) {
+    typedef const __attribute__((address_space(4))) ChunkArgs Args;
+    return ((Args*)__builtin_amdgcn_kernarg_segment_ptr())->job[blockIdx.y];
+}
 
 // Four neighbours of a row to base[at], of which `columns` are there.
 template <class Out, class Four, bool kWhole>
@@ -250,7 +259,7 @@ __device__ __forceinline__ void put(Out* base, long long at, int columns, f32x4 
 constexpr int waves_of(int) { return 2; }
 
 // kDA: rows of the state (a's and b's columns) padded; kW waves of kCT 16-column tiles each.
-// kStates: only each segment's own state, from zero.
+// kStates: only the own state, from zero, of each segment but the last.
 template <class T, int kDA, int kW, int kCT, bool kWhole, bool kStates>
 __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     using In = InputOf<T>;
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     constexpr int kSA = kDA + M::kRowPad, kSB = kDA + M::kColPad, kSC = kDC + M::kColPad, kSP = kC + M::kRowPad;
     __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kC * kSA], lb[kC * kSB], lc[kC * kSC],
         lp[kStates ? 1 : kC * kSP];
-    const ScanArgs& S = A.s;
+    const JobArgs& S = job_of(A);
     const int lane = threadIdx.x % 64, r = lane % 16, g4 = lane / 16 * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int slice = blockIdx.x % A.nslice;
@@ -304,27 +313,29 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
         for (int ct = 0; ct < kCT; ++ct) X[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const long long state0 = static_cast<long long>(bh) * S.da * S.dc;
+    const long long state_size = static_cast<long long>(S.da) * S.dc;
+    // X at each place becomes f(X there, where that lies in a state)
+    auto each_place = [&](auto f) {
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+            for (int ct = 0; ct < kCT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
+                    if (row < S.da && col < S.dc)
+                        X[rt][ct][i] = f(X[rt][ct][i], row * S.row_stride + col * S.col_stride);
+                }
+    };
     if constexpr (!kStates) {
+        if (seg > 0) {
+            const float* w = S.states + (static_cast<long long>(bh) * (A.nseg - 1) + seg - 1) * state_size;
+            each_place([&](float, int at) { return w[at]; });
+        }
         if (S.state_in) {
             const float left = pow2(g * static_cast<float>(min(begin, len)));
-#pragma unroll
-            for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-                for (int ct = 0; ct < kCT; ++ct)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
-                        if (row < S.da && col < S.dc)
-                            X[rt][ct][i] = left * S.state_in[state0 + static_cast<long long>(row) * S.row_stride +
-                                                             static_cast<long long>(col) * S.col_stride];
-                    }
-        }
-        if (seg > 0) {
-            const f32x4* w = reinterpret_cast<const f32x4*>(A.states) +
-                             ((static_cast<long long>(bh) * (A.nseg - 1) + seg - 1) * A.nslice + slice) * (kRT * kCT * kT);
-#pragma unroll
-            for (int k = 0; k < kRT * kCT; ++k) X[k / kCT][k % kCT] += w[k * kT + threadIdx.x];
+            const float* w = S.state_in + bh * state_size;
+            each_place([&](float x, int at) { return x + left * w[at]; });
         }
     }
     // scale_in e^{g (n - off - j)}: what is left at the chunk's end of what enters at step j
@@ -431,7 +442,7 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct) {
                             const int columns = S.dc - (col0 + mine + ct * 16 + g4);
-                            if (A.y_f32) put<float, f32x4, kWhole>(static_cast<float*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
+                            if (S.y_f32) put<float, f32x4, kWhole>(static_cast<float*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
                             else put<typename In::Elem, typename In::Four, kWhole>(static_cast<typename In::Elem*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
                         }
                     }
@@ -472,58 +483,48 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
         }
     }
     if constexpr (kStates) {
-        f32x4* w = reinterpret_cast<f32x4*>(A.states) +
-                   ((static_cast<long long>(bh) * nseg + seg) * A.nslice + slice) * (kRT * kCT * kT);
-#pragma unroll
-        for (int k = 0; k < kRT * kCT; ++k) w[k * kT + threadIdx.x] = X[k / kCT][k % kCT];
+        float* w = S.states + (static_cast<long long>(bh) * nseg + seg) * state_size;
+        each_place([&](float x, int at) { return w[at] = x; });
     } else {
         // steps past the sequence's end
         for (int i = max(begin, len) + wave; i < end; i += kW) {
             const long long at = batch * S.y_stride[0] + i * S.y_stride[1] + h * S.y_stride[2];
             for (int col = col0 + lane; col < col0 + dc_here; col += 64)
-                if (A.y_f32) static_cast<float*>(S.y)[at + col] = 0.f;
+                if (S.y_f32) static_cast<float*>(S.y)[at + col] = 0.f;
                 else static_cast<typename In::Elem*>(S.y)[at + col] = static_cast<typename In::Elem>(0.f);
         }
         if (S.state_out && seg == A.nseg - 1) {
-#pragma unroll
-            for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-                for (int ct = 0; ct < kCT; ++ct)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
-                        if (row < S.da && col < S.dc)
-                            S.state_out[state0 + static_cast<long long>(row) * S.row_stride +
-                                        static_cast<long long>(col) * S.col_stride] = X[rt][ct][i];
-                    }
+            float* w = S.state_out + bh * state_size;
+            each_place([&](float x, int at) { return w[at] = x; });
         }
     }
 }
 
 // Segments' own states to the states that enter the segments after them, in place.
-__global__ void __launch_bounds__(kThreads) k_join(float* states, const float* log_decay, const int32_t* lengths,
-                                                   int heads, int time, int nseg, int seg_steps, int each) {
-    const int bh = blockIdx.y, batch = bh / heads, h = bh - batch * heads;
-    const int e = blockIdx.x * kThreads + threadIdx.x;
-    if (e >= each) return;
-    const int len = lengths ? min(max(lengths[batch], 0), time) : time;
-    const float lg = log_decay[h] * 1.44269504f;
+__global__ void __launch_bounds__(kThreads) k_join(ChunkArgs A) {
+    const JobArgs& S = job_of(A);
+    const int nseg = A.nseg - 1, size = S.da * S.dc, blocks = (size + kThreads - 1) / kThreads;
+    const int bh = blockIdx.x / blocks, e = blockIdx.x % blocks * kThreads + threadIdx.x;
+    if (e >= size) return;
+    const int batch = bh / S.heads, h = bh - batch * S.heads;
+    const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
+    const float lg = S.log_decay[h] * 1.44269504f;
     const float g = lg < -1e4f ? -1e4f : lg;
-    f32x4* w = reinterpret_cast<f32x4*>(states) + static_cast<long long>(bh) * nseg * each + e;
+    float* w = S.states + static_cast<long long>(bh) * nseg * size + e;
     // the segments' loads do not wait for each other
-    constexpr int kAhead = 8;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f}, next[kAhead];
+    constexpr int kAhead = 16;
+    float x = 0.f, next[kAhead];
     for (int s0 = 0; s0 < nseg; s0 += kAhead) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (s0 + k < nseg) next[k] = w[static_cast<long long>(s0 + k) * each];
+            if (s0 + k < nseg) next[k] = w[static_cast<long long>(s0 + k) * size];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const int s = s0 + k;
             if (s < nseg) {
-                const int n = min(max(len - s * seg_steps, 0), seg_steps);
+                const int n = min(max(len - s * A.seg_steps, 0), A.seg_steps);
                 x = x * pow2(g * static_cast<float>(n)) + next[k];
-                w[static_cast<long long>(s) * each] = x;
+                w[static_cast<long long>(s) * size] = x;
             }
         }
     }
@@ -553,71 +554,32 @@ struct Operand {
     int64_t heads, d;
 };
 
-// How a call is cut: state rows padded, waves and their 16-column tiles, slices of c's
-// columns, segments of the steps.
+// How a sum is cut: state rows padded, waves and their 16-column tiles.
 struct Cut {
-    int rows, waves, tiles, nslice, nseg, seg_steps;
-    size_t state_bytes;
+    int rows, waves, tiles;
+    int width() const { return waves * tiles * 16; }
 };
 
-Cut cut_of(int64_t type, int64_t batch, int64_t heads, int64_t time, int64_t da, int64_t dc) {
+Cut cut_of(int64_t da, int64_t dc) {
     Cut c{};
     c.rows = da <= 32 ? 32 : da <= 64 ? 64 : da <= 128 ? 128 : 256;
     c.waves = dc <= 32 ? 2 : 4;
     c.tiles = dc <= 64 || c.rows == 256 ? 1 : 2;
-    const int width = c.waves * c.tiles * 16, chunk = type == HX_BF16 ? MathBf16::kC : MathF32::kC;
-    c.nslice = static_cast<int>((dc + width - 1) / width);
-    const int64_t units = batch * heads * c.nslice, chunks = std::max<int64_t>(1, (time + chunk - 1) / chunk);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 4));
-    const int64_t each = (chunks + want - 1) / want;
-    c.seg_steps = static_cast<int>(each * chunk);
-    c.nseg = static_cast<int>((chunks + each - 1) / each);
-    c.state_bytes = sizeof(float) * (c.nseg - 1) * units * c.rows * width;
     return c;
 }
 
-template <class T, int kDA, int kW, int kCT, bool kWhole>
-hipError_t launch_cut(const ChunkArgs& A, long long bh, hipStream_t st) {
-    if (A.nseg > 1) {
-        k_chunk<T, kDA, kW, kCT, kWhole, true>
-            <<<static_cast<unsigned>(bh * (A.nseg - 1) * A.nslice), kW * 64, 0, st>>>(A);
-        const int each = A.nslice * (kDA / 16) * kCT * kW * 64;
-        k_join<<<dim3((each + kThreads - 1) / kThreads, static_cast<unsigned>(bh)), kThreads, 0, st>>>(
-            A.states, A.s.log_decay, A.s.lengths, A.s.heads, A.s.time, A.nseg - 1, A.seg_steps, each);
-    }
-    k_chunk<T, kDA, kW, kCT, kWhole, false><<<static_cast<unsigned>(bh * A.nseg * A.nslice), kW * 64, 0, st>>>(A);
-    return hipGetLastError();
-}
+// Segments of the steps, the same for all sums of a call.
+struct Segments {
+    int count, steps;
+};
 
-template <class T>
-hipError_t launch_chunks(const ScanArgs& S, int64_t type, long long batch, bool y_f32, void* states, hipStream_t st) {
-    const Cut c = cut_of(type, batch, S.heads, S.time, S.da, S.dc);
-    ChunkArgs A{};
-    A.s = S, A.nslice = c.nslice, A.nseg = c.nseg, A.seg_steps = c.seg_steps;
-    A.states = static_cast<float*>(states);
-    A.y_f32 = y_f32;
-    const long long bh = batch * S.heads;
-    auto go = [&](auto rows, auto whole) {
-        constexpr int kDA = decltype(rows)::value;
-        constexpr bool kWhole = decltype(whole)::value;
-        if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole>(A, bh, st);
-        if constexpr (kDA < 256)
-            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole>(A, bh, st);
-        return launch_cut<T, kDA, 4, 1, kWhole>(A, bh, st);
-    };
-    auto rows = [&](auto whole) {
-        switch (c.rows) {
-            case 32: return go(std::integral_constant<int, 32>{}, whole);
-            case 64: return go(std::integral_constant<int, 64>{}, whole);
-            case 128: return go(std::integral_constant<int, 128>{}, whole);
-            default: return go(std::integral_constant<int, 256>{}, whole);
-        }
-    };
-    constexpr int kP = InputOf<T>::Math::kPiece;
-    constexpr long long kFar = 1 << 23;          // elements from step to step: 64 of them in 32 bits of bytes
-    const bool whole = S.da % kP == 0 && S.dc % kP == 0 && S.a_stride[1] < kFar && S.b_stride[1] < kFar &&
-                       S.c_stride[1] < kFar && S.y_stride[1] < kFar;
-    return whole ? rows(std::true_type{}) : rows(std::false_type{});
+Segments segments_of(const hx_attention_args& A) {
+    const int chunk = A.type == HX_BF16 ? MathBf16::kC : MathF32::kC, width = cut_of(A.dk, A.dv).width();
+    const int64_t units = A.batch * A.heads * ((A.dv + width - 1) / width);
+    const int64_t chunks = std::max<int64_t>(1, (A.time + chunk - 1) / chunk);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 4));
+    const int64_t each = (chunks + want - 1) / want;
+    return {static_cast<int>((chunks + each - 1) / each), static_cast<int>(each * chunk)};
 }
 
 ScanArgs scan_args(const hx_attention_args& A, const Operand& a, const Operand& b, const Operand& c, bool reverse) {
@@ -638,34 +600,93 @@ void contiguous(long long* s, int64_t time, int64_t heads, int64_t d) {
     s[0] = time * heads * d, s[1] = heads * d, s[2] = d;
 }
 
-// Workspace: segments' states, then fp32 gradients by head where heads share an input.
-size_t state_part(const hx_attention_args& A, int64_t da, int64_t dc) {
-    const size_t n = cut_of(A.type, A.batch, A.heads, A.time, da, dc).state_bytes;
+template <class T, int kDA, int kW, int kCT, bool kWhole>
+hipError_t launch_cut(ChunkArgs& A, int jobs, bool states, long long bh, hipStream_t st) {
+    A.nslice = (A.job[0].dc + kW * kCT * 16 - 1) / (kW * kCT * 16);
+    const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice), jobs);
+    if (states) k_chunk<T, kDA, kW, kCT, kWhole, true><<<grid, kW * 64, 0, st>>>(A);
+    else k_chunk<T, kDA, kW, kCT, kWhole, false><<<grid, kW * 64, 0, st>>>(A);
+    return hipGetLastError();
+}
+
+// The jobs of one launch are of one size.
+template <class T>
+hipError_t launch_chunks(ChunkArgs A, int jobs, bool states, long long bh, hipStream_t st) {
+    constexpr int kP = InputOf<T>::Math::kPiece;
+    constexpr long long kFar = 1 << 23;          // elements from step to step: 64 of them in 32 bits of bytes
+    const Cut c = cut_of(A.job[0].da, A.job[0].dc);
+    bool all_whole = A.job[0].da % kP == 0 && A.job[0].dc % kP == 0;
+    for (int i = 0; i < jobs; ++i) {
+        const ScanArgs& S = A.job[i];
+        all_whole =
+            all_whole && S.a_stride[1] < kFar && S.b_stride[1] < kFar && S.c_stride[1] < kFar && S.y_stride[1] < kFar;
+    }
+    auto go = [&](auto rows, auto whole) {
+        constexpr int kDA = decltype(rows)::value;
+        constexpr bool kWhole = decltype(whole)::value;
+        if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole>(A, jobs, states, bh, st);
+        if constexpr (kDA < 256)
+            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole>(A, jobs, states, bh, st);
+        return launch_cut<T, kDA, 4, 1, kWhole>(A, jobs, states, bh, st);
+    };
+    auto rows = [&](auto whole) {
+        switch (c.rows) {
+            case 32: return go(std::integral_constant<int, 32>{}, whole);
+            case 64: return go(std::integral_constant<int, 64>{}, whole);
+            case 128: return go(std::integral_constant<int, 128>{}, whole);
+            default: return go(std::integral_constant<int, 256>{}, whole);
+        }
+    };
+    return all_whole ? rows(std::true_type{}) : rows(std::false_type{});
+}
+
+// What enters each segment but the first, where there are several; the jobs are of one size.
+template <class T>
+hipError_t launch_states(const ChunkArgs& A, int jobs, long long bh, hipStream_t st) {
+    if (A.nseg < 2) return hipSuccess;
+    const hipError_t e = launch_chunks<T>(A, jobs, true, bh, st);
+    if (e != hipSuccess) return e;
+    const long long blocks = (static_cast<long long>(A.job[0].da) * A.job[0].dc + kThreads - 1) / kThreads;
+    k_join<<<dim3(static_cast<unsigned>(bh * blocks), jobs), kThreads, 0, st>>>(A);
+    return hipGetLastError();
+}
+
+// Workspace: the segments' states (of the gradient's two directions), then fp32 gradients by head
+// for each input that heads share.
+size_t state_part(const hx_attention_args& A) {
+    const size_t n = sizeof(float) * (segments_of(A).count - 1) * A.batch * A.heads * A.dk * A.dv;
     return (n + 255) / 256 * 256;
 }
 
 size_t shared_part(const hx_attention_args& A, int64_t heads, int64_t d) {
-    return heads == A.heads ? 0 : sizeof(float) * A.batch * A.time * A.heads * d;
+    const size_t n = heads == A.heads ? 0 : sizeof(float) * A.batch * A.time * A.heads * d;
+    return (n + 255) / 256 * 256;
 }
 
 }  // namespace
 
 size_t attention_workspace(const hx_attention_args& A, bool grad) {
-    const size_t there = state_part(A, A.dk, A.dv);
-    if (!grad) return there;
-    return std::max(there, state_part(A, A.dv, A.dk)) +
-           std::max({shared_part(A, A.q_heads, A.dk), shared_part(A, A.k_heads, A.dk), shared_part(A, A.v_heads, A.dv)});
+    if (!grad) return state_part(A);
+    return 2 * state_part(A) + shared_part(A, A.q_heads, A.dk) + shared_part(A, A.k_heads, A.dk) +
+           shared_part(A, A.v_heads, A.dv);
 }
 
 hipError_t attention_forward(const hx_attention_args& A) {
     const Operand q{A.q, A.q_stride, A.q_heads, A.dk}, k{A.k, A.k_stride, A.k_heads, A.dk},
         v{A.v, A.v_stride, A.v_heads, A.dv};
-    ScanArgs S = scan_args(A, q, k, v, false);
+    const Segments seg = segments_of(A);
+    ChunkArgs C{};
+    C.nseg = seg.count, C.seg_steps = seg.steps;
+    ScanArgs& S = C.job[0];
+    S = scan_args(A, q, k, v, false);
+    S.states = static_cast<float*>(A.workspace);
     S.state_in = A.initial_state, S.state_out = A.end_state, S.row_stride = S.dc, S.col_stride = 1;
     S.y = A.o;
     for (int i = 0; i < 3; ++i) S.y_stride[i] = A.o_stride[i];
     return with_type(A.type, [&](auto t) {
-        return launch_chunks<decltype(t)>(S, A.type, A.batch, false, A.workspace, stream_of(A));
+        using T = decltype(t);
+        const hipError_t e = launch_states<T>(C, 1, A.batch * A.heads, stream_of(A));
+        return e != hipSuccess ? e : launch_chunks<T>(C, 1, false, A.batch * A.heads, stream_of(A));
     });
 }
 
@@ -692,32 +713,65 @@ hipError_t attention_backward(const hx_attention_args& A) {
     const Operand q{A.q, A.q_stride, A.q_heads, A.dk}, k{A.k, A.k_stride, A.k_heads, A.dk},
         v{A.v, A.v_stride, A.v_heads, A.dv}, o{A.grad_o, A.grad_o_stride, A.heads, A.dv};
     const hipStream_t st = stream_of(A);
+    const Segments seg = segments_of(A);
     char* const space = static_cast<char*>(A.workspace);
-    float* const by_head = reinterpret_cast<float*>(
-        space + std::max(state_part(A, A.dk, A.dv), state_part(A, A.dv, A.dk)));
-    auto one = [&](const Operand& a, const Operand& b, const Operand& c, bool reverse, bool transposed,
-                   const float* in, float* out, void* y, int64_t kept) -> hipError_t {
+    float* const ahead = reinterpret_cast<float*>(space);
+    float* const back = reinterpret_cast<float*>(space + state_part(A));
+    char* by_head = space + 2 * state_part(A);
+    const int dv = static_cast<int>(A.dv);
+    const long long bh = A.batch * A.heads;
+
+    // States lie as (dk, dv) whichever way a sum takes them: k v^T going forward, q do^T going
+    // back, the latter for dk and dv alike.
+    enum Columns { kOfKeys, kOfValues };
+    auto sum = [&](const Operand& a, const Operand& b, const Operand& c, bool reverse, Columns columns, float* states,
+                   void* y, int64_t kept) {
         ScanArgs S = scan_args(A, a, b, c, reverse);
-        S.state_in = in, S.state_out = out;
-        S.row_stride = transposed ? 1 : S.dc, S.col_stride = transposed ? S.da : 1;
-        const bool shared = kept != A.heads;
-        S.y = shared ? by_head : y;
+        S.row_stride = columns == kOfKeys ? 1 : dv, S.col_stride = columns == kOfKeys ? dv : 1;
+        S.states = states, S.state_in = reverse ? A.grad_end : A.initial_state;
+        S.y = y, S.y_f32 = kept != A.heads;
+        if (S.y_f32) {
+            S.y = by_head;
+            by_head += shared_part(A, kept, c.d);
+        }
         contiguous(S.y_stride, A.time, A.heads, c.d);
-        return with_type(A.type, [&](auto t) -> hipError_t {
-            using T = decltype(t);
-            const hipError_t e = launch_chunks<T>(S, A.type, A.batch, shared, space, st);
-            if (e != hipSuccess || !A.time || !shared) return e;
-            const long long n = A.batch * A.time;
-            const long long blocks = std::min<long long>((n * kept * c.d + kThreads - 1) / kThreads, 1 << 16);
-            k_share<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(by_head, static_cast<T*>(y), n, S.heads,
-                                                                           static_cast<int>(kept), static_cast<int>(c.d));
-            return hipGetLastError();
-        });
+        return S;
     };
-    hipError_t e = one(o, v, k, false, true, A.initial_state, nullptr, A.grad_q, A.q_heads);
-    if (e == hipSuccess) e = one(v, o, q, true, true, A.grad_end, nullptr, A.grad_k, A.k_heads);
-    if (e == hipSuccess) e = one(k, q, o, true, false, A.grad_end, A.grad_initial, A.grad_v, A.v_heads);
-    return e;
+    ChunkArgs states{}, grads{};
+    states.nseg = grads.nseg = seg.count;
+    states.seg_steps = grads.seg_steps = seg.steps;
+    states.job[0] = sum(q, k, v, false, kOfValues, ahead, nullptr, A.heads);
+    states.job[1] = sum(k, q, o, true, kOfValues, back, nullptr, A.heads);
+    grads.job[0] = sum(o, v, k, false, kOfKeys, ahead, A.grad_q, A.q_heads);
+    grads.job[1] = sum(v, o, q, true, kOfKeys, back, A.grad_k, A.k_heads);
+    grads.job[2] = sum(k, q, o, true, kOfValues, back, A.grad_v, A.v_heads);
+    grads.job[2].state_out = A.grad_initial;
+
+    return with_type(A.type, [&](auto t) -> hipError_t {
+        using T = decltype(t);
+        hipError_t e = launch_states<T>(states, 2, bh, st);
+        if (e != hipSuccess) return e;
+        if (A.dk == A.dv) {
+            e = launch_chunks<T>(grads, 3, false, bh, st);
+        } else {
+            ChunkArgs last = grads;
+            last.job[0] = grads.job[2];
+            e = launch_chunks<T>(grads, 2, false, bh, st);
+            if (e == hipSuccess) e = launch_chunks<T>(last, 1, false, bh, st);
+        }
+        void* const outs[3] = {A.grad_q, A.grad_k, A.grad_v};
+        const int64_t heads[3] = {A.q_heads, A.k_heads, A.v_heads};
+        for (int i = 0; i < 3 && e == hipSuccess && A.time; ++i) {
+            const ScanArgs& S = grads.job[i];
+            if (!S.y_f32) continue;
+            const long long n = A.batch * A.time;
+            const long long blocks = std::min<long long>((n * heads[i] * S.dc + kThreads - 1) / kThreads, 1 << 16);
+            k_share<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(
+                static_cast<const float*>(S.y), static_cast<T*>(outs[i]), n, S.heads, static_cast<int>(heads[i]), S.dc);
+            e = hipGetLastError();
+        }
+        return e;
+    });
 }
 
 }  // namespace hx
