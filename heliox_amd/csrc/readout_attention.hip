@@ -116,8 +116,9 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-// Operand fragments are taken 16 reduction indices at a time, four consecutive ones a lane
-// (lane: index 4 (lane / 16) .. + 3 of row lane % 16).
+// Reduction indices are taken 32 at a time, eight a lane; which eight is free as long as both
+// operands agree, and is chosen so that every LDS access is whole and without bank conflicts
+// (two reads of 8 bytes where one of 16 does: 2400 of 4500 LDS cycles a chunk were conflicts).
 //
 // bf16 inputs: 32 indices an instruction.  Products of inputs are exact in fp32; P and the
 // state as it enters y are rounded to bf16 once, as y is afterwards.  The state itself stays
@@ -125,20 +126,64 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 struct MathBf16 {
     using Elem = __bf16;
     using Frag = bf16x4;
+    using Pair = bf16x8;
     static constexpr int kC = 64, kPiece = 8, kTerms = 3;
-    static constexpr int kRowPad = 8, kColPad = 16;     // LDS rows: 4 / 8 banks on, read by rows / by columns
-    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Frag a0, Frag a1, Frag b0, Frag b1) {
-        const bf16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-        const bf16x8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+    static constexpr int kPadA = 8, kPadB = 0, kPadC = 16, kPadP = 8;
+    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
     }
     static __device__ __forceinline__ Frag frag(f32x4 x) { return __builtin_convertvector(x, Frag); }
     static __device__ __forceinline__ f32x4 wide(Frag x) { return __builtin_convertvector(x, f32x4); }
-    // Column `lane % 16` of the 16 x 16 block at p, rows 4 (lane / 16) .. + 3: the transposing read
-    // takes four neighbours of row (lane % 16) / 4 from each lane.
-    static __device__ __forceinline__ Frag column(const Elem* p, int stride, int lane) {
-        const Elem* at = p + (4 * (lane / 16) + lane % 16 / 4) * stride + 4 * (lane % 4);
+    static __device__ __forceinline__ Pair pair(Frag a, Frag b) {
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // State row (a's and b's column) that accumulator rows g4 .. + 3 of tile rt hold: tiles 2K and
+    // 2K + 1 take turns of four in 32 columns, so that a lane's eight are neighbours in a.
+    static __device__ __forceinline__ int row(int rt, int g4) { return rt / 2 * 32 + g4 * 2 + rt % 2 * 4; }
+    // a in rows: eight neighbours, against the state; or the eight that lie together in b, against b.
+    static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
+        return *reinterpret_cast<const Pair*>(row + k * 32 + g4 * 2);
+    }
+    static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) {
+        const Elem* at = row + k * 32 + g4 / 4 % 2 * 16 + g4 / 8 * 4;
+        return pair(*reinterpret_cast<const Frag*>(at), *reinterpret_cast<const Frag*>(at + 8));
+    }
+    // b is read by rows and by columns: of each 32 columns first tile 2K's, then tile 2K + 1's, and
+    // the 16-byte slots of a row exchanged by an exclusive or with f(row), which differs for 16 rows
+    // and, without its lowest bit, for eight.
+    template <int kDA>
+    static __device__ __forceinline__ int b_at(int row, int place) {
+        constexpr int kSlots = kDA / 8 < 16 ? kDA / 8 : 16, kPer = 16 / kSlots;
+        const int q = row % 16 / kPer;
+        const int f = (q * 2 & (kSlots - 1)) | q / (kSlots / 2);
+        return row * kDA + ((place / 8 ^ f) * 8) + place % 8;
+    }
+    template <int kDA>
+    static __device__ __forceinline__ Pair b_pair(const Elem* lb, int row, int k, int g4) {
+        return *reinterpret_cast<const Pair*>(lb + b_at<kDA>(row, k * 32 + g4 * 2));
+    }
+    template <int kDA>
+    static __device__ __forceinline__ void b_store(Elem* lb, int row, int col, Pair x) {
+        const int place = col / 32 * 32 + col % 32 / 2;
+        *reinterpret_cast<Frag*>(lb + b_at<kDA>(row, place)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+        *reinterpret_cast<Frag*>(lb + b_at<kDA>(row, place + 16)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+    }
+    // Column `lane % 16` of a 16 x 16 block, rows 4 (lane / 16) .. + 3: the transposing read takes
+    // four neighbours of row (lane % 16) / 4 from each lane.
+    static __device__ __forceinline__ Frag turned(const Elem* at) {
         return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) Frag*)at);
+    }
+    template <int kDA>
+    static __device__ __forceinline__ Frag b_column(const Elem* lb, int sb, int rt, int lane) {
+        return turned(lb + b_at<kDA>(sb * 16 + 4 * (lane / 16) + lane % 16 / 4, rt * 16 + 4 * (lane % 4)));
+    }
+    static __device__ __forceinline__ Frag c_column(const Elem* lc, int stride, int sb, int col, int lane) {
+        return turned(lc + (sb * 16 + 4 * (lane / 16) + lane % 16 / 4) * stride + col + 4 * (lane % 4));
+    }
+    // P's columns in the order that c's column fragments have
+    static __device__ __forceinline__ int p_at(int sb, int g4) { return sb / 2 * 32 + g4 * 2 + sb % 2 * 4; }
+    static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
+        return *reinterpret_cast<const Pair*>(row + p_at(sb, g4));
     }
 };
 
@@ -146,20 +191,46 @@ struct MathBf16 {
 struct MathF32 {
     using Elem = float;
     using Frag = f32x4;
+    struct Pair {
+        f32x4 x[2];
+    };
     static constexpr int kC = 32, kPiece = 4, kTerms = 1;
-    static constexpr int kRowPad = 4, kColPad = 4;
-    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Frag a0, Frag a1, Frag b0, Frag b1) {
+    static constexpr int kPadA = 4, kPadB = 4, kPadC = 4, kPadP = 4;
+    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[i], b0[i], acc, 0, 0, 0);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[i], b1[i], acc, 0, 0, 0);
+            for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[h][i], b.x[h][i], acc, 0, 0, 0);
         return acc;
     }
     static __device__ __forceinline__ Frag frag(f32x4 x) { return x; }
     static __device__ __forceinline__ f32x4 wide(Frag x) { return x; }
-    static __device__ __forceinline__ Frag column(const Elem* p, int stride, int lane) {
-        const Elem* at = p + 4 * (lane / 16) * stride + lane % 16;
+    static __device__ __forceinline__ Pair pair(Frag a, Frag b) { return {a, b}; }
+    static __device__ __forceinline__ int row(int rt, int g4) { return rt * 16 + g4; }
+    static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
+        return {*reinterpret_cast<const Frag*>(row + k * 32 + g4), *reinterpret_cast<const Frag*>(row + k * 32 + 16 + g4)};
+    }
+    static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) { return a_pair(row, k, g4); }
+    template <int kDA>
+    static __device__ __forceinline__ Pair b_pair(const Elem* lb, int row, int k, int g4) {
+        return a_pair(lb + row * (kDA + kPadB), k, g4);
+    }
+    template <int kDA>
+    static __device__ __forceinline__ void b_store(Elem* lb, int row, int col, Frag x) {
+        *reinterpret_cast<Frag*>(lb + row * (kDA + kPadB) + col) = x;
+    }
+    static __device__ __forceinline__ Frag c_column(const Elem* lc, int stride, int sb, int col, int lane) {
+        const Elem* at = lc + (sb * 16 + 4 * (lane / 16)) * stride + col + lane % 16;
         return Frag{at[0], at[stride], at[2 * stride], at[3 * stride]};
+    }
+    template <int kDA>
+    static __device__ __forceinline__ Frag b_column(const Elem* lb, int sb, int rt, int lane) {
+        return c_column(lb, kDA + kPadB, sb, rt * 16, lane);
+    }
+    static __device__ __forceinline__ int p_at(int sb, int g4) { return sb * 16 + g4; }
+    static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
+        return {*reinterpret_cast<const Frag*>(row + sb * 16 + g4),
+                *reinterpret_cast<const Frag*>(row + sb * 16 + 16 + g4)};
     }
 };
 
@@ -218,12 +289,13 @@ struct Tile {
             raw[p] = x;
         }
     }
-    __device__ __forceinline__ void store(typename Math::Elem* lds, int stride) const {
+    // put(row, column, piece) for the pieces of this thread
+    template <class F>
+    __device__ __forceinline__ void store(F put) const {
         typedef typename Math::Elem Out __attribute__((ext_vector_type(kP)));
         const int i = threadIdx.x / kRowPieces, j = threadIdx.x % kRowPieces * kP;
 #pragma unroll
-        for (int p = 0; p < kN; ++p)
-            *reinterpret_cast<Out*>(lds + (i + p * kRows) * stride + j) = __builtin_convertvector(raw[p], Out);
+        for (int p = 0; p < kN; ++p) put(i + p * kRows, j, __builtin_convertvector(raw[p], Out));
     }
 };
 
@@ -242,12 +314,13 @@ __device__ __forceinline__ JobArgs& job_of(const ChunkArgs&) {
 }
 
 // Four neighbours of a row to base[at], of which `columns` are there.
-template <class Out, class Four, bool kWhole>
-__device__ __forceinline__ void put(Out* base, long long at, int columns, f32x4 v) {
+template <class V> using Global = __attribute__((address_space(1))) V;
+template <class Out, class Four, bool kWhole, class At>
+__device__ __forceinline__ void put(Global<Out>* base, At at, int columns, f32x4 v) {
     const Four w = __builtin_convertvector(v, Four);
     if constexpr (kWhole) {
         typedef Four Any __attribute__((aligned(sizeof(Out))));
-        if (columns > 0) *reinterpret_cast<Any*>(base + static_cast<unsigned>(at)) = w;
+        if (columns > 0) *(Global<Any>*)(base + at) = w;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -267,9 +340,15 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     using Elem = typename M::Elem;
     using Frag = typename M::Frag;
     constexpr int kC = M::kC, kB = kC / 16, kT = kW * 64, kDC = kW * kCT * 16, kRT = kDA / 16;
-    constexpr int kSA = kDA + M::kRowPad, kSB = kDA + M::kColPad, kSC = kDC + M::kColPad, kSP = kC + M::kRowPad;
+    using Pair = typename M::Pair;
+    typedef Elem Piece __attribute__((ext_vector_type(M::kPiece)));
+    constexpr int kSA = kDA + M::kPadA, kSB = kDA + M::kPadB, kSC = kDC + M::kPadC, kSP = kC + M::kPadP, kK = kRT / 2;
     __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kC * kSA], lb[kC * kSB], lc[kC * kSC],
         lp[kStates ? 1 : kC * kSP];
+    // the chunk's decays, made once: of P's blocks tb - sb + 1 blocks under the diagonal (the first:
+    // over it, nothing) as a lane holds them; of the entering state; of what enters at a step
+    __shared__ f32x4 lfactor[kStates ? 1 : (kB + 1) * 64], lleft[kC / 4];
+    __shared__ float lsince[kStates ? 1 : kC];
     const JobArgs& S = job_of(A);
     const int lane = threadIdx.x % 64, r = lane % 16, g4 = lane / 16 * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -282,7 +361,7 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     const int col0 = slice * kDC;                          // of the slice
     const int mine = wave * kCT * 16;                      // of the wave, in the slice
     const float lg = S.log_decay[h] * 1.44269504f;
-    float g = lg < -1e4f ? -1e4f : lg;                     // -inf: e^{g 0} stays 1
+    const float g = lg < -1e4f ? -1e4f : lg;               // -inf: e^{g 0} stays 1
     const int off = S.reverse ? 0 : 1;
     const float scale = S.scale_in * S.scale_out;
     const int dc_here = min(S.dc - col0, kDC);
@@ -298,14 +377,19 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
     if constexpr (!kStates) ta.start(a0, S.a_stride[1], S.reverse, S.da);
     tb.start(b0, S.b_stride[1], S.reverse, S.da);
     tc.start(c0, S.c_stride[1], S.reverse, dc_here);
-    auto fetch = [&](int i0) {
+    // in two parts: all at once, the pieces would take registers from the products beside them
+    auto fetch = [&](int i0, int part) {
         const int n = min(kC, len - i0);
         const long long t0 = S.reverse ? len - 1 - i0 : i0;
-        if constexpr (!kStates) ta.load(t0 * S.a_stride[1], n);
-        tb.load(t0 * S.b_stride[1], n);
-        tc.load(t0 * S.c_stride[1], n);
+        if (part == 0) {
+            if constexpr (!kStates) ta.load(t0 * S.a_stride[1], n);
+            tc.load(t0 * S.c_stride[1], n);
+        } else {
+            tb.load(t0 * S.b_stride[1], n);
+        }
     };
-    fetch(begin);
+    fetch(begin, 0);
+    fetch(begin, 1);
 
     // The state that enters: what came before the sequence, and the segments before this one.
     f32x4 X[kRT][kCT];
@@ -322,7 +406,7 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
             for (int ct = 0; ct < kCT; ++ct)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = rt * 16 + g4 + i, col = col0 + mine + ct * 16 + r;
+                    const int row = M::row(rt, g4) + i, col = col0 + mine + ct * 16 + r;
                     if (row < S.da && col < S.dc)
                         X[rt][ct][i] = f(X[rt][ct][i], row * S.row_stride + col * S.col_stride);
                 }
@@ -339,116 +423,131 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
         }
     }
     // scale_in e^{g (n - off - j)}: what is left at the chunk's end of what enters at step j
-    auto left = [&](int n, int sb) {
-        f32x4 w;
+    auto make_left = [&](int n) {
+        if (threadIdx.x < kC / 4) {
+            f32x4 w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int ago = n - off - (sb * 16 + g4 + i);
-            w[i] = ago + off > 0 ? S.scale_in * pow2(g * static_cast<float>(ago)) : 0.f;
+            for (int i = 0; i < 4; ++i) {
+                const int j = threadIdx.x * 4 + i;
+                w[i] = j < n ? S.scale_in * pow2(g * static_cast<float>(n - off - j)) : 0.f;
+            }
+            lleft[threadIdx.x] = w;
         }
-        return w;
     };
+    make_left(kC);
+    if constexpr (!kStates) {
+        for (int e = threadIdx.x; e < (kB + 1) * 64; e += kT) {
+            f32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ago = (e / 64 - 1) * 16 + r - g4 - i;
+                w[i] = e >= 64 && ago >= 0 ? scale * pow2(g * static_cast<float>(ago)) : 0.f;
+            }
+            lfactor[e] = w;
+        }
+        if (threadIdx.x < kC) lsince[threadIdx.x] = S.scale_out * pow2(g * static_cast<float>(threadIdx.x + off));
+    }
+    long long y_step = S.y_stride[1];
+    unsigned long long y_base = reinterpret_cast<unsigned long long>(S.y) +
+                                (batch * S.y_stride[0] + h * S.y_stride[2] + col0 + mine) * (S.y_f32 ? 4 : sizeof(T));
+    asm volatile("" : "+s"(y_base), "+s"(y_step));         // held, not read from the arguments at every store
+    const std::conditional_t<kWhole, unsigned, long long> y_lane = (S.reverse ? 15 - r : r) * y_step + g4;
 
     for (int i0 = begin; i0 < end; i0 += kC) {
         const int n = min(kC, len - i0);
         if (n <= 0) break;
         __syncthreads();                       // the chunk before is done with
-        if constexpr (!kStates) ta.store(la, kSA);
-        tb.store(lb, kSB);
-        tc.store(lc, kSC);
+        if (n < kC) make_left(n);
+        if constexpr (!kStates)
+            ta.store([&](int i, int col, Piece x) { *reinterpret_cast<Piece*>(la + i * kSA + col) = x; });
+        tb.store([&](int i, int col, Piece x) { M::template b_store<kDA>(lb, i, col, x); });
+        tc.store([&](int i, int col, Piece x) { *reinterpret_cast<Piece*>(lc + i * kSC + col) = x; });
         __syncthreads();
-        if (i0 + kC < end) fetch(i0 + kC);
-        asm volatile("" : "+v"(g));             // decays are made anew in every chunk: kept, they take 40 registers
         Frag c[kB][kCT];
         if constexpr (!kStates) {
             // P's blocks, as many for each wave (those over the diagonal come out as zero)
             constexpr int kEach = kB * kB / kW;
-            f32x4 p[kEach];
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) p[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            static_assert(kEach * kW == kB * kB && (kEach % kB == 0 || kB % kEach == 0), "whole rows or parts of one");
             const int block0 = wave * kEach;
-#pragma unroll
-            for (int k = 0; k < kRT; k += 2) {
-                Frag a_0, a_1;
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int sb = (block0 + e) % kB;
-                    if (e % kB == 0) {
-                        const Elem* pa = la + ((block0 + e) / kB * 16 + r) * kSA + k * 16 + g4;
-                        a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
-                    }
-                    const Elem* pb = lb + (sb * 16 + r) * kSB + k * 16 + g4;
-                    p[e] = M::mma(p[e], *reinterpret_cast<const Frag*>(pb), *reinterpret_cast<const Frag*>(pb + 16), a_0,
-                                  a_1);
-                }
-            }
-            // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
+            Pair pa[kK];
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
+                if (e % kB == 0)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ago = (tb_ - sb) * 16 + r - g4 - i;
-                    p[e][i] = ago >= 0 ? p[e][i] * (scale * pow2(g * static_cast<float>(ago))) : 0.f;
-                }
-                *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + sb * 16 + g4) = M::frag(p[e]);
+                    for (int k = 0; k < kK; ++k) pa[k] = M::a_like_b(la + (tb_ * 16 + r) * kSA, k, g4);
+                Pair pb[kK];
+#pragma unroll
+                for (int k = 0; k < kK; ++k) pb[k] = M::template b_pair<kDA>(lb, sb * 16 + r, k, g4);
+                f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kK; ++k) p = M::mma(p, pb[k], pa[k]);
+                // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
+                p *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
+                *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4)) = M::frag(p);
             }
         }
 #pragma unroll
         for (int sb = 0; sb < kB; ++sb)
 #pragma unroll
-            for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::column(lc + sb * 16 * kSC + mine + ct * 16, kSC, lane);
+            for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::c_column(lc, kSC, sb, mine + ct * 16, lane);
         if constexpr (!kStates) {
             __syncthreads();                   // P is whole
             // two blocks of steps at a time: what the entering state adds, then the chunk's own steps
 #pragma unroll
             for (int t0 = 0; t0 < kB; t0 += 2) {
+                Pair pa[2][kK], pp[2][kB / 2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int k = 0; k < kK; ++k) pa[t][k] = M::a_pair(la + ((t0 + t) * 16 + r) * kSA, k, g4);
+#pragma unroll
+                    for (int sb = 0; sb <= t0 + t; sb += 2)
+                        pp[t][sb / 2] = M::p_pair(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
+                }
                 f32x4 y[2][kCT];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < kRT; k += 2) {
-                    Frag x0[kCT], x1[kCT];
+                for (int k = 0; k < kK; ++k)
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) x0[ct] = M::frag(X[k][ct]), x1[ct] = M::frag(X[k + 1][ct]);
+                    for (int ct = 0; ct < kCT; ++ct) {
+                        const Pair x = M::pair(M::frag(X[2 * k][ct]), M::frag(X[2 * k + 1][ct]));
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const Elem* pa = la + ((t0 + t) * 16 + r) * kSA + k * 16 + g4;
-                        const Frag a_0 = *reinterpret_cast<const Frag*>(pa), a_1 = *reinterpret_cast<const Frag*>(pa + 16);
-#pragma unroll
-                        for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], x0[ct], x1[ct], a_0, a_1);
+                        for (int t = 0; t < 2; ++t) y[t][ct] = M::mma(y[t][ct], x, pa[t][k]);
                     }
-                }
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const float since = S.scale_out * pow2(g * static_cast<float>((t0 + t) * 16 + r + off));
+                    const float since = lsince[(t0 + t) * 16 + r];
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
+                    for (int ct = 0; ct < kCT; ++ct) {
+                        y[t][ct] *= since;
 #pragma unroll
-                    for (int sb = 0; sb <= t0 + t; sb += 2) {
-                        const Elem* pp = lp + ((t0 + t) * 16 + r) * kSP + sb * 16 + g4;
-                        const Frag p0 = *reinterpret_cast<const Frag*>(pp), p1 = *reinterpret_cast<const Frag*>(pp + 16);
-#pragma unroll
-                        for (int ct = 0; ct < kCT; ++ct) y[t][ct] = M::mma(y[t][ct], c[sb][ct], c[sb + 1][ct], p0, p1);
+                        for (int sb = 0; sb <= t0 + t; sb += 2)
+                            y[t][ct] = M::mma(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp[t][sb / 2]);
                     }
                     // lane: step (t0 + t)*16 + r, columns g4 .. + 3 of each tile
                     const int i1 = i0 + (t0 + t) * 16;
-                    const long long step = S.reverse ? len - 1 - i1 - 15 : i1;         // least of the 16
-                    const long long at = batch * S.y_stride[0] + step * S.y_stride[1] + h * S.y_stride[2] + col0 + mine;
-                    const long long lane_at = (S.reverse ? 15 - r : r) * S.y_stride[1] + g4;
+                    const long long at = (S.reverse ? len - 1 - i1 - 15 : i1) * y_step;     // of the least step
                     if (i1 + r < len) {
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct) {
                             const int columns = S.dc - (col0 + mine + ct * 16 + g4);
-                            if (S.y_f32) put<float, f32x4, kWhole>(static_cast<float*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
-                            else put<typename In::Elem, typename In::Four, kWhole>(static_cast<typename In::Elem*>(S.y) + at + ct * 16, lane_at, columns, y[t][ct]);
+                            if (S.y_f32)
+                                put<float, f32x4, kWhole>((Global<float>*)y_base + at + ct * 16, y_lane,
+                                                          columns, y[t][ct]);
+                            else
+                                put<typename In::Elem, typename In::Four, kWhole>(
+                                    (Global<typename In::Elem>*)y_base + at + ct * 16, y_lane, columns,
+                                    y[t][ct]);
                         }
                     }
                 }
             }
         }
+        if (i0 + kC < end) fetch(i0 + kC, 0);
         // the state that leaves
         const float keep = pow2(g * static_cast<float>(n));
 #pragma unroll
@@ -457,28 +556,39 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
             for (int ct = 0; ct < kCT; ++ct) X[rt][ct] *= keep;
 #pragma unroll
         for (int sb = 0; sb < kB; sb += 2) {
+            if (sb == kB - 2 && i0 + kC < end) fetch(i0 + kC, 1);
+            constexpr int kAhead = kRT < 4 ? kRT : 4;
             Frag wc[M::kTerms][2][kCT];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const f32x4 w0 = left(n, sb + e);
+            for (int rt0 = 0; rt0 < kRT; rt0 += kAhead) {
+                Frag b[kAhead][2];
 #pragma unroll
-                for (int ct = 0; ct < kCT; ++ct) {
-                    f32x4 w = M::wide(c[sb + e][ct]) * w0;
+                for (int rt = 0; rt < kAhead; ++rt)
 #pragma unroll
-                    for (int k = 0; k < M::kTerms; ++k) {
-                        wc[k][e][ct] = M::frag(w);
-                        w -= M::wide(wc[k][e][ct]);
+                    for (int e = 0; e < 2; ++e) b[rt][e] = M::template b_column<kDA>(lb, sb + e, rt0 + rt, lane);
+                if (rt0 == 0) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const f32x4 w0 = lleft[(sb + e) * 4 + g4 / 4];
+#pragma unroll
+                        for (int ct = 0; ct < kCT; ++ct) {
+                            f32x4 w = M::wide(c[sb + e][ct]) * w0;
+#pragma unroll
+                            for (int k = 0; k < M::kTerms; ++k) {
+                                wc[k][e][ct] = M::frag(w);
+                                w -= M::wide(wc[k][e][ct]);
+                            }
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int rt = 0; rt < kRT; ++rt) {
-                const Frag b_0 = M::column(lb + sb * 16 * kSB + rt * 16, kSB, lane);
-                const Frag b_1 = M::column(lb + (sb + 1) * 16 * kSB + rt * 16, kSB, lane);
+                for (int rt = 0; rt < kAhead; ++rt)
 #pragma unroll
-                for (int ct = 0; ct < kCT; ++ct)
+                    for (int ct = 0; ct < kCT; ++ct)
 #pragma unroll
-                    for (int k = 0; k < M::kTerms; ++k) X[rt][ct] = M::mma(X[rt][ct], b_0, b_1, wc[k][0][ct], wc[k][1][ct]);
+                        for (int k = 0; k < M::kTerms; ++k)
+                            X[rt0 + rt][ct] = M::mma(X[rt0 + rt][ct], M::pair(b[rt][0], b[rt][1]),
+                                                     M::pair(wc[k][0][ct], wc[k][1][ct]));
             }
         }
     }
