@@ -6,7 +6,7 @@
 // (w (P - p_r / q_r)); the few entries are written over afterwards.
 #include "readout.h"
 
-#include <algorithm>
+#include <type_traits>
 
 namespace hx {
 namespace {
@@ -110,15 +110,29 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
         }
     };
     const unsigned char* bits = reinterpret_cast<const unsigned char*>(member);
-    for (int p = threadIdx.x; p < pieces; p += kThreads) {
-        const Vec raw = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p) * kP);
+    // f(piece, its logits) for the row's whole pieces, several loads at a time (one alone leaves a
+    // CU with 32 KB on their way, less than it takes to keep the memory busy)
+    auto each_piece = [&](auto f) {
+        constexpr int kAhead = 4;
+        for (int p0 = threadIdx.x; p0 < pieces; p0 += kAhead * kThreads) {
+            Vec raw[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (p0 + k * kThreads < pieces)
+                    raw[k] = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p0 + k * kThreads) * kP);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (p0 + k * kThreads < pieces) f(p0 + k * kThreads, raw[k]);
+        }
+    };
+    each_piece([&](int p, Vec raw) {
         float v[kP];
 #pragma unroll
         for (int i = 0; i < kP; ++i) v[i] = static_cast<float>(raw[i]);
         unsigned in = 0;
         if constexpr (kRest) in = kP == 8 ? bits[p] : bits[p / 2] >> (p % 2 * 4) & 15;
         take(v, kP, in);
-    }
+    });
     if (pieces * kP + static_cast<int>(threadIdx.x) < vocab) {       // fewer than a piece are left
         const int j = pieces * kP + threadIdx.x;
         float v[kP] = {to_f32(x[j])};
@@ -172,12 +186,11 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
     const float w = some > 0.f ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
     const float factor = w * outside / z;
     auto slope = [&](float v) { return some > 0.f ? factor * pow2((v - m) * cold) : 0.f; };
-    for (int p = threadIdx.x; p < pieces; p += kThreads) {
-        Vec raw = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p) * kP);
+    each_piece([&](int p, Vec raw) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) raw[i] = static_cast<decltype(raw[0] + raw[0])>(slope(static_cast<float>(raw[i])));
         *reinterpret_cast<Vec*>(g + static_cast<long long>(p) * kP) = raw;
-    }
+    });
     if (pieces * kP + static_cast<int>(threadIdx.x) < vocab) {
         const int j = pieces * kP + threadIdx.x;
         g[j] = from_f32<T>(slope(to_f32(x[j])));
@@ -214,9 +227,17 @@ hipError_t launch(const hx_distill_args& A) {
 
 template <class T, class U, class I>
 hipError_t pick(const hx_distill_args& A) {
-    const bool wide = A.vocab > 4096;
-    if (A.teacher_lse) return wide ? launch<T, U, I, 1024, true>(A) : launch<T, U, I, 256, true>(A);
-    return wide ? launch<T, U, I, 1024, false>(A) : launch<T, U, I, 256, false>(A);
+    // Threads a row.  A CU holds 2048: rows of a last, thin round run alone, so 512 threads
+    // where that fits all rows into one round and 1024 does not (517 rows of 50021: 42 us with
+    // 1024, 37 with 512); small rows take no more than they have pieces for.
+    const bool small = A.vocab <= 4096, half = A.rows > 512 && A.rows <= 1024;
+    auto go = [&](auto rest) {
+        constexpr bool kRest = decltype(rest)::value;
+        return small  ? launch<T, U, I, 256, kRest>(A)
+               : half ? launch<T, U, I, 512, kRest>(A)
+                      : launch<T, U, I, 1024, kRest>(A);
+    };
+    return A.teacher_lse ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace

@@ -1,11 +1,13 @@
 // The drawing of an answer from logits, one workgroup per row.
 //
 // Masses are whole numbers, so their sums are the same in any order, and integer atomics may
-// make them.  What top_k and top_p leave is "every place over a key, and the first of those at
-// it by index"; the key is found from histograms: one over places in 2048 equal parts of the
-// range that has any mass, then over the keys of the one part where the sum passes the bound.
-// Where top_k leaves at most as many places as the workgroup has threads, those go into LDS and
-// are sorted there instead.  The row itself is read again from the cache in each pass.
+// make them.  What top_k and top_p leave is "every place over a key, and those at it up to an
+// index".  A histogram over 2048 equal parts of the range that has any mass says in which part
+// the cut lies; the places of that part (and, for top_k, of all above) go into LDS where they
+// fit, are sorted there and say the rest.  Where they do not fit (ties without end), histograms
+// over the part's keys go on until one key is left.  The row itself is read again from the cache
+// in each pass: two to four of them as a rule, of which those that make masses of all places
+// (about 25 instructions each) take the time.
 #include "readout.h"
 
 namespace hx {
@@ -37,7 +39,7 @@ __device__ __forceinline__ float value_of(unsigned key) {
 struct Shared {
     u64 bins[kBins];
     u64 part[kWaves];
-    u64 pick[2];
+    u64 pick[3];
     unsigned count;
 };
 
@@ -68,7 +70,7 @@ __device__ __forceinline__ u64 wave_before(u64 x) {       // sum over the lanes 
 }
 
 // Sum of x over the threads before this one; total gets the whole sum.
-__device__ u64 block_before(u64 x, Shared& sh, u64& total) {
+__device__ __forceinline__ u64 block_before(u64 x, Shared& sh, u64& total) {
     const u64 before = wave_before(x);
     __syncthreads();
     if (threadIdx.x % 64 == 63) sh.part[threadIdx.x / 64] = before + x;
@@ -116,69 +118,73 @@ struct Row {
     __device__ __forceinline__ u64 mass(float v) const { return static_cast<u64>(weight(v) * kMass); }
 };
 
-// Of sh.bins from the last to the first, the one where the running sum (from `before`) passes;
-// before gets the sum up to it, and the whole sum is returned where none passes (bin -1).
+struct Cut {
+    int bin;            // -1: the bound is not reached
+    u64 before, at;     // the sums over what comes before it, and of it
+};
+
+// Of sh.bins from the last to the first, the one where the running sum (from `before`) passes.
+// The bins are zero afterwards.
 template <class P>
-__device__ int find_bin(Shared& sh, P passes, u64& before) {
+__device__ __forceinline__ Cut find_bin(Shared& sh, P passes, u64 before) {
     __syncthreads();
     constexpr int kEach = kBins / kThreads;
     const int top = kBins - 1 - threadIdx.x * kEach;
     u64 mine = 0, total;
     for (int i = 0; i < kEach; ++i) mine += sh.bins[top - i];
     u64 sum = before + block_before(mine, sh, total);
-    if (threadIdx.x == 0) {
-        sh.pick[0] = ~0ull;
-        sh.pick[1] = before + total;
-    }
+    if (threadIdx.x == 0) sh.pick[0] = ~0ull;
     __syncthreads();
     if (!passes(sum) && passes(sum + mine))
         for (int i = 0; i < kEach; ++i) {
             if (passes(sum + sh.bins[top - i])) {
                 sh.pick[0] = top - i;
                 sh.pick[1] = sum;
+                sh.pick[2] = sh.bins[top - i];
                 break;
             }
             sum += sh.bins[top - i];
         }
     __syncthreads();
-    const int bin = static_cast<int>(static_cast<long long>(sh.pick[0]));
-    before = sh.pick[1];
-    __syncthreads();
+    const Cut c{static_cast<int>(static_cast<long long>(sh.pick[0])), sh.pick[1], sh.pick[2]};
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
     __syncthreads();
-    return bin;
+    return c;
 }
 
-// The key at which a running sum over the places in descending order passes a bound: value(v)
-// is what a place counts (0: nothing), passes(sum) whether a sum reaches the bound.  before gets
-// the sum over larger keys.  Returns 0 where all places with a mass do not reach the bound.
-// sh.bins are zero before and after.
-template <class T, class V, class P>
-__device__ unsigned select(const Row<T>& R, Shared& sh, V value, P passes, u64& before) {
-    // equal parts of the depth; monotonous, as each rounding is
-    auto part = [&](float v) {
-        const float d = -R.depth(v) * (kBins / kDepth);
-        return d < kBins ? kBins - 1 - static_cast<int>(d) : -1;
-    };
-    R.each([&](int, const float* v, int n) {
+// Which of the equal parts of the range with any mass a logit lies in, the largest in the last;
+// -1: beyond.  Monotonous, as each of its roundings is.
+template <class T>
+__device__ __forceinline__ int part_of(const Row<T>& R, float v) {
+    const float d = -R.depth(v) * (kBins / kDepth);
+    return d < kBins ? kBins - 1 - static_cast<int>(d) : -1;
+}
+
+// Adds value(index, logit) to the bin of each place's part.
+template <class T, class V>
+__device__ __forceinline__ void add_parts(const Row<T>& R, Shared& sh, V value) {
+    R.each([&](int j0, const float* v, int n) {
 #pragma unroll
         for (int i = 0; i < Row<T>::kP; ++i) {
-            const int b = i < n ? part(v[i]) : -1;
+            const int b = i < n ? part_of(R, v[i]) : -1;
             if (b >= 0) {
-                const u64 w = value(v[i]);
+                const u64 w = value(j0 + i, v[i]);
                 if (w) atomicAdd(&sh.bins[b], w);
             }
         }
     });
-    before = 0;
-    const int bin = find_bin(sh, passes, before);
-    if (bin < 0) return 0;
-    // the part's keys: least and largest, then 2048 parts of what lies between, until one key is left
+}
+
+// From the part where a running sum passes to the key where it does: by histograms over what
+// lies between the part's least and largest key, until one key is left.  c is the part's cut
+// and becomes the key's.
+template <class T, class V, class P>
+__device__ __forceinline__ unsigned refine(const Row<T>& R, Shared& sh, V value, P passes, Cut& c) {
     unsigned lo = ~0u, hi = 0;
-    R.each([&](int, const float* v, int n) {
+    R.each([&](int j0, const float* v, int n) {
 #pragma unroll
         for (int i = 0; i < Row<T>::kP; ++i)
-            if (i < n && part(v[i]) == bin && value(v[i])) {
+            if (i < n && part_of(R, v[i]) == c.bin && value(j0 + i, v[i])) {
                 const unsigned k = key_of(v[i]);
                 lo = min(lo, k);
                 hi = max(hi, k);
@@ -189,27 +195,25 @@ __device__ unsigned select(const Row<T>& R, Shared& sh, V value, P passes, u64& 
     while (lo < hi) {
         int shift = 0;
         while ((hi - lo) >> shift >= kBins) ++shift;
-        __syncthreads();
-        R.each([&](int, const float* v, int n) {
+        R.each([&](int j0, const float* v, int n) {
 #pragma unroll
-            for (int i = 0; i < Row<T>::kP; ++i)
-                if (i < n) {
-                    const unsigned k = key_of(v[i]);
-                    if (k >= lo && k <= hi) {
-                        const u64 w = value(v[i]);
-                        if (w) atomicAdd(&sh.bins[(k - lo) >> shift], w);
-                    }
+            for (int i = 0; i < Row<T>::kP; ++i) {
+                const unsigned k = key_of(v[i]);
+                if (i < n && k >= lo && k <= hi) {
+                    const u64 w = value(j0 + i, v[i]);
+                    if (w) atomicAdd(&sh.bins[(k - lo) >> shift], w);
                 }
+            }
         });
-        const int b = find_bin(sh, passes, before);
-        lo += static_cast<unsigned>(b) << shift;
+        c = find_bin(sh, passes, c.before);
+        lo += static_cast<unsigned>(c.bin) << shift;
         hi = min(hi, lo + ((1u << shift) - 1));
     }
     return lo;
 }
 
 // Ascending sort of kThreads keys, one a thread, in LDS.
-__device__ u64 block_sort(u64 key, u64* at) {
+__device__ __forceinline__ u64 block_sort(u64 key, u64* at) {
     for (int size = 2; size <= kThreads; size <<= 1)
         for (int gap = size / 2; gap > 0; gap >>= 1) {
             u64 other;
@@ -227,8 +231,38 @@ __device__ u64 block_sort(u64 key, u64* at) {
     return key;
 }
 
+constexpr u64 kNone = ~0ull;
+__device__ __forceinline__ u64 by_rank(float v, int j) { return static_cast<u64>(~key_of(v)) << 32 | static_cast<unsigned>(j); }
+__device__ __forceinline__ float ranked_value(u64 e) { return value_of(~static_cast<unsigned>(e >> 32)); }
+
+// The places for which take(index, logit) holds, sorted by rank, one a thread (kNone: no more);
+// false, and nothing usable, where they are more than the threads.  Uses sh.bins.
+template <class T, class F>
+__device__ __forceinline__ bool gather(const Row<T>& R, Shared& sh, F take, u64& mine) {
+    u64* const list = sh.bins;
+    static_assert(kBins >= 2 * kThreads, "the list and the sort's own space");
+    R.each([&](int j0, const float* v, int n) {
+#pragma unroll
+        for (int i = 0; i < Row<T>::kP; ++i)
+            if (i < n && take(j0 + i, v[i])) {
+                const unsigned at = atomicAdd(&sh.count, 1u);
+                if (at < kThreads) list[at] = by_rank(v[i], j0 + i);
+            }
+    });
+    __syncthreads();
+    const unsigned count = sh.count;
+    mine = threadIdx.x < min(count, static_cast<unsigned>(kThreads)) ? list[threadIdx.x] : kNone;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    if (count <= kThreads) mine = block_sort(mine, list + kThreads);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) list[i] = 0;
+    __syncthreads();
+    return count <= kThreads;
+}
+
 // How many places at a key stay: those with less than the bound before them, of at most n.
-__device__ u64 count_under(double bound, u64 before, u64 mass, u64 n) {
+__device__ __forceinline__ u64 count_under(double bound, u64 before, u64 mass, u64 n) {
     u64 lo = 1, hi = n > 1 ? n : 1;
     while (lo < hi) {
         const u64 mid = (lo + hi + 1) / 2;
@@ -238,16 +272,61 @@ __device__ u64 count_under(double bound, u64 before, u64 mass, u64 n) {
     return lo;
 }
 
-__device__ __forceinline__ u64 aim_of(float u, u64 total) {
-    const double share = fmin(fmax(static_cast<double>(u), 0.0), 1.0);
-    const u64 aim = static_cast<u64>(floor(share * static_cast<double>(total)));
-    return aim < total ? aim : total - 1;
+// The place where the running sum of value(index, logit), in index order, passes an aim: each
+// wave's turns are summed, then the turn where it passes is looked at by itself.  aim_of(whole
+// sum) is the aim; found(index, logit, whole sum) is called by the one thread that holds the place.
+template <class T, class V, class A, class F>
+__device__ __forceinline__ void at_running_sum(const Row<T>& R, Shared& sh, u64* segments, V value, A aim_of, F found) {
+    constexpr int kP = Row<T>::kP;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    int turn = 0;
+    R.each([&](int j0, const float* v, int n) {
+        u64 m = 0;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) m += i < n ? value(j0 + i, v[i]) : 0;
+        for (int s = 32; s > 0; s >>= 1) m += __shfl_xor(m, s);
+        if (lane == 0) segments[turn * kWaves + wave] = m;
+        ++turn;
+    });
+    __syncthreads();
+    const int nseg = turn * kWaves, per = (nseg + kThreads - 1) / kThreads;
+    const int s0 = min(static_cast<int>(threadIdx.x) * per, nseg), s1 = min(s0 + per, nseg);
+    u64 mine = 0, total;
+    for (int s = s0; s < s1; ++s) mine += segments[s];
+    u64 before = block_before(mine, sh, total);
+    const u64 aim = aim_of(total);
+    if (mine && before <= aim && aim < before + mine) {
+        int s = s0;
+        while (before + segments[s] <= aim) before += segments[s++];
+        sh.pick[0] = s;
+        sh.pick[1] = before;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        const int seg = static_cast<int>(sh.pick[0]);
+        const int j0 = ((seg / kWaves) * kThreads + seg % kWaves * 64 + lane) * kP;
+        u64 m[kP], sum = 0;
+        float v[kP];
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+            v[i] = j0 + i < R.n ? to_f32(R.x[j0 + i]) : -INFINITY;
+            m[i] = j0 + i < R.n ? value(j0 + i, v[i]) : 0;
+            sum += m[i];
+        }
+        before = sh.pick[1] + wave_before(sum);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+            if (m[i] && before <= aim && aim < before + m[i]) found(j0 + i, v[i], total);
+            before += m[i];
+        }
+    }
+    __syncthreads();
 }
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
     __shared__ Shared sh;
-    extern __shared__ u64 segments[];          // mass of each wave's turn in each()
+    extern __shared__ u64 segments[];          // sums of each wave's turns in each()
     using R_ = Row<T>;
     constexpr int kP = R_::kP;
     const long long row = blockIdx.x;
@@ -255,12 +334,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
     R.x = static_cast<const T*>(A.logits) + row * A.logits_stride;
     R.n = static_cast<int>(A.vocab);
     const float temp = A.temperature ? A.temperature[row] : static_cast<float>(A.temperature_value);
-    long long top_k = A.top_k ? A.top_k[row] : A.top_k_value;
+    const long long top_k = A.top_k ? A.top_k[row] : A.top_k_value;
     const float top_p = A.top_p ? A.top_p[row] : static_cast<float>(A.top_p_value);
     const float min_p = fminf(A.min_p ? A.min_p[row] : static_cast<float>(A.min_p_value), 1.f);
     const bool greedy = !(temp > 0.f);
-    if (greedy) top_k = 1;
-    if (top_k >= R.n) top_k = 0;
     R.cold = greedy ? 1.f : 1.f / temp;
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
     if (threadIdx.x == 0) sh.count = 0;
@@ -282,165 +359,110 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
         }
         return;
     }
-
-    // Places stay whose key is over `least`, and the first `ties` by index of the `at` at it.
-    unsigned least = 0;
-    u64 ties = R.n, at = R.n;
-    if (top_k > 0) {
-        u64 before;
-        least = select(R, sh, [](float v) { return u64(v == v); },
-                       [&](u64 n) { return n >= static_cast<u64>(top_k); }, before);
-        if (least) ties = top_k - before;
-        // (where fewer than top_k places have a mass, all that have one stay)
-    }
-    if (top_k > 0 && top_k <= kThreads) {
-        // those places into LDS, in whatever order
-        u64* const list = sh.bins;
-        static_assert(kBins >= 2 * kThreads, "the list and the sort's own space");
-        R.each([&](int j0, const float* v, int n) {
+    if (greedy) {
+        int first = R.n;
+        R.each([&](int j0, const float* v, int) {
 #pragma unroll
             for (int i = 0; i < kP; ++i)
-                if (i < n && R.mass(v[i])) {
-                    const unsigned k = key_of(v[i]);
-                    if (k > least) list[atomicAdd(&sh.count, 1u)] = static_cast<u64>(~k) << 32 | (j0 + i);
-                }
+                if (v[i] == R.most) first = min(first, j0 + i);
         });
-        __syncthreads();
-        const unsigned first = sh.count;
-        // the first `ties` by index of those at the key: by their rank among the row's
-        u64 seen = 0;
-        if (least)
-            R.each([&](int j0, const float* v, int n) {
-                unsigned mine = 0;
-#pragma unroll
-                for (int i = 0; i < kP; ++i) mine += i < n && v[i] == v[i] && key_of(v[i]) == least;
-                if (seen >= ties) return;      // the same for all threads
-                u64 turn;
-                u64 rank = seen + block_before(mine, sh, turn);
-                seen += turn;
-#pragma unroll
-                for (int i = 0; i < kP; ++i)
-                    if (i < n && v[i] == v[i] && key_of(v[i]) == least) {
-                        if (rank < ties) list[first + rank] = static_cast<u64>(~least) << 32 | (j0 + i);
-                        ++rank;
-                    }
-            });
-        __syncthreads();
-        const unsigned count = first + static_cast<unsigned>(least ? ties : 0);
-        u64 key = threadIdx.x < count ? list[threadIdx.x] : ~0ull;
-        __syncthreads();
-        key = block_sort(key, list + kThreads);
-        // in rank order now
-        const bool there = threadIdx.x < count;
-        const float v = there ? value_of(~static_cast<unsigned>(key >> 32)) : -INFINITY;
-        u64 m = there ? R.mass(v) : 0, total;
-        u64 before = block_before(m, sh, total);
-        if (!(top_p >= 1.f)) {
-            const double bound = fmax(static_cast<double>(top_p) * static_cast<double>(total), 0.5);
-            if (!(static_cast<double>(before) < bound)) m = 0;
-        }
-        if (there && !(R.weight(v) >= min_p)) m = 0;
-        // and in index order
-        key = block_sort(m ? key << 32 | key >> 32 : ~0ull, list + kThreads);
-        const bool stays = key != ~0ull;
-        const float w = stays ? value_of(~static_cast<unsigned>(key)) : -INFINITY;
-        m = stays ? R.mass(w) : 0;
-        before = block_before(m, sh, total);
-        const u64 aim = aim_of(A.u[row], total);
-        if (m && before <= aim && aim < before + m) answer(static_cast<int>(key >> 32), w, total);
+        first = block_reduce(first, sh, [](int a, int b) { return min(a, b); });
+        if (threadIdx.x == 0) answer(first, R.most, static_cast<u64>(kMass));
         return;
     }
-
-    if (!(top_p >= 1.f)) {
-        auto counted = [&](float v) { return key_of(v) >= least ? R.mass(v) : 0; };
-        u64 over = 0, same = 0;
-        R.each([&](int, const float* v, int n) {
-#pragma unroll
-            for (int i = 0; i < kP; ++i)
-                if (i < n) {
-                    const unsigned k = key_of(v[i]);
-                    if (k > least) over += R.mass(v[i]);
-                    same += k == least;
-                }
-        });
-        over = block_sum(over, sh);
-        at = block_sum(same, sh);
-        const u64 stay = min(at, ties);
-        const u64 m_least = least ? R.mass(value_of(least)) : 0;
-        // the largest stays whatever the bound is
-        const double bound = fmax(static_cast<double>(top_p) * static_cast<double>(over + stay * m_least), 0.5);
-        u64 before;
-        const unsigned cut = select(R, sh, counted, [&](u64 s) { return static_cast<double>(s) >= bound; }, before);
-        ties = count_under(bound, before, R.mass(value_of(cut)), cut > least ? R.n : stay);
-        least = cut;
-    }
-    // Only some of the places at the key stay: up to which index?
-    int last = R.n;
-    if (least) {
-        u64 seen = 0;
-        int found = R.n;
-        R.each([&](int j0, const float* v, int n) {
-            if (seen >= ties) return;          // the same for all threads
-            unsigned mine = 0;
-#pragma unroll
-            for (int i = 0; i < kP; ++i) mine += i < n && key_of(v[i]) == least;
-            u64 turn;
-            u64 rank = seen + block_before(mine, sh, turn);
-            seen += turn;
-#pragma unroll
-            for (int i = 0; i < kP; ++i)
-                if (i < n && key_of(v[i]) == least && ++rank == ties) found = j0 + i;
-        });
-        last = block_reduce(found, sh, [](int a, int b) { return min(a, b); });
-    }
-    auto kept = [&](int j, float v) -> u64 {
-        const unsigned k = key_of(v);
-        const float w = R.weight(v);
-        return (k > least || (k == least && j <= last)) && w >= min_p ? static_cast<u64>(w * kMass) : 0;
+    auto aim = [&](u64 total) {
+        const double u = fmin(fmax(static_cast<double>(A.u[row]), 0.0), 1.0);
+        const u64 a = static_cast<u64>(floor(u * static_cast<double>(total)));
+        return a < total ? a : total - 1;
     };
-    // What stays of each wave's turns, their running sum, and in the turn where it passes u of
-    // the whole the place itself.
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    int turn = 0;
-    R.each([&](int j0, const float* v, int n) {
-        u64 m = 0;
-#pragma unroll
-        for (int i = 0; i < kP; ++i) m += i < n ? kept(j0 + i, v[i]) : 0;
-        for (int s = 32; s > 0; s >>= 1) m += __shfl_xor(m, s);
-        if (lane == 0) segments[turn * kWaves + wave] = m;
-        ++turn;
-    });
-    __syncthreads();
-    const int nseg = turn * kWaves, per = (nseg + kThreads - 1) / kThreads;
-    const int s0 = min(static_cast<int>(threadIdx.x) * per, nseg), s1 = min(s0 + per, nseg);
-    u64 mine = 0, total;
-    for (int s = s0; s < s1; ++s) mine += segments[s];
-    u64 before = block_before(mine, sh, total);
-    const u64 aim = aim_of(A.u[row], total);
-    if (mine && before <= aim && aim < before + mine) {
-        int s = s0;
-        while (before + segments[s] <= aim) before += segments[s++];
-        sh.pick[0] = s;
-        sh.pick[1] = before;
+    // The largest place stays whatever top_p is.
+    auto bound_of = [&](u64 total) { return fmax(static_cast<double>(top_p) * static_cast<double>(total), 0.5); };
+
+    // Places stay whose key is over `least`, and those at it up to index `last`.
+    unsigned least = 0;
+    int last = R.n;
+    auto stays = [&](int j, float v) {
+        const unsigned k = key_of(v);
+        return k > least || (k == least && j <= last);
+    };
+    auto last_of = [&](u64 ties) {             // the index of so many places at the key
+        at_running_sum(R, sh, segments, [&](int, float v) { return u64(v == v && key_of(v) == least); },
+                       [&](u64) { return ties - 1; }, [&](int j, float, u64) { sh.pick[2] = j; });
+        last = static_cast<int>(sh.pick[2]);
+        __syncthreads();
+    };
+    if (top_k > 0 && top_k < R.n) {
+        auto passes = [&](u64 n) { return n >= static_cast<u64>(top_k); };
+        auto one = [](int, float v) { return u64(v == v); };
+        add_parts(R, sh, one);
+        Cut c = find_bin(sh, passes, 0);
+        // (where fewer than top_k places have a mass, all that have one stay)
+        u64 mine = kNone;
+        bool listed = false;
+        if (c.bin >= 0 && c.before + c.at <= kThreads) {
+            listed = gather(R, sh, [&](int, float v) { return part_of(R, v) >= c.bin; }, mine);
+            if (threadIdx.x >= top_k) mine = kNone;
+        } else if (c.bin >= 0) {
+            least = refine(R, sh, one, passes, c);
+            if (top_k - c.before < c.at) last_of(top_k - c.before);
+            if (top_k <= kThreads) listed = gather(R, sh, stays, mine);
+        }
+        if (listed) {
+            // in rank order
+            const float v = mine != kNone ? ranked_value(mine) : -INFINITY;
+            u64 m = mine != kNone ? R.mass(v) : 0, total;
+            u64 before = block_before(m, sh, total);
+            if (!(top_p >= 1.f) && !(static_cast<double>(before) < bound_of(total))) m = 0;
+            if (!(R.weight(v) >= min_p)) m = 0;
+            // and in index order
+            mine = block_sort(m ? mine << 32 | mine >> 32 : kNone, sh.bins + kThreads);
+            const float w = mine != kNone ? value_of(~static_cast<unsigned>(mine)) : -INFINITY;
+            m = mine != kNone ? R.mass(w) : 0;
+            before = block_before(m, sh, total);
+            const u64 to = aim(total);
+            if (m && before <= to && to < before + m) answer(static_cast<int>(mine >> 32), w, total);
+            return;
+        }
     }
-    __syncthreads();
-    if (wave != 0) return;
-    const int seg = static_cast<int>(sh.pick[0]);
-    const int j0 = ((seg / kWaves) * kThreads + seg % kWaves * 64 + lane) * kP;
-    u64 m[kP], sum = 0;
-    float v[kP];
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-        v[i] = j0 + i < R.n ? to_f32(R.x[j0 + i]) : -INFINITY;
-        m[i] = j0 + i < R.n ? kept(j0 + i, v[i]) : 0;
-        sum += m[i];
+    if (!(top_p >= 1.f)) {
+        auto counted = [&](int j, float v) { return stays(j, v) ? R.mass(v) : 0; };
+        add_parts(R, sh, counted);
+        __syncthreads();
+        u64 total = 0;
+        for (int i = threadIdx.x; i < kBins; i += kThreads) total += sh.bins[i];
+        const double bound = bound_of(block_sum(total, sh));
+        auto passes = [&](u64 s) { return static_cast<double>(s) >= bound; };
+        Cut c = find_bin(sh, passes, 0);
+        u64 mine;
+        if (gather(R, sh, [&](int j, float v) { return part_of(R, v) == c.bin && stays(j, v); }, mine)) {
+            const u64 m = mine != kNone ? R.mass(ranked_value(mine)) : 0;
+            u64 all;
+            const u64 before = c.before + block_before(m, sh, all);
+            // the last place that stays: less than the bound before it, not after it
+            if (m && !passes(before) && passes(before + m)) {
+                sh.pick[0] = ~static_cast<unsigned>(mine >> 32);
+                sh.pick[1] = static_cast<unsigned>(mine);
+            }
+            __syncthreads();
+            least = static_cast<unsigned>(sh.pick[0]);
+            last = static_cast<int>(sh.pick[1]);
+            __syncthreads();
+        } else {
+            const unsigned cut = refine(R, sh, counted, passes, c);
+            const u64 m = R.mass(value_of(cut)), at = c.at / m;
+            const u64 ties = count_under(bound, c.before, m, at);
+            if (cut != least) last = R.n;
+            least = cut;
+            if (ties < at) last_of(ties);
+        }
     }
-    before = sh.pick[1] + wave_before(sum);
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-        if (m[i] && before <= aim && aim < before + m[i]) answer(j0 + i, v[i], total);
-        before += m[i];
-    }
+    at_running_sum(
+        R, sh, segments,
+        [&](int j, float v) {
+            const float w = R.weight(v);
+            return stays(j, v) && w >= min_p ? static_cast<u64>(w * kMass) : 0;
+        },
+        aim, answer);
 }
 
 }  // namespace
