@@ -235,9 +235,9 @@ struct MathF32 {
 };
 
 template <class T> struct InputOf;      // math, and a piece of a row as it is loaded
-template <> struct InputOf<float> { using Math = MathF32; using Elem = float; using Raw = f32x4; using Four = f32x4; };
-template <> struct InputOf<__half> { using Math = MathF32; using Elem = _Float16; using Raw = f16x4; using Four = f16x4; };
-template <> struct InputOf<__hip_bfloat16> { using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; using Four = bf16x4; };
+template <> struct InputOf<float> { static constexpr int kType = HX_F32; using Math = MathF32; using Elem = float; using Raw = f32x4; using Four = f32x4; };
+template <> struct InputOf<__half> { static constexpr int kType = HX_F16; using Math = MathF32; using Elem = _Float16; using Raw = f16x4; using Four = f16x4; };
+template <> struct InputOf<__hip_bfloat16> { static constexpr int kType = HX_BF16; using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; using Four = bf16x4; };
 
 // Rows [0, n) of a chunk into registers, kD columns padded with zeros, R rows a round of the
 // workgroup.  kWhole: d is a whole number of pieces and a round's rows are within 2 GiB, so that
@@ -328,13 +328,12 @@ __device__ __forceinline__ void put(Global<Out>* base, At at, int columns, f32x4
     }
 }
 
-// Waves a SIMD that the registers have to leave room for.
-constexpr int waves_of(int) { return 2; }
-
 // kDA: rows of the state (a's and b's columns) padded; kW waves of kCT 16-column tiles each.
+// kFull: the state fills its padding; else products of nothing but padding are left out (96 x 80
+// of 128 x 128 is half the work), at the price of branches between the others.
 // kStates: only the own state, from zero, of each segment but the last.
-template <class T, int kDA, int kW, int kCT, bool kWhole, bool kStates>
-__global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
+template <class T, int kDA, int kW, int kCT, bool kWhole, bool kFull, bool kStates>
+__global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A) {
     using In = InputOf<T>;
     using M = typename In::Math;
     using Elem = typename M::Elem;
@@ -463,28 +462,37 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
         tb.store([&](int i, int col, Piece x) { M::template b_store<kDA>(lb, i, col, x); });
         tc.store([&](int i, int col, Piece x) { *reinterpret_cast<Piece*>(lc + i * kSC + col) = x; });
         __syncthreads();
+        // whether columns 32 k .. of a and b are there, and the wave's column tile ct
+        auto there = [&](int k) { return kFull || k * 32 < S.da; };
+        auto column = [&](int ct) { return kFull || col0 + mine + ct * 16 < S.dc; };
         Frag c[kB][kCT];
         if constexpr (!kStates) {
             // P's blocks, as many for each wave (those over the diagonal come out as zero)
-            constexpr int kEach = kB * kB / kW;
-            static_assert(kEach * kW == kB * kB && (kEach % kB == 0 || kB % kEach == 0), "whole rows or parts of one");
+            constexpr int kEach = kB * kB > kW ? kB * kB / kW : 1;
+            static_assert((kEach * kW == kB * kB || kEach == 1) && (kEach % kB == 0 || kB % kEach == 0),
+                          "whole rows or parts of one");
             const int block0 = wave * kEach;
-            Pair pa[kK];
+            if (kEach * kW == kB * kB || block0 < kB * kB) {
+                f32x4 p[kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
-                if (e % kB == 0)
+                for (int e = 0; e < kEach; ++e) p[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < kK; ++k) pa[k] = M::a_like_b(la + (tb_ * 16 + r) * kSA, k, g4);
-                Pair pb[kK];
+                for (int k = 0; k < kK; ++k)
+                    if (there(k)) {
+                        Pair pa;
 #pragma unroll
-                for (int k = 0; k < kK; ++k) pb[k] = M::template b_pair<kDA>(lb, sb * 16 + r, k, g4);
-                f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < kK; ++k) p = M::mma(p, pb[k], pa[k]);
+                        for (int e = 0; e < kEach; ++e) {
+                            if (e % kB == 0) pa = M::a_like_b(la + ((block0 + e) / kB * 16 + r) * kSA, k, g4);
+                            p[e] = M::mma(p[e], M::template b_pair<kDA>(lb, (block0 + e) % kB * 16 + r, k, g4), pa);
+                        }
+                    }
                 // lane: step tb*16 + r, earlier steps sb*16 + g4 .. + 3
-                p *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
-                *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4)) = M::frag(p);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
+                    p[e] *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
+                    *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4)) = M::frag(p[e]);
+                }
             }
         }
 #pragma unroll
@@ -496,15 +504,7 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
             // two blocks of steps at a time: what the entering state adds, then the chunk's own steps
 #pragma unroll
             for (int t0 = 0; t0 < kB; t0 += 2) {
-                Pair pa[2][kK], pp[2][kB / 2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                    for (int k = 0; k < kK; ++k) pa[t][k] = M::a_pair(la + ((t0 + t) * 16 + r) * kSA, k, g4);
-#pragma unroll
-                    for (int sb = 0; sb <= t0 + t; sb += 2)
-                        pp[t][sb / 2] = M::p_pair(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
-                }
+                if (!column(0)) break;
                 f32x4 y[2][kCT];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -512,21 +512,28 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
                     for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < kK; ++k)
+                    if (there(k)) {
+                        Pair pa[2];
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) {
-                        const Pair x = M::pair(M::frag(X[2 * k][ct]), M::frag(X[2 * k + 1][ct]));
+                        for (int t = 0; t < 2; ++t) pa[t] = M::a_pair(la + ((t0 + t) * 16 + r) * kSA, k, g4);
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) y[t][ct] = M::mma(y[t][ct], x, pa[t][k]);
+                        for (int ct = 0; ct < kCT; ++ct) {
+                            const Pair x = M::pair(M::frag(X[2 * k][ct]), M::frag(X[2 * k + 1][ct]));
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) y[t][ct] = M::mma(y[t][ct], x, pa[t]);
+                        }
                     }
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const float since = lsince[(t0 + t) * 16 + r];
 #pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct) {
-                        y[t][ct] *= since;
+                    for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
 #pragma unroll
-                        for (int sb = 0; sb <= t0 + t; sb += 2)
-                            y[t][ct] = M::mma(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp[t][sb / 2]);
+                    for (int sb = 0; sb <= t0 + t; sb += 2) {
+                        const Pair pp = M::p_pair(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
+#pragma unroll
+                        for (int ct = 0; ct < kCT; ++ct)
+                            y[t][ct] = M::mma(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp);
                     }
                     // lane: step (t0 + t)*16 + r, columns g4 .. + 3 of each tile
                     const int i1 = i0 + (t0 + t) * 16;
@@ -557,39 +564,35 @@ __global__ void __launch_bounds__(kW * 64, waves_of(kDA)) k_chunk(ChunkArgs A) {
 #pragma unroll
         for (int sb = 0; sb < kB; sb += 2) {
             if (sb == kB - 2 && i0 + kC < end) fetch(i0 + kC, 1);
-            constexpr int kAhead = kRT < 4 ? kRT : 4;
+            if (!column(0)) continue;
             Frag wc[M::kTerms][2][kCT];
 #pragma unroll
-            for (int rt0 = 0; rt0 < kRT; rt0 += kAhead) {
-                Frag b[kAhead][2];
+            for (int e = 0; e < 2; ++e) {
+                const f32x4 w0 = lleft[(sb + e) * 4 + g4 / 4];
 #pragma unroll
-                for (int rt = 0; rt < kAhead; ++rt)
+                for (int ct = 0; ct < kCT; ++ct) {
+                    f32x4 w = M::wide(c[sb + e][ct]) * w0;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) b[rt][e] = M::template b_column<kDA>(lb, sb + e, rt0 + rt, lane);
-                if (rt0 == 0) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const f32x4 w0 = lleft[(sb + e) * 4 + g4 / 4];
-#pragma unroll
-                        for (int ct = 0; ct < kCT; ++ct) {
-                            f32x4 w = M::wide(c[sb + e][ct]) * w0;
-#pragma unroll
-                            for (int k = 0; k < M::kTerms; ++k) {
-                                wc[k][e][ct] = M::frag(w);
-                                w -= M::wide(wc[k][e][ct]);
-                            }
-                        }
+                    for (int k = 0; k < M::kTerms; ++k) {
+                        wc[k][e][ct] = M::frag(w);
+                        w -= M::wide(wc[k][e][ct]);
                     }
                 }
-#pragma unroll
-                for (int rt = 0; rt < kAhead; ++rt)
-#pragma unroll
-                    for (int ct = 0; ct < kCT; ++ct)
-#pragma unroll
-                        for (int k = 0; k < M::kTerms; ++k)
-                            X[rt0 + rt][ct] = M::mma(X[rt0 + rt][ct], M::pair(b[rt][0], b[rt][1]),
-                                                     M::pair(wc[k][0][ct], wc[k][1][ct]));
             }
+#pragma unroll
+            for (int k = 0; k < kK; ++k)
+                if (there(k)) {
+#pragma unroll
+                    for (int rt = 2 * k; rt < 2 * k + 2; ++rt) {
+                        const Pair b = M::pair(M::template b_column<kDA>(lb, sb, rt, lane),
+                                               M::template b_column<kDA>(lb, sb + 1, rt, lane));
+#pragma unroll
+                        for (int ct = 0; ct < kCT; ++ct)
+#pragma unroll
+                            for (int t = 0; t < M::kTerms; ++t)
+                                X[rt][ct] = M::mma(X[rt][ct], b, M::pair(wc[t][0][ct], wc[t][1][ct]));
+                    }
+                }
         }
     }
     if constexpr (kStates) {
@@ -670,11 +673,22 @@ struct Cut {
     int width() const { return waves * tiles * 16; }
 };
 
-Cut cut_of(int64_t da, int64_t dc) {
+Cut cut_of(int64_t type, int64_t da, int64_t dc) {
     Cut c{};
     c.rows = da <= 32 ? 32 : da <= 64 ? 64 : da <= 128 ? 128 : 256;
     c.waves = dc <= 32 ? 2 : 4;
-    c.tiles = dc <= 64 || c.rows == 256 ? 1 : 2;
+    c.tiles = 1;
+    if (dc > 64 && c.rows < 256) {
+        // 128 columns: in bf16 two tiles a wave (LDS reads serve twice: 165 us for 65536 steps, 8
+        // heads, 128 x 128, against 200 with eight waves of one); fp32 products take so much longer
+        // that more waves pay instead (777 steps, 156 sequences and heads: 114 us against 123)
+        if (type == HX_BF16) {
+            c.tiles = 2;
+        } else {
+            c.waves = 8;
+            c.rows = std::max(c.rows, 64);
+        }
+    }
     return c;
 }
 
@@ -684,7 +698,7 @@ struct Segments {
 };
 
 Segments segments_of(const hx_attention_args& A) {
-    const int chunk = A.type == HX_BF16 ? MathBf16::kC : MathF32::kC, width = cut_of(A.dk, A.dv).width();
+    const int chunk = A.type == HX_BF16 ? MathBf16::kC : MathF32::kC, width = cut_of(A.type, A.dk, A.dv).width();
     const int64_t units = A.batch * A.heads * ((A.dv + width - 1) / width);
     const int64_t chunks = std::max<int64_t>(1, (A.time + chunk - 1) / chunk);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 4));
@@ -710,12 +724,12 @@ void contiguous(long long* s, int64_t time, int64_t heads, int64_t d) {
     s[0] = time * heads * d, s[1] = heads * d, s[2] = d;
 }
 
-template <class T, int kDA, int kW, int kCT, bool kWhole>
+template <class T, int kDA, int kW, int kCT, bool kWhole, bool kFull>
 hipError_t launch_cut(ChunkArgs& A, int jobs, bool states, long long bh, hipStream_t st) {
     A.nslice = (A.job[0].dc + kW * kCT * 16 - 1) / (kW * kCT * 16);
     const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice), jobs);
-    if (states) k_chunk<T, kDA, kW, kCT, kWhole, true><<<grid, kW * 64, 0, st>>>(A);
-    else k_chunk<T, kDA, kW, kCT, kWhole, false><<<grid, kW * 64, 0, st>>>(A);
+    if (states) k_chunk<T, kDA, kW, kCT, kWhole, kFull, true><<<grid, kW * 64, 0, st>>>(A);
+    else k_chunk<T, kDA, kW, kCT, kWhole, kFull, false><<<grid, kW * 64, 0, st>>>(A);
     return hipGetLastError();
 }
 
@@ -724,30 +738,36 @@ template <class T>
 hipError_t launch_chunks(ChunkArgs A, int jobs, bool states, long long bh, hipStream_t st) {
     constexpr int kP = InputOf<T>::Math::kPiece;
     constexpr long long kFar = 1 << 23;          // elements from step to step: 64 of them in 32 bits of bytes
-    const Cut c = cut_of(A.job[0].da, A.job[0].dc);
+    const Cut c = cut_of(InputOf<T>::kType, A.job[0].da, A.job[0].dc);
     bool all_whole = A.job[0].da % kP == 0 && A.job[0].dc % kP == 0;
     for (int i = 0; i < jobs; ++i) {
         const ScanArgs& S = A.job[i];
         all_whole =
             all_whole && S.a_stride[1] < kFar && S.b_stride[1] < kFar && S.c_stride[1] < kFar && S.y_stride[1] < kFar;
     }
-    auto go = [&](auto rows, auto whole) {
+    const bool full = A.job[0].da == c.rows && A.job[0].dc % c.width() == 0;
+    auto go = [&](auto rows, auto whole, auto fills) {
         constexpr int kDA = decltype(rows)::value;
-        constexpr bool kWhole = decltype(whole)::value;
-        if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole>(A, jobs, states, bh, st);
-        if constexpr (kDA < 256)
-            if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole>(A, jobs, states, bh, st);
-        return launch_cut<T, kDA, 4, 1, kWhole>(A, jobs, states, bh, st);
+        constexpr bool kWhole = decltype(whole)::value, kFull = decltype(fills)::value;
+        if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole, kFull>(A, jobs, states, bh, st);
+        if constexpr (std::is_same_v<typename InputOf<T>::Math, MathBf16>) {
+            if constexpr (kDA < 256)
+                if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole, kFull>(A, jobs, states, bh, st);
+        } else if constexpr (kDA == 64 || kDA == 128) {
+            if (c.waves == 8) return launch_cut<T, kDA, 8, 1, kWhole, kFull>(A, jobs, states, bh, st);
+        }
+        return launch_cut<T, kDA, 4, 1, kWhole, kFull>(A, jobs, states, bh, st);
     };
-    auto rows = [&](auto whole) {
+    auto rows = [&](auto whole, auto fills) {
         switch (c.rows) {
-            case 32: return go(std::integral_constant<int, 32>{}, whole);
-            case 64: return go(std::integral_constant<int, 64>{}, whole);
-            case 128: return go(std::integral_constant<int, 128>{}, whole);
-            default: return go(std::integral_constant<int, 256>{}, whole);
+            case 32: return go(std::integral_constant<int, 32>{}, whole, fills);
+            case 64: return go(std::integral_constant<int, 64>{}, whole, fills);
+            case 128: return go(std::integral_constant<int, 128>{}, whole, fills);
+            default: return go(std::integral_constant<int, 256>{}, whole, fills);
         }
     };
-    return all_whole ? rows(std::true_type{}) : rows(std::false_type{});
+    if (all_whole && full) return rows(std::true_type{}, std::true_type{});
+    return all_whole ? rows(std::true_type{}, std::false_type{}) : rows(std::false_type{}, std::false_type{});
 }
 
 // What enters each segment but the first, where there are several; the jobs are of one size.
