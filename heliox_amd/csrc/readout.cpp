@@ -58,6 +58,8 @@ int attention_space(const char* call, const hx_attention_args* A, bool grad) {
     const size_t need = hx::attention_workspace(*A, grad);
     if (need && (!A->workspace || A->workspace_bytes < 0 || static_cast<size_t>(A->workspace_bytes) < need))
         return refuse("%s: the workspace has to hold %zu bytes", call, need);
+    if (need && reinterpret_cast<uintptr_t>(A->workspace) % 16)
+        return refuse("%s: the workspace has to start at a multiple of 16 bytes", call);
     return 0;
 }
 

@@ -310,7 +310,7 @@ struct ChunkArgs {
 typedef const __attribute__((address_space(4))) ScanArgs JobArgs;
 __device__ __forceinline__ JobArgs& job_of(const ChunkArgs&) {
     typedef const __attribute__((address_space(4))) ChunkArgs Args;
-    return ((Args*)__builtin_amdgcn_kernarg_segment_ptr())->job[blockIdx.y];
+    return ((Args*)__builtin_amdgcn_kernarg_segment_ptr())->job[blockIdx.z];
 }
 
 // Four neighbours of a row to base[at], of which `columns` are there.
@@ -613,20 +613,23 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     }
 }
 
-// Segments' own states to the states that enter the segments after them, in place.
+// Segments' own states to the states that enter the segments after them, in place; kV values
+// a thread.
+template <int kV>
 __global__ void __launch_bounds__(kThreads) k_join(ChunkArgs A) {
+    typedef float Vec __attribute__((ext_vector_type(kV)));
     const JobArgs& S = job_of(A);
-    const int nseg = A.nseg - 1, size = S.da * S.dc, blocks = (size + kThreads - 1) / kThreads;
-    const int bh = blockIdx.x / blocks, e = blockIdx.x % blocks * kThreads + threadIdx.x;
+    const int nseg = A.nseg - 1, size = S.da * S.dc / kV;
+    const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x;
     if (e >= size) return;
     const int batch = bh / S.heads, h = bh - batch * S.heads;
     const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
     const float lg = S.log_decay[h] * 1.44269504f;
     const float g = lg < -1e4f ? -1e4f : lg;
-    float* w = S.states + static_cast<long long>(bh) * nseg * size + e;
+    Vec* w = reinterpret_cast<Vec*>(S.states) + static_cast<long long>(bh) * nseg * size + e;
     // the segments' loads do not wait for each other
     constexpr int kAhead = 16;
-    float x = 0.f, next[kAhead];
+    Vec x = {}, next[kAhead];
     for (int s0 = 0; s0 < nseg; s0 += kAhead) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
@@ -727,7 +730,7 @@ void contiguous(long long* s, int64_t time, int64_t heads, int64_t d) {
 template <class T, int kDA, int kW, int kCT, bool kWhole, bool kFull>
 hipError_t launch_cut(ChunkArgs& A, int jobs, bool states, long long bh, hipStream_t st) {
     A.nslice = (A.job[0].dc + kW * kCT * 16 - 1) / (kW * kCT * 16);
-    const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice), jobs);
+    const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice), 1, jobs);
     if (states) k_chunk<T, kDA, kW, kCT, kWhole, kFull, true><<<grid, kW * 64, 0, st>>>(A);
     else k_chunk<T, kDA, kW, kCT, kWhole, kFull, false><<<grid, kW * 64, 0, st>>>(A);
     return hipGetLastError();
@@ -776,8 +779,11 @@ hipError_t launch_states(const ChunkArgs& A, int jobs, long long bh, hipStream_t
     if (A.nseg < 2) return hipSuccess;
     const hipError_t e = launch_chunks<T>(A, jobs, true, bh, st);
     if (e != hipSuccess) return e;
-    const long long blocks = (static_cast<long long>(A.job[0].da) * A.job[0].dc + kThreads - 1) / kThreads;
-    k_join<<<dim3(static_cast<unsigned>(bh * blocks), jobs), kThreads, 0, st>>>(A);
+    // (several segments are made of 512 sequences and heads at most: within a grid's second dimension)
+    const int size = A.job[0].da * A.job[0].dc, width = size % 4 == 0 ? 4 : 1;
+    const dim3 grid((size / width + kThreads - 1) / kThreads, static_cast<unsigned>(bh), jobs);
+    if (width == 4) k_join<4><<<grid, kThreads, 0, st>>>(A);
+    else k_join<1><<<grid, kThreads, 0, st>>>(A);
     return hipGetLastError();
 }
 

@@ -535,7 +535,7 @@ typedef struct hx_attention_args {
     float* state;
     const int32_t* slots;
     int64_t n_slots;
-    void* workspace;
+    void* workspace;                                      /* starts at a multiple of 16 bytes */
     int64_t workspace_bytes;
     void* stream;
 } hx_attention_args;

@@ -243,3 +243,46 @@ def test_captured_into_a_graph():
         want = work()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(replayed, want)), n
+
+
+def test_python_refuses_what_does_not_fit():
+    q, k, v, g, state, do, dend = make(29, torch.bfloat16, 2, 9, 4, 4, 2, 4, 16, 24)
+    bad = [
+        (ValueError, lambda: readout.linear_attention(q, k[:, :8], v, g)),
+        (ValueError, lambda: readout.linear_attention(q, k[..., :15], v, g)),
+        (ValueError, lambda: readout.linear_attention(q[0], k[0], v[0], g)),
+        (TypeError, lambda: readout.linear_attention(q, k.half(), v, g)),
+        (TypeError, lambda: readout.linear_attention(q.double(), k.double(), v.double(), g)),
+        (TypeError, lambda: readout.linear_attention(q, k, v, g.double())),
+        (TypeError, lambda: readout.linear_attention(q, k, v, None)),
+        (ValueError, lambda: readout.linear_attention(q, k, v, g.cpu())),
+        (ValueError, lambda: readout.linear_attention(q, k, v, g, initial_state=state[:1])),
+        (TypeError, lambda: readout.linear_attention(q, k, v, g, lengths=torch.tensor([1, 2], device="cuda"))),
+        (ValueError, lambda: readout.linear_attention_grad(q, k, v, g, do[..., :23])),
+        (TypeError, lambda: readout.linear_attention_grad(q, k, v, g, do.float())),
+        (TypeError, lambda: readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state.transpose(2, 3))),
+        (ValueError, lambda: readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state[:, :3].contiguous())),
+        (RuntimeError, lambda: readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state[:1])),
+        (RuntimeError, lambda: readout.linear_attention(q, k, v, g[:3])),
+        (RuntimeError, lambda: readout.linear_attention(q, k, v, g, scale=float("nan"))),
+        (ValueError, lambda: readout.sample(q[:, 0, 0], g)),
+        (TypeError, lambda: readout.sample(q[:, 0, 0], g[:2], top_k=g[:2])),
+        (ValueError, lambda: readout.distill_loss(q[:, 0, 0], torch.zeros(3, 1, dtype=torch.int32, device="cuda"),
+                                                  torch.zeros(3, 1, device="cuda"))),
+        (TypeError, lambda: readout.distill_loss(q[:, 0, 0], torch.zeros(2, 1, device="cuda"),
+                                                 torch.zeros(2, 1, device="cuda"))),
+        (ValueError, lambda: readout.distill_loss_grad(q[:, 0, 0], torch.zeros(2, 1, dtype=torch.int32, device="cuda"),
+                                                       torch.zeros(2, 1, device="cuda"), out=q[:, 0, 0].t())),
+    ]
+    for error, call in bad:
+        with pytest.raises(error):
+            call()
+
+
+def test_decays_are_clamped_like_the_recurrence():
+    """Very strong decays (and none) in one call, over several chunks and segments."""
+    q, k, v, *_ = make(31, torch.float32, 1, 2100, 4, 4, 4, 4, 16, 16)
+    g = torch.tensor([-1e30, -200.0, -20.0, 0.0], device="cuda")
+    o, end = readout.linear_attention(q, k, v, g)
+    want = ref.attention(q, k, v, g, 0.25)
+    assert ref.rel(o, want[0]) <= bound(torch.float32) and ref.rel(end, want[1]) <= bound(torch.float32)

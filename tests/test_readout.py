@@ -110,3 +110,19 @@ def test_records_are_as_long_as_the_header_says(tmp_path):
                    check=True)
     got = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout
     assert got.split() == [str(r.size) for r in (readout._ATTENTION, readout._DISTILL, readout._SAMPLE)]
+
+
+def test_a_workspace_that_does_not_fit_is_refused():
+    """Pointers are only compared here: the call ends before anything is launched."""
+    long = dict(GOOD, batch=1, time=5000)
+    need = lib().hx_linear_attention_workspace(attention(**long), 0)
+    assert need > 0
+    fields = list(readout._ATTENTION.unpack(attention(**long)))
+    for i in (9, 10, 11, 21, 25):       # q, k, v, log_decay, o
+        fields[i] = 4096
+    for space, size in ((0, need), (4096, need - 1), (4096, -1)):
+        fields[-3:-1] = space, size
+        assert lib().hx_linear_attention(readout._ATTENTION.pack(*fields)) == -1
+        assert "workspace" in error()
+    fields[-3:-1] = 4104, need
+    assert lib().hx_linear_attention(readout._ATTENTION.pack(*fields)) == -1 and "16 bytes" in error()
