@@ -39,7 +39,8 @@ struct ScanArgs {
 // ------------------------------------------------------------------- one step
 // One workgroup per (sequence, head).  Lanes lie along a state's rows, kV columns each, so that
 // the state streams through as it lies in memory; k and q wait in LDS.  Bound by the state's
-// bytes, read and written once.
+// bytes, read and written once: 256 x 16 states of 128 x 128 in 102 us, 5.3 TB/s (a copy of as
+// much reaches 4.8).  A single row is bound by the call (11 us, 4 of them on the GPU).
 template <class T, int kV>
 __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, const int32_t* slots, long long n_slots,
                                                    int lanes) {
@@ -103,14 +104,24 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
 // ------------------------------------------------------------------- whole sequences
 // Chunks of kC steps.  With i, j counted inside a chunk of n steps, X the state that enters it
 // and off 1 (forward) or 0 (reverse, where a state has not decayed before its first step):
-//   P_ij = scale_in e^{g (i - j)} (a_i . b_j) for j <= i
-//   y_i  = scale_out (sum_j P_ij c_j + e^{g (i + off)} X^T a_i)
+//   P_ij = scale_in scale_out e^{g (i - j)} (a_i . b_j) for j <= i
+//   y_i  = sum_j P_ij c_j + scale_out e^{g (i + off)} X^T a_i
 //   X'   = e^{g n} X + sum_j b_j (scale_in e^{g (n - off - j)} c_j)^T
 // are products of matrices.  A workgroup walks through the chunks of one (sequence, head,
 // slice of c's columns, segment of the steps); each wave keeps X^T's rows for its own columns
 // in accumulator registers, whose layout (lane: one column, four rows) is at the same time
 // that of an operand, so X enters y's product without leaving the registers.  y and P are made
 // transposed for the same reason: P goes to LDS, and y to memory, four neighbours a lane.
+//
+// Few sequences are cut into segments: their own states first (from zero, in a launch that reads
+// b and c alone), joined one after another, then every segment with the state that enters it.
+// The price is b and c read twice.
+//
+// What bounds it, bf16, 65536 steps of 8 heads of 128 x 128 (537 MB, 113 us at a copy's rate):
+// 69 us for the segments' states (3.9 TB/s), 15 to join them, 136 for the rest, in which a wave
+// issues 2500 cycles of matrix and 3200 of other instructions a chunk, two waves a SIMD: neither
+// memory nor matrix cores are full, barriers and LDS reads lie between.  fp32 matrix instructions
+// take 16 times as long: there they bound it.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -745,8 +756,8 @@ hipError_t launch_chunks(ChunkArgs A, int jobs, bool states, long long bh, hipSt
     bool all_whole = A.job[0].da % kP == 0 && A.job[0].dc % kP == 0;
     for (int i = 0; i < jobs; ++i) {
         const ScanArgs& S = A.job[i];
-        all_whole =
-            all_whole && S.a_stride[1] < kFar && S.b_stride[1] < kFar && S.c_stride[1] < kFar && S.y_stride[1] < kFar;
+        for (long long stride : {S.a_stride[1], S.b_stride[1], S.c_stride[1], S.y_stride[1]})
+            all_whole = all_whole && stride >= 0 && stride < kFar;
     }
     const bool full = A.job[0].da == c.rows && A.job[0].dc % c.width() == 0;
     auto go = [&](auto rows, auto whole, auto fills) {

@@ -2,20 +2,20 @@
 //
 // Masses are whole numbers, so their sums are the same in any order, and integer atomics may
 // make them.  What top_k and top_p leave is "every place over a key, and those at it up to an
-// index".  A histogram over 2048 equal parts of the range that has any mass says in which part
-// the cut lies; the places of that part (and, for top_k, of all above) go into LDS where they
-// fit, are sorted there and say the rest.  Where they do not fit (ties without end), histograms
+// index".  A histogram over equal parts (two a thread) of the range that has any mass says in
+// which part the cut lies; the places of that part (and, for top_k, of all above) go into LDS
+// where they fit, are sorted there and say the rest.  Where they do not fit (ties without end), histograms
 // over the part's keys go on until one key is left.  The row itself is read again from the cache
 // in each pass: two to four of them as a rule, of which those that make masses of all places
-// (about 25 instructions each) take the time.
+// (about 40 instructions each) take the time: 256 rows of 131072 bf16 logits, each with its own
+// settings, take 121 us, nine times what reading them once would, 16 waves a CU busy throughout.
 #include "readout.h"
+
+#include <type_traits>
 
 namespace hx {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
 constexpr float kMass = 1099511627776.f;      // 2^40
 constexpr float kDepth = 27.8f;               // e^-27.8 < 2^-40: no mass beyond
 typedef unsigned long long u64;
@@ -36,7 +36,9 @@ __device__ __forceinline__ float value_of(unsigned key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+template <int kT>
 struct Shared {
+    static constexpr int kThreads = kT, kWaves = kT / 64, kBins = 2 * kT;
     u64 bins[kBins];
     u64 part[kWaves];
     u64 pick[3];
@@ -44,18 +46,19 @@ struct Shared {
 };
 
 // x reduced over the workgroup; every thread gets the result.
-template <class V, class F>
-__device__ __forceinline__ V block_reduce(V x, Shared& sh, F op) {
+template <class Sh, class V, class F>
+__device__ __forceinline__ V block_reduce(V x, Sh& sh, F op) {
     for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
     __syncthreads();
     if (threadIdx.x % 64 == 0) sh.part[threadIdx.x / 64] = x;
     __syncthreads();
     x = static_cast<V>(sh.part[0]);
-    for (int w = 1; w < kWaves; ++w) x = op(x, static_cast<V>(sh.part[w]));
+    for (int w = 1; w < Sh::kWaves; ++w) x = op(x, static_cast<V>(sh.part[w]));
     return x;
 }
 
-__device__ __forceinline__ u64 block_sum(u64 x, Shared& sh) {
+template <class Sh>
+__device__ __forceinline__ u64 block_sum(u64 x, Sh& sh) {
     return block_reduce(x, sh, [](u64 a, u64 b) { return a + b; });
 }
 
@@ -70,21 +73,22 @@ __device__ __forceinline__ u64 wave_before(u64 x) {       // sum over the lanes 
 }
 
 // Sum of x over the threads before this one; total gets the whole sum.
-__device__ __forceinline__ u64 block_before(u64 x, Shared& sh, u64& total) {
+template <class Sh>
+__device__ __forceinline__ u64 block_before(u64 x, Sh& sh, u64& total) {
     const u64 before = wave_before(x);
     __syncthreads();
     if (threadIdx.x % 64 == 63) sh.part[threadIdx.x / 64] = before + x;
     __syncthreads();
     u64 base = 0;
     total = 0;
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < Sh::kWaves; ++w) {
         if (w < static_cast<int>(threadIdx.x / 64)) base += sh.part[w];
         total += sh.part[w];
     }
     return base + before;
 }
 
-template <class T>
+template <class T, int kThreads>
 struct Row {
     using Vec = typename PieceOf<T>::Vec;
     static constexpr int kP = sizeof(Vec) / sizeof(T);
@@ -125,8 +129,9 @@ struct Cut {
 
 // Of sh.bins from the last to the first, the one where the running sum (from `before`) passes.
 // The bins are zero afterwards.
-template <class P>
-__device__ __forceinline__ Cut find_bin(Shared& sh, P passes, u64 before) {
+template <class Sh, class P>
+__device__ __forceinline__ Cut find_bin(Sh& sh, P passes, u64 before) {
+    constexpr int kThreads = Sh::kThreads, kBins = Sh::kBins;
     __syncthreads();
     constexpr int kEach = kBins / kThreads;
     const int top = kBins - 1 - threadIdx.x * kEach;
@@ -154,19 +159,19 @@ __device__ __forceinline__ Cut find_bin(Shared& sh, P passes, u64 before) {
 
 // Which of the equal parts of the range with any mass a logit lies in, the largest in the last;
 // -1: beyond.  Monotonous, as each of its roundings is.
-template <class T>
-__device__ __forceinline__ int part_of(const Row<T>& R, float v) {
+template <int kBins, class R_>
+__device__ __forceinline__ int part_of(const R_& R, float v) {
     const float d = -R.depth(v) * (kBins / kDepth);
     return d < kBins ? kBins - 1 - static_cast<int>(d) : -1;
 }
 
 // Adds value(index, logit) to the bin of each place's part.
-template <class T, class V>
-__device__ __forceinline__ void add_parts(const Row<T>& R, Shared& sh, V value) {
+template <class R_, class Sh, class V>
+__device__ __forceinline__ void add_parts(const R_& R, Sh& sh, V value) {
     R.each([&](int j0, const float* v, int n) {
 #pragma unroll
-        for (int i = 0; i < Row<T>::kP; ++i) {
-            const int b = i < n ? part_of(R, v[i]) : -1;
+        for (int i = 0; i < R_::kP; ++i) {
+            const int b = i < n ? part_of<Sh::kBins>(R, v[i]) : -1;
             if (b >= 0) {
                 const u64 w = value(j0 + i, v[i]);
                 if (w) atomicAdd(&sh.bins[b], w);
@@ -178,13 +183,14 @@ __device__ __forceinline__ void add_parts(const Row<T>& R, Shared& sh, V value) 
 // From the part where a running sum passes to the key where it does: by histograms over what
 // lies between the part's least and largest key, until one key is left.  c is the part's cut
 // and becomes the key's.
-template <class T, class V, class P>
-__device__ __forceinline__ unsigned refine(const Row<T>& R, Shared& sh, V value, P passes, Cut& c) {
+template <class R_, class Sh, class V, class P>
+__device__ __forceinline__ unsigned refine(const R_& R, Sh& sh, V value, P passes, Cut& c) {
+    constexpr int kBins = Sh::kBins;
     unsigned lo = ~0u, hi = 0;
     R.each([&](int j0, const float* v, int n) {
 #pragma unroll
-        for (int i = 0; i < Row<T>::kP; ++i)
-            if (i < n && part_of(R, v[i]) == c.bin && value(j0 + i, v[i])) {
+        for (int i = 0; i < R_::kP; ++i)
+            if (i < n && part_of<kBins>(R, v[i]) == c.bin && value(j0 + i, v[i])) {
                 const unsigned k = key_of(v[i]);
                 lo = min(lo, k);
                 hi = max(hi, k);
@@ -197,7 +203,7 @@ __device__ __forceinline__ unsigned refine(const Row<T>& R, Shared& sh, V value,
         while ((hi - lo) >> shift >= kBins) ++shift;
         R.each([&](int j0, const float* v, int n) {
 #pragma unroll
-            for (int i = 0; i < Row<T>::kP; ++i) {
+            for (int i = 0; i < R_::kP; ++i) {
                 const unsigned k = key_of(v[i]);
                 if (i < n && k >= lo && k <= hi) {
                     const u64 w = value(j0 + i, v[i]);
@@ -213,6 +219,7 @@ __device__ __forceinline__ unsigned refine(const Row<T>& R, Shared& sh, V value,
 }
 
 // Ascending sort of kThreads keys, one a thread, in LDS.
+template <int kThreads>
 __device__ __forceinline__ u64 block_sort(u64 key, u64* at) {
     for (int size = 2; size <= kThreads; size <<= 1)
         for (int gap = size / 2; gap > 0; gap >>= 1) {
@@ -237,13 +244,14 @@ __device__ __forceinline__ float ranked_value(u64 e) { return value_of(~static_c
 
 // The places for which take(index, logit) holds, sorted by rank, one a thread (kNone: no more);
 // false, and nothing usable, where they are more than the threads.  Uses sh.bins.
-template <class T, class F>
-__device__ __forceinline__ bool gather(const Row<T>& R, Shared& sh, F take, u64& mine) {
+template <class R_, class Sh, class F>
+__device__ __forceinline__ bool gather(const R_& R, Sh& sh, F take, u64& mine) {
+    constexpr int kThreads = Sh::kThreads, kBins = Sh::kBins;
     u64* const list = sh.bins;
     static_assert(kBins >= 2 * kThreads, "the list and the sort's own space");
     R.each([&](int j0, const float* v, int n) {
 #pragma unroll
-        for (int i = 0; i < Row<T>::kP; ++i)
+        for (int i = 0; i < R_::kP; ++i)
             if (i < n && take(j0 + i, v[i])) {
                 const unsigned at = atomicAdd(&sh.count, 1u);
                 if (at < kThreads) list[at] = by_rank(v[i], j0 + i);
@@ -254,7 +262,7 @@ __device__ __forceinline__ bool gather(const Row<T>& R, Shared& sh, F take, u64&
     mine = threadIdx.x < min(count, static_cast<unsigned>(kThreads)) ? list[threadIdx.x] : kNone;
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
-    if (count <= kThreads) mine = block_sort(mine, list + kThreads);
+    if (count <= kThreads) mine = block_sort<kThreads>(mine, list + kThreads);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) list[i] = 0;
     __syncthreads();
@@ -275,9 +283,9 @@ __device__ __forceinline__ u64 count_under(double bound, u64 before, u64 mass, u
 // The place where the running sum of value(index, logit), in index order, passes an aim: each
 // wave's turns are summed, then the turn where it passes is looked at by itself.  aim_of(whole
 // sum) is the aim; found(index, logit, whole sum) is called by the one thread that holds the place.
-template <class T, class V, class A, class F>
-__device__ __forceinline__ void at_running_sum(const Row<T>& R, Shared& sh, u64* segments, V value, A aim_of, F found) {
-    constexpr int kP = Row<T>::kP;
+template <class R_, class Sh, class V, class A, class F>
+__device__ __forceinline__ void at_running_sum(const R_& R, Sh& sh, u64* segments, V value, A aim_of, F found) {
+    constexpr int kP = R_::kP, kThreads = Sh::kThreads, kWaves = Sh::kWaves;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     int turn = 0;
     R.each([&](int j0, const float* v, int n) {
@@ -323,12 +331,13 @@ __device__ __forceinline__ void at_running_sum(const Row<T>& R, Shared& sh, u64*
     __syncthreads();
 }
 
-template <class T>
+template <class T, int kThreads>
 __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
-    __shared__ Shared sh;
+    using R_ = Row<T, kThreads>;
+    using Sh = Shared<kThreads>;
+    constexpr int kP = R_::kP, kBins = Sh::kBins;
+    __shared__ Sh sh;
     extern __shared__ u64 segments[];          // sums of each wave's turns in each()
-    using R_ = Row<T>;
-    constexpr int kP = R_::kP;
     const long long row = blockIdx.x;
     R_ R;
     R.x = static_cast<const T*>(A.logits) + row * A.logits_stride;
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
         u64 mine = kNone;
         bool listed = false;
         if (c.bin >= 0 && c.before + c.at <= kThreads) {
-            listed = gather(R, sh, [&](int, float v) { return part_of(R, v) >= c.bin; }, mine);
+            listed = gather(R, sh, [&](int, float v) { return part_of<kBins>(R, v) >= c.bin; }, mine);
             if (threadIdx.x >= top_k) mine = kNone;
         } else if (c.bin >= 0) {
             least = refine(R, sh, one, passes, c);
@@ -415,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
             if (!(top_p >= 1.f) && !(static_cast<double>(before) < bound_of(total))) m = 0;
             if (!(R.weight(v) >= min_p)) m = 0;
             // and in index order
-            mine = block_sort(m ? mine << 32 | mine >> 32 : kNone, sh.bins + kThreads);
+            mine = block_sort<kThreads>(m ? mine << 32 | mine >> 32 : kNone, sh.bins + kThreads);
             const float w = mine != kNone ? value_of(~static_cast<unsigned>(mine)) : -INFINITY;
             m = mine != kNone ? R.mass(w) : 0;
             before = block_before(m, sh, total);
@@ -426,7 +435,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
     }
     if (!(top_p >= 1.f)) {
         auto counted = [&](int j, float v) { return stays(j, v) ? R.mass(v) : 0; };
-        add_parts(R, sh, counted);
+        if (least) add_parts(R, sh, counted);
+        else add_parts(R, sh, [&](int, float v) { return R.mass(v); });
         __syncthreads();
         u64 total = 0;
         for (int i = threadIdx.x; i < kBins; i += kThreads) total += sh.bins[i];
@@ -434,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
         auto passes = [&](u64 s) { return static_cast<double>(s) >= bound; };
         Cut c = find_bin(sh, passes, 0);
         u64 mine;
-        if (gather(R, sh, [&](int j, float v) { return part_of(R, v) == c.bin && stays(j, v); }, mine)) {
+        if (gather(R, sh, [&](int j, float v) { return part_of<kBins>(R, v) == c.bin && stays(j, v); }, mine)) {
             const u64 m = mine != kNone ? R.mass(ranked_value(mine)) : 0;
             u64 all;
             const u64 before = c.before + block_before(m, sh, all);
@@ -471,15 +481,23 @@ hipError_t sample_launch(const hx_sample_args& A) {
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     return with_type(A.type, [&](auto t) {
         using T = decltype(t);
-        constexpr int64_t turn = static_cast<int64_t>(kThreads) * Row<T>::kP;
-        const size_t lds = sizeof(u64) * kWaves * ((A.vocab + turn - 1) / turn);
-        if (lds > 32768) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_sample<T>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, 140000);
-            if (e != hipSuccess) return e;
-        }
-        k_sample<T><<<static_cast<unsigned>(A.rows), kThreads, lds, st>>>(A);
-        return hipGetLastError();
+        auto go = [&](auto threads) {
+            constexpr int kThreads = decltype(threads)::value;
+            constexpr int64_t turn = static_cast<int64_t>(kThreads) * Row<T, kThreads>::kP;
+            const size_t lds = sizeof(u64) * (kThreads / 64) * ((A.vocab + turn - 1) / turn);
+            if (lds > 32768) {
+                const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_sample<T, kThreads>),
+                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 140000);
+                if (e != hipSuccess) return e;
+            }
+            k_sample<T, kThreads><<<static_cast<unsigned>(A.rows), kThreads, lds, st>>>(A);
+            return hipGetLastError();
+        };
+        // Threads a row.  A row that has a CU to itself takes 1024 (16000 places: 12 us against 20
+        // with 256); small ones and many are faster with 256, whose barriers and sorts are short
+        // (1500 rows: of 600 places 24 us against 131, of 16000 places 112 against 176).
+        return A.vocab <= 4096 || A.rows >= 1024 ? go(std::integral_constant<int, 256>{})
+                                                 : go(std::integral_constant<int, 1024>{});
     });
 }
 
