@@ -23,6 +23,8 @@ int launched(const char* call, hipError_t e) {
 
 bool known_type(int64_t t) { return t == HX_F32 || t == HX_F16 || t == HX_BF16; }
 
+constexpr int64_t kMaxRows = 1 << 21;     // of 1024 threads each: a grid has under 2^32
+
 int64_t checked_product(int64_t a, int64_t b) {
     int64_t p = 0;
     return __builtin_mul_overflow(a, b, &p) ? INT64_MAX : p;
@@ -42,9 +44,9 @@ int attention_sizes(const char* call, const hx_attention_args* A) {
     if (A->dk < 1 || A->dk > hx::kAttnMaxDim || A->dv < 1 || A->dv > hx::kAttnMaxDim)
         return refuse("%s: dk (%lld) and dv (%lld) have to be in 1..%d", call, (long long)A->dk, (long long)A->dv,
                       hx::kAttnMaxDim);
-    // one workgroup or more for each (sequence, head): the grid's own limit, with room for its splits
-    if (checked_product(A->batch, A->heads) > (1 << 24) || A->time > (int64_t(1) << 30))
-        return refuse("%s: batch x heads is at most 2^24 and time at most 2^30", call);
+    // up to twelve workgroups of 256 threads for each (sequence, head): a grid has under 2^32 threads
+    if (checked_product(A->batch, A->heads) > (1 << 20) || A->time > (int64_t(1) << 30))
+        return refuse("%s: batch x heads is at most 2^20 and time at most 2^30", call);
     if (!std::isfinite(A->scale)) return refuse("%s: scale is not finite", call);
     return 0;
 }
@@ -116,7 +118,7 @@ int hx_distill_loss(const hx_distill_args* A) {
     if (!A) return refuse("%s: no arguments", call);
     if (!known_type(A->type) || !known_type(A->teacher_type)) return refuse("%s: type is not known", call);
     if (A->index_bits != 32 && A->index_bits != 64) return refuse("%s: indexes have 32 or 64 bits", call);
-    if (A->rows < 0 || A->rows > INT32_MAX) return refuse("%s: rows has to be in 0..2^31-1", call);
+    if (A->rows < 0 || A->rows > kMaxRows) return refuse("%s: rows has to be in 0..2^21", call);
     if (A->vocab < 1 || A->vocab > hx::kDistillMaxVocab)
         return refuse("%s: vocab (%lld) has to be in 1..%lld", call, (long long)A->vocab,
                       (long long)hx::kDistillMaxVocab);
@@ -134,7 +136,7 @@ int hx_sample(const hx_sample_args* A) {
     const char* call = "hx_sample";
     if (!A) return refuse("%s: no arguments", call);
     if (!known_type(A->type)) return refuse("%s: type is not known", call);
-    if (A->rows < 0 || A->rows > INT32_MAX) return refuse("%s: rows has to be in 0..2^31-1", call);
+    if (A->rows < 0 || A->rows > kMaxRows) return refuse("%s: rows has to be in 0..2^21", call);
     // masses count to 2^40 each: 2^22 of them stay inside 63 bits
     if (A->vocab < 1 || A->vocab > (1 << 22)) return refuse("%s: vocab has to be in 1..2^22", call);
     if (!A->rows) return 0;

@@ -313,15 +313,15 @@ struct Tile {
 constexpr int kJobs = 3;               // sums of one launch: the gradients are three
 struct ChunkArgs {
     ScanArgs job[kJobs];
-    int nslice, nseg, seg_steps;       // seg_steps a multiple of the chunk
+    int jobs, nslice, nseg, seg_steps; // seg_steps a multiple of the chunk
 };
 
-// The block's job where it lies among the kernel's arguments (indexed as a value, the array
+// A job where it lies among the kernel's arguments (indexed as a value, the array
 // would be copied to every lane's scratch memory first: 157 -> 452 us).
 typedef const __attribute__((address_space(4))) ScanArgs JobArgs;
-__device__ __forceinline__ JobArgs& job_of(const ChunkArgs&) {
+__device__ __forceinline__ JobArgs& job_of(int job) {
     typedef const __attribute__((address_space(4))) ChunkArgs Args;
-    return ((Args*)__builtin_amdgcn_kernarg_segment_ptr())->job[blockIdx.z];
+    return ((Args*)__builtin_amdgcn_kernarg_segment_ptr())->job[job];
 }
 
 // Four neighbours of a row to base[at], of which `columns` are there.
@@ -359,11 +359,11 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     // over it, nothing) as a lane holds them; of the entering state; of what enters at a step
     __shared__ f32x4 lfactor[kStates ? 1 : (kB + 1) * 64], lleft[kC / 4];
     __shared__ float lsince[kStates ? 1 : kC];
-    const JobArgs& S = job_of(A);
+    // neighbouring workgroups take the jobs of one segment, which read much the same
+    const JobArgs& S = job_of(blockIdx.x % A.jobs);
     const int lane = threadIdx.x % 64, r = lane % 16, g4 = lane / 16 * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int slice = blockIdx.x % A.nslice;
-    const int unit = blockIdx.x / A.nslice;
+    const int part = blockIdx.x / A.jobs, slice = part % A.nslice, unit = part / A.nslice;
     const int nseg = kStates ? A.nseg - 1 : A.nseg;
     const int seg = unit % nseg, bh = unit / nseg;
     const int batch = bh / S.heads, h = bh - batch * S.heads;
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
 template <int kV>
 __global__ void __launch_bounds__(kThreads) k_join(ChunkArgs A) {
     typedef float Vec __attribute__((ext_vector_type(kV)));
-    const JobArgs& S = job_of(A);
+    const JobArgs& S = job_of(blockIdx.z);
     const int nseg = A.nseg - 1, size = S.da * S.dc / kV;
     const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x;
     if (e >= size) return;
@@ -706,7 +706,10 @@ Cut cut_of(int64_t type, int64_t da, int64_t dc) {
     return c;
 }
 
-// Segments of the steps, the same for all sums of a call.
+// Segments of the steps, the same for all sums of a call: 512 workgroups in all, two chunks or
+// more each.  Two segments would read twice what they halve, and three of one chunk or two wait
+// longer for two more launches than for the chunks: forward and backward, bf16, 4 heads of 64,
+// 500 steps 49 us cut and 56 whole, but 16 sequences of 300 steps 53 cut in two and 38 whole.
 struct Segments {
     int count, steps;
 };
@@ -715,8 +718,8 @@ Segments segments_of(const hx_attention_args& A) {
     const int chunk = A.type == HX_BF16 ? MathBf16::kC : MathF32::kC, width = cut_of(A.type, A.dk, A.dv).width();
     const int64_t units = A.batch * A.heads * ((A.dv + width - 1) / width);
     const int64_t chunks = std::max<int64_t>(1, (A.time + chunk - 1) / chunk);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 4));
-    const int64_t each = (chunks + want - 1) / want;
+    const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 2);
+    const int64_t each = want < 3 ? chunks : (chunks + want - 1) / want;
     return {static_cast<int>((chunks + each - 1) / each), static_cast<int>(each * chunk)};
 }
 
@@ -741,7 +744,8 @@ void contiguous(long long* s, int64_t time, int64_t heads, int64_t d) {
 template <class T, int kDA, int kW, int kCT, bool kWhole, bool kFull>
 hipError_t launch_cut(ChunkArgs& A, int jobs, bool states, long long bh, hipStream_t st) {
     A.nslice = (A.job[0].dc + kW * kCT * 16 - 1) / (kW * kCT * 16);
-    const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice), 1, jobs);
+    A.jobs = jobs;
+    const dim3 grid(static_cast<unsigned>(bh * (A.nseg - states) * A.nslice * jobs));
     if (states) k_chunk<T, kDA, kW, kCT, kWhole, kFull, true><<<grid, kW * 64, 0, st>>>(A);
     else k_chunk<T, kDA, kW, kCT, kWhole, kFull, false><<<grid, kW * 64, 0, st>>>(A);
     return hipGetLastError();

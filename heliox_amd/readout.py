@@ -32,7 +32,6 @@ _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_NO_STRIDE = (0, 0, 0)
 
 
 # A call's checks are most of a small call's time, so each goes the short way first (attributes
@@ -113,7 +112,8 @@ def _like(x: torch.Tensor, what: str, q: torch.Tensor, device: int) -> None:
 
 
 def _attention_inputs(q, k, v, log_decay, ndim: int):
-    """q, k, v with contiguous last dimensions, and their sizes as the record takes them."""
+    """The tensors with contiguous last dimensions (kept by the caller until its call is queued),
+    and the record's fields up to log_decay: sizes, pointers, strides."""
     device = _on_gpu(q, "q")
     _like(k, "k", q, device)
     _like(v, "v", q, device)
@@ -130,14 +130,15 @@ def _attention_inputs(q, k, v, log_decay, ndim: int):
     if log_decay is None:
         raise TypeError("log_decay has to be a tensor")
     log_decay = _array(log_decay, "log_decay", torch.float32, (heads,), device)
-    time = sq[1] if ndim == 4 else 1
-    sizes = (kind, sq[0], time, heads, sq[-2], sk[-2], sv[-2], sq[-1], sv[-1])
-    return device, _rows(q), _rows(k), _rows(v), log_decay, sizes
-
-
-def _strides(x: torch.Tensor) -> tuple:
-    s = x.stride()
-    return s[:3] if len(s) == 4 else (s[0], 0, s[1])
+    rows = q, k, v = _rows(q), _rows(k), _rows(v)
+    a, b, c = q.stride(), k.stride(), v.stride()
+    if ndim == 4:
+        fields = (kind, sq[0], sq[1], heads, sq[2], sk[2], sv[2], sq[3], sv[3], q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2], log_decay.data_ptr())
+    else:
+        fields = (kind, sq[0], 1, heads, sq[1], sk[1], sv[1], sq[2], sv[2], q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), a[0], 0, a[1], b[0], 0, b[1], c[0], 0, c[1], log_decay.data_ptr())
+    return device, (rows, log_decay), fields
 
 
 def _lengths(lengths, batch: int, device) -> Optional[torch.Tensor]:
@@ -161,15 +162,14 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Within a sequence a non-finite k or v may reach outputs of up to 63 steps before it (chunks
     of steps are products of matrices).
     """
-    device, q, k, v, log_decay, sizes = _attention_inputs(q, k, v, log_decay, 4)
-    _, batch, time, heads, _, _, _, dk, dv = sizes
+    device, kept, fields = _attention_inputs(q, k, v, log_decay, 4)
+    _, batch, time, heads, _, _, _, dk, dv = fields[:9]
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, heads, dk, dv), device)
     lengths = _lengths(lengths, batch, device)
     o = torch.empty((batch, time, heads, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((batch, heads, dk, dv), dtype=torch.float32, device=q.device)
-    head = (*sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay),
-            _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, _ptr(o), *_strides(o),
-            _ptr(end), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    head = (*fields, _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, o.data_ptr(),
+            time * heads * dv, heads * dv, dv, end.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     _run_attention("hx_linear_attention", device, head, 0)
     return o, end
 
@@ -199,8 +199,8 @@ def linear_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     share adds up over them; zero beyond a sequence's length) and the gradient by initial_state
     (None where that is None).  Decays are time constants of the readout: no gradient is made
     for them."""
-    device, q, k, v, log_decay, sizes = _attention_inputs(q, k, v, log_decay, 4)
-    _, batch, time, heads, _, _, _, dk, dv = sizes
+    device, kept, fields = _attention_inputs(q, k, v, log_decay, 4)
+    _, batch, time, heads, _, _, _, dk, dv = fields[:9]
     _like(do, "do", q, device)
     if do.shape != (batch, time, heads, dv):
         raise ValueError(f"do has shape {tuple(do.shape)}, expected {(batch, time, heads, dv)}")
@@ -210,9 +210,9 @@ def linear_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     lengths = _lengths(lengths, batch, device)
     dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
     dinitial = None if initial_state is None else torch.empty_like(initial_state)
-    head = (*sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay),
-            _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, 0, *_NO_STRIDE, 0, _ptr(do),
-            *_strides(do), _ptr(dstate), _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dinitial), 0, 0, 0)
+    head = (*fields, _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, 0, 0, 0, 0, 0,
+            do.data_ptr(), *do.stride()[:3], _ptr(dstate), dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(),
+            _ptr(dinitial), 0, 0, 0)
     _run_attention("hx_linear_attention_grad", device, head, 1)
     return dq, dk_, dv_, dinitial
 
@@ -224,18 +224,17 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     v alike; state (n_slots, heads, dk, dv) fp32, contiguous, is updated in place.  Row i's state
     is slot slots[i] (int32, distinct; a slot outside 0..n_slots-1 leaves the row out and its
     output zero), slot i unless given.  Returns o (batch, heads, dv)."""
-    device, q, k, v, log_decay, sizes = _attention_inputs(q, k, v, log_decay, 3)
-    _, batch, _, heads, _, _, _, dk, dv = sizes
-    if _on_gpu(state, "state") != device or state.dtype != torch.float32 or not state.is_contiguous():
+    device, kept, fields = _attention_inputs(q, k, v, log_decay, 3)
+    _, batch, _, heads, _, _, _, dk, dv = fields[:9]
+    if _on_gpu(state, "state") != device or state.dtype is not torch.float32 or not state.is_contiguous():
         raise TypeError(f"state has to be a contiguous float32 tensor on {q.device}")
     if state.dim() != 4 or state.shape[1:] != (heads, dk, dv):
         raise ValueError(f"state has shape {tuple(state.shape)}, expected (n_slots, {heads}, {dk}, {dv})")
     slots = _array(slots, "slots", torch.int32, (batch,), device)
     o = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
-        *sizes, _ptr(q), _ptr(k), _ptr(v), *_strides(q), *_strides(k), *_strides(v), _ptr(log_decay), 0, 0,
-        dk ** -0.5 if scale is None else scale, _ptr(o), *_strides(o), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, _ptr(state),
-        _ptr(slots), state.shape[0], 0, 0, _stream(device)))
+        *fields, 0, 0, dk ** -0.5 if scale is None else scale, o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
+        0, 0, state.data_ptr(), _ptr(slots), state.shape[0], 0, 0, _stream(device)))
     return o
 
 

@@ -511,7 +511,7 @@ enum { HX_F32 = 0, HX_F16 = 1, HX_BF16 = 2 };
  * past a sequence's length are zero, whatever its inputs hold there.  Head h reads head
  * h q_heads / heads of q, and so on: q_heads, k_heads and v_heads each divide heads.
  * g = log_decay[h] is at most 0 (-inf: no memory).  States are (batch, heads, dk, dv) fp32,
- * contiguous.  dk and dv are at most 256. */
+ * contiguous.  dk and dv are at most 256, batch x heads 2^20, time 2^30. */
 typedef struct hx_attention_args {
     int64_t type, batch, time, heads, q_heads, k_heads, v_heads, dk, dv;
     const void *q, *k, *v;                                /* (batch, time, heads of each, d) */
@@ -557,7 +557,7 @@ int hx_linear_attention_step(const hx_attention_args* args);
  * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself. */
 typedef struct hx_distill_args {
     int64_t type, teacher_type, index_bits;               /* index_bits 32 or 64 */
-    int64_t rows, vocab, top;                             /* vocab <= 2^20, top <= 2048 */
+    int64_t rows, vocab, top;                             /* at most 2^21, 2^20 and 2048 */
     const void* logits;
     int64_t logits_stride;
     const void* index;
@@ -583,7 +583,7 @@ int hx_distill_loss(const hx_distill_args* args);
  * takes the largest logit.  NaN counts as -inf; a row of nothing but -inf gives token -1 and
  * logprob -inf.  Each setting is an array (rows) or, where that is NULL, one value. */
 typedef struct hx_sample_args {
-    int64_t type, rows, vocab;
+    int64_t type, rows, vocab;                            /* rows at most 2^21, vocab 2^22 */
     const void* logits;
     int64_t logits_stride;
     const float* u;

@@ -286,3 +286,32 @@ def test_decays_are_clamped_like_the_recurrence():
     o, end = readout.linear_attention(q, k, v, g)
     want = ref.attention(q, k, v, g, 0.25)
     assert ref.rel(o, want[0]) <= bound(torch.float32) and ref.rel(end, want[1]) <= bound(torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_past_32_bits(dtype):
+    """Sequences 2^31 elements apart, steps 2^24 apart, and a state pool of over 2^31 values."""
+    far = 2 ** 31 + 64
+    space = torch.empty(far + 40 * 2 ** 24 + 64, dtype=dtype, device="cuda")
+    gen = torch.Generator().manual_seed(37)
+    q, k, v = (torch.randn(2, 40, 1, 16, generator=gen).to(dtype).cuda() for _ in range(3))
+    apart = []
+    for n, x in enumerate((q, k, v)):
+        y = space.as_strided(x.shape, (far, 2 ** 24, 16, 1), 16 * n)
+        y.copy_(x)
+        apart.append(y)
+    g = torch.tensor([-0.05], device="cuda")
+    near, far_ = readout.linear_attention(q, k, v, g), readout.linear_attention(*apart, g)
+    assert all(torch.equal(a, b) for a, b in zip(near, far_))
+    do = torch.randn(2, 40, 1, 16, generator=gen).to(dtype).cuda()
+    near, far_ = readout.linear_attention_grad(q, k, v, g, do), readout.linear_attention_grad(*apart, g, do)
+    assert all(torch.equal(a, b) for a, b in zip(near[:3], far_[:3]))
+    del space, apart, y
+    pool = torch.empty(2 ** 31 // (128 * 128) + 3, 1, 128, 128, device="cuda")
+    slots = torch.tensor([pool.shape[0] - 1, 0], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(2, 1, 128, generator=gen).to(dtype).cuda() for _ in range(3))
+    state = torch.randn(2, 1, 128, 128, generator=gen).cuda()
+    pool[slots.long()] = state
+    o = readout.linear_attention_step(q, k, v, g, pool, slots=slots)
+    assert torch.equal(o, readout.linear_attention_step(q, k, v, g, state))
+    assert torch.equal(pool[slots.long()], state)

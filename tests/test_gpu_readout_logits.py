@@ -286,3 +286,17 @@ def test_sample_strides():
     check_draws(x, u, 1.0, 30, 0.8, 0.0)
     flipped = x.t().contiguous().t()            # last dimension not contiguous
     assert all(torch.equal(p, q) for p, q in zip(readout.sample(flipped, u, top_k=30, top_p=0.8), a))
+
+
+def test_rows_more_than_32_bits_apart():
+    far = 2 ** 31 + 24
+    space = torch.empty(far + 5000, dtype=torch.bfloat16, device="cuda")
+    x, index, t, lse, weight = problem(9, torch.bfloat16, 2, 5000, 12, 1.0)
+    apart = space.as_strided(x.shape, (far, 1))
+    apart.copy_(x)
+    near = readout.distill_loss_grad(x, index, t, teacher_lse=lse, weight=weight)
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    drawn = readout.sample(x, u, top_p=0.9)
+    assert all(torch.equal(a, b) for a, b in zip(readout.sample(apart, u, top_p=0.9), drawn))
+    loss, grad = readout.distill_loss_grad(apart, index, t, teacher_lse=lse, weight=weight, out=apart)
+    assert torch.equal(loss, near[0]) and torch.equal(grad, near[1])
