@@ -120,12 +120,14 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
 // What bounds it, bf16, 65536 steps of 8 heads of 128 x 128 (537 MB, 113 us at a copy's rate):
 // 69 us for the segments' states (3.9 TB/s), 15 to join them, 136 for the rest, in which a wave
 // issues 2500 cycles of matrix and 3200 of other instructions a chunk, two waves a SIMD: neither
-// memory nor matrix cores are full, barriers and LDS reads lie between.  fp32 matrix instructions
-// take 16 times as long: there they bound it.
+// memory nor matrix cores are full, barriers and LDS reads lie between.  Short sequences are
+// chains of chunks, 4 to 8 us each (777 steps of 13 x 12 sequences and heads, 96 x 80 in fp16: 31,
+// 6 and 69 us).  fp32 matrix instructions take 16 times as long: there they bound it.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // Reduction indices are taken 32 at a time, eight a lane; which eight is free as long as both
 // operands agree, and is chosen so that every LDS access is whole and without bank conflicts
@@ -136,9 +138,11 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 // fp32: its weighted c enters as three bf16 terms (24 bits).
 struct MathBf16 {
     using Elem = __bf16;
+    using Raw = bf16x8;
     using Frag = bf16x4;
     using Pair = bf16x8;
-    static constexpr int kC = 64, kPiece = 8, kTerms = 3;
+    using Term = bf16x4;
+    static constexpr int kC = 64, kPiece = 8, kPlanes = 1, kTerms = 3;
     static constexpr int kPadA = 8, kPadB = 0, kPadC = 16, kPadP = 8;
     static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
@@ -148,13 +152,28 @@ struct MathBf16 {
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) {
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    // b times weighted c in terms
+    static __device__ __forceinline__ Term term(f32x4 x) { return frag(x); }
+    static __device__ __forceinline__ f32x4 wide_term(Term x) { return wide(x); }
+    static __device__ __forceinline__ f32x4 mma_terms(f32x4 acc, Pair b, const Term (&w0)[kTerms], const Term (&w1)[kTerms]) {
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) acc = mma(acc, b, pair(w0[t], w1[t]));
+        return acc;
+    }
+    // pieces and fragments to LDS (arrays of several planes: kPlane from one to the next)
+    template <int kPlane>
+    static __device__ __forceinline__ void store(Elem* at, Raw x) { *reinterpret_cast<Raw*>(at) = x; }
+    template <int kPlane>
+    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) { *reinterpret_cast<Frag*>(at) = x; }
     // State row (a's and b's column) that accumulator rows g4 .. + 3 of tile rt hold: tiles 2K and
     // 2K + 1 take turns of four in 32 columns, so that a lane's eight are neighbours in a.
     static __device__ __forceinline__ int row(int rt, int g4) { return rt / 2 * 32 + g4 * 2 + rt % 2 * 4; }
     // a in rows: eight neighbours, against the state; or the eight that lie together in b, against b.
+    template <int kPlane>
     static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
         return *reinterpret_cast<const Pair*>(row + k * 32 + g4 * 2);
     }
+    template <int kPlane>
     static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) {
         const Elem* at = row + k * 32 + g4 / 4 % 2 * 16 + g4 / 8 * 4;
         return pair(*reinterpret_cast<const Frag*>(at), *reinterpret_cast<const Frag*>(at + 8));
@@ -188,24 +207,114 @@ struct MathBf16 {
     static __device__ __forceinline__ Frag b_column(const Elem* lb, int sb, int rt, int lane) {
         return turned(lb + b_at<kDA>(sb * 16 + 4 * (lane / 16) + lane % 16 / 4, rt * 16 + 4 * (lane % 4)));
     }
+    template <int kPlane>
     static __device__ __forceinline__ Frag c_column(const Elem* lc, int stride, int sb, int col, int lane) {
         return turned(lc + (sb * 16 + 4 * (lane / 16) + lane % 16 / 4) * stride + col + 4 * (lane % 4));
     }
     // P's columns in the order that c's column fragments have
     static __device__ __forceinline__ int p_at(int sb, int g4) { return sb / 2 * 32 + g4 * 2 + sb % 2 * 4; }
+    template <int kPlane>
     static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
         return *reinterpret_cast<const Pair*>(row + p_at(sb, g4));
     }
 };
 
-// fp32 and fp16 inputs, in fp32 throughout (fp16's range would not hold P or the states).
+// fp16 inputs: each exactly the sum of two bf16 numbers (8 and 3 bits; fp16 itself has not the
+// range that P and states need), held in LDS as two planes.  P and the state as it enters y are
+// two bf16 terms, good to 2^-17; of four products of terms the three larger ones are made, five
+// of six in the state's update, which misses 2^-25 (13 x 777 steps, 12 heads of 96 x 80: 99 us, with
+// fp32 instructions 117).  An infinite input gives NaN where it would give infinity.
+struct MathF16 {
+    using One = MathBf16;
+    using Elem = __bf16;
+    using Raw = f16x8;
+    struct Frag {
+        bf16x4 h, l;
+    };
+    struct Pair {
+        bf16x8 h, l;
+    };
+    using Term = bf16x4;
+    static constexpr int kC = 32, kPiece = 8, kPlanes = 2, kTerms = 3;
+    static constexpr int kPadA = One::kPadA, kPadB = One::kPadB, kPadC = One::kPadC, kPadP = One::kPadP;
+    static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
+        return One::mma(One::mma(One::mma(acc, a.h, b.l), a.l, b.h), a.h, b.h);
+    }
+    static __device__ __forceinline__ Frag frag(f32x4 x) {
+        const bf16x4 h = One::frag(x);
+        return {h, One::frag(x - One::wide(h))};
+    }
+    static __device__ __forceinline__ f32x4 wide(Frag x) { return One::wide(x.h) + One::wide(x.l); }
+    static __device__ __forceinline__ Pair pair(Frag a, Frag b) { return {One::pair(a.h, b.h), One::pair(a.l, b.l)}; }
+    static __device__ __forceinline__ Term term(f32x4 x) { return One::frag(x); }
+    static __device__ __forceinline__ f32x4 wide_term(Term x) { return One::wide(x); }
+    static __device__ __forceinline__ f32x4 mma_terms(f32x4 acc, Pair b, const Term (&w0)[kTerms], const Term (&w1)[kTerms]) {
+#pragma unroll
+        for (int t = kTerms - 1; t >= 0; --t) {
+            const bf16x8 w = One::pair(w0[t], w1[t]);
+            if (t < kTerms - 1) acc = One::mma(acc, b.l, w);
+            acc = One::mma(acc, b.h, w);
+        }
+        return acc;
+    }
+    static __device__ __forceinline__ Pair split(Raw x) {
+        typedef float f32x8 __attribute__((ext_vector_type(8)));
+        const f32x8 w = __builtin_convertvector(x, f32x8);
+        const bf16x8 h = __builtin_convertvector(w, bf16x8);
+        return {h, __builtin_convertvector(w - __builtin_convertvector(h, f32x8), bf16x8)};
+    }
+    template <int kPlane>
+    static __device__ __forceinline__ void store(Elem* at, Raw x) {
+        const Pair p = split(x);
+        One::store<0>(at, p.h), One::store<0>(at + kPlane, p.l);
+    }
+    template <int kPlane>
+    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) {
+        One::store_frag<0>(at, x.h), One::store_frag<0>(at + kPlane, x.l);
+    }
+    static __device__ __forceinline__ int row(int rt, int g4) { return One::row(rt, g4); }
+    template <int kPlane>
+    static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
+        return {One::a_pair<0>(row, k, g4), One::a_pair<0>(row + kPlane, k, g4)};
+    }
+    template <int kPlane>
+    static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) {
+        return {One::a_like_b<0>(row, k, g4), One::a_like_b<0>(row + kPlane, k, g4)};
+    }
+    template <int kDA>
+    static __device__ __forceinline__ Pair b_pair(const Elem* lb, int row, int k, int g4) {
+        return {One::b_pair<kDA>(lb, row, k, g4), One::b_pair<kDA>(lb + kC * kDA, row, k, g4)};
+    }
+    template <int kDA>
+    static __device__ __forceinline__ void b_store(Elem* lb, int row, int col, Raw x) {
+        const Pair p = split(x);
+        One::b_store<kDA>(lb, row, col, p.h), One::b_store<kDA>(lb + kC * kDA, row, col, p.l);
+    }
+    template <int kDA>
+    static __device__ __forceinline__ Frag b_column(const Elem* lb, int sb, int rt, int lane) {
+        return {One::b_column<kDA>(lb, sb, rt, lane), One::b_column<kDA>(lb + kC * kDA, sb, rt, lane)};
+    }
+    template <int kPlane>
+    static __device__ __forceinline__ Frag c_column(const Elem* lc, int stride, int sb, int col, int lane) {
+        return {One::c_column<0>(lc, stride, sb, col, lane), One::c_column<0>(lc + kPlane, stride, sb, col, lane)};
+    }
+    static __device__ __forceinline__ int p_at(int sb, int g4) { return One::p_at(sb, g4); }
+    template <int kPlane>
+    static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
+        return {One::p_pair<0>(row, sb, g4), One::p_pair<0>(row + kPlane, sb, g4)};
+    }
+};
+
+// fp32 inputs, in fp32 throughout.
 struct MathF32 {
     using Elem = float;
+    using Raw = f32x4;
     using Frag = f32x4;
     struct Pair {
         f32x4 x[2];
     };
-    static constexpr int kC = 32, kPiece = 4, kTerms = 1;
+    using Term = f32x4;
+    static constexpr int kC = 32, kPiece = 4, kPlanes = 1, kTerms = 1;
     static constexpr int kPadA = 4, kPadB = 4, kPadC = 4, kPadP = 4;
     static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
 #pragma unroll
@@ -217,38 +326,51 @@ struct MathF32 {
     static __device__ __forceinline__ Frag frag(f32x4 x) { return x; }
     static __device__ __forceinline__ f32x4 wide(Frag x) { return x; }
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) { return {a, b}; }
+    static __device__ __forceinline__ Term term(f32x4 x) { return x; }
+    static __device__ __forceinline__ f32x4 wide_term(Term x) { return x; }
+    static __device__ __forceinline__ f32x4 mma_terms(f32x4 acc, Pair b, const Term (&w0)[kTerms], const Term (&w1)[kTerms]) {
+        return mma(acc, b, pair(w0[0], w1[0]));
+    }
+    template <int kPlane>
+    static __device__ __forceinline__ void store(Elem* at, Raw x) { *reinterpret_cast<Raw*>(at) = x; }
+    template <int kPlane>
+    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) { *reinterpret_cast<Frag*>(at) = x; }
     static __device__ __forceinline__ int row(int rt, int g4) { return rt * 16 + g4; }
+    template <int kPlane>
     static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
         return {*reinterpret_cast<const Frag*>(row + k * 32 + g4), *reinterpret_cast<const Frag*>(row + k * 32 + 16 + g4)};
     }
-    static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) { return a_pair(row, k, g4); }
+    template <int kPlane>
+    static __device__ __forceinline__ Pair a_like_b(const Elem* row, int k, int g4) { return a_pair<0>(row, k, g4); }
     template <int kDA>
     static __device__ __forceinline__ Pair b_pair(const Elem* lb, int row, int k, int g4) {
-        return a_pair(lb + row * (kDA + kPadB), k, g4);
+        return a_pair<0>(lb + row * (kDA + kPadB), k, g4);
     }
     template <int kDA>
     static __device__ __forceinline__ void b_store(Elem* lb, int row, int col, Frag x) {
         *reinterpret_cast<Frag*>(lb + row * (kDA + kPadB) + col) = x;
     }
+    template <int kPlane>
     static __device__ __forceinline__ Frag c_column(const Elem* lc, int stride, int sb, int col, int lane) {
         const Elem* at = lc + (sb * 16 + 4 * (lane / 16)) * stride + col + lane % 16;
         return Frag{at[0], at[stride], at[2 * stride], at[3 * stride]};
     }
     template <int kDA>
     static __device__ __forceinline__ Frag b_column(const Elem* lb, int sb, int rt, int lane) {
-        return c_column(lb, kDA + kPadB, sb, rt * 16, lane);
+        return c_column<0>(lb, kDA + kPadB, sb, rt * 16, lane);
     }
     static __device__ __forceinline__ int p_at(int sb, int g4) { return sb * 16 + g4; }
+    template <int kPlane>
     static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
         return {*reinterpret_cast<const Frag*>(row + sb * 16 + g4),
                 *reinterpret_cast<const Frag*>(row + sb * 16 + 16 + g4)};
     }
 };
 
-template <class T> struct InputOf;      // math, and a piece of a row as it is loaded
-template <> struct InputOf<float> { static constexpr int kType = HX_F32; using Math = MathF32; using Elem = float; using Raw = f32x4; using Four = f32x4; };
-template <> struct InputOf<__half> { static constexpr int kType = HX_F16; using Math = MathF32; using Elem = _Float16; using Raw = f16x4; using Four = f16x4; };
-template <> struct InputOf<__hip_bfloat16> { static constexpr int kType = HX_BF16; using Math = MathBf16; using Elem = __bf16; using Raw = bf16x8; using Four = bf16x4; };
+template <class T> struct InputOf;      // the products' mathematics, the input's type and four of them
+template <> struct InputOf<float> { static constexpr int kType = HX_F32; using Math = MathF32; using Elem = float; using Four = f32x4; };
+template <> struct InputOf<__half> { static constexpr int kType = HX_F16; using Math = MathF16; using Elem = _Float16; using Four = f16x4; };
+template <> struct InputOf<__hip_bfloat16> { static constexpr int kType = HX_BF16; using Math = MathBf16; using Elem = __bf16; using Four = bf16x4; };
 
 // Rows [0, n) of a chunk into registers, kD columns padded with zeros, R rows a round of the
 // workgroup.  kWhole: d is a whole number of pieces and a round's rows are within 2 GiB, so that
@@ -260,9 +382,10 @@ template <class T, int kD, int kT, bool kWhole>
 struct Tile {
     using In = InputOf<T>;
     using Math = typename In::Math;
-    static constexpr int kP = Math::kPiece, kRowPieces = kD / kP, kRows = kT / kRowPieces, kN = Math::kC / kRows;
-    static_assert(kRows * kRowPieces == kT && kN * kRows == Math::kC, "whole rounds of rows");
-    typedef typename In::Raw Raw;
+    static constexpr int kP = Math::kPiece, kRowPieces = kD / kP, kRows = kT / kRowPieces;
+    static constexpr int kN = kRows < Math::kC ? Math::kC / kRows : 1;
+    static_assert(kRows * kRowPieces == kT && (kN * kRows == Math::kC || kN == 1), "whole rounds of rows");
+    typedef typename Math::Raw Raw;
     typedef Raw Any __attribute__((aligned(sizeof(T))));
     Raw raw[kN];
     const T* base;          // row 0 of the sequence (reverse: row R - 1 of a round that starts there)
@@ -303,10 +426,10 @@ struct Tile {
     // put(row, column, piece) for the pieces of this thread
     template <class F>
     __device__ __forceinline__ void store(F put) const {
-        typedef typename Math::Elem Out __attribute__((ext_vector_type(kP)));
         const int i = threadIdx.x / kRowPieces, j = threadIdx.x % kRowPieces * kP;
 #pragma unroll
-        for (int p = 0; p < kN; ++p) put(i + p * kRows, j, __builtin_convertvector(raw[p], Out));
+        for (int p = 0; p < kN; ++p)
+            if (kRows <= Math::kC || i < Math::kC) put(i + p * kRows, j, raw[p]);
     }
 };
 
@@ -351,10 +474,11 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     using Frag = typename M::Frag;
     constexpr int kC = M::kC, kB = kC / 16, kT = kW * 64, kDC = kW * kCT * 16, kRT = kDA / 16;
     using Pair = typename M::Pair;
-    typedef Elem Piece __attribute__((ext_vector_type(M::kPiece)));
+    using Raw = typename M::Raw;
     constexpr int kSA = kDA + M::kPadA, kSB = kDA + M::kPadB, kSC = kDC + M::kPadC, kSP = kC + M::kPadP, kK = kRT / 2;
-    __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kC * kSA], lb[kC * kSB], lc[kC * kSC],
-        lp[kStates ? 1 : kC * kSP];
+    constexpr int kPlaneA = kC * kSA, kPlaneC = kC * kSC, kPlaneP = kC * kSP, kPlanes = M::kPlanes;
+    __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kPlaneA * kPlanes], lb[kC * kSB * kPlanes],
+        lc[kPlaneC * kPlanes], lp[kStates ? 1 : kPlaneP * kPlanes];
     // the chunk's decays, made once: of P's blocks tb - sb + 1 blocks under the diagonal (the first:
     // over it, nothing) as a lane holds them; of the entering state; of what enters at a step
     __shared__ f32x4 lfactor[kStates ? 1 : (kB + 1) * 64], lleft[kC / 4];
@@ -469,9 +593,9 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
         __syncthreads();                       // the chunk before is done with
         if (n < kC) make_left(n);
         if constexpr (!kStates)
-            ta.store([&](int i, int col, Piece x) { *reinterpret_cast<Piece*>(la + i * kSA + col) = x; });
-        tb.store([&](int i, int col, Piece x) { M::template b_store<kDA>(lb, i, col, x); });
-        tc.store([&](int i, int col, Piece x) { *reinterpret_cast<Piece*>(lc + i * kSC + col) = x; });
+            ta.store([&](int i, int col, Raw x) { M::template store<kPlaneA>(la + i * kSA + col, x); });
+        tb.store([&](int i, int col, Raw x) { M::template b_store<kDA>(lb, i, col, x); });
+        tc.store([&](int i, int col, Raw x) { M::template store<kPlaneC>(lc + i * kSC + col, x); });
         __syncthreads();
         // whether columns 32 k .. of a and b are there, and the wave's column tile ct
         auto there = [&](int k) { return kFull || k * 32 < S.da; };
@@ -493,7 +617,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                         Pair pa;
 #pragma unroll
                         for (int e = 0; e < kEach; ++e) {
-                            if (e % kB == 0) pa = M::a_like_b(la + ((block0 + e) / kB * 16 + r) * kSA, k, g4);
+                            if (e % kB == 0) pa = M::template a_like_b<kPlaneA>(la + ((block0 + e) / kB * 16 + r) * kSA, k, g4);
                             p[e] = M::mma(p[e], M::template b_pair<kDA>(lb, (block0 + e) % kB * 16 + r, k, g4), pa);
                         }
                     }
@@ -502,14 +626,14 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                 for (int e = 0; e < kEach; ++e) {
                     const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
                     p[e] *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
-                    *reinterpret_cast<Frag*>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4)) = M::frag(p[e]);
+                    M::template store_frag<kPlaneP>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4), M::frag(p[e]));
                 }
             }
         }
 #pragma unroll
         for (int sb = 0; sb < kB; ++sb)
 #pragma unroll
-            for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::c_column(lc, kSC, sb, mine + ct * 16, lane);
+            for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::template c_column<kPlaneC>(lc, kSC, sb, mine + ct * 16, lane);
         if constexpr (!kStates) {
             __syncthreads();                   // P is whole
             // two blocks of steps at a time: what the entering state adds, then the chunk's own steps
@@ -526,7 +650,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                     if (there(k)) {
                         Pair pa[2];
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) pa[t] = M::a_pair(la + ((t0 + t) * 16 + r) * kSA, k, g4);
+                        for (int t = 0; t < 2; ++t) pa[t] = M::template a_pair<kPlaneA>(la + ((t0 + t) * 16 + r) * kSA, k, g4);
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct) {
                             const Pair x = M::pair(M::frag(X[2 * k][ct]), M::frag(X[2 * k + 1][ct]));
@@ -541,7 +665,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                     for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
 #pragma unroll
                     for (int sb = 0; sb <= t0 + t; sb += 2) {
-                        const Pair pp = M::p_pair(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
+                        const Pair pp = M::template p_pair<kPlaneP>(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct)
                             y[t][ct] = M::mma(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp);
@@ -576,7 +700,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
         for (int sb = 0; sb < kB; sb += 2) {
             if (sb == kB - 2 && i0 + kC < end) fetch(i0 + kC, 1);
             if (!column(0)) continue;
-            Frag wc[M::kTerms][2][kCT];
+            typename M::Term wc[2][kCT][M::kTerms];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const f32x4 w0 = lleft[(sb + e) * 4 + g4 / 4];
@@ -585,8 +709,8 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                     f32x4 w = M::wide(c[sb + e][ct]) * w0;
 #pragma unroll
                     for (int k = 0; k < M::kTerms; ++k) {
-                        wc[k][e][ct] = M::frag(w);
-                        w -= M::wide(wc[k][e][ct]);
+                        wc[e][ct][k] = M::term(w);
+                        w -= M::wide_term(wc[e][ct][k]);
                     }
                 }
             }
@@ -599,9 +723,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                                                M::template b_column<kDA>(lb, sb + 1, rt, lane));
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct)
-#pragma unroll
-                            for (int t = 0; t < M::kTerms; ++t)
-                                X[rt][ct] = M::mma(X[rt][ct], b, M::pair(wc[t][0][ct], wc[t][1][ct]));
+                            X[rt][ct] = M::mma_terms(X[rt][ct], b, wc[0][ct], wc[1][ct]);
                     }
                 }
         }
@@ -696,7 +818,7 @@ Cut cut_of(int64_t type, int64_t da, int64_t dc) {
         // 128 columns: in bf16 two tiles a wave (LDS reads serve twice: 165 us for 65536 steps, 8
         // heads, 128 x 128, against 200 with eight waves of one); fp32 products take so much longer
         // that more waves pay instead (777 steps, 156 sequences and heads: 114 us against 123)
-        if (type == HX_BF16) {
+        if (type != HX_F32) {
             c.tiles = 2;
         } else {
             c.waves = 8;
@@ -715,7 +837,8 @@ struct Segments {
 };
 
 Segments segments_of(const hx_attention_args& A) {
-    const int chunk = A.type == HX_BF16 ? MathBf16::kC : MathF32::kC, width = cut_of(A.type, A.dk, A.dv).width();
+    const int chunk = with_type(A.type, [](auto t) { return InputOf<decltype(t)>::Math::kC; });
+    const int width = cut_of(A.type, A.dk, A.dv).width();
     const int64_t units = A.batch * A.heads * ((A.dv + width - 1) / width);
     const int64_t chunks = std::max<int64_t>(1, (A.time + chunk - 1) / chunk);
     const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(units, 1), chunks / 2);
@@ -768,7 +891,7 @@ hipError_t launch_chunks(ChunkArgs A, int jobs, bool states, long long bh, hipSt
         constexpr int kDA = decltype(rows)::value;
         constexpr bool kWhole = decltype(whole)::value, kFull = decltype(fills)::value;
         if (c.waves == 2) return launch_cut<T, kDA, 2, 1, kWhole, kFull>(A, jobs, states, bh, st);
-        if constexpr (std::is_same_v<typename InputOf<T>::Math, MathBf16>) {
+        if constexpr (InputOf<T>::kType != HX_F32) {
             if constexpr (kDA < 256)
                 if (c.tiles == 2) return launch_cut<T, kDA, 4, 2, kWhole, kFull>(A, jobs, states, bh, st);
         } else if constexpr (kDA == 64 || kDA == 128) {

@@ -160,7 +160,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Returns o (batch, time, heads, dv) of q's type and the state at each sequence's end.
 
     Within a sequence a non-finite k or v may reach outputs of up to 63 steps before it (chunks
-    of steps are products of matrices).
+    of steps are products of matrices), and may do so as NaN.
     """
     device, kept, fields = _attention_inputs(q, k, v, log_decay, 4)
     _, batch, time, heads, _, _, _, dk, dv = fields[:9]
