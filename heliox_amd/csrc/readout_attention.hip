@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
 //
 // What bounds it, bf16, 65536 steps of 8 heads of 128 x 128 (537 MB, 113 us at a copy's rate):
 // 69 us for the segments' states (3.9 TB/s), 15 to join them, 136 for the rest, in which a wave
-// issues 2500 cycles of matrix and 3200 of other instructions a chunk, two waves a SIMD: neither
+// issues 2500 cycles of matrix and 2400 of other instructions a chunk, two waves a SIMD: neither
 // memory nor matrix cores are full, barriers and LDS reads lie between.  Short sequences are
 // chains of chunks, 4 to 8 us each (777 steps of 13 x 12 sequences and heads, 96 x 80 in fp16: 31,
 // 6 and 69 us).  fp32 matrix instructions take 16 times as long: there they bound it.
