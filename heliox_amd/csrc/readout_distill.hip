@@ -20,14 +20,14 @@ template <> struct PieceOf<__hip_bfloat16> { typedef __bf16 Vec __attribute__((e
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // x reduced over the workgroup's waves; every thread gets the result.
-template <int kThreads, class F>
-__device__ __forceinline__ float block_reduce(float x, float* sh, F op) {
+template <int kThreads, class V, class F>
+__device__ __forceinline__ V block_reduce(V x, double* sh, F op) {
     for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
     __syncthreads();
     if (threadIdx.x % 64 == 0) sh[threadIdx.x / 64] = x;
     __syncthreads();
-    x = sh[0];
-    for (int w = 1; w < kThreads / 64; ++w) x = op(x, sh[w]);
+    x = static_cast<V>(sh[threadIdx.x % (kThreads / 64)]);
+    for (int m = kThreads / 128; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
     return x;
 }
 
@@ -40,13 +40,14 @@ __device__ __forceinline__ int entry(const void* index, long long at, int vocab)
 // LDS: places and teacher's shares of the row's entries, the student's logits there, and, where
 // the rest is one class, one bit for each place of the vocabulary that holds an entry.
 // Weights are 2^((x - max) cold), cold = log2 e / temperature: the difference comes first, so
-// that an error of the product is one of the small difference and not of the logit.
+// that an error of the product is one of the small difference and not of the logit.  What the
+// few entries take, logarithms that nearly cancel, is 64 bits wide; per = 1 / temperature.
 template <class T, class U, class I, int kThreads, bool kRest>
-__global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float cold) {
+__global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, float cold, double per) {
     using Vec = typename PieceOf<T>::Vec;
     constexpr int kP = sizeof(Vec) / sizeof(T);
     extern __shared__ int lds[];
-    __shared__ float red[kThreads / 64];
+    __shared__ double red[kThreads / 64];
     const int top = static_cast<int>(A.top), vocab = static_cast<int>(A.vocab);
     int* place = lds;
     float* share = reinterpret_cast<float*>(lds + top);
@@ -56,8 +57,11 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
     const T* x = static_cast<const T*>(A.logits) + row * A.logits_stride;
     const U* t = static_cast<const U*>(A.teacher) + row * A.teacher_stride;
     const float tau = static_cast<float>(A.temperature);
-    auto add = [](float a, float b) { return a + b; };
+    auto add = [](auto a, auto b) { return a + b; };
     auto most = [](float a, float b) { return fmaxf(a, b); };
+    const float per_f = static_cast<float>(per);
+    // fp32 logits have the time for the exact exponential (14 instructions; 16 bits a place have not)
+    auto weight = [&](float d) { return sizeof(T) == 4 ? expf(d * per_f) : pow2(d * cold); };
 
     if constexpr (kRest) {
         for (int w = threadIdx.x; w < (vocab + 31) / 32; w += kThreads) member[w] = 0;
@@ -67,7 +71,7 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
     for (int k = threadIdx.x; k < top; k += kThreads) {
         const int j = entry<I>(A.index, row * A.index_stride + k, vocab);
         place[k] = j;
-        share[k] = j >= 0 ? to_f32(t[k]) / tau : -INFINITY;
+        share[k] = j >= 0 ? to_f32(t[k]) : -INFINITY;
         logit[k] = j >= 0 ? to_f32(x[j]) : 0.f;
         if (j >= 0) {
             some = 1.f;
@@ -87,7 +91,7 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
         for (int i = 1; i < kP; ++i)
             if (i < n) c = fmaxf(c, v[i]);
         if (c > m) {
-            const float keep = pow2((m - c) * cold);     // m = -inf: 0
+            const float keep = weight(m - c);     // m = -inf: 0
             z *= keep;
             others *= keep;
             m = c;
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
         float e[kP], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-            e[i] = i < n ? pow2((v[i] - from) * cold) : 0.f;
+            e[i] = i < n ? weight(v[i] - from) : 0.f;
             sum += e[i];
         }
         z += sum;
@@ -143,49 +147,50 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
     const float mine = m;
     m = block_reduce<kThreads>(m, red, most);
     if (m == -INFINITY) m = 0.f;
-    const float scale = pow2((mine - m) * cold);
-    z = block_reduce<kThreads>(z * scale, red, add);
-    if constexpr (kRest) others = block_reduce<kThreads>(others * scale, red, add);
-    const float logz = logf(z);
+    const float scale = weight(mine - m);
+    const double whole = block_reduce<kThreads>(static_cast<double>(z * scale), red, add), logz = log(whole);
+    double rest = 0.;
+    if constexpr (kRest) rest = block_reduce<kThreads>(static_cast<double>(others * scale), red, add);
 
     // the teacher's shares and the row's loss
-    float norm;
+    double norm;
     if constexpr (kRest) {
         norm = A.teacher_lse[row];
     } else {
         float mass = 0.f;
         for (int k = threadIdx.x; k < top; k += kThreads)
-            if (share[k] != -INFINITY) mass += share[k] == tmax ? 1.f : expf(share[k] - tmax);
-        norm = tmax + logf(block_reduce<kThreads>(mass, red, add));
+            if (share[k] != -INFINITY) mass += share[k] == tmax ? 1.f : expf((share[k] - tmax) / tau);
+        norm = tmax * per + log(static_cast<double>(block_reduce<kThreads>(mass, red, add)));
     }
-    float loss = 0.f, psum = 0.f;
+    double loss = 0., psum = 0.;
     for (int k = threadIdx.x; k < top; k += kThreads) {
         float p = 0.f;
         if (share[k] != -INFINITY) {
-            const float logp = share[k] - norm;
-            p = expf(logp);
-            if (p != 0.f) loss += p * (logp - ((logit[k] - m) / tau - logz));
+            const double logp = share[k] * per - norm;
+            p = expf(static_cast<float>(logp));
+            if (p != 0.f) loss += p * (logp - ((static_cast<double>(logit[k]) - m) * per - logz));
         }
         share[k] = p;
         psum += p;
     }
     loss = block_reduce<kThreads>(loss, red, add);
     psum = block_reduce<kThreads>(psum, red, add);
-    float inside = psum, outside = psum;
+    double inside = psum, outside = psum;
     if constexpr (kRest) {
-        const float pr = fmaxf(0.f, 1.f - psum), qr = others / z;
-        if (pr > 0.f && qr > 0.f) {
-            loss += pr * (logf(pr) - logf(qr));
+        const double pr = fmax(0., 1. - psum), qr = rest / whole;
+        if (pr > 0. && qr > 0.) {
+            loss += pr * log(pr / qr);
             inside = psum + pr;
             outside = inside - pr / qr;
         }
     }
-    if (threadIdx.x == 0) A.loss[row] = some > 0.f ? loss * tau * tau : 0.f;
+    if (threadIdx.x == 0) A.loss[row] = some > 0.f ? static_cast<float>(loss * tau * tau) : 0.f;
     if (!A.grad) return;
     T* g = static_cast<T*>(A.grad) + row * A.grad_stride;
     const float w = some > 0.f ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
-    const float factor = w * outside / z;
-    auto slope = [&](float v) { return some > 0.f ? factor * pow2((v - m) * cold) : 0.f; };
+    const float factor = static_cast<float>(w * outside / whole),
+                within = static_cast<float>(inside / whole);
+    auto slope = [&](float v) { return some > 0.f ? factor * weight(v - m) : 0.f; };
     each_piece([&](int p, Vec raw) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) raw[i] = static_cast<decltype(raw[0] + raw[0])>(slope(static_cast<float>(raw[i])));
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) k_distill(hx_distill_args A, float c
                 p += share[i];
                 if (i < k) first = false;
             }
-        if (first) g[j] = from_f32<T>(w * (inside / z * pow2((logit[k] - m) * cold) - p));
+        if (first) g[j] = from_f32<T>(w * (within * weight(logit[k] - m) - p));
     }
 }
 
@@ -221,7 +226,7 @@ hipError_t launch(const hx_distill_args& A) {
         if (e != hipSuccess) return e;
     }
     kernel<<<static_cast<unsigned>(A.rows), kThreads, lds, static_cast<hipStream_t>(A.stream)>>>(
-        A, static_cast<float>(1.4426950408889634 / A.temperature));
+        A, static_cast<float>(1.4426950408889634 / A.temperature), 1.0 / A.temperature);
     return hipGetLastError();
 }
 
