@@ -134,15 +134,22 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // (two reads of 8 bytes where one of 16 does: 2400 of 4500 LDS cycles a chunk were conflicts).
 //
 // bf16 inputs: 32 indices an instruction.  Products of inputs are exact in fp32; P and the
-// state as it enters y are rounded to bf16 once, as y is afterwards.  The state itself stays
-// fp32: its weighted c enters as three bf16 terms (24 bits).
+// state as it enters y (Sum) are two bf16 terms, good to 2^-17, so that the only rounding of y
+// that counts is its own.  The state itself stays fp32: its weighted c enters as three bf16
+// terms (24 bits).
 struct MathBf16 {
     using Elem = __bf16;
     using Raw = bf16x8;
     using Frag = bf16x4;
     using Pair = bf16x8;
     using Term = bf16x4;
-    static constexpr int kC = 64, kPiece = 8, kPlanes = 1, kTerms = 3;
+    struct Sum {
+        bf16x4 h, l;
+    };
+    struct SumPair {
+        bf16x8 h, l;
+    };
+    static constexpr int kC = 64, kPiece = 8, kPlanes = 1, kPlanesP = 2, kTerms = 3;
     static constexpr int kPadA = 8, kPadB = 0, kPadC = 16, kPadP = 8;
     static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
@@ -152,6 +159,13 @@ struct MathBf16 {
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) {
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    static __device__ __forceinline__ Sum sum(f32x4 x) {
+        const Frag h = frag(x);
+        return {h, frag(x - wide(h))};
+    }
+    static __device__ __forceinline__ SumPair sum_pair(Sum a, Sum b) { return {pair(a.h, b.h), pair(a.l, b.l)}; }
+    static __device__ __forceinline__ f32x4 mma_sum(f32x4 acc, SumPair x, Pair a) { return mma(mma(acc, x.l, a), x.h, a); }
+    static __device__ __forceinline__ f32x4 mma_by_sum(f32x4 acc, Pair c, SumPair p) { return mma(mma(acc, c, p.l), c, p.h); }
     // b times weighted c in terms
     static __device__ __forceinline__ Term term(f32x4 x) { return frag(x); }
     static __device__ __forceinline__ f32x4 wide_term(Term x) { return wide(x); }
@@ -164,7 +178,10 @@ struct MathBf16 {
     template <int kPlane>
     static __device__ __forceinline__ void store(Elem* at, Raw x) { *reinterpret_cast<Raw*>(at) = x; }
     template <int kPlane>
-    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) { *reinterpret_cast<Frag*>(at) = x; }
+    static __device__ __forceinline__ void store_sum(Elem* at, Sum x) {
+        *reinterpret_cast<Frag*>(at) = x.h;
+        *reinterpret_cast<Frag*>(at + kPlane) = x.l;
+    }
     // State row (a's and b's column) that accumulator rows g4 .. + 3 of tile rt hold: tiles 2K and
     // 2K + 1 take turns of four in 32 columns, so that a lane's eight are neighbours in a.
     static __device__ __forceinline__ int row(int rt, int g4) { return rt / 2 * 32 + g4 * 2 + rt % 2 * 4; }
@@ -214,14 +231,14 @@ struct MathBf16 {
     // P's columns in the order that c's column fragments have
     static __device__ __forceinline__ int p_at(int sb, int g4) { return sb / 2 * 32 + g4 * 2 + sb % 2 * 4; }
     template <int kPlane>
-    static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
-        return *reinterpret_cast<const Pair*>(row + p_at(sb, g4));
+    static __device__ __forceinline__ SumPair p_pair(const Elem* row, int sb, int g4) {
+        return {*reinterpret_cast<const Pair*>(row + p_at(sb, g4)), *reinterpret_cast<const Pair*>(row + kPlane + p_at(sb, g4))};
     }
 };
 
 // fp16 inputs: each exactly the sum of two bf16 numbers (8 and 3 bits; fp16 itself has not the
 // range that P and states need), held in LDS as two planes.  P and the state as it enters y are
-// two bf16 terms, good to 2^-17; of four products of terms the three larger ones are made, five
+// two bf16 terms as they are for bf16; of four products of terms the three larger ones are made, five
 // of six in the state's update, which misses 2^-25 (13 x 777 steps, 12 heads of 96 x 80: 99 us, with
 // fp32 instructions 117).  An infinite input gives NaN where it would give infinity.
 struct MathF16 {
@@ -235,15 +252,17 @@ struct MathF16 {
         bf16x8 h, l;
     };
     using Term = bf16x4;
-    static constexpr int kC = 32, kPiece = 8, kPlanes = 2, kTerms = 3;
+    using Sum = One::Sum;
+    using SumPair = One::SumPair;
+    static constexpr int kC = 32, kPiece = 8, kPlanes = 2, kPlanesP = 2, kTerms = 3;
     static constexpr int kPadA = One::kPadA, kPadB = One::kPadB, kPadC = One::kPadC, kPadP = One::kPadP;
     static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
         return One::mma(One::mma(One::mma(acc, a.h, b.l), a.l, b.h), a.h, b.h);
     }
-    static __device__ __forceinline__ Frag frag(f32x4 x) {
-        const bf16x4 h = One::frag(x);
-        return {h, One::frag(x - One::wide(h))};
-    }
+    static __device__ __forceinline__ Sum sum(f32x4 x) { return One::sum(x); }
+    static __device__ __forceinline__ SumPair sum_pair(Sum a, Sum b) { return One::sum_pair(a, b); }
+    static __device__ __forceinline__ f32x4 mma_sum(f32x4 acc, SumPair x, Pair a) { return mma(acc, {x.h, x.l}, a); }
+    static __device__ __forceinline__ f32x4 mma_by_sum(f32x4 acc, Pair c, SumPair p) { return mma(acc, c, {p.h, p.l}); }
     static __device__ __forceinline__ f32x4 wide(Frag x) { return One::wide(x.h) + One::wide(x.l); }
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) { return {One::pair(a.h, b.h), One::pair(a.l, b.l)}; }
     static __device__ __forceinline__ Term term(f32x4 x) { return One::frag(x); }
@@ -269,9 +288,7 @@ struct MathF16 {
         One::store<0>(at, p.h), One::store<0>(at + kPlane, p.l);
     }
     template <int kPlane>
-    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) {
-        One::store_frag<0>(at, x.h), One::store_frag<0>(at + kPlane, x.l);
-    }
+    static __device__ __forceinline__ void store_sum(Elem* at, Sum x) { One::store_sum<kPlane>(at, x); }
     static __device__ __forceinline__ int row(int rt, int g4) { return One::row(rt, g4); }
     template <int kPlane>
     static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
@@ -300,9 +317,7 @@ struct MathF16 {
     }
     static __device__ __forceinline__ int p_at(int sb, int g4) { return One::p_at(sb, g4); }
     template <int kPlane>
-    static __device__ __forceinline__ Pair p_pair(const Elem* row, int sb, int g4) {
-        return {One::p_pair<0>(row, sb, g4), One::p_pair<0>(row + kPlane, sb, g4)};
-    }
+    static __device__ __forceinline__ SumPair p_pair(const Elem* row, int sb, int g4) { return One::p_pair<kPlane>(row, sb, g4); }
 };
 
 // fp32 inputs, in fp32 throughout.
@@ -314,7 +329,9 @@ struct MathF32 {
         f32x4 x[2];
     };
     using Term = f32x4;
-    static constexpr int kC = 32, kPiece = 4, kPlanes = 1, kTerms = 1;
+    using Sum = f32x4;
+    using SumPair = Pair;
+    static constexpr int kC = 32, kPiece = 4, kPlanes = 1, kPlanesP = 1, kTerms = 1;
     static constexpr int kPadA = 4, kPadB = 4, kPadC = 4, kPadP = 4;
     static __device__ __forceinline__ f32x4 mma(f32x4 acc, Pair a, Pair b) {
 #pragma unroll
@@ -323,9 +340,12 @@ struct MathF32 {
             for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[h][i], b.x[h][i], acc, 0, 0, 0);
         return acc;
     }
-    static __device__ __forceinline__ Frag frag(f32x4 x) { return x; }
     static __device__ __forceinline__ f32x4 wide(Frag x) { return x; }
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) { return {a, b}; }
+    static __device__ __forceinline__ Sum sum(f32x4 x) { return x; }
+    static __device__ __forceinline__ SumPair sum_pair(Sum a, Sum b) { return {a, b}; }
+    static __device__ __forceinline__ f32x4 mma_sum(f32x4 acc, SumPair x, Pair a) { return mma(acc, x, a); }
+    static __device__ __forceinline__ f32x4 mma_by_sum(f32x4 acc, Pair c, SumPair p) { return mma(acc, c, p); }
     static __device__ __forceinline__ Term term(f32x4 x) { return x; }
     static __device__ __forceinline__ f32x4 wide_term(Term x) { return x; }
     static __device__ __forceinline__ f32x4 mma_terms(f32x4 acc, Pair b, const Term (&w0)[kTerms], const Term (&w1)[kTerms]) {
@@ -334,7 +354,7 @@ struct MathF32 {
     template <int kPlane>
     static __device__ __forceinline__ void store(Elem* at, Raw x) { *reinterpret_cast<Raw*>(at) = x; }
     template <int kPlane>
-    static __device__ __forceinline__ void store_frag(Elem* at, Frag x) { *reinterpret_cast<Frag*>(at) = x; }
+    static __device__ __forceinline__ void store_sum(Elem* at, Sum x) { *reinterpret_cast<Frag*>(at) = x; }
     static __device__ __forceinline__ int row(int rt, int g4) { return rt * 16 + g4; }
     template <int kPlane>
     static __device__ __forceinline__ Pair a_pair(const Elem* row, int k, int g4) {
@@ -478,7 +498,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     constexpr int kSA = kDA + M::kPadA, kSB = kDA + M::kPadB, kSC = kDC + M::kPadC, kSP = kC + M::kPadP, kK = kRT / 2;
     constexpr int kPlaneA = kC * kSA, kPlaneC = kC * kSC, kPlaneP = kC * kSP, kPlanes = M::kPlanes;
     __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kPlaneA * kPlanes], lb[kC * kSB * kPlanes],
-        lc[kPlaneC * kPlanes], lp[kStates ? 1 : kPlaneP * kPlanes];
+        lc[kPlaneC * kPlanes], lp[kStates ? 1 : kPlaneP * M::kPlanesP];
     // the chunk's decays, made once: of P's blocks tb - sb + 1 blocks under the diagonal (the first:
     // over it, nothing) as a lane holds them; of the entering state; of what enters at a step
     __shared__ f32x4 lfactor[kStates ? 1 : (kB + 1) * 64], lleft[kC / 4];
@@ -626,7 +646,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                 for (int e = 0; e < kEach; ++e) {
                     const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
                     p[e] *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
-                    M::template store_frag<kPlaneP>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4), M::frag(p[e]));
+                    M::template store_sum<kPlaneP>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4), M::sum(p[e]));
                 }
             }
         }
@@ -636,42 +656,41 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
             for (int ct = 0; ct < kCT; ++ct) c[sb][ct] = M::template c_column<kPlaneC>(lc, kSC, sb, mine + ct * 16, lane);
         if constexpr (!kStates) {
             __syncthreads();                   // P is whole
-            // two blocks of steps at a time: what the entering state adds, then the chunk's own steps
+            // all blocks of steps at a time, so that the state's terms are made once and not kept: what
+            // the entering state adds, then the chunk's own steps
+            if (column(0)) {
+                f32x4 y[kB][kCT];
 #pragma unroll
-            for (int t0 = 0; t0 < kB; t0 += 2) {
-                if (!column(0)) break;
-                f32x4 y[2][kCT];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < kB; ++t)
 #pragma unroll
                     for (int ct = 0; ct < kCT; ++ct) y[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < kK; ++k)
                     if (there(k)) {
-                        Pair pa[2];
+                        Pair pa[kB];
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) pa[t] = M::template a_pair<kPlaneA>(la + ((t0 + t) * 16 + r) * kSA, k, g4);
+                        for (int t = 0; t < kB; ++t) pa[t] = M::template a_pair<kPlaneA>(la + (t * 16 + r) * kSA, k, g4);
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct) {
-                            const Pair x = M::pair(M::frag(X[2 * k][ct]), M::frag(X[2 * k + 1][ct]));
+                            const typename M::SumPair x = M::sum_pair(M::sum(X[2 * k][ct]), M::sum(X[2 * k + 1][ct]));
 #pragma unroll
-                            for (int t = 0; t < 2; ++t) y[t][ct] = M::mma(y[t][ct], x, pa[t]);
+                            for (int t = 0; t < kB; ++t) y[t][ct] = M::mma_sum(y[t][ct], x, pa[t]);
                         }
                     }
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const float since = lsince[(t0 + t) * 16 + r];
+                for (int t = 0; t < kB; ++t) {
+                    const float since = lsince[t * 16 + r];
 #pragma unroll
                     for (int ct = 0; ct < kCT; ++ct) y[t][ct] *= since;
 #pragma unroll
-                    for (int sb = 0; sb <= t0 + t; sb += 2) {
-                        const Pair pp = M::template p_pair<kPlaneP>(lp + ((t0 + t) * 16 + r) * kSP, sb, g4);
+                    for (int sb = 0; sb <= t; sb += 2) {
+                        const typename M::SumPair pp = M::template p_pair<kPlaneP>(lp + (t * 16 + r) * kSP, sb, g4);
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct)
-                            y[t][ct] = M::mma(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp);
+                            y[t][ct] = M::mma_by_sum(y[t][ct], M::pair(c[sb][ct], c[sb + 1][ct]), pp);
                     }
-                    // lane: step (t0 + t)*16 + r, columns g4 .. + 3 of each tile
-                    const int i1 = i0 + (t0 + t) * 16;
+                    // lane: step t*16 + r, columns g4 .. + 3 of each tile
+                    const int i1 = i0 + t * 16;
                     const long long at = (S.reverse ? len - 1 - i1 - 15 : i1) * y_step;     // of the least step
                     if (i1 + r < len) {
 #pragma unroll

@@ -315,3 +315,26 @@ def test_offsets_past_32_bits(dtype):
     o = readout.linear_attention_step(q, k, v, g, pool, slots=slots)
     assert torch.equal(o, readout.linear_attention_step(q, k, v, g, state))
     assert torch.equal(pool[slots.long()], state)
+
+
+def by_head(x, dim):
+    """(..., heads, ...) as (heads, everything else)."""
+    return x.detach().cpu().double().movedim(dim, 0).flatten(1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 100, 8, 64, 64), (2, 600, 4, 128, 128), (1, 300, 8, 96, 80), (1, 200, 4, 256, 100)])
+def test_outputs_of_16_bits_are_rounded_once(dtype, shape):
+    """Head by head, outputs and gradients are as far from the 64-bit result as that result rounded
+    to their type: the products' own terms (2^-17 each, a dozen of them at most) add next to nothing
+    to a rounding of 2^-9 or 2^-12."""
+    batch, time, heads, dk, dv = shape
+    print(f"case rounding {dtype} {shape}", flush=True)
+    q, k, v, g, state, do, dend = make(41, dtype, batch, time, heads, heads, heads, heads, dk, dv)
+    o, _ = readout.linear_attention(q, k, v, g, initial_state=state)
+    got = (o, *readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)[:3])
+    want = ref.attention(q, k, v, g, dk ** -0.5, state, None, do, dend)
+    for x, w in zip(got, (want[0], *want[2:5])):
+        x, least, w = by_head(x, 2), by_head(w.to(dtype), 2), by_head(w, 2)
+        off, least = (x - w).norm(dim=1), (least - w).norm(dim=1)
+        assert bool((off <= 1.01 * least + 12 * 2.0 ** -17 * w.norm(dim=1)).all()), (off / least).tolist()
