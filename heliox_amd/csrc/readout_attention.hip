@@ -22,7 +22,8 @@ __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x
 struct ScanArgs {
     const void *a, *b, *c;
     long long a_stride[3], b_stride[3], c_stride[3];
-    int a_heads, b_heads, c_heads, heads, da, dc, time;
+    int a_each, b_each, c_each;       // heads that share one of a, b, c: head h reads head h / each
+    int heads, da, dc, time;
     bool reverse;
     float scale_in, scale_out;       // of what enters the state, and of y
     const float* log_decay;
@@ -64,9 +65,9 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
     };
     fetch(group);
     const float decay = expf(S.log_decay[h]);
-    const T* a = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
-    const T* b = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
-    const T* c = static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2];
+    const T* a = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h / S.a_each) * S.a_stride[2];
+    const T* b = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h / S.b_each) * S.b_stride[2];
+    const T* c = static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h / S.c_each) * S.c_stride[2];
     if (threadIdx.x < S.da) {
         lq[threadIdx.x] = to_f32(a[threadIdx.x]);
         lk[threadIdx.x] = to_f32(b[threadIdx.x]);
@@ -520,10 +521,10 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     const float scale = S.scale_in * S.scale_out;
     const int dc_here = min(S.dc - col0, kDC);
 
-    const T* a0 = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h * S.a_heads / S.heads) * S.a_stride[2];
-    const T* b0 = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h * S.b_heads / S.heads) * S.b_stride[2];
+    const T* a0 = static_cast<const T*>(S.a) + batch * S.a_stride[0] + (h / S.a_each) * S.a_stride[2];
+    const T* b0 = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h / S.b_each) * S.b_stride[2];
     const T* c0 =
-        static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h * S.c_heads / S.heads) * S.c_stride[2] + col0;
+        static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h / S.c_each) * S.c_stride[2] + col0;
     const int begin = seg * A.seg_steps, end = min(begin + A.seg_steps, S.time);
 
     Tile<T, kDA, kT, kWhole> ta, tb;
@@ -869,7 +870,8 @@ ScanArgs scan_args(const hx_attention_args& A, const Operand& a, const Operand& 
     ScanArgs S{};
     S.a = a.p, S.b = b.p, S.c = c.p;
     for (int i = 0; i < 3; ++i) S.a_stride[i] = a.stride[i], S.b_stride[i] = b.stride[i], S.c_stride[i] = c.stride[i];
-    S.a_heads = static_cast<int>(a.heads), S.b_heads = static_cast<int>(b.heads), S.c_heads = static_cast<int>(c.heads);
+    S.a_each = static_cast<int>(A.heads / a.heads), S.b_each = static_cast<int>(A.heads / b.heads);
+    S.c_each = static_cast<int>(A.heads / c.heads);
     S.heads = static_cast<int>(A.heads), S.da = static_cast<int>(a.d), S.dc = static_cast<int>(c.d);
     S.time = static_cast<int>(A.time);
     S.reverse = reverse, S.scale_in = reverse ? static_cast<float>(A.scale) : 1.f;

@@ -338,3 +338,28 @@ def test_outputs_of_16_bits_are_rounded_once(dtype, shape):
         x, least, w = by_head(x, 2), by_head(w.to(dtype), 2), by_head(w, 2)
         off, least = (x - w).norm(dim=1), (least - w).norm(dim=1)
         assert bool((off <= 1.01 * least + 12 * 2.0 ** -17 * w.norm(dim=1)).all()), (off / least).tolist()
+
+
+@pytest.mark.parametrize("share", [1, 2])
+def test_heads_up_to_the_limit(share):
+    """2^20 heads: each gives what it gives in a call of its own few.  (heads x heads passes 32 bits from
+    46341 heads on.)"""
+    heads = 2 ** 20
+    print(f"case heads {heads} shared by {share}", flush=True)
+    q, k, v, g, state, do, dend = make(43, torch.float32, 1, 3, heads, heads, heads // share, heads, 2, 1)
+    o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+    grads = readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)
+    stepped = state.clone()
+    step = readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, stepped)
+    for first in (0, 40000, 2 ** 19, heads - 16):
+        at, few = slice(first, first + 16), slice(first // share, (first + 16) // share)
+        own = q[:, :, at], k[:, :, few], v[:, :, at], g[at]
+        want = readout.linear_attention(*own, initial_state=state[:, at])
+        assert torch.equal(o[:, :, at], want[0]) and torch.equal(end[:, at], want[1])
+        want = readout.linear_attention_grad(*own, do[:, :, at], initial_state=state[:, at], dstate=dend[:, at])
+        for x, w, part in zip(grads, want, (at, few, at)):
+            assert torch.equal(x[:, :, part], w)
+        assert torch.equal(grads[3][:, at], want[3])
+        one = state[:, at].clone()
+        want = readout.linear_attention_step(q[:, 0, at], k[:, 0, few], v[:, 0, at], g[at], one)
+        assert torch.equal(step[:, at], want) and torch.equal(stepped[:, at], one)
