@@ -1,9 +1,15 @@
 // The loss against a teacher's top logits, and its gradient by the student's, one workgroup
 // per row.
 //
-// Two passes over a row: the running maximum and sums of a softmax, then the gradient, which
-// reads the row again from the cache.  Every place outside the teacher's entries has one factor
-// (w (P - p_r / q_r)); the few entries are written over afterwards.
+// Two passes over a row: the running maximum and sum of a softmax, then the gradient, which
+// reads the row again from the cache.  Every place outside the teacher's entries has one factor;
+// the few entries are written over afterwards.
+//
+// Where the rest is one class, the running maximum m_o and the sum z_o are those of the other
+// places alone, and the entries are added from their list.  A student that is sure of its
+// entries leaves the others a mass q_r far below what fp32 holds beside the largest logit;
+// log q_r = (m_o - m) / t + log z_o - log z and the others' gradient
+// w (P e^{(m_o - m) / t} / z - p_r / z_o) e^{(x - m_o) / t} have no such limit (z_o is at least 1).
 #include "readout.h"
 
 #include <type_traits>
@@ -48,6 +54,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     constexpr int kP = sizeof(Vec) / sizeof(T);
     extern __shared__ int lds[];
     __shared__ double red[kThreads / 64];
+    __shared__ int twice;                    // whether two entries stand at one place
     const int top = static_cast<int>(A.top), vocab = static_cast<int>(A.vocab);
     int* place = lds;
     float* share = reinterpret_cast<float*>(lds + top);
@@ -65,9 +72,10 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
 
     if constexpr (kRest) {
         for (int w = threadIdx.x; w < (vocab + 31) / 32; w += kThreads) member[w] = 0;
+        if (threadIdx.x == 0) twice = 0;
         __syncthreads();
     }
-    float tmax = -INFINITY, some = 0.f;
+    float tmax = -INFINITY, some = 0.f, lead = -INFINITY;
     for (int k = threadIdx.x; k < top; k += kThreads) {
         const int j = entry<I>(A.index, row * A.index_stride + k, vocab);
         place[k] = j;
@@ -76,42 +84,37 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
         if (j >= 0) {
             some = 1.f;
             tmax = fmaxf(tmax, share[k]);
-            if constexpr (kRest) atomicOr(member + j / 32, 1u << (j % 32));
+            lead = fmaxf(lead, logit[k]);
+            if constexpr (kRest)
+                if (atomicOr(member + j / 32, 1u << (j % 32)) >> (j % 32) & 1) twice = 1;
         }
     }
     some = block_reduce<kThreads>(some, red, most);
     if constexpr (!kRest) tmax = block_reduce<kThreads>(tmax, red, most);
 
-    // the student's maximum and sums: all places, and those without an entry
-    float m = -INFINITY, z = 0.f, others = 0.f;
+    // the student's running maximum and sum over all places, or over those without an entry (bits
+    // of `in`: an entry)
+    float m = -INFINITY, z = 0.f;
     const int pieces = vocab / kP;
-    auto take = [&](const float* v, int n, unsigned in) {
+    auto take = [&](float* v, int n, unsigned in) {
+        if (kRest && in) {
+#pragma unroll
+            for (int i = 0; i < kP; ++i)
+                if (in >> i & 1) v[i] = -INFINITY;
+        }
         float c = v[0];
 #pragma unroll
         for (int i = 1; i < kP; ++i)
             if (i < n) c = fmaxf(c, v[i]);
         if (c > m) {
-            const float keep = weight(m - c);     // m = -inf: 0
-            z *= keep;
-            others *= keep;
+            z *= weight(m - c);                          // m = -inf: 0
             m = c;
         }
         const float from = m == -INFINITY ? 0.f : m;     // nothing but -inf yet: its weights are 0, not NaN
-        float e[kP], sum = 0.f;
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < kP; ++i) {
-            e[i] = i < n ? weight(v[i] - from) : 0.f;
-            sum += e[i];
-        }
+        for (int i = 0; i < kP; ++i) sum += i < n ? weight(v[i] - from) : 0.f;
         z += sum;
-        if constexpr (kRest) {
-            if (in) {
-                sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < kP; ++i) sum += in >> i & 1 ? 0.f : e[i];
-            }
-            others += sum;
-        }
     };
     const unsigned char* bits = reinterpret_cast<const unsigned char*>(member);
     // f(piece, its logits) for the row's whole pieces, several loads at a time (one alone leaves a
@@ -147,10 +150,25 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     const float mine = m;
     m = block_reduce<kThreads>(m, red, most);
     if (m == -INFINITY) m = 0.f;
-    const float scale = weight(mine - m);
-    const double whole = block_reduce<kThreads>(static_cast<double>(z * scale), red, add), logz = log(whole);
-    double rest = 0.;
-    if constexpr (kRest) rest = block_reduce<kThreads>(static_cast<double>(others * scale), red, add);
+    double whole = block_reduce<kThreads>(static_cast<double>(z * weight(mine - m)), red, add);
+    const float base = m;                       // what the other places' weights are relative to
+    const double beside = whole;                // their sum (0: nothing but -inf)
+    double under = 1.;                          // e^{(base - m) / t}
+    if constexpr (kRest) {
+        lead = block_reduce<kThreads>(lead, red, most);
+        m = beside != 0. ? fmaxf(base, lead) : lead > -INFINITY ? lead : 0.f;
+        under = beside != 0. ? exp((static_cast<double>(base) - m) * per) : 0.;
+        float own = 0.f;
+        for (int k = threadIdx.x; k < top; k += kThreads) {
+            bool counts = place[k] >= 0;
+            if (twice)                          // a place counts once
+                for (int i = 0; i < k; ++i) counts = counts && place[i] != place[k];
+            if (counts) own += weight(logit[k] - m);
+        }
+        own = block_reduce<kThreads>(own, red, add);
+        whole = beside * under + own;
+    }
+    const double logz = log(whole);
 
     // the teacher's shares and the row's loss
     double norm;
@@ -167,30 +185,33 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
         float p = 0.f;
         if (share[k] != -INFINITY) {
             const double logp = share[k] * per - norm;
-            p = expf(static_cast<float>(logp));
+            // 1 - sum p is a share of its own: in 64 bits
+            const double wide = kRest ? exp(logp) : static_cast<double>(expf(static_cast<float>(logp)));
+            p = static_cast<float>(wide);
+            psum += wide;
             if (p != 0.f) loss += p * (logp - ((static_cast<double>(logit[k]) - m) * per - logz));
         }
         share[k] = p;
-        psum += p;
     }
     loss = block_reduce<kThreads>(loss, red, add);
     psum = block_reduce<kThreads>(psum, red, add);
-    double inside = psum, outside = psum;
+    double inside = psum, pull = 0.;            // pull: p_r / z_o
     if constexpr (kRest) {
-        const double pr = fmax(0., 1. - psum), qr = rest / whole;
-        if (pr > 0. && qr > 0.) {
-            loss += pr * log(pr / qr);
+        const double pr = fmax(0., 1. - psum);
+        if (pr > 0. && beside * under > 0.) {   // a mass of 0 in 64 bits is that of masked places
+            loss += pr * (log(pr / beside) - ((static_cast<double>(base) - m) * per - logz));
             inside = psum + pr;
-            outside = inside - pr / qr;
+            pull = pr / beside;
         }
     }
     if (threadIdx.x == 0) A.loss[row] = some > 0.f ? static_cast<float>(loss * tau * tau) : 0.f;
     if (!A.grad) return;
     T* g = static_cast<T*>(A.grad) + row * A.grad_stride;
     const float w = some > 0.f ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
-    const float factor = static_cast<float>(w * outside / whole),
+    const float factor = static_cast<float>(w * (inside * under / whole - pull)),
                 within = static_cast<float>(inside / whole);
-    auto slope = [&](float v) { return some > 0.f ? factor * weight(v - m) : 0.f; };
+    // (entries may lie far above the base; theirs are written over below)
+    auto slope = [&](float v) { return some > 0.f ? factor * weight(v - base) : 0.f; };
     each_piece([&](int p, Vec raw) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) raw[i] = static_cast<decltype(raw[0] + raw[0])>(slope(static_cast<float>(raw[i])));

@@ -278,7 +278,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
     or int64; a place outside the vocabulary is an absent entry).  Without teacher_lse the
     teacher is the softmax over its entries.  With teacher_lse (rows,) fp32, the logarithm of
     sum exp(logit / temperature) over the teacher's whole vocabulary, its mass on all other
-    places is one more class.  A row without entries has loss 0."""
+    places is one more class, but where the student's mask leaves none of them (their mass is
+    under 2^-1074).  A row without entries has loss 0."""
     return _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, None, None)
 
 

@@ -552,7 +552,9 @@ int hx_linear_attention_step(const hx_attention_args* args);
  * outside 0..vocab-1 is absent; entries at one place add up), and
  *   teacher_lse NULL: p = softmax of teacher / t over the row's entries, no p_r term;
  *   else:  p_k = exp(teacher_k / t - teacher_lse_i), p_r = max(0, 1 - sum_k p_k) and q_r the
- *          student's mass of all other places (no such term where p_r or q_r is 0).
+ *          student's mass of all other places (no such term where p_r is 0, or q_r under
+ *          2^-1074, the least number of 64 bits: -inf or a type's lowest value on every one of
+ *          them is a mask).
  * A row without entries has loss 0 and gradient 0.  grad (NULL: not made) receives
  * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself. */
 typedef struct hx_distill_args {

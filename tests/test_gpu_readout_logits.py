@@ -300,3 +300,78 @@ def test_rows_more_than_32_bits_apart():
     assert all(torch.equal(a, b) for a, b in zip(readout.sample(apart, u, top_p=0.9), drawn))
     loss, grad = readout.distill_loss_grad(apart, index, t, teacher_lse=lse, weight=weight, out=apart)
     assert torch.equal(loss, near[0]) and torch.equal(grad, near[1])
+
+
+# ---------------------------------------------------------- distillation, students far from the teacher
+def sure(seed, dtype, gap, tau, rows=3, vocab=203, top=5, masked=None, below=True):
+    """Students whose other places lie `gap` temperatures under their entries (below) or over them;
+    the teacher has a tenth of its mass beside the entries."""
+    gen = torch.Generator().manual_seed(seed)
+    index = torch.stack([torch.randperm(vocab, generator=gen)[:top] for _ in range(rows)])
+    x = torch.randn(rows, vocab, generator=gen) * tau - (gap * tau if below else 0.0)
+    x.scatter_(1, index, torch.randn(rows, top, generator=gen) * tau - (0.0 if below else gap * tau))
+    if masked is not None:
+        ruled = torch.arange(vocab) % 3 == 0
+        ruled[index.unique()] = False
+        x[:, ruled] = -math.inf if masked == "inf" else torch.finfo(dtype).min
+    t = torch.randn(rows, top, generator=gen).to(dtype)
+    lse = torch.logsumexp(t.double() / tau, 1) - math.log(0.9)
+    return x.to(dtype).cuda(), index.to(torch.int32).cuda(), t.cuda(), lse.float().cuda()
+
+
+def check_sure(x, index, t, tau, lse, weight, dtype):
+    """Losses as everywhere; gradients row by row, the entries and the others each by themselves."""
+    want, dwant = ref.distill(x, index, t, tau, lse, weight)
+    loss, grad = readout.distill_loss_grad(x, index, t, temperature=tau, teacher_lse=lse, weight=weight)
+    assert bool(torch.isfinite(dwant).all()) and bool(torch.isfinite(grad).all())
+    assert torch.equal(loss, readout.distill_loss(x, index, t, temperature=tau, teacher_lse=lse))
+    assert bool(((loss.cpu().double() - want).abs() <= tau * tau * loss_bound(want / (tau * tau))).all()), (loss, want)
+    entries = torch.zeros(x.shape, dtype=torch.bool).scatter_(1, index.cpu().long(), True)
+    for part in (entries, ~entries):
+        got, exact = (torch.where(part, g.cpu().double(), 0.0) for g in (grad, dwant))
+        assert bool(((got - exact).norm(dim=1) <= grad_bound(dtype) * exact.norm(dim=1)).all()), (got - exact).norm(dim=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau", [0.25, 0.5, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("gap", [20, 46, 60, 87, 90, 95, 100, 104, 200, 400, 700])
+def test_distill_the_rest_of_a_sure_student(dtype, tau, gap):
+    print(f"case sure student {dtype} gap={gap} tau={tau}", flush=True)
+    weight = torch.tensor([16.0, 256.0, 1000.0], device="cuda")
+    for masked in (None, "inf", "lowest"):
+        x, index, t, lse = sure(gap, dtype, gap, tau, masked=masked)
+        check_sure(x, index, t, tau, lse, weight, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gap", [30, 100, 400])
+def test_distill_a_student_sure_of_other_places(dtype, gap):
+    x, index, t, lse = sure(gap, dtype, gap, 1.0, below=False)
+    check_sure(x, index, t, 1.0, lse, torch.tensor([16.0, 256.0, 1000.0], device="cuda"), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_entries_twice_and_absent_beside_a_far_rest(dtype):
+    x, index, t, lse = sure(5, dtype, 100, 1.0, rows=4)
+    lse = lse + 1.0                   # room for an entry that comes twice
+    index[0, 3] = index[0, 1]
+    index[1, 2] = -1
+    index[2, 4] = index[2, 0]
+    index[2, 1] = 203
+    want, dwant = ref.distill(x, index, t, 1.0, lse)
+    loss, grad = readout.distill_loss_grad(x, index, t, teacher_lse=lse)
+    assert bool(((loss.cpu().double() - want).abs() <= loss_bound(want)).all())
+    assert bool(((grad.cpu().double() - dwant).norm(dim=1) <= grad_bound(dtype) * dwant.norm(dim=1)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low", ["inf", "lowest"])
+def test_distill_nothing_left_beside_the_entries(dtype, low):
+    """Every other place is masked: their class is not there, and they have no gradient."""
+    x, index, t, lse = sure(6, dtype, 0, 1.0)
+    others = torch.ones_like(x, dtype=torch.bool).scatter_(1, index.long(), False)
+    x[others] = -math.inf if low == "inf" else torch.finfo(dtype).min
+    want, dwant = ref.distill(x, index, t, 1.0, lse)
+    loss, grad = readout.distill_loss_grad(x, index, t, teacher_lse=lse)
+    assert bool(((loss.cpu().double() - want).abs() <= loss_bound(want)).all())
+    assert not grad[others].any() and ref.rel(grad, dwant) <= grad_bound(dtype)
