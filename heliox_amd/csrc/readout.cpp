@@ -124,8 +124,9 @@ int hx_distill_loss(const hx_distill_args* A) {
                       (long long)hx::kDistillMaxVocab);
     if (A->top < 0 || A->top > hx::kDistillMaxTop)
         return refuse("%s: top (%lld) has to be in 0..%lld", call, (long long)A->top, (long long)hx::kDistillMaxTop);
-    if (!(A->temperature > 0) || !std::isfinite(A->temperature))
-        return refuse("%s: temperature has to be positive", call);
+    // it and its reciprocal times log2 e are fp32 numbers in the kernel
+    if (!(A->temperature >= 0x1p-126) || !(A->temperature <= 0x1p126))
+        return refuse("%s: temperature has to be positive, in 2^-126..2^126", call);
     if (!A->rows) return 0;
     if (!A->logits || !A->loss || (A->top && (!A->index || !A->teacher)))
         return refuse("%s: logits, index, teacher or loss is missing", call);

@@ -555,7 +555,8 @@ int hx_linear_attention_step(const hx_attention_args* args);
  *          student's mass of all other places (no such term where p_r is 0, or q_r under
  *          2^-1074, the least number of 64 bits: -inf or a type's lowest value on every one of
  *          them is a mask).
- * A row without entries has loss 0 and gradient 0.  grad (NULL: not made) receives
+ * t is in 2^-126..2^126.  A row without entries has loss 0 and gradient 0; one whose logits
+ * are all -inf has no softmax (NaN).  grad (NULL: not made) receives
  * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself. */
 typedef struct hx_distill_args {
     int64_t type, teacher_type, index_bits;               /* index_bits 32 or 64 */

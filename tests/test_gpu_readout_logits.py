@@ -375,3 +375,19 @@ def test_distill_nothing_left_beside_the_entries(dtype, low):
     loss, grad = readout.distill_loss_grad(x, index, t, teacher_lse=lse)
     assert bool(((loss.cpu().double() - want).abs() <= loss_bound(want)).all())
     assert not grad[others].any() and ref.rel(grad, dwant) <= grad_bound(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_temperatures_at_the_ends(dtype):
+    """The coldest student is its largest logit, the hottest knows nothing: finite either way."""
+    x, index, t, lse, weight = problem(12, dtype, 3, 300, 5, 1.0)
+    x = x.float().cummax(1).values + 0.125 * torch.arange(300, device="cuda")     # one largest, the last
+    x = x.to(dtype)
+    index[:, 0] = 299
+    loss, grad = readout.distill_loss_grad(x, index, t, temperature=2.0 ** -126)
+    assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(grad).all())
+    _, grad = readout.distill_loss_grad(x, index, t, temperature=2.0 ** 126, weight=torch.full_like(weight, 2.0 ** -126))
+    assert bool(torch.isfinite(grad).all())
+    outside = torch.ones(300, dtype=torch.bool, device="cuda")
+    outside[index.long().unique()] = False
+    assert torch.allclose(grad.float()[:, outside], torch.full_like(grad.float()[:, outside], 1 / 300), rtol=2 ** -7)

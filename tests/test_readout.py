@@ -126,3 +126,15 @@ def test_a_workspace_that_does_not_fit_is_refused():
         assert "workspace" in error()
     fields[-3:-1] = 4104, need
     assert lib().hx_linear_attention(readout._ATTENTION.pack(*fields)) == -1 and "16 bytes" in error()
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -127, 1e-300, 2.0 ** 127, 1e300, -1.0])
+def test_temperatures_that_fp32_cannot_hold_are_refused(temperature):
+    """Its reciprocal, or the temperature itself, would be infinite in the kernel and the result NaN."""
+    assert lib().hx_distill_loss(distill(temperature=temperature)) == -1
+    assert "temperature" in error()
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -126, 2.0 ** 126])
+def test_temperatures_at_the_ends_are_taken(temperature):
+    assert lib().hx_distill_loss(distill(rows=0, temperature=temperature)) == 0
