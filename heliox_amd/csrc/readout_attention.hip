@@ -16,8 +16,10 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// 2^x by the instruction: one unit off at most, 0 under 2^-126.
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+// The logarithm of a decay, finite: -inf as a number whose exponential is 0 after one step, so
+// that e^{g 0} stays 1.  Decays are expf(g n), made once a workgroup or once a chunk: g goes in as
+// it is, and their error is that of one product and one exponential.
+__device__ __forceinline__ float decay_of(float log_decay) { return log_decay < -1e4f ? -1e4f : log_decay; }
 
 struct ScanArgs {
     const void *a, *b, *c;
@@ -515,8 +517,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
     const int col0 = slice * kDC;                          // of the slice
     const int mine = wave * kCT * 16;                      // of the wave, in the slice
-    const float lg = S.log_decay[h] * 1.44269504f;
-    const float g = lg < -1e4f ? -1e4f : lg;               // -inf: e^{g 0} stays 1
+    const float g = decay_of(S.log_decay[h]);
     const int off = S.reverse ? 0 : 1;
     const float scale = S.scale_in * S.scale_out;
     const int dc_here = min(S.dc - col0, kDC);
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
             each_place([&](float, int at) { return w[at]; });
         }
         if (S.state_in) {
-            const float left = pow2(g * static_cast<float>(min(begin, len)));
+            const float left = expf(g * static_cast<float>(min(begin, len)));
             const float* w = S.state_in + bh * state_size;
             each_place([&](float x, int at) { return x + left * w[at]; });
         }
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = threadIdx.x * 4 + i;
-                w[i] = j < n ? S.scale_in * pow2(g * static_cast<float>(n - off - j)) : 0.f;
+                w[i] = j < n ? S.scale_in * expf(g * static_cast<float>(n - off - j)) : 0.f;
             }
             lleft[threadIdx.x] = w;
         }
@@ -596,11 +597,11 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int ago = (e / 64 - 1) * 16 + r - g4 - i;
-                w[i] = e >= 64 && ago >= 0 ? scale * pow2(g * static_cast<float>(ago)) : 0.f;
+                w[i] = e >= 64 && ago >= 0 ? scale * expf(g * static_cast<float>(ago)) : 0.f;
             }
             lfactor[e] = w;
         }
-        if (threadIdx.x < kC) lsince[threadIdx.x] = S.scale_out * pow2(g * static_cast<float>(threadIdx.x + off));
+        if (threadIdx.x < kC) lsince[threadIdx.x] = S.scale_out * expf(g * static_cast<float>(threadIdx.x + off));
     }
     long long y_step = S.y_stride[1];
     unsigned long long y_base = reinterpret_cast<unsigned long long>(S.y) +
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
         }
         if (i0 + kC < end) fetch(i0 + kC, 0);
         // the state that leaves
-        const float keep = pow2(g * static_cast<float>(n));
+        const float keep = expf(g * static_cast<float>(n));
 #pragma unroll
         for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
@@ -777,8 +778,7 @@ __global__ void __launch_bounds__(kThreads) k_join(ChunkArgs A) {
     if (e >= size) return;
     const int batch = bh / S.heads, h = bh - batch * S.heads;
     const int len = S.lengths ? min(max(S.lengths[batch], 0), S.time) : S.time;
-    const float lg = S.log_decay[h] * 1.44269504f;
-    const float g = lg < -1e4f ? -1e4f : lg;
+    const float g = decay_of(S.log_decay[h]);
     Vec* w = reinterpret_cast<Vec*>(S.states) + static_cast<long long>(bh) * nseg * size + e;
     // the segments' loads do not wait for each other
     constexpr int kAhead = 16;
@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(kThreads) k_join(ChunkArgs A) {
             const int s = s0 + k;
             if (s < nseg) {
                 const int n = min(max(len - s * A.seg_steps, 0), A.seg_steps);
-                x = x * pow2(g * static_cast<float>(n)) + next[k];
+                x = x * expf(g * static_cast<float>(n)) + next[k];
                 w[static_cast<long long>(s) * size] = x;
             }
         }

@@ -363,3 +363,30 @@ def test_heads_up_to_the_limit(share):
         one = state[:, at].clone()
         want = readout.linear_attention_step(q[:, 0, at], k[:, 0, few], v[:, 0, at], g[at], one)
         assert torch.equal(step[:, at], want) and torch.equal(stepped[:, at], one)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_decays_are_the_exponentials(dtype):
+    """One input at the first step, seen later: e^{g t}, with decays whose products with whole numbers
+    are exact.  What is left are the exponentials' own units: three for each chunk gone through (one
+    exponential of at most two units, one product), 16 for the rest."""
+    time = 1281
+    g = torch.tensor([-1 / 16, -3 / 16, -5 / 16, -13 / 16, -23 / 16, -7 / 8], device="cuda")
+    heads = g.shape[0]
+    lengths = torch.tensor([1, 2, 33, 50, 64, 65, 97, 129, 256, 300, 511, 800, 1100, 1281], dtype=torch.int32, device="cuda")
+    one = torch.ones(1, time, heads, 1, dtype=dtype, device="cuda")
+    first = torch.zeros_like(one)
+    first[:, 0] = 1
+    o, _ = readout.linear_attention(one, first, one, g, scale=1.0)
+    batch = lambda x: x.expand(lengths.shape[0], -1, -1, -1)  # noqa: E731
+    _, end = readout.linear_attention(batch(one), batch(first), batch(one), g, scale=1.0, lengths=lengths)
+    t = torch.arange(time, device="cuda").double()
+    courses = [(end[:, :, 0, 0].double(), lengths.double() - 1)]
+    if dtype == torch.float32:
+        courses.append((o[0, :, :, 0].double(), t))
+    for got, ago in courses:
+        want = torch.exp(g.double() * ago[:, None])
+        bound_ = (3 * ago[:, None] / 32 + 16) * ref.UNIT[torch.float32]
+        seen = g.double() * ago[:, None] > -80
+        off = (got / want - 1).abs()
+        assert bool((off <= bound_)[seen].all()), float((off / bound_)[seen].max())
