@@ -110,7 +110,9 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
 //   P_ij = scale_in scale_out e^{g (i - j)} (a_i . b_j) for j <= i
 //   y_i  = sum_j P_ij c_j + scale_out e^{g (i + off)} X^T a_i
 //   X'   = e^{g n} X + sum_j b_j (scale_in e^{g (n - off - j)} c_j)^T
-// are products of matrices.  A workgroup walks through the chunks of one (sequence, head,
+// are products of matrices.  P over the diagonal is made zero, not multiplied by it, and a chunk
+// ends before a step whose c holds an infinity or a NaN (zero times that is NaN), unless that is
+// its first step: no step's output looks at a later one.  A workgroup walks through the chunks of one (sequence, head,
 // slice of c's columns, segment of the steps); each wave keeps X^T's rows for its own columns
 // in accumulator registers, whose layout (lane: one column, four rows) is at the same time
 // that of an operand, so X enters y's product without leaving the registers.  y and P are made
@@ -390,10 +392,30 @@ struct MathF32 {
     }
 };
 
-template <class T> struct InputOf;      // the products' mathematics, the input's type and four of them
-template <> struct InputOf<float> { static constexpr int kType = HX_F32; using Math = MathF32; using Elem = float; using Four = f32x4; };
-template <> struct InputOf<__half> { static constexpr int kType = HX_F16; using Math = MathF16; using Elem = _Float16; using Four = f16x4; };
-template <> struct InputOf<__hip_bfloat16> { static constexpr int kType = HX_BF16; using Math = MathBf16; using Elem = __bf16; using Four = bf16x4; };
+// The products' mathematics, the input's type and four of them, the exponent's bits and lowest bit
+// of the numbers in 32 bits.
+template <class T> struct InputOf;
+template <> struct InputOf<float> {
+    static constexpr int kType = HX_F32;
+    static constexpr unsigned kExponent = 0x7f800000u, kUnit = 0x00800000u;
+    using Math = MathF32;
+    using Elem = float;
+    using Four = f32x4;
+};
+template <> struct InputOf<__half> {
+    static constexpr int kType = HX_F16;
+    static constexpr unsigned kExponent = 0x7c007c00u, kUnit = 0x04000400u;
+    using Math = MathF16;
+    using Elem = _Float16;
+    using Four = f16x4;
+};
+template <> struct InputOf<__hip_bfloat16> {
+    static constexpr int kType = HX_BF16;
+    static constexpr unsigned kExponent = 0x7f807f80u, kUnit = 0x00800080u;
+    using Math = MathBf16;
+    using Elem = __bf16;
+    using Four = bf16x4;
+};
 
 // Rows [0, n) of a chunk into registers, kD columns padded with zeros, R rows a round of the
 // workgroup.  kWhole: d is a whole number of pieces and a round's rows are within 2 GiB, so that
@@ -448,11 +470,32 @@ struct Tile {
     }
     // put(row, column, piece) for the pieces of this thread
     template <class F>
-    __device__ __forceinline__ void store(F put) const {
-        const int i = threadIdx.x / kRowPieces, j = threadIdx.x % kRowPieces * kP;
+    __device__ __forceinline__ void store(F put, int thread = threadIdx.x) const {
+        const int i = thread / kRowPieces, j = thread % kRowPieces * kP;
 #pragma unroll
         for (int p = 0; p < kN; ++p)
             if (kRows <= Math::kC || i < Math::kC) put(i + p * kRows, j, raw[p]);
+    }
+    // Whether an infinity or a NaN is among the pieces (their exponents are nothing but ones, and one
+    // more of their lowest bit passes on).
+    static __device__ __forceinline__ unsigned exponents(Raw x) {
+        typedef unsigned Words __attribute__((ext_vector_type(4)));
+        const Words w = (__builtin_bit_cast(Words, x) & In::kExponent) + In::kUnit;
+        return w[0] | w[1] | w[2] | w[3];
+    }
+    static constexpr unsigned kOdd = In::kExponent + In::kUnit;
+    __device__ __forceinline__ bool odd() const {
+        unsigned any = 0;
+#pragma unroll
+        for (int p = 0; p < kN; ++p) any |= exponents(raw[p]);
+        return (any & kOdd) != 0;
+    }
+    // f(row) for the pieces with one among them
+    template <class F>
+    __device__ __forceinline__ void each_odd(F f) const {
+#pragma unroll
+        for (int p = 0; p < kN; ++p)
+            if ((exponents(raw[p]) & kOdd) != 0) f(static_cast<int>(threadIdx.x) / kRowPieces + p * kRows);
     }
 };
 
@@ -503,9 +546,10 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     __shared__ __attribute__((aligned(16))) Elem la[kStates ? 1 : kPlaneA * kPlanes], lb[kC * kSB * kPlanes],
         lc[kPlaneC * kPlanes], lp[kStates ? 1 : kPlaneP * M::kPlanesP];
     // the chunk's decays, made once: of P's blocks tb - sb + 1 blocks under the diagonal (the first:
-    // over it, nothing) as a lane holds them; of the entering state; of what enters at a step
+    // over it) as a lane holds them, NaN for later steps; of the entering state; of what enters at a step
     __shared__ f32x4 lfactor[kStates ? 1 : (kB + 1) * 64], lleft[kC / 4];
     __shared__ float lsince[kStates ? 1 : kC];
+    __shared__ int lodd;                                   // the first step but 0 whose c is not finite
     // neighbouring workgroups take the jobs of one segment, which read much the same
     const JobArgs& S = job_of(blockIdx.x % A.jobs);
     const int lane = threadIdx.x % 64, r = lane % 16, g4 = lane / 16 * 4;
@@ -526,7 +570,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     const T* b0 = static_cast<const T*>(S.b) + batch * S.b_stride[0] + (h / S.b_each) * S.b_stride[2];
     const T* c0 =
         static_cast<const T*>(S.c) + batch * S.c_stride[0] + (h / S.c_each) * S.c_stride[2] + col0;
-    const int begin = seg * A.seg_steps, end = min(begin + A.seg_steps, S.time);
+    const int begin = seg * A.seg_steps, end = min(begin + A.seg_steps, S.time), stop = min(end, len);
 
     Tile<T, kDA, kT, kWhole> ta, tb;
     Tile<T, kDC, kT, kWhole> tc;
@@ -535,7 +579,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     tc.start(c0, S.c_stride[1], S.reverse, dc_here);
     // in two parts: all at once, the pieces would take registers from the products beside them
     auto fetch = [&](int i0, int part) {
-        const int n = min(kC, len - i0);
+        const int n = min(kC, stop - i0);
         const long long t0 = S.reverse ? len - 1 - i0 : i0;
         if (part == 0) {
             if constexpr (!kStates) ta.load(t0 * S.a_stride[1], n);
@@ -591,13 +635,15 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
         }
     };
     make_left(kC);
+    int left_of = kC;                                      // the steps that lleft is made for
+    if (threadIdx.x == 0) lodd = kC;
     if constexpr (!kStates) {
         for (int e = threadIdx.x; e < (kB + 1) * 64; e += kT) {
             f32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int ago = (e / 64 - 1) * 16 + r - g4 - i;
-                w[i] = e >= 64 && ago >= 0 ? scale * expf(g * static_cast<float>(ago)) : 0.f;
+                w[i] = e >= 64 && ago >= 0 ? scale * expf(g * static_cast<float>(ago)) : __builtin_nanf("");
             }
             lfactor[e] = w;
         }
@@ -609,22 +655,27 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
     asm volatile("" : "+s"(y_base), "+s"(y_step));         // held, not read from the arguments at every store
     const std::conditional_t<kWhole, unsigned, long long> y_lane = (S.reverse ? 15 - r : r) * y_step + g4;
 
-    for (int i0 = begin; i0 < end; i0 += kC) {
-        const int n = min(kC, len - i0);
-        if (n <= 0) break;
+    for (int i0 = begin, n; i0 < stop; i0 += n) {
+        n = min(kC, stop - i0);
         __syncthreads();                       // the chunk before is done with
-        if (n < kC) make_left(n);
+        if (n != left_of) make_left(left_of = n);
         if constexpr (!kStates)
             ta.store([&](int i, int col, Raw x) { M::template store<kPlaneA>(la + i * kSA + col, x); });
         tb.store([&](int i, int col, Raw x) { M::template b_store<kDA>(lb, i, col, x); });
         tc.store([&](int i, int col, Raw x) { M::template store<kPlaneC>(lc + i * kSC + col, x); });
+        if constexpr (!kStates)
+            if (tc.odd())
+                tc.each_odd([&](int i) {
+                    if (i > 0) atomicMin(&lodd, i);
+                });
         __syncthreads();
         // whether columns 32 k .. of a and b are there, and the wave's column tile ct
         auto there = [&](int k) { return kFull || k * 32 < S.da; };
         auto column = [&](int ct) { return kFull || col0 + mine + ct * 16 < S.dc; };
         Frag c[kB][kCT];
         if constexpr (!kStates) {
-            // P's blocks, as many for each wave (those over the diagonal come out as zero)
+            const int first_odd = lodd;
+            // P's blocks, as many for each wave
             constexpr int kEach = kB * kB > kW ? kB * kB / kW : 1;
             static_assert((kEach * kW == kB * kB || kEach == 1) && (kEach % kB == 0 || kB % kEach == 0),
                           "whole rows or parts of one");
@@ -647,9 +698,28 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
                     const int tb_ = (block0 + e) / kB, sb = (block0 + e) % kB;
-                    p[e] *= lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
+                    const f32x4 w = lfactor[(max(tb_ - sb, -1) + 1) * 64 + lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[e][i] = w[i] == w[i] ? p[e][i] * w[i] : 0.f;
                     M::template store_sum<kPlaneP>(lp + (tb_ * 16 + r) * kSP + M::p_at(sb, g4), M::sum(p[e]));
                 }
+            }
+            // (P is made with the steps that this takes out: in the rows that stay it is zero there)
+            const int odd = __builtin_amdgcn_readfirstlane(first_odd);
+            if (odd < n) {
+                n = odd;
+                __syncthreads();               // all have read it
+                if (threadIdx.x == 0) lodd = kC;
+                make_left(left_of = n);
+                int thread = threadIdx.x;
+                asm volatile("" : "+v"(thread));       // its addresses are made here, not kept
+                tb.store([&](int i, int col, Raw) {
+                    if (i >= n) M::template b_store<kDA>(lb, i, col, Raw{});
+                }, thread);
+                tc.store([&](int i, int col, Raw) {
+                    if (i >= n) M::template store<kPlaneC>(lc + i * kSC + col, Raw{});
+                }, thread);
+                __syncthreads();
             }
         }
 #pragma unroll
@@ -694,7 +764,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                     // lane: step t*16 + r, columns g4 .. + 3 of each tile
                     const int i1 = i0 + t * 16;
                     const long long at = (S.reverse ? len - 1 - i1 - 15 : i1) * y_step;     // of the least step
-                    if (i1 + r < len) {
+                    if (t * 16 + r < n) {
 #pragma unroll
                         for (int ct = 0; ct < kCT; ++ct) {
                             const int columns = S.dc - (col0 + mine + ct * 16 + g4);
@@ -710,7 +780,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
                 }
             }
         }
-        if (i0 + kC < end) fetch(i0 + kC, 0);
+        if (i0 + n < stop) fetch(i0 + n, 0);
         // the state that leaves
         const float keep = expf(g * static_cast<float>(n));
 #pragma unroll
@@ -719,7 +789,7 @@ __global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A)
             for (int ct = 0; ct < kCT; ++ct) X[rt][ct] *= keep;
 #pragma unroll
         for (int sb = 0; sb < kB; sb += 2) {
-            if (sb == kB - 2 && i0 + kC < end) fetch(i0 + kC, 1);
+            if (sb == kB - 2 && i0 + n < stop) fetch(i0 + n, 1);
             if (!column(0)) continue;
             typename M::Term wc[2][kCT][M::kTerms];
 #pragma unroll

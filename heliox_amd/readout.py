@@ -159,8 +159,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     (int32; all of time unless given); its outputs beyond are zero, whatever its inputs hold.
     Returns o (batch, time, heads, dv) of q's type and the state at each sequence's end.
 
-    Within a sequence a non-finite k or v may reach outputs of up to 63 steps before it (chunks
-    of steps are products of matrices), and may do so as NaN.
+    An infinite or NaN input reaches what it reaches in the recurrence, and no earlier step, but as
+    NaN where that may have an infinity.
     """
     device, kept, fields = _attention_inputs(q, k, v, log_decay, 4)
     _, batch, time, heads, _, _, _, dk, dv = fields[:9]

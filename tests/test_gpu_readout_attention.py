@@ -390,3 +390,46 @@ def test_decays_are_the_exponentials(dtype):
         seen = g.double() * ago[:, None] > -80
         off = (got / want - 1).abs()
         assert bool((off <= bound_)[seen].all()), float((off / bound_)[seen].max())
+
+
+def check_reach(got, want, dtype, what):
+    """Finite where the recurrence is, and as near to it as everywhere; not finite where it is not."""
+    got, want = got.detach().cpu().double(), want.double()
+    there = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), there), (what, int((torch.isfinite(got) != there).sum()))
+    got, want = torch.where(there, got, 0.0), torch.where(there, want, 0.0)
+    assert float((got - want).norm()) <= bound(dtype) * float(want.norm()), what
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("shape", [(2, 200, 2, 2, 2, 2, 48, 40), (1, 130, 8, 8, 4, 8, 64, 64), (1, 1500, 1, 1, 1, 1, 33, 100)])
+def test_what_is_not_finite_reaches_no_earlier_step(dtype, value, shape):
+    """One infinity or NaN in one of q, k, v, do: outputs, states and gradients that the recurrence
+    does not bring it to are as without it."""
+    batch, time, heads, qh, kh, vh, dk, dv = shape
+    print(f"case reach {dtype} {value} {shape}", flush=True)
+    for n, step in enumerate((0, 5, 63, 64, time // 2 + 1, time - 1)):
+        q, k, v, g, state, do, dend = make(47 + n, dtype, *shape)
+        name = ("q", "k", "v", "do")[n % 4]
+        x = {"q": q, "k": k, "v": v, "do": do}[name]
+        x[0, step, 0, 3] = value
+        if n == 4:                       # two in one chunk
+            v[0, step + 3, 0, 1] = value
+        o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+        grads = readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend)
+        want = ref.attention(q, k, v, g, dk ** -0.5, state, None, do, dend)
+        for x, w, kind, part in zip((o, end, *grads), want, (dtype, torch.float32, dtype, dtype, dtype, torch.float32),
+                                    ("o", "end", "dq", "dk", "dv", "dinitial")):
+            check_reach(x, w, kind, (name, step, part))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_but_nan_ends(dtype):
+    """Every step is a chunk of its own then."""
+    q, k, v, g, state, *_ = make(59, dtype, 2, 300, 2, 2, 2, 2, 32, 64)
+    v[0] = float("nan")
+    o, end = readout.linear_attention(q, k, v, g, initial_state=state)
+    want = ref.attention(q, k, v, g, 32 ** -0.5, state)
+    check_reach(o, want[0], dtype, "o")
+    check_reach(end, want[1], torch.float32, "end")
