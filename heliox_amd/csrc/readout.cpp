@@ -56,6 +56,16 @@ int attention_inputs(const char* call, const hx_attention_args* A) {
     return 0;
 }
 
+// The states that a call writes are not those it reads: workgroups of other segments read them
+// while the last one writes.
+int attention_states(const char* call, const hx_attention_args* A, const float* out, const char* out_name, const float* in,
+                     const char* in_name) {
+    const uintptr_t bytes = sizeof(float) * A->batch * A->heads * A->dk * A->dv;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+    if (o && i && o < i + bytes && i < o + bytes) return refuse("%s: %s overlaps %s", call, out_name, in_name);
+    return 0;
+}
+
 int attention_space(const char* call, const hx_attention_args* A, bool grad) {
     const size_t need = hx::attention_workspace(*A, grad);
     if (need && (!A->workspace || A->workspace_bytes < 0 || static_cast<size_t>(A->workspace_bytes) < need))
@@ -84,6 +94,7 @@ int hx_linear_attention(const hx_attention_args* A) {
     if (!A->log_decay) return refuse("%s: log_decay is missing", call);
     if (A->time && attention_inputs(call, A)) return -1;
     if (A->time && !A->o) return refuse("%s: o is missing", call);
+    if (attention_states(call, A, A->end_state, "end_state", A->initial_state, "initial_state")) return -1;
     if (attention_space(call, A, false)) return -1;
     return launched(call, hx::attention_forward(*A));
 }
@@ -96,6 +107,9 @@ int hx_linear_attention_grad(const hx_attention_args* A) {
     if (A->time && attention_inputs(call, A)) return -1;
     if (A->time && (!A->grad_o || !A->grad_q || !A->grad_k || !A->grad_v))
         return refuse("%s: grad_o, grad_q, grad_k or grad_v is missing", call);
+    if (attention_states(call, A, A->grad_initial, "grad_initial", A->initial_state, "initial_state") ||
+        attention_states(call, A, A->grad_initial, "grad_initial", A->grad_end, "grad_end"))
+        return -1;
     if (attention_space(call, A, true)) return -1;
     return launched(call, hx::attention_backward(*A));
 }

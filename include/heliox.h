@@ -511,7 +511,9 @@ enum { HX_F32 = 0, HX_F16 = 1, HX_BF16 = 2 };
  * past a sequence's length are zero, whatever its inputs hold there.  Head h reads head
  * h q_heads / heads of q, and so on: q_heads, k_heads and v_heads each divide heads.
  * g = log_decay[h] is at most 0 (-inf: no memory).  States are (batch, heads, dk, dv) fp32,
- * contiguous.  dk and dv are at most 256, batch x heads 2^20, time 2^30. */
+ * contiguous.  dk and dv are at most 256, batch x heads 2^20, time 2^30.  What a call writes
+ * overlaps nothing that it reads (end_state and grad_initial that do are refused), but for the
+ * single step's state. */
 typedef struct hx_attention_args {
     int64_t type, batch, time, heads, q_heads, k_heads, v_heads, dk, dv;
     const void *q, *k, *v;                                /* (batch, time, heads of each, d) */

@@ -138,3 +138,18 @@ def test_temperatures_that_fp32_cannot_hold_are_refused(temperature):
 @pytest.mark.parametrize("temperature", [2.0 ** -126, 2.0 ** 126])
 def test_temperatures_at_the_ends_are_taken(temperature):
     assert lib().hx_distill_loss(distill(rows=0, temperature=temperature)) == 0
+
+
+@pytest.mark.parametrize("call,out,inp", [("hx_linear_attention", 29, 22), ("hx_linear_attention_grad", 38, 22),
+                                          ("hx_linear_attention_grad", 38, 34)])
+def test_states_written_over_those_read_are_refused(call, out, inp):
+    """Pointers are only compared here: the call ends before anything is launched (no workspace)."""
+    long = dict(GOOD, batch=1, time=5000)
+    fields = list(readout._ATTENTION.unpack(attention(**long)))
+    for i in (9, 10, 11, 21, 25, 30, 35, 36, 37):       # q, k, v, log_decay, o, grad_o, grad_q, grad_k, grad_v
+        fields[i] = 1 << 40
+    size = 4 * 4 * 16 * 24
+    for apart, refused in ((0, True), (size - 4, True), (4 - size, True), (size, False), (-size, False)):
+        fields[inp], fields[out] = 1 << 20, (1 << 20) + apart
+        assert getattr(lib(), call)(readout._ATTENTION.pack(*fields)) == -1
+        assert ("overlaps" in error()) == refused and ("workspace" in error()) != refused
