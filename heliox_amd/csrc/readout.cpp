@@ -75,6 +75,24 @@ int attention_space(const char* call, const hx_attention_args* A, bool grad) {
     return 0;
 }
 
+// grad is the logits themselves, row for row, or apart from them; its rows are apart from each other.
+int distill_gradient(const char* call, const hx_distill_args* A) {
+    typedef __int128 Wide;
+    const int64_t size = A->type == HX_F32 ? 4 : 2;
+    const Wide width = static_cast<Wide>(A->vocab) * size, gs = static_cast<Wide>(A->grad_stride) * size,
+               xs = static_cast<Wide>(A->logits_stride) * size;
+    if (A->rows > 1 && (gs < 0 ? -gs : gs) < width) return refuse("%s: rows of grad overlap each other", call);
+    const Wide g = reinterpret_cast<uintptr_t>(A->grad), x = reinterpret_cast<uintptr_t>(A->logits);
+    if (g == x && (A->rows == 1 || gs == xs)) return 0;
+    auto lowest = [&](Wide at, Wide stride) { return stride < 0 ? at + (A->rows - 1) * stride : at; };
+    auto end = [&](Wide at, Wide stride) { return (stride < 0 ? at : at + (A->rows - 1) * stride) + width; };
+    if (end(g, gs) <= lowest(x, xs) || end(x, xs) <= lowest(g, gs)) return 0;
+    // views side by side of one wider array
+    const Wide step = gs < 0 ? -gs : gs, apart = step ? ((g - x) % step + step) % step : 0;
+    if (A->rows > 1 && gs == xs && apart >= width && apart <= step - width) return 0;
+    return refuse("%s: grad overlaps logits without being them", call);
+}
+
 }  // namespace
 
 extern "C" {
@@ -144,6 +162,7 @@ int hx_distill_loss(const hx_distill_args* A) {
     if (!A->rows) return 0;
     if (!A->logits || !A->loss || (A->top && (!A->index || !A->teacher)))
         return refuse("%s: logits, index, teacher or loss is missing", call);
+    if (A->grad && distill_gradient(call, A)) return -1;
     return launched(call, hx::distill_launch(*A));
 }
 

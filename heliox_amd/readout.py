@@ -14,7 +14,8 @@ a trained network, and the gradients of both.
 They take and return torch tensors on one GPU (fp32, fp16 or bf16), work on torch's current
 stream, wait for nothing, and may be captured into a graph.  Sums, softmax statistics and
 states are fp32 or wider whatever the inputs are.  Arguments that do not fit raise ValueError
-or TypeError; a failing library call raises HelioxError.
+or TypeError; sizes, values and overlaps that the library refuses, and launches that fail, raise
+HelioxError.
 """
 from __future__ import annotations
 
@@ -289,7 +290,7 @@ def distill_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
                       out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """distill_loss and, in the same pass, the gradient of sum_i weight_i loss_i by the logits
     (weight (rows,) fp32, 1 unless given), of the logits' type.  The gradient goes to ``out``
-    where that is given; it may be the logits themselves."""
+    where that is given; it may be the logits themselves, but not overlap them otherwise."""
     if out is None:
         _on_gpu(logits, "logits")
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)

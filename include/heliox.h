@@ -559,7 +559,8 @@ int hx_linear_attention_step(const hx_attention_args* args);
  *          them is a mask).
  * t is in 2^-126..2^126.  A row without entries has loss 0 and gradient 0; one whose logits
  * are all -inf has no softmax (NaN).  grad (NULL: not made) receives
- * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself. */
+ * weight_i dloss_i/dlogits (weight NULL: 1); it may be logits itself, else it overlaps nothing
+ * that the call reads (logits in part: refused). */
 typedef struct hx_distill_args {
     int64_t type, teacher_type, index_bits;               /* index_bits 32 or 64 */
     int64_t rows, vocab, top;                             /* at most 2^21, 2^20 and 2048 */

@@ -391,3 +391,18 @@ def test_distill_temperatures_at_the_ends(dtype):
     outside = torch.ones(300, dtype=torch.bool, device="cuda")
     outside[index.long().unique()] = False
     assert torch.allclose(grad.float()[:, outside], torch.full_like(grad.float()[:, outside], 1 / 300), rtol=2 ** -7)
+
+
+def test_distill_gradients_beside_the_logits():
+    """Halves of one array, and an array of its own with rows further apart, are taken; parts are refused."""
+    x, index, t, lse, weight = problem(13, torch.float32, 6, 500, 9, 1.0)
+    want = readout.distill_loss_grad(x, index, t, teacher_lse=lse, weight=weight)[1]
+    both = torch.cat([x, torch.zeros_like(x)], dim=1)
+    for out in (both[:, 500:], torch.zeros(6, 777, device="cuda")[:, 5:505]):
+        readout.distill_loss_grad(both[:, :500], index, t, teacher_lse=lse, weight=weight, out=out)
+        assert torch.equal(out, want) and torch.equal(both[:, :500], x)
+    one = x[:1].expand(6, -1)
+    for logits, out in ((x, torch.zeros(1, 500, device="cuda").expand(6, -1)), (both[:, :500], both[:, 1:501]), (one, one)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            readout.distill_loss_grad(logits, index, t, teacher_lse=lse, out=out)
+    assert torch.equal(readout.distill_loss_grad(one, index, t)[1], readout.distill_loss_grad(one.contiguous(), index, t)[1])

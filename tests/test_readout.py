@@ -153,3 +153,25 @@ def test_states_written_over_those_read_are_refused(call, out, inp):
         fields[inp], fields[out] = 1 << 20, (1 << 20) + apart
         assert getattr(lib(), call)(readout._ATTENTION.pack(*fields)) == -1
         assert ("overlaps" in error()) == refused and ("workspace" in error()) != refused
+
+
+@pytest.mark.parametrize("kind,size", [(0, 4), (1, 2)])
+@pytest.mark.parametrize("rows,vocab,apart,logits_stride,grad_stride,text", [
+    (4, 10, 0, 10, 0, "each other"),        # an expanded row
+    (4, 10, 500, 10, 9, "each other"),
+    (4, 10, 500, 10, -9, "each other"),
+    (4, 10, 1, 10, 10, "without being"),    # one element further
+    (4, 10, -39, 10, 10, "without being"),
+    (4, 10, 0, 10, 20, "without being"),    # the same start, other rows
+    (4, 10, 10, 20, 30, "without being"),
+    (4, 10, 9, 20, 20, "without being"),
+    (4, 10, 0, 0, 10, "without being"),
+    (1, 10, 9, 0, 0, "without being"),
+    (4, 10, -30, -10, 10, "without being")])
+def test_a_gradient_that_overlaps_is_refused(kind, size, rows, vocab, apart, logits_stride, grad_stride, text):
+    """Pointers are only compared here: the call ends before anything is launched."""
+    at = 1 << 20
+    record = readout._DISTILL.pack(kind, 0, 32, rows, vocab, 0, at, logits_stride, 0, 0, 0, 0, 0, 0, 1.0, 1 << 30,
+                                   at + apart * size, grad_stride, 0)
+    assert lib().hx_distill_loss(record) == -1
+    assert text in error()
