@@ -20,6 +20,7 @@ HelioxError.
 from __future__ import annotations
 
 import functools
+import operator
 import struct
 from typing import Optional, Tuple, Union
 
@@ -75,6 +76,33 @@ def _array(x: Optional[torch.Tensor], what: str, dtype: torch.dtype, shape: tupl
     if x.shape != shape:
         raise ValueError(f"{what} has shape {tuple(x.shape)}, expected {tuple(shape)}")
     return x if x.is_contiguous() else x.contiguous()
+
+
+def _real(x, what: str) -> float:
+    if type(x) is float:
+        return x
+    try:
+        if isinstance(x, (str, bytes)):
+            raise TypeError
+        return float(x)
+    except OverflowError:
+        raise ValueError(f"{what} is too large a number") from None
+    except (TypeError, ValueError):
+        raise TypeError(f"{what} has to be a number, got {type(x).__name__}") from None
+
+
+def _scale(scale, dk: int) -> float:
+    return dk ** -0.5 if scale is None else _real(scale, "scale")
+
+
+def _whole(x, what: str) -> int:
+    try:
+        x = operator.index(x)
+    except TypeError:
+        raise TypeError(f"{what} has to be a whole number, got {type(x).__name__}") from None
+    if not -2 ** 63 <= x < 2 ** 63:
+        raise ValueError(f"{what} is too large a number")
+    return x
 
 
 def _ptr(x: Optional[torch.Tensor]) -> int:
@@ -169,7 +197,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     lengths = _lengths(lengths, batch, device)
     o = torch.empty((batch, time, heads, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((batch, heads, dk, dv), dtype=torch.float32, device=q.device)
-    head = (*fields, _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, o.data_ptr(),
+    head = (*fields, _ptr(initial_state), _ptr(lengths), _scale(scale, dk), o.data_ptr(),
             time * heads * dv, heads * dv, dv, end.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     _run_attention("hx_linear_attention", device, head, 0)
     return o, end
@@ -211,7 +239,7 @@ def linear_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     lengths = _lengths(lengths, batch, device)
     dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
     dinitial = None if initial_state is None else torch.empty_like(initial_state)
-    head = (*fields, _ptr(initial_state), _ptr(lengths), dk ** -0.5 if scale is None else scale, 0, 0, 0, 0, 0,
+    head = (*fields, _ptr(initial_state), _ptr(lengths), _scale(scale, dk), 0, 0, 0, 0, 0,
             do.data_ptr(), *do.stride()[:3], _ptr(dstate), dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(),
             _ptr(dinitial), 0, 0, 0)
     _run_attention("hx_linear_attention_grad", device, head, 1)
@@ -234,7 +262,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     slots = _array(slots, "slots", torch.int32, (batch,), device)
     o = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
-        *fields, 0, 0, dk ** -0.5 if scale is None else scale, o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
+        *fields, 0, 0, _scale(scale, dk), o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
         0, 0, state.data_ptr(), _ptr(slots), state.shape[0], 0, 0, _stream(device)))
     return o
 
@@ -267,8 +295,8 @@ def _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, we
     _call("hx_distill_loss", device, _DISTILL.pack(
         kind, teacher_kind, 32 if teacher_index.dtype == torch.int32 else 64, rows, vocab, teacher_index.shape[1],
         _ptr(logits), logits.stride(0), _ptr(teacher_index), teacher_index.stride(0), _ptr(teacher_logits),
-        teacher_logits.stride(0), _ptr(teacher_lse), _ptr(weight), temperature, _ptr(loss), _ptr(grad),
-        0 if grad is None else grad.stride(0), _stream(device)))
+        teacher_logits.stride(0), _ptr(teacher_lse), _ptr(weight), _real(temperature, "temperature"), _ptr(loss),
+        _ptr(grad), 0 if grad is None else grad.stride(0), _stream(device)))
     return loss
 
 
@@ -331,7 +359,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
             values.append(0)
         else:
             pointers.append(None)
-            values.append(x)
+            values.append(_whole(x, name) if dtype is torch.int32 else _real(x, name))
     token = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
     _call("hx_sample", device, _SAMPLE.pack(

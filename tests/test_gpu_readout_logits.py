@@ -406,3 +406,33 @@ def test_distill_gradients_beside_the_logits():
         with pytest.raises(RuntimeError, match="overlap"):
             readout.distill_loss_grad(logits, index, t, teacher_lse=lse, out=out)
     assert torch.equal(readout.distill_loss_grad(one, index, t)[1], readout.distill_loss_grad(one.contiguous(), index, t)[1])
+
+
+def test_settings_that_are_no_numbers_are_refused():
+    x, index, t, *_ = problem(14, torch.float32, 2, 50, 3, 1.0)
+    u = torch.rand(2, device="cuda")
+    q = torch.randn(1, 3, 2, 8, device="cuda")
+    g = torch.zeros(2, device="cuda")
+    bad = [
+        (TypeError, lambda: readout.sample(x, u, top_k=50.0)),
+        (TypeError, lambda: readout.sample(x, u, top_k="5")),
+        (TypeError, lambda: readout.sample(x, u, top_k=None)),
+        (ValueError, lambda: readout.sample(x, u, top_k=2 ** 63)),
+        (TypeError, lambda: readout.sample(x, u, temperature="1.0")),
+        (TypeError, lambda: readout.sample(x, u, top_p=None)),
+        (TypeError, lambda: readout.sample(x, u, min_p=[0.1])),
+        (ValueError, lambda: readout.sample(x, u, temperature=10 ** 400)),
+        (TypeError, lambda: readout.distill_loss(x, index, t, temperature="warm")),
+        (ValueError, lambda: readout.distill_loss_grad(x, index, t, temperature=10 ** 400)),
+        (TypeError, lambda: readout.linear_attention(q, q, q, g, scale="1")),
+        (TypeError, lambda: readout.linear_attention_grad(q, q, q, g, q, scale=[1.0])),
+        (ValueError, lambda: readout.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g, q.new_zeros(1, 2, 8, 8), scale=10 ** 400)),
+    ]
+    for error, call in bad:
+        with pytest.raises(error):
+            call()
+    import numpy as np
+    same = readout.sample(x, u, temperature=0.5, top_k=5, top_p=0.75, min_p=0.25)
+    other = readout.sample(x, u, temperature=np.float32(0.5), top_k=np.int64(5), top_p=np.float64(0.75), min_p=np.float32(0.25))
+    assert all(torch.equal(a, b) for a, b in zip(same, other))
+    assert all(torch.equal(a, b) for a, b in zip(readout.sample(x, u, temperature=1, top_p=1, min_p=0), readout.sample(x, u)))
