@@ -15,7 +15,8 @@ They take and return torch tensors on one GPU (fp32, fp16 or bf16), work on torc
 stream, wait for nothing, and may be captured into a graph.  Sums, softmax statistics and
 states are fp32 or wider whatever the inputs are.  Arguments that do not fit raise ValueError
 or TypeError; sizes, values and overlaps that the library refuses, and launches that fail, raise
-HelioxError.
+HelioxError.  Results carry no graph for autograd: gradients are calls of their own, and the calls
+that have one refuse inputs that require a gradient while torch records.
 """
 from __future__ import annotations
 
@@ -39,6 +40,16 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 # A call's checks are most of a small call's time, so each goes the short way first (attributes
 # compared as they are, devices as numbers, 50-80 ns each) and finds out what is wrong only where
 # something is.
+
+
+def _no_graph(call: str, instead: str, *inputs: Optional[torch.Tensor]) -> None:
+    """Results here carry no autograd graph: where one is being recorded, a gradient that an input
+    asks for would be lost in silence."""
+    if torch.is_grad_enabled():
+        for x in inputs:
+            if x is not None and x.requires_grad:
+                raise ValueError(f"{call} records no graph for autograd, and an input requires a gradient: "
+                                 f"{instead}, and call {call} under torch.no_grad() or in an autograd.Function")
 
 
 def _type(x: torch.Tensor, what: str) -> int:
@@ -194,6 +205,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     device, kept, fields = _attention_inputs(q, k, v, log_decay, 4)
     _, batch, time, heads, _, _, _, dk, dv = fields[:9]
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, heads, dk, dv), device)
+    _no_graph("linear_attention", "take it from linear_attention_grad", q, k, v, log_decay, initial_state)
     lengths = _lengths(lengths, batch, device)
     o = torch.empty((batch, time, heads, dv), dtype=q.dtype, device=q.device)
     end = torch.empty((batch, heads, dk, dv), dtype=torch.float32, device=q.device)
@@ -259,6 +271,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         raise TypeError(f"state has to be a contiguous float32 tensor on {q.device}")
     if state.dim() != 4 or state.shape[1:] != (heads, dk, dv):
         raise ValueError(f"state has shape {tuple(state.shape)}, expected (n_slots, {heads}, {dk}, {dv})")
+    _no_graph("linear_attention_step", "take it from linear_attention_grad over the steps", q, k, v, log_decay, state)
     slots = _array(slots, "slots", torch.int32, (batch,), device)
     o = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
@@ -309,6 +322,9 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
     sum exp(logit / temperature) over the teacher's whole vocabulary, its mass on all other
     places is one more class, but where the student's mask leaves none of them (their mass is
     under 2^-1074).  A row without entries has loss 0."""
+    for x, name in ((logits, "logits"), (teacher_logits, "teacher_logits")):
+        _on_gpu(x, name)
+    _no_graph("distill_loss", "take it from distill_loss_grad", logits, teacher_logits, teacher_lse)
     return _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, None, None)
 
 
@@ -344,7 +360,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 
     Masses are whole numbers (2^-40 of the largest), so that an answer does not depend on the
     order of a sum: what is less than 2^-40 times as probable as the largest is never drawn.
-    NaN counts as -inf; a row without a finite logit gives token -1."""
+    NaN counts as -inf; a row without a finite logit gives token -1.  Neither result carries a
+    gradient."""
     device, kind, logits = _logits(logits)
     rows, vocab = logits.shape
     u = _array(u, "u", torch.float32, (rows,), device)

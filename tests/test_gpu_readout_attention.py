@@ -433,3 +433,51 @@ def test_nothing_but_nan_ends(dtype):
     want = ref.attention(q, k, v, g, 32 ** -0.5, state)
     check_reach(o, want[0], dtype, "o")
     check_reach(end, want[1], torch.float32, "end")
+
+
+def test_gradients_are_not_lost_in_silence():
+    """While torch records, inputs that require a gradient are refused; under no_grad they are not."""
+    q, k, v, g, state, do, dend = make(61, torch.float32, 1, 9, 2, 2, 2, 2, 8, 8)
+    x, index, t = q[0, :, 0], torch.zeros(9, 1, dtype=torch.int32, device="cuda"), torch.zeros(9, 1, device="cuda")
+    lse = torch.ones(9, device="cuda")
+
+    def calls(q=q, k=k, v=v, g=g, state=state, x=x, t=t, lse=lse):
+        return {"attention": lambda: readout.linear_attention(q, k, v, g, initial_state=state),
+                "step": lambda: readout.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state),
+                "distill": lambda: readout.distill_loss(x, index, t, teacher_lse=lse)}
+
+    asks = lambda y: y.clone().requires_grad_()  # noqa: E731
+    for names, given in ((("attention", "step"), {"q": asks(q)}), (("attention", "step"), {"k": asks(k)}),
+                         (("attention", "step"), {"v": asks(v)}), (("attention", "step"), {"g": asks(g)}),
+                         (("attention", "step"), {"state": asks(state)}), (("distill",), {"x": asks(x)}),
+                         (("distill",), {"t": asks(t)}), (("distill",), {"lse": asks(lse)})):
+        for name in names:
+            with pytest.raises(ValueError, match="_grad"):
+                calls(**given)[name]()
+            with torch.no_grad():
+                calls(**given)[name]()
+    # the calls that make gradients take what their gradients are for
+    readout.linear_attention_grad(asks(q), asks(k), asks(v), g, do, initial_state=asks(state))
+    readout.distill_loss_grad(asks(x), index, t)
+    readout.sample(asks(x), lse * 0.5)
+
+
+def test_the_pair_of_calls_in_an_autograd_function():
+    """As a model whose other parts are torch's would use them."""
+    class Attention(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, g):
+            ctx.save_for_backward(q, k, v, g)
+            return readout.linear_attention(q, k, v, g)
+
+        @staticmethod
+        def backward(ctx, do, dstate):
+            q, k, v, g = ctx.saved_tensors
+            return (*readout.linear_attention_grad(q, k, v, g, do, dstate=dstate)[:3], None)
+
+    q, k, v, g, state, do, dend = make(67, torch.float32, 2, 70, 4, 4, 2, 4, 16, 24)
+    leaves = [y.clone().requires_grad_() for y in (q, k, v)]
+    o, end = Attention.apply(*leaves, g)
+    torch.autograd.backward([o, end], [do, dend])
+    want = readout.linear_attention_grad(q, k, v, g, do, dstate=dend)
+    assert all(torch.equal(y.grad, w) for y, w in zip(leaves, want))
