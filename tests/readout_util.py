@@ -104,3 +104,21 @@ def rel(got, want):
     norm = float(want.norm())
     off = float((got - want).norm())
     return off / norm if norm else off
+
+
+def captured(call, change):
+    """The call, captured once and replayed three times with other inputs and its own eager runs in
+    between, gives what it gives by itself."""
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for n in range(3):
+        change(torch.Generator().manual_seed(n))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [x.clone() for x in got]
+        want = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, want)), n

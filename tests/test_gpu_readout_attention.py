@@ -481,3 +481,61 @@ def test_the_pair_of_calls_in_an_autograd_function():
     torch.autograd.backward([o, end], [do, dend])
     want = readout.linear_attention_grad(q, k, v, g, do, dstate=dend)
     assert all(torch.equal(y.grad, w) for y, w in zip(leaves, want))
+
+
+def head_bounds(got, want, dtype, dim):
+    """Head by head, so that slow heads do not drown fast ones.  16 bits: as far off as the result's own
+    rounding, and a dozen terms of 2^-17.  fp32: sums of up to 2^8 terms a chunk and 2^6 chunks whose
+    roundings are independent, 2^4 units, and the decays' units, 2^4 more."""
+    x, w = by_head(got, dim), by_head(want, dim)
+    off, size = (x - w).norm(dim=1), w.norm(dim=1)
+    if dtype == torch.float32:
+        return off, 2 ** 5 * ref.UNIT[dtype] * size
+    return off, 1.01 * (by_head(want.to(dtype), dim) - w).norm(dim=1) + 12 * 2.0 ** -17 * size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,lengths", [
+    ((1, 900, 4, 4, 4, 4, 128, 128), None), ((2, 700, 3, 3, 1, 3, 96, 80), [700, 333]),
+    ((1, 800, 2, 2, 2, 2, 256, 256), None), ((2, 1100, 2, 2, 2, 2, 33, 47), [1100, 20]),
+    ((1, 1600, 4, 4, 4, 4, 64, 64), None), ((2, 1000, 4, 4, 4, 4, 64, 64), [400, 1000]),
+    ((1, 1300, 2, 1, 2, 2, 47, 33), [900]), ((1, 800, 2, 2, 2, 2, 160, 200), [500])])
+def test_segments_of_every_cut(dtype, shape, lengths):
+    """Recordings long enough to be cut into segments, at head sizes of each way to lay them out."""
+    batch, time, heads, qh, kh, vh, dk, dv = shape
+    print(f"case segments {dtype} {shape} {lengths}", flush=True)
+    q, k, v, g, state, do, dend = make(71, dtype, *shape)
+    at = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    o, end = readout.linear_attention(q, k, v, g, initial_state=state, lengths=at)
+    got = readout.linear_attention_grad(q, k, v, g, do, initial_state=state, lengths=at, dstate=dend)
+    want = ref.attention(q, k, v, g, dk ** -0.5, state, lengths, do, dend)
+    kinds = (dtype, torch.float32, dtype, dtype, dtype, torch.float32)
+    for x, w, kind, dim, name in zip((o, end, *got), want, kinds, (2, 1, 2, 2, 2, 1), ("o", "end", "dq", "dk", "dv", "d0")):
+        off, most = head_bounds(x, w, kind, dim)
+        assert bool((off <= most).all()), (name, (off / most).tolist())
+
+
+def test_products_past_the_largest_fp16():
+    """q.k and the state pass 65504, the outputs do not."""
+    q, k, v, g, *_ = make(73, torch.float16, 1, 130, 2, 2, 2, 2, 64, 64)
+    g = torch.full((2,), -0.003, device="cuda")
+    q, k = q * 100, k * 100
+    dots = (q.double().transpose(1, 2) @ k.double().transpose(1, 2).transpose(2, 3)).tril()
+    assert float(dots.abs().max()) > 3 * 65504
+    o, end = readout.linear_attention(q, k, v * 20, g, scale=1e-5)
+    want = ref.attention(q, k, v * 20, g, 1e-5)
+    assert float(want[1].abs().max()) > 1e4 and float(want[0].abs().max()) < 65504
+    off, most = head_bounds(o, want[0], torch.float16, 2)
+    assert bool((off <= most).all())
+    off, most = head_bounds(end, want[1], torch.float32, 1)
+    assert bool((off <= most).all())
+
+
+def test_gradient_captured_into_a_graph():
+    q, k, v, g, state, do, dend = make(79, torch.bfloat16, 1, 900, 4, 4, 2, 4, 64, 48)
+
+    def change(gen):
+        q.copy_(torch.randn(q.shape, generator=gen).to(q.dtype))
+        do.copy_(torch.randn(do.shape, generator=gen).to(do.dtype))
+
+    ref.captured(lambda: readout.linear_attention_grad(q, k, v, g, do, initial_state=state, dstate=dend), change)

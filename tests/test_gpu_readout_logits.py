@@ -436,3 +436,45 @@ def test_settings_that_are_no_numbers_are_refused():
     other = readout.sample(x, u, temperature=np.float32(0.5), top_k=np.int64(5), top_p=np.float64(0.75), min_p=np.float32(0.25))
     assert all(torch.equal(a, b) for a, b in zip(same, other))
     assert all(torch.equal(a, b) for a, b in zip(readout.sample(x, u, temperature=1, top_p=1, min_p=0), readout.sample(x, u)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_rows_of_half_a_chip(dtype, rest):
+    """600 rows take 512 threads each."""
+    x, index, t, lse, weight = problem(15, dtype, 600, 5003, 12, 1.0)
+    check(x, index, t, 1.0, lse if rest else None, weight, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_many_rows_of_several_turns(dtype):
+    """1100 rows take 256 threads each, and a row of 5003 places several turns of them."""
+    gen = torch.Generator().manual_seed(16)
+    x = (torch.randn(1100, 5003, generator=gen) * 3).to(dtype).cuda()
+    u = torch.rand(1100, generator=gen).cuda()
+    pick = lambda *v: torch.tensor(v)[torch.randint(len(v), (1100,), generator=gen)].cuda()  # noqa: E731
+    check_draws(x, u, pick(0.0, 0.5, 1.0, 2.0), pick(0, 1, 7, 100, 900).to(torch.int32), pick(0.3, 0.9, 1.0), pick(0.0, 0.05))
+
+
+@pytest.mark.parametrize("vocab", [1000, 600_001])     # the bit map of the latter: over 64 KB of LDS
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_captured_into_a_graph(rest, vocab):
+    x, index, t, lse, weight = problem(17, torch.bfloat16, 3, vocab, 20, 1.0)
+    lse = lse if rest else None
+    ref.captured(lambda: (readout.distill_loss(x, index, t, teacher_lse=lse),
+                          *readout.distill_loss_grad(x, index, t, teacher_lse=lse, weight=weight)),
+                 lambda gen: x.copy_((torch.randn(x.shape, generator=gen) * 3).to(x.dtype)))
+
+
+@pytest.mark.parametrize("vocab", [1000, 3_000_000])   # the sums by turn of the latter: over 32 KB of LDS
+def test_sample_captured_into_a_graph(vocab):
+    x = torch.zeros(3, vocab, dtype=torch.bfloat16, device="cuda")
+    u = torch.zeros(3, device="cuda")
+
+    def change(gen):
+        x.copy_((torch.randn(x.shape, generator=gen) * 3).to(x.dtype))
+        u.copy_(torch.rand(3, generator=gen))
+
+    change(torch.Generator().manual_seed(9))
+    ref.captured(lambda: (*readout.sample(x, u), *readout.sample(x, u, top_k=30, top_p=0.9), *readout.sample(x, u, top_p=0.8)),
+                 change)
