@@ -37,6 +37,24 @@ template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(f
     return __float2bfloat16(x);
 }
 
+// 16 bytes of a row of logits; pieces start at any element.
+template <class T> struct PieceOf;
+template <> struct PieceOf<float> { typedef float Vec __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct PieceOf<__half> { typedef _Float16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct PieceOf<__hip_bfloat16> { typedef __bf16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
+
+// x reduced over the workgroup's waves, by way of sh (one for each wave); every thread gets the result.
+template <int kThreads, class W, class V, class F>
+__device__ __forceinline__ V block_reduce(V x, W* sh, F op) {
+    for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) sh[threadIdx.x / 64] = x;
+    __syncthreads();
+    x = static_cast<V>(sh[threadIdx.x % (kThreads / 64)]);
+    for (int m = kThreads / 128; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
+    return x;
+}
+
 // Calls f with a value of the element type that `type` names.
 template <class F>
 auto with_type(int64_t type, F&& f) {

@@ -17,25 +17,8 @@
 namespace hx {
 namespace {
 
-template <class T> struct PieceOf;
-template <> struct PieceOf<float> { typedef float Vec __attribute__((ext_vector_type(4), aligned(4))); };
-template <> struct PieceOf<__half> { typedef _Float16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
-template <> struct PieceOf<__hip_bfloat16> { typedef __bf16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
-
 // 2^x by the instruction: one unit off at most, 0 under 2^-126.
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// x reduced over the workgroup's waves; every thread gets the result.
-template <int kThreads, class V, class F>
-__device__ __forceinline__ V block_reduce(V x, double* sh, F op) {
-    for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) sh[threadIdx.x / 64] = x;
-    __syncthreads();
-    x = static_cast<V>(sh[threadIdx.x % (kThreads / 64)]);
-    for (int m = kThreads / 128; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
-    return x;
-}
 
 template <class I>
 __device__ __forceinline__ int entry(const void* index, long long at, int vocab) {

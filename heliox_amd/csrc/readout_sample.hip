@@ -20,11 +20,6 @@ constexpr float kMass = 1099511627776.f;      // 2^40
 constexpr float kDepth = 27.8f;               // e^-27.8 < 2^-40: no mass beyond
 typedef unsigned long long u64;
 
-template <class T> struct PieceOf;
-template <> struct PieceOf<float> { typedef float Vec __attribute__((ext_vector_type(4), aligned(4))); };
-template <> struct PieceOf<__half> { typedef _Float16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
-template <> struct PieceOf<__hip_bfloat16> { typedef __bf16 Vec __attribute__((ext_vector_type(8), aligned(2))); };
-
 // Order-preserving key of a logit: larger key, larger logit; -0 and 0 alike, NaN as -inf.
 __device__ __forceinline__ unsigned key_of(float x) {
     if (x != x) x = -INFINITY;
@@ -45,21 +40,9 @@ struct Shared {
     unsigned count;
 };
 
-// x reduced over the workgroup; every thread gets the result.
-template <class Sh, class V, class F>
-__device__ __forceinline__ V block_reduce(V x, Sh& sh, F op) {
-    for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) sh.part[threadIdx.x / 64] = x;
-    __syncthreads();
-    x = static_cast<V>(sh.part[0]);
-    for (int w = 1; w < Sh::kWaves; ++w) x = op(x, static_cast<V>(sh.part[w]));
-    return x;
-}
-
 template <class Sh>
 __device__ __forceinline__ u64 block_sum(u64 x, Sh& sh) {
-    return block_reduce(x, sh, [](u64 a, u64 b) { return a + b; });
+    return block_reduce<Sh::kThreads>(x, sh.part, [](u64 a, u64 b) { return a + b; });
 }
 
 __device__ __forceinline__ u64 wave_before(u64 x) {       // sum over the lanes before this one
@@ -196,8 +179,8 @@ __device__ __forceinline__ unsigned refine(const R_& R, Sh& sh, V value, P passe
                 hi = max(hi, k);
             }
     });
-    lo = block_reduce(lo, sh, [](unsigned a, unsigned b) { return min(a, b); });
-    hi = block_reduce(hi, sh, [](unsigned a, unsigned b) { return max(a, b); });
+    lo = block_reduce<Sh::kThreads>(lo, sh.part, [](unsigned a, unsigned b) { return min(a, b); });
+    hi = block_reduce<Sh::kThreads>(hi, sh.part, [](unsigned a, unsigned b) { return max(a, b); });
     while (lo < hi) {
         int shift = 0;
         while ((hi - lo) >> shift >= kBins) ++shift;
@@ -356,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) most = fmaxf(most, v[i]);
     });
-    R.most = value_of(block_reduce(key_of(most), sh, [](unsigned a, unsigned b) { return max(a, b); }));
+    R.most = value_of(block_reduce<kThreads>(key_of(most), sh.part, [](unsigned a, unsigned b) { return max(a, b); }));
     auto answer = [&](int j, float v, u64 total) {
         A.token[row] = j;
         A.logprob[row] = R.depth(v) - logf(static_cast<float>(total) / kMass);
@@ -375,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(hx_sample_args A) {
             for (int i = 0; i < kP; ++i)
                 if (v[i] == R.most) first = min(first, j0 + i);
         });
-        first = block_reduce(first, sh, [](int a, int b) { return min(a, b); });
+        first = block_reduce<kThreads>(first, sh.part, [](int a, int b) { return min(a, b); });
         if (threadIdx.x == 0) answer(first, R.most, static_cast<u64>(kMass));
         return;
     }
