@@ -20,10 +20,21 @@ namespace {
 // 2^x by the instruction: one unit off at most, 0 under 2^-126.
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <class I>
-__device__ __forceinline__ int entry(const void* index, long long at, int vocab) {
-    const I j = static_cast<const I*>(index)[at];
-    return j >= 0 && j < vocab ? static_cast<int>(j) : -1;
+// The k-th of a row's entries: its place (-1: absent), and the teacher's logit.  Indexes and teachers
+// of every type go through one kernel: only the few entries are read so.
+__device__ __forceinline__ int place_of(const hx_distill_args& A, long long row, int k) {
+    const long long at = row * A.index_stride + k;
+    const long long j = A.index_bits == 64 ? static_cast<const int64_t*>(A.index)[at] : static_cast<const int32_t*>(A.index)[at];
+    return j >= 0 && j < A.vocab ? static_cast<int>(j) : -1;
+}
+
+__device__ __forceinline__ float teacher_of(const hx_distill_args& A, long long row, int k) {
+    const long long at = row * A.teacher_stride + k;
+    switch (A.teacher_type) {
+        case HX_F16: return to_f32(static_cast<const __half*>(A.teacher)[at]);
+        case HX_BF16: return to_f32(static_cast<const __hip_bfloat16*>(A.teacher)[at]);
+        default: return static_cast<const float*>(A.teacher)[at];
+    }
 }
 
 // LDS: places and teacher's shares of the row's entries, the student's logits there, and, where
@@ -31,7 +42,7 @@ __device__ __forceinline__ int entry(const void* index, long long at, int vocab)
 // Weights are 2^((x - max) cold), cold = log2 e / temperature: the difference comes first, so
 // that an error of the product is one of the small difference and not of the logit.  What the
 // few entries take, logarithms that nearly cancel, is 64 bits wide; per = 1 / temperature.
-template <class T, class U, class I, int kThreads, bool kRest>
+template <class T, int kThreads, bool kRest>
 __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, float cold, double per) {
     using Vec = typename PieceOf<T>::Vec;
     constexpr int kP = sizeof(Vec) / sizeof(T);
@@ -45,7 +56,6 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     unsigned* member = reinterpret_cast<unsigned*>(logit + top);
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(A.logits) + row * A.logits_stride;
-    const U* t = static_cast<const U*>(A.teacher) + row * A.teacher_stride;
     const float tau = static_cast<float>(A.temperature);
     auto add = [](auto a, auto b) { return a + b; };
     auto most = [](float a, float b) { return fmaxf(a, b); };
@@ -60,9 +70,9 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     }
     float tmax = -INFINITY, some = 0.f, lead = -INFINITY;
     for (int k = threadIdx.x; k < top; k += kThreads) {
-        const int j = entry<I>(A.index, row * A.index_stride + k, vocab);
+        const int j = place_of(A, row, k);
         place[k] = j;
-        share[k] = j >= 0 ? to_f32(t[k]) : -INFINITY;
+        share[k] = j >= 0 ? teacher_of(A, row, k) : -INFINITY;
         logit[k] = j >= 0 ? to_f32(x[j]) : 0.f;
         if (j >= 0) {
             some = 1.f;
@@ -220,10 +230,10 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     }
 }
 
-template <class T, class U, class I, int kThreads, bool kRest>
+template <class T, int kThreads, bool kRest>
 hipError_t launch(const hx_distill_args& A) {
     const size_t lds = sizeof(int) * (3 * A.top + (kRest ? (A.vocab + 31) / 32 : 0));
-    auto kernel = k_distill<T, U, I, kThreads, kRest>;
+    auto kernel = k_distill<T, kThreads, kRest>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, 163840 - 256);
@@ -234,7 +244,7 @@ hipError_t launch(const hx_distill_args& A) {
     return hipGetLastError();
 }
 
-template <class T, class U, class I>
+template <class T>
 hipError_t pick(const hx_distill_args& A) {
     // Threads a row.  A CU holds 2048: rows of a last, thin round run alone, so 512 threads
     // where that fits all rows into one round and 1024 does not (517 rows of 50021: 42 us with
@@ -242,9 +252,9 @@ hipError_t pick(const hx_distill_args& A) {
     const bool small = A.vocab <= 4096, half = A.rows > 512 && A.rows <= 1024;
     auto go = [&](auto rest) {
         constexpr bool kRest = decltype(rest)::value;
-        return small  ? launch<T, U, I, 256, kRest>(A)
-               : half ? launch<T, U, I, 512, kRest>(A)
-                      : launch<T, U, I, 1024, kRest>(A);
+        return small  ? launch<T, 256, kRest>(A)
+               : half ? launch<T, 512, kRest>(A)
+                      : launch<T, 1024, kRest>(A);
     };
     return A.teacher_lse ? go(std::true_type{}) : go(std::false_type{});
 }
@@ -252,13 +262,7 @@ hipError_t pick(const hx_distill_args& A) {
 }  // namespace
 
 hipError_t distill_launch(const hx_distill_args& A) {
-    return with_type(A.type, [&](auto t) {
-        return with_type(A.teacher_type, [&](auto u) {
-            using T = decltype(t);
-            using U = decltype(u);
-            return A.index_bits == 64 ? pick<T, U, int64_t>(A) : pick<T, U, int32_t>(A);
-        });
-    });
+    return with_type(A.type, [&](auto t) { return pick<decltype(t)>(A); });
 }
 
 }  // namespace hx
