@@ -160,7 +160,14 @@ struct MathBf16 {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
     }
     static __device__ __forceinline__ Frag frag(f32x4 x) { return __builtin_convertvector(x, Frag); }
-    static __device__ __forceinline__ f32x4 wide(Frag x) { return __builtin_convertvector(x, f32x4); }
+    // (from the packed bits: converted one by one, the numbers are rounded once more for it)
+    static __device__ __forceinline__ f32x4 wide(Frag x) {
+        typedef unsigned Two __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const Two u = __builtin_bit_cast(Two, x);
+        const f32x2 even = __builtin_bit_cast(f32x2, u << 16), odd = __builtin_bit_cast(f32x2, u & 0xffff0000u);
+        return f32x4{even[0], odd[0], even[1], odd[1]};
+    }
     static __device__ __forceinline__ Pair pair(Frag a, Frag b) {
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
@@ -284,8 +291,8 @@ struct MathF16 {
     static __device__ __forceinline__ Pair split(Raw x) {
         typedef float f32x8 __attribute__((ext_vector_type(8)));
         const f32x8 w = __builtin_convertvector(x, f32x8);
-        const bf16x8 h = __builtin_convertvector(w, bf16x8);
-        return {h, __builtin_convertvector(w - __builtin_convertvector(h, f32x8), bf16x8)};
+        const SumPair p = One::sum_pair(One::sum(w.lo), One::sum(w.hi));
+        return {p.h, p.l};
     }
     template <int kPlane>
     static __device__ __forceinline__ void store(Elem* at, Raw x) {
