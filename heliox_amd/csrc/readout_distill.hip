@@ -48,7 +48,8 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     constexpr int kP = sizeof(Vec) / sizeof(T);
     extern __shared__ int lds[];
     __shared__ double red[kThreads / 64];
-    __shared__ int twice;                    // whether two entries stand at one place
+    __shared__ float made[3];
+    __shared__ int any, twice;               // whether there is an entry, and whether two stand at one place
     const int top = static_cast<int>(A.top), vocab = static_cast<int>(A.vocab);
     int* place = lds;
     float* share = reinterpret_cast<float*>(lds + top);
@@ -65,25 +66,38 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
 
     if constexpr (kRest) {
         for (int w = threadIdx.x; w < (vocab + 31) / 32; w += kThreads) member[w] = 0;
-        if (threadIdx.x == 0) twice = 0;
-        __syncthreads();
     }
-    float tmax = -INFINITY, some = 0.f, lead = -INFINITY;
+    if (threadIdx.x == 0) any = twice = 0;
+    __syncthreads();
+    float tmax = -INFINITY, lead = -INFINITY;    // the entries' largest logits, the teacher's and the student's
     for (int k = threadIdx.x; k < top; k += kThreads) {
         const int j = place_of(A, row, k);
         place[k] = j;
         share[k] = j >= 0 ? teacher_of(A, row, k) : -INFINITY;
         logit[k] = j >= 0 ? to_f32(x[j]) : 0.f;
         if (j >= 0) {
-            some = 1.f;
+            any = 1;
             tmax = fmaxf(tmax, share[k]);
             lead = fmaxf(lead, logit[k]);
             if constexpr (kRest)
                 if (atomicOr(member + j / 32, 1u << (j % 32)) >> (j % 32) & 1) twice = 1;
         }
     }
-    some = block_reduce<kThreads>(some, red, most);
-    if constexpr (!kRest) tmax = block_reduce<kThreads>(tmax, red, most);
+    if constexpr (kRest) lead = block_reduce<kThreads>(lead, red, most);
+    else tmax = block_reduce<kThreads>(tmax, red, most);
+    const bool some = any;
+    double own = 0.;                             // the entries' weights, relative to the largest of them
+    if constexpr (kRest) {
+        if (lead == -INFINITY) lead = 0.f;
+        float mine = 0.f;
+        for (int k = threadIdx.x; k < top; k += kThreads) {
+            bool counts = place[k] >= 0;
+            if (twice)                           // a place counts once
+                for (int i = 0; i < k; ++i) counts = counts && place[i] != place[k];
+            if (counts) mine += weight(logit[k] - lead);
+        }
+        own = block_reduce<kThreads>(static_cast<double>(mine), red, add);
+    }
 
     // the student's running maximum and sum over all places, or over those without an entry (bits
     // of `in`: an entry)
@@ -146,22 +160,21 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     double whole = block_reduce<kThreads>(static_cast<double>(z * weight(mine - m)), red, add);
     const float base = m;                       // what the other places' weights are relative to
     const double beside = whole;                // their sum (0: nothing but -inf)
-    double under = 1.;                          // e^{(base - m) / t}
-    if constexpr (kRest) {
-        lead = block_reduce<kThreads>(lead, red, most);
-        m = beside != 0. ? fmaxf(base, lead) : lead > -INFINITY ? lead : 0.f;
-        under = beside != 0. ? exp((static_cast<double>(base) - m) * per) : 0.;
-        float own = 0.f;
-        for (int k = threadIdx.x; k < top; k += kThreads) {
-            bool counts = place[k] >= 0;
-            if (twice)                          // a place counts once
-                for (int i = 0; i < k; ++i) counts = counts && place[i] != place[k];
-            if (counts) own += weight(logit[k] - m);
+    // From here to the gradient it is the row as a whole and its entries: waves without entries leave
+    // the 64-bit exponentials and logarithms to the others (made by all 16 waves of a row they took
+    // 3 to 8% of the call).
+    const bool works = threadIdx.x < 64 || static_cast<int>(threadIdx.x) / 64 * 64 < top;
+    double under = 1., logz = 0.;               // under: e^{(base - m) / t}
+    // (a side that has no weight at all does not count)
+    if constexpr (kRest) m = beside == 0. ? lead : own == 0. ? base : fmaxf(base, lead);
+    if (works) {
+        if constexpr (kRest) {
+            const double less = exp((static_cast<double>(fminf(base, lead)) - m) * per);
+            under = beside == 0. ? 0. : base < m ? less : 1.;
+            whole = beside * under + own * (lead < m ? less : 1.);
         }
-        own = block_reduce<kThreads>(own, red, add);
-        whole = beside * under + own;
+        logz = log(whole);
     }
-    const double logz = log(whole);
 
     // the teacher's shares and the row's loss
     double norm;
@@ -171,7 +184,8 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
         float mass = 0.f;
         for (int k = threadIdx.x; k < top; k += kThreads)
             if (share[k] != -INFINITY) mass += share[k] == tmax ? 1.f : expf((share[k] - tmax) / tau);
-        norm = tmax * per + log(static_cast<double>(block_reduce<kThreads>(mass, red, add)));
+        norm = block_reduce<kThreads>(static_cast<double>(mass), red, add);
+        if (works) norm = tmax * per + log(norm);
     }
     double loss = 0., psum = 0.;
     for (int k = threadIdx.x; k < top; k += kThreads) {
@@ -188,23 +202,29 @@ __global__ void __launch_bounds__(kThreads, 8) k_distill(hx_distill_args A, floa
     }
     loss = block_reduce<kThreads>(loss, red, add);
     psum = block_reduce<kThreads>(psum, red, add);
-    double inside = psum, pull = 0.;            // pull: p_r / z_o
-    if constexpr (kRest) {
-        const double pr = fmax(0., 1. - psum);
-        if (pr > 0. && beside * under > 0.) {   // a mass of 0 in 64 bits is that of masked places
-            loss += pr * (log(pr / beside) - ((static_cast<double>(base) - m) * per - logz));
-            inside = psum + pr;
-            pull = pr / beside;
+    if (threadIdx.x < 64) {
+        double inside = psum, pull = 0.;        // pull: p_r / z_o
+        if constexpr (kRest) {
+            const double pr = fmax(0., 1. - psum);
+            if (pr > 0. && beside * under > 0.) {   // a mass of 0 in 64 bits is that of masked places
+                loss += pr * (log(pr / beside) - ((static_cast<double>(base) - m) * per - logz));
+                inside = psum + pr;
+                pull = pr / beside;
+            }
+        }
+        if (threadIdx.x == 0) {
+            A.loss[row] = some ? static_cast<float>(loss * tau * tau) : 0.f;
+            made[0] = some ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
+            made[1] = static_cast<float>(made[0] * (inside * under / whole - pull));
+            made[2] = static_cast<float>(inside / whole);
         }
     }
-    if (threadIdx.x == 0) A.loss[row] = some > 0.f ? static_cast<float>(loss * tau * tau) : 0.f;
     if (!A.grad) return;
+    __syncthreads();
     T* g = static_cast<T*>(A.grad) + row * A.grad_stride;
-    const float w = some > 0.f ? tau * (A.weight ? A.weight[row] : 1.f) : 0.f;
-    const float factor = static_cast<float>(w * (inside * under / whole - pull)),
-                within = static_cast<float>(inside / whole);
+    const float w = made[0], factor = made[1], within = made[2];
     // (entries may lie far above the base; theirs are written over below)
-    auto slope = [&](float v) { return some > 0.f ? factor * weight(v - base) : 0.f; };
+    auto slope = [&](float v) { return some ? factor * weight(v - base) : 0.f; };
     each_piece([&](int p, Vec raw) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) raw[i] = static_cast<decltype(raw[0] + raw[0])>(slope(static_cast<float>(raw[i])));
