@@ -42,8 +42,10 @@ struct ScanArgs {
 // ------------------------------------------------------------------- one step
 // One workgroup per (sequence, head).  Lanes lie along a state's rows, kV columns each, so that
 // the state streams through as it lies in memory; k and q wait in LDS.  Bound by the state's
-// bytes, read and written once: 256 x 16 states of 128 x 128 in 102 us, 5.3 TB/s (a copy of as
-// much reaches 4.8).  A single row is bound by the call (11 us, 4 of them on the GPU).
+// bytes, read and written once: 256 x 16 states of 128 x 128, a twentieth of the rows without a
+// slot (510 MB), in 96 to 101 us, 5.1 to 5.3 TB/s (a copy of 2 GiB reaches 4.8; of a pool of
+// 315 MB some may stay cached from call to call).  A single row is bound by the call (11 us, 4.6
+// of them on the GPU).
 template <class T, int kV>
 __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, const int32_t* slots, long long n_slots,
                                                    int lanes) {
@@ -110,24 +112,28 @@ __global__ void __launch_bounds__(kThreads) k_step(ScanArgs S, float* states, co
 //   P_ij = scale_in scale_out e^{g (i - j)} (a_i . b_j) for j <= i
 //   y_i  = sum_j P_ij c_j + scale_out e^{g (i + off)} X^T a_i
 //   X'   = e^{g n} X + sum_j b_j (scale_in e^{g (n - off - j)} c_j)^T
-// are products of matrices.  P over the diagonal is made zero, not multiplied by it, and a chunk
-// ends before a step whose c holds an infinity or a NaN (zero times that is NaN), unless that is
-// its first step: no step's output looks at a later one.  A workgroup walks through the chunks of one (sequence, head,
-// slice of c's columns, segment of the steps); each wave keeps X^T's rows for its own columns
-// in accumulator registers, whose layout (lane: one column, four rows) is at the same time
-// that of an operand, so X enters y's product without leaving the registers.  y and P are made
-// transposed for the same reason: P goes to LDS, and y to memory, four neighbours a lane.
+// are products of matrices.  A workgroup walks through the chunks of one (sequence, head, slice of
+// c's columns, segment of the steps); each wave keeps X^T's rows for its own columns in
+// accumulator registers, whose layout (lane: one column, four rows) is at the same time that of
+// an operand, so X enters y's product without leaving the registers.  y and P are made transposed
+// for the same reason: P goes to LDS, and y to memory, four neighbours a lane.
+//
+// No step's output looks at a later step: P over the diagonal is made zero, not multiplied by it,
+// and a chunk ends before a step whose c holds an infinity or a NaN (zero times that is NaN),
+// unless that is its first.  An input of nothing but NaN makes every step a chunk.
 //
 // Few sequences are cut into segments: their own states first (from zero, in a launch that reads
 // b and c alone), joined one after another, then every segment with the state that enters it.
 // The price is b and c read twice.
 //
 // What bounds it, bf16, 65536 steps of 8 heads of 128 x 128 (537 MB, 113 us at a copy's rate):
-// 69 us for the segments' states (3.9 TB/s), 15 to join them, 136 for the rest, in which a wave
-// issues 2500 cycles of matrix and 2400 of other instructions a chunk, two waves a SIMD: neither
-// memory nor matrix cores are full, barriers and LDS reads lie between.  Short sequences are
-// chains of chunks, 4 to 8 us each (777 steps of 13 x 12 sequences and heads, 96 x 80 in fp16: 31,
-// 6 and 69 us).  fp32 matrix instructions take 16 times as long: there they bound it.
+// 236 us, of which about 66 for the segments' states (4 TB/s), 15 to join them and 155 for the
+// rest, in which a wave issues 3200 cycles of matrix and 3300 of other vector instructions a chunk
+// of its 16,900, two waves a SIMD: neither memory nor matrix cores are full, barriers and LDS reads
+// lie between.  Short sequences are chains of chunks, 4 to 8 us each (777 steps of 13 x 12 sequences
+// and heads, 96 x 80 in fp16: 29, 6 and 65 us).  fp32 matrix instructions take 16 times as long:
+// there they bound it.  Sizes that are no whole number of pieces load and store element by element,
+// and some of their kernels spill (36 to 304 bytes a lane; 128 x 128 in bf16: 156).
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -251,7 +257,7 @@ struct MathBf16 {
 // fp16 inputs: each exactly the sum of two bf16 numbers (8 and 3 bits; fp16 itself has not the
 // range that P and states need), held in LDS as two planes.  P and the state as it enters y are
 // two bf16 terms as they are for bf16; of four products of terms the three larger ones are made, five
-// of six in the state's update, which misses 2^-25 (13 x 777 steps, 12 heads of 96 x 80: 99 us, with
+// of six in the state's update, which misses 2^-25 (13 x 777 steps, 12 heads of 96 x 80: 95 us; with
 // fp32 instructions 117).  An infinite input gives NaN where it would give infinity.
 struct MathF16 {
     using One = MathBf16;
@@ -539,8 +545,14 @@ __device__ __forceinline__ void put(Global<Out>* base, At at, int columns, f32x4
 // kFull: the state fills its padding; else products of nothing but padding are left out (96 x 80
 // of 128 x 128 is half the work), at the price of branches between the others.
 // kStates: only the own state, from zero, of each segment but the last.
+// Waves a SIMD.  Small states in chunks of 32 steps leave registers for four (2 x 4000 steps of 8 heads,
+// 33 x 47, with gradient: 153 us in fp16 and fp32, with three 171 and 163).
+template <class T, int kDA, int kW, int kCT>
+constexpr int kWavesASimd =
+    kW == 8 || (kW == 4 && kCT == 1 && kDA <= 64 && InputOf<T>::Math::kC == 32) ? 4 : 2;
+
 template <class T, int kDA, int kW, int kCT, bool kWhole, bool kFull, bool kStates>
-__global__ void __launch_bounds__(kW * 64, kW == 8 ? 4 : 2) k_chunk(ChunkArgs A) {
+__global__ void __launch_bounds__(kW * 64, (kWavesASimd<T, kDA, kW, kCT>)) k_chunk(ChunkArgs A) {
     using In = InputOf<T>;
     using M = typename In::Math;
     using Elem = typename M::Elem;
@@ -912,9 +924,10 @@ Cut cut_of(int64_t type, int64_t da, int64_t dc) {
     c.waves = dc <= 32 ? 2 : 4;
     c.tiles = 1;
     if (dc > 64 && c.rows < 256) {
-        // 128 columns: in bf16 two tiles a wave (LDS reads serve twice: 165 us for 65536 steps, 8
-        // heads, 128 x 128, against 200 with eight waves of one); fp32 products take so much longer
-        // that more waves pay instead (777 steps, 156 sequences and heads: 114 us against 123)
+        // 128 columns: in 16 bits two tiles a wave (LDS reads serve twice: 224 us for 65536 steps, 8
+        // heads, 128 x 128 in bf16, against 295 with eight waves of one); fp32 products take so much
+        // longer that more waves pay instead (777 steps, 156 sequences and heads, 96 x 80: 115 us
+        // against 136)
         if (type != HX_F32) {
             c.tiles = 2;
         } else {
@@ -928,7 +941,7 @@ Cut cut_of(int64_t type, int64_t da, int64_t dc) {
 // Segments of the steps, the same for all sums of a call: 512 workgroups in all, two chunks or
 // more each.  Two segments would read twice what they halve, and three of one chunk or two wait
 // longer for two more launches than for the chunks: forward and backward, bf16, 4 heads of 64,
-// 500 steps 49 us cut and 56 whole, but 16 sequences of 300 steps 53 cut in two and 38 whole.
+// 500 steps 46 us cut and 51 whole, but 16 sequences of 300 steps 50 cut in two and 37 whole.
 struct Segments {
     int count, steps;
 };

@@ -267,8 +267,8 @@ hipError_t launch(const hx_distill_args& A) {
 template <class T>
 hipError_t pick(const hx_distill_args& A) {
     // Threads a row.  A CU holds 2048: rows of a last, thin round run alone, so 512 threads
-    // where that fits all rows into one round and 1024 does not (517 rows of 50021: 42 us with
-    // 1024, 37 with 512); small rows take no more than they have pieces for.
+    // where that fits all rows into one round and 1024 does not (517 rows of 50021: 48 us with
+    // 1024, 38 with 512); small rows take no more than they have pieces for.
     const bool small = A.vocab <= 4096, half = A.rows > 512 && A.rows <= 1024;
     auto go = [&](auto rest) {
         constexpr bool kRest = decltype(rest)::value;
