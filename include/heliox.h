@@ -508,7 +508,8 @@ enum { HX_F32 = 0, HX_F16 = 1, HX_BF16 = 2 };
 
 /* S_t = e^g S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, for t < length; S_{-1} is the initial
  * state (NULL: zero), end_state is S_{length-1} (the initial state where length is 0); outputs
- * past a sequence's length are zero, whatever its inputs hold there.  Head h reads head
+ * past a sequence's length are zero, whatever its inputs hold there, and an infinity or a NaN
+ * within it reaches no earlier step (but as NaN where this may have an infinity).  Head h reads head
  * h q_heads / heads of q, and so on: q_heads, k_heads and v_heads each divide heads.
  * g = log_decay[h] is at most 0 (-inf: no memory).  States are (batch, heads, dk, dv) fp32,
  * contiguous.  dk and dv are at most 256, batch x heads 2^20, time 2^30.  What a call writes
