@@ -66,13 +66,17 @@ int attention_states(const char* call, const hx_attention_args* A, const float* 
     return 0;
 }
 
-int attention_space(const char* call, const hx_attention_args* A, bool grad) {
-    const size_t need = hx::attention_workspace(*A, grad);
-    if (need && (!A->workspace || A->workspace_bytes < 0 || static_cast<size_t>(A->workspace_bytes) < need))
+// Workspace of `need` bytes as the call got it.
+int space_fits(const char* call, size_t need, const void* space, int64_t bytes) {
+    if (need && (!space || bytes < 0 || static_cast<size_t>(bytes) < need))
         return refuse("%s: the workspace has to hold %zu bytes", call, need);
-    if (need && reinterpret_cast<uintptr_t>(A->workspace) % 16)
+    if (need && reinterpret_cast<uintptr_t>(space) % 16)
         return refuse("%s: the workspace has to start at a multiple of 16 bytes", call);
     return 0;
+}
+
+int attention_space(const char* call, const hx_attention_args* A, bool grad) {
+    return space_fits(call, hx::attention_workspace(*A, grad), A->workspace, A->workspace_bytes);
 }
 
 // grad is the logits themselves, row for row, or apart from them; its rows are apart from each other.
@@ -91,6 +95,17 @@ int distill_gradient(const char* call, const hx_distill_args* A) {
     const Wide step = gs < 0 ? -gs : gs, apart = step ? ((g - x) % step + step) % step : 0;
     if (A->rows > 1 && gs == xs && apart >= width && apart <= step - width) return 0;
     return refuse("%s: grad overlaps logits without being them", call);
+}
+
+int norm_sizes(const char* call, const hx_norm_args* A) {
+    if (!A) return refuse("%s: no arguments", call);
+    if (!known_type(A->type) || !known_type(A->weight_type)) return refuse("%s: type is not known", call);
+    if (A->rows < 0 || A->rows > INT32_MAX) return refuse("%s: rows has to be in 0..2^31 - 1", call);
+    if (A->width < 1 || A->width > (1 << 24))
+        return refuse("%s: width (%lld) has to be in 1..2^24", call, (long long)A->width);
+    if (!(A->eps >= 0) || !std::isfinite(A->eps)) return refuse("%s: eps has to be a number, at least 0", call);
+    if (!A->grad_weight != !A->grad_bias) return refuse("%s: grad_weight and grad_bias come together", call);
+    return 0;
 }
 
 }  // namespace
@@ -177,6 +192,28 @@ int hx_sample(const hx_sample_args* A) {
     if (!A->logits || !A->u || !A->token || !A->logprob)
         return refuse("%s: logits, u, token or logprob is missing", call);
     return launched(call, hx::sample_launch(*A));
+}
+
+int64_t hx_layer_norm_workspace(const hx_norm_args* A) {
+    if (norm_sizes("hx_layer_norm_workspace", A)) return -1;
+    return A->rows ? static_cast<int64_t>(hx::norm_workspace(*A)) : 0;
+}
+
+int hx_layer_norm(const hx_norm_args* A) {
+    const char* call = "hx_layer_norm";
+    if (norm_sizes(call, A)) return -1;
+    if (!A->rows) return 0;
+    if (!A->x || !A->y || !A->mean || !A->rstd) return refuse("%s: x, y, mean or rstd is missing", call);
+    return launched(call, hx::norm_forward(*A));
+}
+
+int hx_layer_norm_grad(const hx_norm_args* A) {
+    const char* call = "hx_layer_norm_grad";
+    if (norm_sizes(call, A)) return -1;
+    if (A->rows && (!A->x || !A->mean || !A->rstd || !A->grad_y || !A->grad_x))
+        return refuse("%s: x, mean, rstd, grad_y or grad_x is missing", call);
+    if (A->rows && space_fits(call, hx::norm_workspace(*A), A->workspace, A->workspace_bytes)) return -1;
+    return launched(call, hx::norm_backward(*A));
 }
 
 }  // extern "C"

@@ -1,6 +1,8 @@
 // Readout operators over a network's captured outputs: linear attention with a decay for
-// each head (readout_attention.hip), the loss against a teacher's top logits
-// (readout_distill.hip) and the drawing of an answer (readout_sample.hip).  readout.cpp holds
+// each head (readout_attention.hip), a gated recurrence (readout_recurrence.hip), layer norm
+// (readout_norm.hip), the loss against a teacher's top logits (readout_distill.hip), log
+// probabilities of given tokens (readout_logprob.hip), the drawing of an answer
+// (readout_sample.hip) and the step of the parameters (readout_adamw.hip).  readout.cpp holds
 // the C entry points and their checks; the kernels take the checked arguments.
 #pragma once
 #include <hip/hip_bf16.h>
@@ -24,6 +26,17 @@ hipError_t attention_backward(const hx_attention_args& A);
 hipError_t attention_step(const hx_attention_args& A);
 hipError_t distill_launch(const hx_distill_args& A);
 hipError_t sample_launch(const hx_sample_args& A);
+size_t norm_workspace(const hx_norm_args& A);
+hipError_t norm_forward(const hx_norm_args& A);
+hipError_t norm_backward(const hx_norm_args& A);
+size_t recurrence_workspace(const hx_recurrence_args& A, bool grad);
+hipError_t recurrence_forward(const hx_recurrence_args& A);
+hipError_t recurrence_backward(const hx_recurrence_args& A);
+hipError_t recurrence_step(const hx_recurrence_args& A);
+size_t logprob_workspace(const hx_logprob_args& A);
+hipError_t logprob_launch(const hx_logprob_args& A);
+hipError_t logprob_gradient(const hx_logprob_args& A);
+hipError_t adamw_launch(const hx_adamw_args& A);
 
 template <class T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }

@@ -8,6 +8,7 @@ a trained network, and the gradients of both.
   linear_attention, linear_attention_grad   a temporal readout over whole recordings: linear
                                             attention whose state decays as a synapse's does
   linear_attention_step                     the same for one tick of a running network
+  layer_norm, layer_norm_grad               rows brought to one mean and size, for recordings and ticks alike
   distill_loss, distill_loss_grad           the loss against a teacher's top logits
   sample                                    an answer drawn from logits
 
@@ -32,6 +33,7 @@ from .sim import HelioxError, lib
 # The records of include/heliox.h, field by field (8 bytes each).
 _ATTENTION = struct.Struct("=9q 3Q 9q 3Q d Q 3q Q Q 3q Q 3Q Q Q Q q Q q Q")
 _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
+_NORM = struct.Struct("=4q Q q 2Q d Q q 2Q Q q Q q 2Q Q q Q")
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -143,12 +145,12 @@ def _call(name: str, device: int, *args) -> int:
     return got
 
 
-def _like(x: torch.Tensor, what: str, q: torch.Tensor, device: int) -> None:
+def _like(x: torch.Tensor, what: str, q: torch.Tensor, device: int, other: str = "q") -> None:
     if not isinstance(x, torch.Tensor) or x.get_device() != device:
         if _on_gpu(x, what) != device:
-            raise ValueError(f"{what} is on {x.device}, q on cuda:{device}")
+            raise ValueError(f"{what} is on {x.device}, {other} on cuda:{device}")
     if x.dtype is not q.dtype:
-        raise TypeError(f"{what} is {x.dtype}, q is {q.dtype}")
+        raise TypeError(f"{what} is {x.dtype}, {other} is {q.dtype}")
 
 
 def _attention_inputs(q, k, v, log_decay, ndim: int):
@@ -278,6 +280,85 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         *fields, 0, 0, _scale(scale, dk), o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
         0, 0, state.data_ptr(), _ptr(slots), state.shape[0], 0, 0, _stream(device)))
     return o
+
+
+def _flat_rows(x: torch.Tensor) -> torch.Tensor:
+    """x as (rows, its last dimension), the last contiguous (a copy only where no view is one)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(0, x.shape[-1])
+    return _rows(x)
+
+
+def _norm_inputs(x, weight, bias):
+    device = _on_gpu(x, "x")
+    kind = _type(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x has to be (..., width) with at least one value a row, got shape {tuple(x.shape)}")
+    width, weight_kind = x.shape[-1], 0
+    for w, what in ((weight, "weight"), (bias, "bias")):
+        if w is not None:
+            if not isinstance(w, torch.Tensor):
+                raise TypeError(f"{what} has to be a tensor, got {type(w).__name__}")
+            weight_kind = _type(w, what)
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise TypeError(f"weight is {weight.dtype}, bias is {bias.dtype}")
+    weight, bias = (None if w is None else _array(w, what, w.dtype, (width,), device)
+                    for w, what in ((weight, "weight"), (bias, "bias")))
+    return device, kind, weight_kind, _flat_rows(x), weight, bias
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_space(kind: int, rows: int, width: int) -> int:
+    need = lib().hx_layer_norm_workspace(_NORM.pack(kind, 0, rows, width, *[0] * 4, 0.0, *[0] * 8, 1, 1, 0, 0, 0))
+    if need < 0:
+        raise HelioxError(lib().hx_readout_error().decode())
+    return need
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+               eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension of x (..., width);
+    weight and bias (width,) are of one type, fp32, fp16 or bf16, whatever x's is (1 and 0 unless
+    given).  Returns y of x's shape and type, and each row's mean and 1 / sqrt(variance + eps)
+    (fp32, x's shape without the last), which layer_norm_grad takes."""
+    device, kind, weight_kind, rows, weight, bias = _norm_inputs(x, weight, bias)
+    _no_graph("layer_norm", "take it from layer_norm_grad", x, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    n, width = rows.shape
+    _call("hx_layer_norm", device, _NORM.pack(
+        kind, weight_kind, n, width, rows.data_ptr(), rows.stride(0), _ptr(weight), _ptr(bias), _real(eps, "eps"),
+        y.data_ptr(), width, mean.data_ptr(), rstd.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, _stream(device)))
+    return y, mean, rstd
+
+
+def layer_norm_grad(x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor,
+                    dy: torch.Tensor, *, parameters: bool = True):
+    """Gradients of layer_norm from its mean and rstd: dy is the loss's gradient by y.  Returns dx of
+    x's shape and type, and the gradients by weight and by bias (width,) fp32, summed over the rows
+    in an order of the sizes alone (None, None with parameters=False)."""
+    device, kind, weight_kind, rows, weight, _ = _norm_inputs(x, weight, None)
+    _like(dy, "dy", x, device, "x")
+    if dy.shape != x.shape:
+        raise ValueError(f"dy has shape {tuple(dy.shape)}, x {tuple(x.shape)}")
+    if mean is None or rstd is None:
+        raise TypeError("mean and rstd have to be tensors")
+    mean = _array(mean, "mean", torch.float32, x.shape[:-1], device)
+    rstd = _array(rstd, "rstd", torch.float32, x.shape[:-1], device)
+    dy = _flat_rows(dy)
+    n, width = rows.shape
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight = dbias = space = None
+    need = 0
+    if parameters:
+        dweight, dbias = (torch.empty(width, dtype=torch.float32, device=x.device) for _ in range(2))
+        need = _norm_space(kind, n, width)
+        space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call("hx_layer_norm_grad", device, _NORM.pack(
+        kind, weight_kind, n, width, rows.data_ptr(), rows.stride(0), _ptr(weight), 0, 0.0, 0, 0, mean.data_ptr(),
+        rstd.data_ptr(), dy.data_ptr(), dy.stride(0), dx.data_ptr(), width, _ptr(dweight), _ptr(dbias), _ptr(space), need,
+        _stream(device)))
+    return dx, dweight, dbias
 
 
 def _logits(logits: torch.Tensor):

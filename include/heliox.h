@@ -497,8 +497,9 @@ int hx_get_replay_kernel_time(hx_sim* sim, double* ms, long long* launches);
 
 /* ---- Readout operators (no counterpart in the reference, which leaves what turns captured
  *      output voltages into answers, and their loss, to its caller): linear attention with a
- *      decay for each head, the loss against a teacher's top logits, the drawing of an answer.
- *      They need no model.  Every pointer is device memory of the current device; work is
+ *      decay for each head, a gated recurrence, layer norm, the loss against a teacher's top
+ *      logits, log probabilities of given tokens, the drawing of an answer, and the step that
+ *      trains such a readout's parameters. They need no model.  Every pointer is device memory of the current device; work is
  *      queued on `stream` (a hipStream_t, NULL: the default stream) and nothing is allocated,
  *      copied to the host or waited for, so calls may be captured into a graph.  Sizes and
  *      strides are in elements; the last dimension of every array is contiguous.  0 on
@@ -604,6 +605,143 @@ typedef struct hx_sample_args {
     void* stream;
 } hx_sample_args;
 int hx_sample(const hx_sample_args* args);
+/* Layer norm of each row: y = (x - mean) rstd weight + bias with the row's mean and
+ * rstd = 1 / sqrt(variance + eps) (mean over the width of (x - mean)^2).  Its gradient, from the
+ * same mean and rstd: with n = (x - mean) rstd and g = grad_y weight,
+ *   grad_x = rstd (g - mean(g) - n mean(g n)),  grad_weight = sum over rows of grad_y n,
+ *   grad_bias = sum over rows of grad_y
+ * (fp32, added in an order of the sizes alone).  grad_weight and grad_bias are both made or both NULL.
+ * rows is at most 2^31 - 1, width at most 2^24.  What a call writes overlaps nothing that it reads. */
+typedef struct hx_norm_args {
+    int64_t type, weight_type;                            /* weight and bias are of weight_type */
+    int64_t rows, width;
+    const void* x;
+    int64_t x_stride;                                     /* of rows, as the others */
+    const void *weight, *bias;                            /* (width) each, or NULL: 1 and 0 */
+    double eps;                                           /* at least 0 */
+    void* y;
+    int64_t y_stride;
+    float *mean, *rstd;                                   /* (rows) each: written, read by the gradient */
+    const void* grad_y;
+    int64_t grad_y_stride;
+    void* grad_x;
+    int64_t grad_x_stride;
+    float *grad_weight, *grad_bias;                       /* (width) each, or both NULL */
+    void* workspace;                                      /* starts at a multiple of 16 bytes */
+    int64_t workspace_bytes;
+    void* stream;
+} hx_norm_args;
+/* Bytes of workspace that hx_layer_norm_grad needs for these sizes; -1 if they are refused. */
+int64_t hx_layer_norm_workspace(const hx_norm_args* args);
+int hx_layer_norm(const hx_norm_args* args);
+int hx_layer_norm_grad(const hx_norm_args* args);
+
+/* h_t = a_t h_{t-1} + (1 - a_t) x_t for each channel, a = 1 / (1 + e^-gate) (1 - a taken as
+ * 1 / (1 + e^gate)), o_t = h_t: the exponential step of a membrane towards x whose conductance
+ * is the gate's.  h_{-1} is the initial state (NULL: zero), end_state the state after a
+ * sequence's last step; outputs past its length are zero, whatever its inputs hold there.  The
+ * gradient: with l_t = grad_o_t + a_{t+1} l_{t+1} (past the end: grad_end),
+ *   grad_x = (1 - a) l,  grad_gate = a (1 - a) l (h_{t-1} - x_t),  grad_initial = a_0 l_0.
+ * States are (batch, channels) fp32, contiguous.  time is at most 2^30, batch x channels 2^31 - 1.
+ * What a call writes overlaps nothing that it reads (end_state and grad_initial that do are
+ * refused), but for the single step's state. */
+typedef struct hx_recurrence_args {
+    int64_t type, batch, time, channels;
+    const void *x, *gate;                                 /* (batch, time, channels) */
+    int64_t x_stride[2], gate_stride[2];                  /* batch, time */
+    const float* initial_state;                           /* or NULL */
+    const int32_t* lengths;                               /* (batch), 0..time; NULL: all of time */
+    void* o;
+    int64_t o_stride[2];
+    float* end_state;                                     /* or NULL */
+    /* gradient: grad_o in; grad_x and grad_gate out, contiguous */
+    const void* grad_o;
+    int64_t grad_o_stride[2];
+    const float* grad_end;                                /* or NULL: zero */
+    void *grad_x, *grad_gate;
+    float* grad_initial;                                  /* or NULL */
+    /* single step: time is 1; the state of row i is slot slots[i] of state (n_slots, channels),
+     * updated in place; a slot outside 0..n_slots-1 leaves its row out (o is zero); the slots of
+     * one call are distinct.  slots NULL: slot i for row i. */
+    float* state;
+    const int32_t* slots;
+    int64_t n_slots;
+    void* workspace;                                      /* starts at a multiple of 16 bytes */
+    int64_t workspace_bytes;
+    void* stream;
+} hx_recurrence_args;
+/* Bytes of workspace that the call with these sizes needs (grad: hx_gated_recurrence_grad); -1 if
+ * the sizes are refused.  The pointers are not looked at. */
+int64_t hx_gated_recurrence_workspace(const hx_recurrence_args* args, int grad);
+int hx_gated_recurrence(const hx_recurrence_args* args);
+int hx_gated_recurrence_grad(const hx_recurrence_args* args);
+int hx_gated_recurrence_step(const hx_recurrence_args* args);
+
+/* Of each row of logits, with q = softmax(logits / temperature): logprob = log q of the row's
+ * token (0 for a token outside 0..vocab-1), entropy = -sum q log q (0 log 0 is 0), and the top
+ * largest logits, largest first (ties: the lowest index first; NaN ranks as -inf), as indexes and
+ * log q.  Where fewer than top places are above -inf, -inf fills the rest, by index.  stats (rows,
+ * 2) receives the largest logit m and log sum exp((logits - m) / temperature).  A row of nothing
+ * but -inf has logprob -inf, entropy 0 and stats -inf, -inf; one with a NaN or +inf has NaN.
+ * The gradient, from the same stats and entropy: grad_j =
+ *   [grad_logprob (1[j = token] - q_j) - grad_entropy q_j (log q_j + entropy)] / temperature
+ * (the first term 0 for a token outside the vocabulary; all 0 for a row of nothing but -inf); it may
+ * be the logits themselves, else it overlaps nothing that the call reads (logits in part: refused). */
+typedef struct hx_logprob_args {
+    int64_t type, index_bits;                             /* of tokens: 32 or 64 */
+    int64_t rows, vocab, top;                             /* at most 2^21, 2^22, 256 (and vocab) */
+    const void* logits;
+    int64_t logits_stride;
+    const void* tokens;                                   /* (rows) */
+    double temperature;                                   /* in 2^-126..2^126 */
+    float *logprob, *entropy, *stats;
+    float* top_logprob;                                   /* (rows, top) */
+    int64_t* top_index;
+    const float *grad_logprob, *grad_entropy;             /* (rows) each, or NULL: 0 */
+    void* grad;
+    int64_t grad_stride;
+    void* workspace;                                      /* starts at a multiple of 16 bytes */
+    int64_t workspace_bytes;
+    void* stream;
+} hx_logprob_args;
+/* Bytes of workspace that hx_token_logprobs needs for these sizes; -1 if they are refused. */
+int64_t hx_token_logprobs_workspace(const hx_logprob_args* args);
+int hx_token_logprobs(const hx_logprob_args* args);
+int hx_token_logprobs_grad(const hx_logprob_args* args);
+
+/* One AdamW step over many tensors: with t = *step + 1 and g = grad_scale grad,
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps),
+ * in fp32, p rounded once to its type; *step becomes t.  Moments lie in two arrays for all the
+ * tensors, tensor i's from element `start` (a multiple of 256) on.  bits 32: m and v as fp32.
+ * bits 8: m and sqrt(v) as 8-bit floating-point numbers (4 bits of exponent, 3 of mantissa, no
+ * infinity: largest 448), each 256 elements relative to m_scale and v_scale, the largest of them
+ * / 448 (fp32; 0, and the numbers 0, where that largest is under 2^-100), rounded to nearest even;
+ * a root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
+ * that is not finite reaches its block's 256 elements in 8 bits.
+ * The parameters of a call do not overlap each other or the gradients (refused); arrays of moments
+ * are the caller's to keep apart.  `step` (two int64: the count, and a zero that the call uses and
+ * leaves zero) is device memory, so that a captured step counts on at every replay. */
+typedef struct hx_adamw_tensor {
+    int64_t type, grad_type;
+    void* param;                                          /* contiguous, elements of them */
+    const void* grad;
+    int64_t elements, start;
+    double weight_decay;
+} hx_adamw_tensor;
+typedef struct hx_adamw_args {
+    int64_t bits, count;
+    const hx_adamw_tensor* tensors;                       /* (count), host memory */
+    void *m, *v;
+    float *m_scale, *v_scale;
+    int64_t moments;                                      /* elements of m and of v */
+    double lr, beta1, beta2, eps, grad_scale;
+    const float* grad_scale_ptr;                          /* device memory; NULL: grad_scale */
+    const float* lr_ptr;                                  /* device memory; NULL: lr */
+    int64_t* step;
+    void* stream;
+} hx_adamw_args;
+int hx_adamw_step(const hx_adamw_args* args);
 const char* hx_readout_error(void);
 
 /* Host emulation of the device tree solve (no counterpart in the reference;
