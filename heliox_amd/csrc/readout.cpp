@@ -75,6 +75,25 @@ int space_fits(const char* call, size_t need, const void* space, int64_t bytes) 
     return 0;
 }
 
+// States of (batch, channels); those that a call writes are not those it reads.
+int recurrence_states(const char* call, const hx_recurrence_args* A, const float* out, const char* out_name,
+                      const float* in, const char* in_name) {
+    const uintptr_t bytes = sizeof(float) * A->batch * A->channels;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+    if (o && i && o < i + bytes && i < o + bytes) return refuse("%s: %s overlaps %s", call, out_name, in_name);
+    return 0;
+}
+
+int recurrence_sizes(const char* call, const hx_recurrence_args* A) {
+    if (!A) return refuse("%s: no arguments", call);
+    if (!known_type(A->type)) return refuse("%s: type %lld is not known", call, (long long)A->type);
+    if (A->batch < 0 || A->time < 0) return refuse("%s: negative batch or time", call);
+    if (A->channels < 1) return refuse("%s: channels has to be at least 1", call);
+    if (checked_product(A->batch, A->channels) > INT32_MAX || A->channels > INT32_MAX || A->time > (int64_t(1) << 30))
+        return refuse("%s: batch x channels is at most 2^31 - 1 and time at most 2^30", call);
+    return 0;
+}
+
 int attention_space(const char* call, const hx_attention_args* A, bool grad) {
     return space_fits(call, hx::attention_workspace(*A, grad), A->workspace, A->workspace_bytes);
 }
@@ -192,6 +211,47 @@ int hx_sample(const hx_sample_args* A) {
     if (!A->logits || !A->u || !A->token || !A->logprob)
         return refuse("%s: logits, u, token or logprob is missing", call);
     return launched(call, hx::sample_launch(*A));
+}
+
+int64_t hx_gated_recurrence_workspace(const hx_recurrence_args* A, int grad) {
+    if (recurrence_sizes("hx_gated_recurrence_workspace", A)) return -1;
+    return A->batch ? static_cast<int64_t>(hx::recurrence_workspace(*A, grad != 0)) : 0;
+}
+
+int hx_gated_recurrence(const hx_recurrence_args* A) {
+    const char* call = "hx_gated_recurrence";
+    if (recurrence_sizes(call, A)) return -1;
+    if (!A->batch) return 0;
+    if (A->time && (!A->x || !A->gate || !A->o)) return refuse("%s: x, gate or o is missing", call);
+    if (recurrence_states(call, A, A->end_state, "end_state", A->initial_state, "initial_state")) return -1;
+    if (space_fits(call, hx::recurrence_workspace(*A, false), A->workspace, A->workspace_bytes)) return -1;
+    return launched(call, hx::recurrence_forward(*A));
+}
+
+int hx_gated_recurrence_grad(const hx_recurrence_args* A) {
+    const char* call = "hx_gated_recurrence_grad";
+    if (recurrence_sizes(call, A)) return -1;
+    if (!A->batch) return 0;
+    if (A->time && (!A->x || !A->gate || !A->grad_o || !A->grad_x || !A->grad_gate))
+        return refuse("%s: x, gate, grad_o, grad_x or grad_gate is missing", call);
+    if (recurrence_states(call, A, A->grad_initial, "grad_initial", A->initial_state, "initial_state") ||
+        recurrence_states(call, A, A->grad_initial, "grad_initial", A->grad_end, "grad_end"))
+        return -1;
+    if (space_fits(call, hx::recurrence_workspace(*A, true), A->workspace, A->workspace_bytes)) return -1;
+    return launched(call, hx::recurrence_backward(*A));
+}
+
+int hx_gated_recurrence_step(const hx_recurrence_args* A) {
+    const char* call = "hx_gated_recurrence_step";
+    if (recurrence_sizes(call, A)) return -1;
+    if (A->time != 1) return refuse("%s: time has to be 1", call);
+    if (A->n_slots < 0) return refuse("%s: n_slots is negative", call);
+    if (!A->slots && A->batch > A->n_slots) return refuse("%s: %lld rows, but only %lld states", call,
+                                                          (long long)A->batch, (long long)A->n_slots);
+    if (!A->batch) return 0;
+    if (!A->x || !A->gate || !A->o || (A->n_slots && !A->state))
+        return refuse("%s: x, gate, o or state is missing", call);
+    return launched(call, hx::recurrence_step(*A));
 }
 
 int64_t hx_layer_norm_workspace(const hx_norm_args* A) {

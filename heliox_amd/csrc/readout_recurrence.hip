@@ -1,0 +1,552 @@
+// A gated recurrence for each channel, h_t = (1 - z_t) h_{t-1} + z_t x_t, z = 1 / (1 + e^gate), and
+// its gradient.
+//
+// A run of steps takes what enters it to P h + Y (P the product of the a = 1 - z, Y what the run
+// makes of nothing), and runs join: that is the scan.  What is left of P and h is h - z h in one
+// rounding, not a h: a channel that remembers for a thousand steps has a = 0.999, whose last bit
+// counts a thousand times, while z keeps all of its bits.
+//
+// Lanes lie along channels, kC each, so that a step's row is read and written as it lies in
+// memory; a wave takes kU steps in registers, a workgroup's kW waves take kW kU steps in a row
+// and join in LDS.  Where sequences and channels alone fill the chip a workgroup walks along its
+// whole sequence, one pass over the data.  Where they do not, sequences are cut into segments:
+// one launch makes each segment's P and Y, one joins them, one walks the segments.  The gradient
+// goes that way always, a segment being kW kU steps: what the future hands back to a run,
+// G = R + P G', joins from the right as h does from the left, and both meet in the run's registers.
+#include "readout.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace hx {
+namespace {
+
+constexpr int kU = 8, kW = 8, kTile = kU * kW, kThreads = 64 * kW;
+
+struct RecurrenceArgs {
+    const void *x, *gate, *grad_o;
+    long long x_stride[2], gate_stride[2], grad_o_stride[2], o_stride[2];
+    void *o, *grad_x, *grad_gate;
+    const int32_t* lengths;
+    const float *initial, *grad_end;
+    float *end, *grad_initial;
+    float *p, *y, *r;                // (batch, segments, channels): P, Y and R of each segment
+    float *enter, *leave;            // the same: what enters it from the left and, going back, from the right
+    int time, channels, blocks;      // blocks: of 64 kC channels
+    int segments, steps;             // steps: of a segment
+    long long batch;
+};
+
+template <class T, int kC> struct Packed;
+template <> struct Packed<float, 1> { typedef float Vec; };
+template <> struct Packed<__half, 2> { typedef _Float16 Vec __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Packed<__hip_bfloat16, 2> { typedef __bf16 Vec __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Packed<__half, 1> { typedef _Float16 Vec; };
+template <> struct Packed<__hip_bfloat16, 1> { typedef __bf16 Vec; };
+
+template <class Vec, int kC>
+__device__ __forceinline__ float part(const Vec& v, int c) {
+    if constexpr (kC == 1) return static_cast<float>(v);
+    else return static_cast<float>(v[c]);
+}
+
+template <class Vec, int kC>
+__device__ __forceinline__ void set(Vec& v, int c, float x) {
+    if constexpr (kC == 1) v = static_cast<Vec>(x);
+    else v[c] = static_cast<decltype(v[0] + v[0])>(x);
+}
+
+template <int kC> struct Floats { typedef float Vec __attribute__((ext_vector_type(kC), aligned(4))); };
+
+__device__ __forceinline__ float get(const float* p, int c) { return p[c]; }
+
+// e^gate; infinite over 88.
+__device__ __forceinline__ float rise(float gate) { return __builtin_amdgcn_exp2f(gate * 1.44269504088896341f); }
+// 1 / (1 + e^gate) from e^gate
+__device__ __forceinline__ float opening(float e) { return __builtin_amdgcn_rcpf(1.f + e); }
+
+// What an opening z leaves of h, and h moved by it towards x.
+__device__ __forceinline__ float left(float h, float z) { return fmaf(-z, h, h); }
+__device__ __forceinline__ float moved(float h, float z, float x) { return fmaf(z, x, left(h, z)); }
+
+// A workgroup's place: sequence, segment, channels.
+struct Where {
+    long long batch;
+    int segment, channel, length;
+    template <int kC>
+    __device__ __forceinline__ static Where of(const RecurrenceArgs& A, long long id) {
+        Where w;
+        const long long row = id / A.blocks;
+        // lanes past the last channel do the last channels over again, and write the same values
+        w.channel = min(static_cast<int>(id - row * A.blocks) * 64 * kC + static_cast<int>(threadIdx.x) % 64 * kC,
+                        A.channels - kC);
+        w.batch = row / A.segments;
+        w.segment = static_cast<int>(row - w.batch * A.segments);
+        w.length = A.lengths ? min(max(A.lengths[w.batch], 0), A.time) : A.time;
+        return w;
+    }
+    __device__ __forceinline__ long long at(const RecurrenceArgs& A) const {
+        return (batch * A.segments + segment) * A.channels + channel;
+    }
+};
+
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
+// kU steps from t on of one array; steps past the length are not read.
+template <class T, int kC, int kN>
+__device__ __forceinline__ void fetch(typename Packed<T, kC>::Vec (&to)[kN], const void* base, const long long (&stride)[2],
+                                      const Where& w, int t) {
+    using Vec = typename Packed<T, kC>::Vec;
+    const T* at = static_cast<const T*>(base) + w.batch * stride[0] + t * stride[1];
+    if (t + kN <= w.length) {
+#pragma unroll
+        for (int u = 0; u < kN; ++u, at += stride[1]) to[u] = *reinterpret_cast<const Vec*>(at + w.channel);
+    } else {
+#pragma unroll
+        for (int u = 0; u < kN; ++u, at += stride[1])
+            to[u] = t + u < w.length ? *reinterpret_cast<const Vec*>(at + w.channel) : Vec{};
+    }
+}
+
+// The whole walk.
+template <class T, int kC>
+__global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
+    using Vec = typename Packed<T, kC>::Vec;
+    using F = typename Floats<kC>::Vec;
+    __shared__ float ends[2][kW][2 * kC][64];
+    const int wave = wave_of(), lane = threadIdx.x % 64;
+    int turn = 0;
+    for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
+        const Where w = Where::of<kC>(A, id);
+        const int first = w.segment * A.steps, last = min(first + A.steps, A.time);
+        float h[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            h[c] = 0.f;
+            if (A.segments > 1) h[c] = A.enter[w.at(A) + c];
+            else if (A.initial) h[c] = A.initial[w.batch * A.channels + w.channel + c];
+        }
+        Vec x[kU], g[kU];
+        fetch<T, kC>(x, A.x, A.x_stride, w, first + wave * kU);
+        fetch<T, kC>(g, A.gate, A.gate_stride, w, first + wave * kU);
+        for (int tile = first; tile < last; tile += kTile, turn ^= 1) {
+            const int t = tile + wave * kU;
+            float p[kU][kC], y[kU][kC];
+            auto run = [&](auto whole) {
+                float pp[kC], yy[kC];
+#pragma unroll
+                for (int c = 0; c < kC; ++c) pp[c] = 1.f, yy[c] = 0.f;
+#pragma unroll
+                for (int u = 0; u < kU; ++u) {
+                    const bool live = decltype(whole)::value || t + u < w.length;
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) {
+                        const float z = live ? opening(rise(part<Vec, kC>(g[u], c))) : 0.f;
+                        const float v = live ? part<Vec, kC>(x[u], c) : 0.f;
+                        p[u][c] = pp[c] = left(pp[c], z);
+                        y[u][c] = yy[c] = moved(yy[c], z, v);
+                    }
+                }
+            };
+            if (t + kU <= w.length) run(std::true_type{});
+            else run(std::false_type{});
+            if (tile + kTile < last) {
+                fetch<T, kC>(x, A.x, A.x_stride, w, t + kTile);
+                fetch<T, kC>(g, A.gate, A.gate_stride, w, t + kTile);
+            }
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                ends[turn][wave][c][lane] = p[kU - 1][c];
+                ends[turn][wave][kC + c][lane] = y[kU - 1][c];
+            }
+            __syncthreads();
+            float mine[kC];
+#pragma unroll
+            for (int c = 0; c < kC; ++c) mine[c] = h[c];
+#pragma unroll
+            for (int v = 0; v < kW; ++v)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    if (v == wave) mine[c] = h[c];
+                    h[c] = fmaf(ends[turn][v][c][lane], h[c], ends[turn][v][kC + c][lane]);
+                }
+            T* o = static_cast<T*>(A.o) + w.batch * A.o_stride[0] + t * A.o_stride[1];
+            auto write = [&](auto whole) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u, o += A.o_stride[1]) {
+                    Vec out;
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) {
+                        const float v = fmaf(p[u][c], mine[c], y[u][c]);
+                        set<Vec, kC>(out, c, decltype(whole)::value || t + u < w.length ? v : 0.f);
+                    }
+                    if (decltype(whole)::value || t + u < A.time) *reinterpret_cast<Vec*>(o + w.channel) = out;
+                }
+            };
+            if (t + kU <= w.length) write(std::true_type{});
+            else write(std::false_type{});
+        }
+        if (A.end && w.segment == A.segments - 1 && wave == 0)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) A.end[w.batch * A.channels + w.channel + c] = h[c];
+    }
+}
+
+// P, Y (and, for the gradient, R) of each segment: every wave takes a share of its steps.
+template <class T, int kC, bool kGrad>
+__global__ void __launch_bounds__(kThreads, 4) k_segments(RecurrenceArgs A) {
+    using Vec = typename Packed<T, kC>::Vec;
+    constexpr int kN = kGrad ? 3 : 2;
+    __shared__ float ends[kW][kN * kC][64];
+    const int wave = wave_of(), lane = threadIdx.x % 64;
+    for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
+        const Where w = Where::of<kC>(A, id);
+        const int each = A.steps / kW, first = w.segment * A.steps + wave * each;
+        const int last = min(first + each, w.length);
+        float p[kC], y[kC], r[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) p[c] = 1.f, y[c] = r[c] = 0.f;
+        for (int t = first; t < last; t += kU) {
+            Vec x[kU], g[kU], d[kU];
+            fetch<T, kC>(x, A.x, A.x_stride, w, t);
+            fetch<T, kC>(g, A.gate, A.gate_stride, w, t);
+            if constexpr (kGrad) fetch<T, kC>(d, A.grad_o, A.grad_o_stride, w, t);
+            auto run = [&](auto whole) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u)
+                    if (decltype(whole)::value || t + u < last)
+#pragma unroll
+                        for (int c = 0; c < kC; ++c) {
+                            const float z = opening(rise(part<Vec, kC>(g[u], c)));
+                            p[c] = left(p[c], z);
+                            y[c] = moved(y[c], z, part<Vec, kC>(x[u], c));
+                            if constexpr (kGrad) r[c] = fmaf(p[c], part<Vec, kC>(d[u], c), r[c]);
+                        }
+            };
+            if (t + kU <= last) run(std::true_type{});
+            else run(std::false_type{});
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            ends[wave][c][lane] = p[c];
+            ends[wave][kC + c][lane] = y[c];
+            if constexpr (kGrad) ends[wave][2 * kC + c][lane] = r[c];
+        }
+        __syncthreads();
+        if (wave == 0)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                float pp = p[c], yy = y[c], rr = r[c];
+#pragma unroll
+                for (int v = 1; v < kW; ++v) {
+                    const float q = ends[v][c][lane];
+                    yy = fmaf(q, yy, ends[v][kC + c][lane]);
+                    if constexpr (kGrad) rr = fmaf(pp, ends[v][2 * kC + c][lane], rr);
+                    pp *= q;
+                }
+                A.p[w.at(A) + c] = pp;
+                A.y[w.at(A) + c] = yy;
+                if constexpr (kGrad) A.r[w.at(A) + c] = rr;
+            }
+    }
+}
+
+// What enters each segment from the left, and going back from the right: 64 channels a workgroup,
+// sixteen runs of segments, which join in LDS.
+template <bool kGrad>
+__global__ void __launch_bounds__(1024) k_join(RecurrenceArgs A) {
+    constexpr int kRuns = 16;
+    __shared__ float sp[kRuns][64], sy[kRuns][64], sr[kRuns][64];
+    const int lane = threadIdx.x % 64, run = threadIdx.x / 64, blocks = (A.channels + 63) / 64;
+    const int each = (A.segments + kRuns - 1) / kRuns, first = run * each, last = min(first + each, A.segments);
+    for (long long id = blockIdx.x; id < A.batch * blocks; id += gridDim.x) {
+        const long long batch = id / blocks;
+        const int channel = min(static_cast<int>(id - batch * blocks) * 64 + lane, A.channels - 1);
+        const long long state = batch * A.channels + channel, at = batch * A.segments * A.channels + channel;
+        float p = 1.f, y = 0.f, r = 0.f;
+        for (int s = first; s < last; ++s) {
+            const long long i = at + static_cast<long long>(s) * A.channels;
+            const float q = A.p[i];
+            y = fmaf(q, y, A.y[i]);
+            if constexpr (kGrad) r = fmaf(p, A.r[i], r);
+            p *= q;
+        }
+        __syncthreads();
+        sp[run][lane] = p, sy[run][lane] = y, sr[run][lane] = r;
+        __syncthreads();
+        float h = A.initial ? A.initial[state] : 0.f;
+        for (int v = 0; v < run; ++v) h = fmaf(sp[v][lane], h, sy[v][lane]);
+        for (int s = first; s < last; ++s) {
+            const long long i = at + static_cast<long long>(s) * A.channels;
+            A.enter[i] = h;
+            h = fmaf(A.p[i], h, A.y[i]);
+        }
+        if constexpr (kGrad) {
+            float g = A.grad_end ? A.grad_end[state] : 0.f;
+            for (int v = kRuns - 1; v > run; --v) g = fmaf(sp[v][lane], g, sr[v][lane]);
+            for (int s = last - 1; s >= first; --s) {
+                const long long i = at + static_cast<long long>(s) * A.channels;
+                A.leave[i] = g;
+                g = fmaf(A.p[i], g, A.r[i]);
+            }
+            if (run == 0 && A.grad_initial) A.grad_initial[state] = g;
+        }
+    }
+}
+
+// The gradients of kTile steps, from what enters them on both sides.
+template <class T, int kC>
+__global__ void __launch_bounds__(kThreads, 4) k_grad(RecurrenceArgs A) {
+    using Vec = typename Packed<T, kC>::Vec;
+    __shared__ float ends[kW][3 * kC][64];
+    const int wave = wave_of(), lane = threadIdx.x % 64;
+    for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
+        const Where w = Where::of<kC>(A, id);
+        const int t = w.segment * kTile + wave * kU;
+        Vec x[kU], g[kU], d[kU];
+        fetch<T, kC>(x, A.x, A.x_stride, w, t);
+        fetch<T, kC>(g, A.gate, A.gate_stride, w, t);
+        fetch<T, kC>(d, A.grad_o, A.grad_o_stride, w, t);
+        float h[kC], back[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            h[c] = back[c] = 0.f;
+            if (A.segments > 1) {
+                h[c] = A.enter[w.at(A) + c];
+                back[c] = A.leave[w.at(A) + c];
+            } else {
+                if (A.initial) h[c] = A.initial[w.batch * A.channels + w.channel + c];
+                if (A.grad_end) back[c] = A.grad_end[w.batch * A.channels + w.channel + c];
+            }
+        }
+        float z[kU][kC], a[kU][kC], p[kC], y[kC], r[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) p[c] = 1.f, y[c] = r[c] = 0.f;
+        auto run = [&](auto whole) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const bool live = decltype(whole)::value || t + u < w.length;
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const float gate = part<Vec, kC>(g[u], c), e = rise(gate);
+                    z[u][c] = live ? opening(e) : 0.f;
+                    a[u][c] = !live || gate > 80.f ? 1.f : e * z[u][c];
+                    p[c] = left(p[c], z[u][c]);
+                    if (live) {                  // what lies past the length may be no number
+                        y[c] = moved(y[c], z[u][c], part<Vec, kC>(x[u], c));
+                        r[c] = fmaf(p[c], part<Vec, kC>(d[u], c), r[c]);
+                    }
+                }
+            }
+        };
+        const bool whole_wave = t + kU <= w.length;
+        if (whole_wave) run(std::true_type{});
+        else run(std::false_type{});
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            ends[wave][c][lane] = p[c];
+            ends[wave][kC + c][lane] = y[c];
+            ends[wave][2 * kC + c][lane] = r[c];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < kW - 1; ++v)
+            if (v < wave)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) h[c] = fmaf(ends[v][c][lane], h[c], ends[v][kC + c][lane]);
+#pragma unroll
+        for (int v = kW - 1; v > 0; --v)
+            if (v > wave)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) back[c] = fmaf(ends[v][c][lane], back[c], ends[v][2 * kC + c][lane]);
+        auto out = [&](auto whole) {
+            float off[kU][kC];                   // h_{t-1} - x_t
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const bool live = decltype(whole)::value || t + u < w.length;
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const float v = part<Vec, kC>(x[u], c);
+                    off[u][c] = h[c] - v;
+                    if (live) h[c] = moved(h[c], z[u][c], v);
+                }
+            }
+            T* dx = static_cast<T*>(A.grad_x) + (w.batch * A.time + t) * A.channels;
+            T* dg = static_cast<T*>(A.grad_gate) + (w.batch * A.time + t) * A.channels;
+#pragma unroll
+            for (int u = kU - 1; u >= 0; --u) {
+                const bool live = decltype(whole)::value || t + u < w.length;
+                Vec vx, vg;
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const float l = part<Vec, kC>(d[u], c) + back[c], zl = z[u][c] * l;
+                    set<Vec, kC>(vx, c, live ? zl : 0.f);
+                    set<Vec, kC>(vg, c, live ? a[u][c] * zl * off[u][c] : 0.f);
+                    if (live) back[c] = left(l, z[u][c]);
+                }
+                if (decltype(whole)::value || t + u < A.time) {
+                    *reinterpret_cast<Vec*>(dx + static_cast<long long>(u) * A.channels + w.channel) = vx;
+                    *reinterpret_cast<Vec*>(dg + static_cast<long long>(u) * A.channels + w.channel) = vg;
+                }
+            }
+        };
+        if (whole_wave) out(std::true_type{});
+        else out(std::false_type{});
+        if (A.segments == 1 && A.grad_initial && wave == 0)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) A.grad_initial[w.batch * A.channels + w.channel + c] = back[c];
+    }
+}
+
+// One step for a batch of running sequences: kV channels a thread.
+template <class T, int kV>
+__global__ void __launch_bounds__(256) k_step(RecurrenceArgs A, float* states, const int32_t* slots, long long n_slots) {
+    const int each = A.channels / kV;
+    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= A.batch * each) return;
+    const long long batch = i / each;
+    const int c = static_cast<int>(i - batch * each) * kV;
+    const long long slot = slots ? slots[batch] : batch;
+    const T* x = static_cast<const T*>(A.x) + batch * A.x_stride[0] + c;
+    const T* g = static_cast<const T*>(A.gate) + batch * A.gate_stride[0] + c;
+    T* o = static_cast<T*>(A.o) + batch * A.o_stride[0] + c;
+    struct alignas(sizeof(T)) Few { T v[kV]; };
+    struct alignas(4) Held { float v[kV]; };
+    Few out{};
+    if (slot >= 0 && slot < n_slots) {
+        const Few xs = *reinterpret_cast<const Few*>(x), gs = *reinterpret_cast<const Few*>(g);
+        Held* const at = reinterpret_cast<Held*>(states + slot * A.channels + c);
+        Held h = *at;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
+            h.v[v] = moved(h.v[v], opening(rise(to_f32(gs.v[v]))), to_f32(xs.v[v]));
+            out.v[v] = from_f32<T>(h.v[v]);
+        }
+        *at = h;
+    } else {
+#pragma unroll
+        for (int v = 0; v < kV; ++v) out.v[v] = from_f32<T>(0.f);
+    }
+    *reinterpret_cast<Few*>(o) = out;
+}
+
+int channels_a_lane(const hx_recurrence_args& A) { return A.type == HX_F32 || A.channels == 1 ? 1 : 2; }
+
+struct Cut { int segments, steps; };
+
+// Segments of whole tiles.  The gradient's are one tile each.  Forward, 128 workgroups and more walk
+// along whole sequences; fewer are cut until there are 512, as far as there are tiles.
+Cut cut_of(const hx_recurrence_args& A, bool grad) {
+    const long long tiles = std::max<long long>(1, (A.time + kTile - 1) / kTile);
+    const long long width = 64 * channels_a_lane(A), walks = A.batch * ((A.channels + width - 1) / width);
+    long long segments = grad ? tiles : walks >= 128 ? 1 : std::min(tiles, (512 + walks - 1) / walks);
+    const long long each = (tiles + segments - 1) / segments;
+    segments = (tiles + each - 1) / each;
+    return {static_cast<int>(segments), static_cast<int>(each * kTile)};
+}
+
+// The workspace's parts, one after another.
+size_t part_bytes(const hx_recurrence_args& A, const Cut& cut) {
+    return sizeof(float) * A.batch * cut.segments * A.channels;
+}
+
+RecurrenceArgs recurrence_args(const hx_recurrence_args& A, const Cut& cut) {
+    RecurrenceArgs R{};
+    R.x = A.x, R.gate = A.gate, R.grad_o = A.grad_o;
+    R.o = A.o, R.grad_x = A.grad_x, R.grad_gate = A.grad_gate;
+    for (int i = 0; i < 2; ++i) {
+        R.x_stride[i] = A.x_stride[i], R.gate_stride[i] = A.gate_stride[i];
+        R.grad_o_stride[i] = A.grad_o_stride[i], R.o_stride[i] = A.o_stride[i];
+    }
+    R.lengths = A.lengths, R.initial = A.initial_state, R.grad_end = A.grad_end;
+    R.end = A.end_state, R.grad_initial = A.grad_initial;
+    R.time = static_cast<int>(A.time), R.channels = static_cast<int>(A.channels), R.batch = A.batch;
+    const int width = 64 * channels_a_lane(A);
+    R.blocks = (R.channels + width - 1) / width;
+    R.segments = cut.segments, R.steps = cut.steps;
+    if (cut.segments > 1) {
+        float* const space = static_cast<float*>(A.workspace);
+        const size_t n = part_bytes(A, cut) / sizeof(float);
+        R.p = space, R.y = space + n, R.enter = space + 2 * n, R.r = space + 3 * n, R.leave = space + 4 * n;
+    }
+    return R;
+}
+
+// Calls f(element type, channels a lane).
+template <class F>
+hipError_t with_lanes(const hx_recurrence_args& A, F&& f) {
+    return with_type(A.type, [&](auto t) {
+        using T = decltype(t);
+        if constexpr (!std::is_same_v<T, float>)
+            if (channels_a_lane(A) == 2) return f(t, std::integral_constant<int, 2>{});
+        return f(t, std::integral_constant<int, 1>{});
+    });
+}
+
+unsigned workgroups(long long n) { return static_cast<unsigned>(std::min<long long>(n, 1 << 22)); }
+
+template <bool kGrad>
+hipError_t join(const RecurrenceArgs& R, hipStream_t st) {
+    k_join<kGrad><<<workgroups(R.batch * ((R.channels + 63) / 64)), 1024, 0, st>>>(R);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t recurrence_workspace(const hx_recurrence_args& A, bool grad) {
+    const Cut cut = cut_of(A, grad);
+    return cut.segments > 1 ? (grad ? 5 : 3) * part_bytes(A, cut) : 0;
+}
+
+hipError_t recurrence_forward(const hx_recurrence_args& A) {
+    const RecurrenceArgs R = recurrence_args(A, cut_of(A, false));
+    const hipStream_t st = static_cast<hipStream_t>(A.stream);
+    const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
+    return with_lanes(A, [&](auto t, auto c) -> hipError_t {
+        using T = decltype(t);
+        constexpr int kC = decltype(c)::value;
+        if (R.segments > 1) {
+            k_segments<T, kC, false><<<grid, kThreads, 0, st>>>(R);
+            hipError_t e = hipGetLastError();
+            if (e == hipSuccess) e = join<false>(R, st);
+            if (e != hipSuccess) return e;
+        }
+        k_walk<T, kC><<<grid, kThreads, 0, st>>>(R);
+        return hipGetLastError();
+    });
+}
+
+hipError_t recurrence_backward(const hx_recurrence_args& A) {
+    const RecurrenceArgs R = recurrence_args(A, cut_of(A, true));
+    const hipStream_t st = static_cast<hipStream_t>(A.stream);
+    const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
+    return with_lanes(A, [&](auto t, auto c) -> hipError_t {
+        using T = decltype(t);
+        constexpr int kC = decltype(c)::value;
+        if (R.segments > 1) {
+            k_segments<T, kC, true><<<grid, kThreads, 0, st>>>(R);
+            hipError_t e = hipGetLastError();
+            if (e == hipSuccess) e = join<true>(R, st);
+            if (e != hipSuccess) return e;
+        }
+        k_grad<T, kC><<<grid, kThreads, 0, st>>>(R);
+        return hipGetLastError();
+    });
+}
+
+hipError_t recurrence_step(const hx_recurrence_args& A) {
+    const RecurrenceArgs R = recurrence_args(A, Cut{1, kTile});
+    const hipStream_t st = static_cast<hipStream_t>(A.stream);
+    const int v = A.channels % 4 == 0 ? 4 : 1;
+    const unsigned grid = static_cast<unsigned>((A.batch * (A.channels / v) + 255) / 256);
+    return with_type(A.type, [&](auto t) {
+        using T = decltype(t);
+        if (v == 4) k_step<T, 4><<<grid, 256, 0, st>>>(R, A.state, A.slots, A.n_slots);
+        else k_step<T, 1><<<grid, 256, 0, st>>>(R, A.state, A.slots, A.n_slots);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace hx

@@ -8,6 +8,9 @@ a trained network, and the gradients of both.
   linear_attention, linear_attention_grad   a temporal readout over whole recordings: linear
                                             attention whose state decays as a synapse's does
   linear_attention_step                     the same for one tick of a running network
+  gated_recurrence, gated_recurrence_grad   a state for each channel that moves to its input as far as its gate
+                                            lets it, over whole recordings
+  gated_recurrence_step                     the same for one tick
   layer_norm, layer_norm_grad               rows brought to one mean and size, for recordings and ticks alike
   distill_loss, distill_loss_grad           the loss against a teacher's top logits
   sample                                    an answer drawn from logits
@@ -34,6 +37,7 @@ from .sim import HelioxError, lib
 _ATTENTION = struct.Struct("=9q 3Q 9q 3Q d Q 3q Q Q 3q Q 3Q Q Q Q q Q q Q")
 _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
 _NORM = struct.Struct("=4q Q q 2Q d Q q 2Q Q q Q q 2Q Q q Q")
+_RECURRENCE = struct.Struct("=4q 2Q 4q 2Q Q 2q Q Q 2q Q 2Q Q 2Q q Q q Q")
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -279,6 +283,110 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
         *fields, 0, 0, _scale(scale, dk), o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
         0, 0, state.data_ptr(), _ptr(slots), state.shape[0], 0, 0, _stream(device)))
+    return o
+
+
+def _recurrence_inputs(x, gate, ndim: int):
+    """The tensors with contiguous last dimensions (kept by the caller until its call is queued),
+    and the record's fields up to gate_stride."""
+    device = _on_gpu(x, "x")
+    _like(gate, "gate", x, device, "x")
+    kind = _type(x, "x and gate")
+    shape = x.shape
+    if len(shape) != ndim or shape[-1] < 1:
+        want = "(batch, time, channels)" if ndim == 3 else "(batch, channels)"
+        raise ValueError(f"x has to be {want} with at least one channel, got shape {tuple(shape)}")
+    if gate.shape != shape:
+        raise ValueError(f"gate has shape {tuple(gate.shape)}, x {tuple(shape)}")
+    rows = x, gate = _rows(x), _rows(gate)
+    a, b = x.stride(), gate.stride()
+    if ndim == 3:
+        fields = (kind, shape[0], shape[1], shape[2], x.data_ptr(), gate.data_ptr(), a[0], a[1], b[0], b[1])
+    else:
+        fields = (kind, shape[0], 1, shape[1], x.data_ptr(), gate.data_ptr(), a[0], 0, b[0], 0)
+    return device, rows, fields
+
+
+@functools.lru_cache(maxsize=1024)
+def _recurrence_space(sizes: tuple, grad: int) -> int:
+    need = lib().hx_gated_recurrence_workspace(_RECURRENCE.pack(*sizes, *[0] * 25), grad)
+    if need < 0:
+        raise HelioxError(lib().hx_readout_error().decode())
+    return need
+
+
+def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, *, initial_state: Optional[torch.Tensor] = None,
+                     lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A state for each channel that moves to its input as far as its gate lets it, over whole
+    sequences: with a = sigmoid(gate),
+
+        h_t = a_t h_{t-1} + (1 - a_t) x_t,   o_t = h_t,
+
+    a membrane's exponential step towards x.  x and gate (batch, time, channels) are of one type;
+    initial_state (batch, channels) fp32 is zero unless given.  Sequence i ends after lengths[i]
+    steps (int32; all of time unless given); its outputs beyond are zero, whatever its inputs hold.
+    Returns o of x's shape and type and the state (batch, channels) fp32 at each sequence's end.
+
+    An infinite or NaN input reaches what it reaches in the recurrence, and no earlier step, but as
+    NaN where that may have an infinity."""
+    device, kept, fields = _recurrence_inputs(x, gate, 3)
+    _, batch, time, channels = sizes = fields[:4]
+    initial_state = _array(initial_state, "initial_state", torch.float32, (batch, channels), device)
+    _no_graph("gated_recurrence", "take it from gated_recurrence_grad", x, gate, initial_state)
+    lengths = _lengths(lengths, batch, device)
+    o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    end = torch.empty((batch, channels), dtype=torch.float32, device=x.device)
+    need = _recurrence_space(sizes, 0)
+    space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call("hx_gated_recurrence", device, _RECURRENCE.pack(
+        *fields, _ptr(initial_state), _ptr(lengths), o.data_ptr(), time * channels, channels, end.data_ptr(),
+        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, _ptr(space), need, _stream(device)))
+    return o, end
+
+
+def gated_recurrence_grad(x: torch.Tensor, gate: torch.Tensor, do: torch.Tensor, *,
+                          initial_state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                          dstate: Optional[torch.Tensor] = None):
+    """Gradients of gated_recurrence: do is the loss's gradient by o, dstate by the end states (zero
+    unless given).  Returns dx and dgate of x's shape and type (zero beyond a sequence's length)
+    and the gradient by initial_state (None where that is None)."""
+    device, kept, fields = _recurrence_inputs(x, gate, 3)
+    _, batch, _, channels = sizes = fields[:4]
+    _like(do, "do", x, device, "x")
+    if do.shape != x.shape:
+        raise ValueError(f"do has shape {tuple(do.shape)}, x {tuple(x.shape)}")
+    do = _rows(do)
+    initial_state = _array(initial_state, "initial_state", torch.float32, (batch, channels), device)
+    dstate = _array(dstate, "dstate", torch.float32, (batch, channels), device)
+    lengths = _lengths(lengths, batch, device)
+    dx, dgate = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    dinitial = None if initial_state is None else torch.empty_like(initial_state)
+    need = _recurrence_space(sizes, 1)
+    space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call("hx_gated_recurrence_grad", device, _RECURRENCE.pack(
+        *fields, _ptr(initial_state), _ptr(lengths), 0, 0, 0, 0, do.data_ptr(), *do.stride()[:2], _ptr(dstate),
+        dx.data_ptr(), dgate.data_ptr(), _ptr(dinitial), 0, 0, 0, _ptr(space), need, _stream(device)))
+    return dx, dgate, dinitial
+
+
+def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *,
+                          slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step of gated_recurrence for a batch of running sequences: x and gate (batch, channels);
+    state (n_slots, channels) fp32, contiguous, is updated in place.  Row i's state is slot slots[i]
+    (int32, distinct; a slot outside 0..n_slots-1 leaves the row out and its output zero), slot i
+    unless given.  Returns o (batch, channels)."""
+    device, kept, fields = _recurrence_inputs(x, gate, 2)
+    batch, channels = x.shape
+    if _on_gpu(state, "state") != device or state.dtype is not torch.float32 or not state.is_contiguous():
+        raise TypeError(f"state has to be a contiguous float32 tensor on {x.device}")
+    if state.dim() != 2 or state.shape[1] != channels:
+        raise ValueError(f"state has shape {tuple(state.shape)}, expected (n_slots, {channels})")
+    _no_graph("gated_recurrence_step", "take it from gated_recurrence_grad over the steps", x, gate, state)
+    slots = _array(slots, "slots", torch.int32, (batch,), device)
+    o = torch.empty((batch, channels), dtype=x.dtype, device=x.device)
+    _call("hx_gated_recurrence_step", device, _RECURRENCE.pack(
+        *fields, 0, 0, o.data_ptr(), channels, 0, 0, 0, 0, 0, 0, 0, 0, 0, state.data_ptr(), _ptr(slots), state.shape[0],
+        0, 0, _stream(device)))
     return o
 
 

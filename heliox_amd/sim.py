@@ -183,6 +183,10 @@ SIGNATURES = {
     "hx_linear_attention_step": (C.c_int, [C.c_char_p]),
     "hx_distill_loss": (C.c_int, [C.c_char_p]),
     "hx_sample": (C.c_int, [C.c_char_p]),
+    "hx_gated_recurrence_workspace": (C.c_int64, [C.c_char_p, C.c_int]),
+    "hx_gated_recurrence": (C.c_int, [C.c_char_p]),
+    "hx_gated_recurrence_grad": (C.c_int, [C.c_char_p]),
+    "hx_gated_recurrence_step": (C.c_int, [C.c_char_p]),
     "hx_layer_norm_workspace": (C.c_int64, [C.c_char_p]),
     "hx_layer_norm": (C.c_int, [C.c_char_p]),
     "hx_layer_norm_grad": (C.c_int, [C.c_char_p]),
