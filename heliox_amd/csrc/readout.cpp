@@ -99,7 +99,8 @@ int attention_space(const char* call, const hx_attention_args* A, bool grad) {
 }
 
 // grad is the logits themselves, row for row, or apart from them; its rows are apart from each other.
-int distill_gradient(const char* call, const hx_distill_args* A) {
+template <class Args>
+int logits_gradient(const char* call, const Args* A) {
     typedef __int128 Wide;
     const int64_t size = A->type == HX_F32 ? 4 : 2;
     const Wide width = static_cast<Wide>(A->vocab) * size, gs = static_cast<Wide>(A->grad_stride) * size,
@@ -114,6 +115,21 @@ int distill_gradient(const char* call, const hx_distill_args* A) {
     const Wide step = gs < 0 ? -gs : gs, apart = step ? ((g - x) % step + step) % step : 0;
     if (A->rows > 1 && gs == xs && apart >= width && apart <= step - width) return 0;
     return refuse("%s: grad overlaps logits without being them", call);
+}
+
+int logprob_sizes(const char* call, const hx_logprob_args* A) {
+    if (!A) return refuse("%s: no arguments", call);
+    if (!known_type(A->type)) return refuse("%s: type is not known", call);
+    if (A->index_bits != 32 && A->index_bits != 64) return refuse("%s: tokens have 32 or 64 bits", call);
+    if (A->rows < 0 || A->rows > kMaxRows) return refuse("%s: rows has to be in 0..2^21", call);
+    if (A->vocab < 1 || A->vocab > (1 << 22)) return refuse("%s: vocab has to be in 1..2^22", call);
+    if (A->top < 0 || A->top > hx::kLogprobMaxTop || A->top > A->vocab)
+        return refuse("%s: top (%lld) has to be in 0..%lld, and at most the vocabulary", call, (long long)A->top,
+                      (long long)hx::kLogprobMaxTop);
+    // it and its reciprocal times log2 e are fp32 numbers in the kernel
+    if (!(A->temperature >= 0x1p-126) || !(A->temperature <= 0x1p126))
+        return refuse("%s: temperature has to be positive, in 2^-126..2^126", call);
+    return 0;
 }
 
 int norm_sizes(const char* call, const hx_norm_args* A) {
@@ -196,7 +212,7 @@ int hx_distill_loss(const hx_distill_args* A) {
     if (!A->rows) return 0;
     if (!A->logits || !A->loss || (A->top && (!A->index || !A->teacher)))
         return refuse("%s: logits, index, teacher or loss is missing", call);
-    if (A->grad && distill_gradient(call, A)) return -1;
+    if (A->grad && logits_gradient(call, A)) return -1;
     return launched(call, hx::distill_launch(*A));
 }
 
@@ -211,6 +227,32 @@ int hx_sample(const hx_sample_args* A) {
     if (!A->logits || !A->u || !A->token || !A->logprob)
         return refuse("%s: logits, u, token or logprob is missing", call);
     return launched(call, hx::sample_launch(*A));
+}
+
+int64_t hx_token_logprobs_workspace(const hx_logprob_args* A) {
+    if (logprob_sizes("hx_token_logprobs_workspace", A)) return -1;
+    return A->rows ? static_cast<int64_t>(hx::logprob_workspace(*A)) : 0;
+}
+
+int hx_token_logprobs(const hx_logprob_args* A) {
+    const char* call = "hx_token_logprobs";
+    if (logprob_sizes(call, A)) return -1;
+    if (!A->rows) return 0;
+    if (!A->logits || !A->tokens || !A->logprob || !A->entropy || !A->stats)
+        return refuse("%s: logits, tokens, logprob, entropy or stats is missing", call);
+    if (A->top && (!A->top_logprob || !A->top_index)) return refuse("%s: top_logprob or top_index is missing", call);
+    if (space_fits(call, hx::logprob_workspace(*A), A->workspace, A->workspace_bytes)) return -1;
+    return launched(call, hx::logprob_launch(*A));
+}
+
+int hx_token_logprobs_grad(const hx_logprob_args* A) {
+    const char* call = "hx_token_logprobs_grad";
+    if (logprob_sizes(call, A)) return -1;
+    if (!A->rows) return 0;
+    if (!A->logits || !A->tokens || !A->entropy || !A->stats || !A->grad)
+        return refuse("%s: logits, tokens, entropy, stats or grad is missing", call);
+    if (logits_gradient(call, A)) return -1;
+    return launched(call, hx::logprob_gradient(*A));
 }
 
 int64_t hx_gated_recurrence_workspace(const hx_recurrence_args* A, int grad) {

@@ -18,6 +18,7 @@ namespace hx {
 constexpr int kAttnMaxDim = 256;
 constexpr int64_t kDistillMaxVocab = 1 << 20;
 constexpr int64_t kDistillMaxTop = 2048;
+constexpr int64_t kLogprobMaxTop = 256;
 
 // Each launches on the arguments' stream; the sizes are checked and not zero.
 size_t attention_workspace(const hx_attention_args& A, bool grad);

@@ -1,0 +1,466 @@
+// Log probabilities of given tokens with the entropy and the top alternatives of each row of
+// logits, and their gradient.
+//
+// One pass over a row gives z = sum 2^y and s = sum y 2^y, y = (x - base) log2 e / t, from which
+// log q = (x - base) / t - ln z and the entropy ln z - ln 2 s / z follow.  The base is the largest
+// logit of the row's first pieces; a thread that meets one far above it moves its own.  The top
+// places come out of the same pass: every wave's lanes hold the largest logit of their first
+// pieces, and a bound that enough of these reach lets few of the row's logits through, a few
+// hundred of a hundred thousand.  They wait in LDS as whole numbers, logit above index, and each
+// counts those above it.  Where the bound lets too many through (logits that rise along the row,
+// or are all the same) the top places' own bound is found byte by byte from histograms.
+//
+// Few long rows are cut into parts, which a second launch joins.  Bound by the logits' bytes, read
+// once; the gradient reads and writes them once.
+#include "readout.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace hx {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kAhead = 4;                  // pieces a thread asks for at a time
+constexpr float kFar = 64.f;               // a base is moved where weights pass 2^64
+constexpr float kNone = -200.f;            // 2^y is 0 from here on; y = -inf would make y 2^y no number
+constexpr double kLn2 = 0.6931471805599453;
+
+struct LogprobArgs {
+    const void *logits, *tokens;
+    long long stride;
+    int vocab, top, index_bits, parts, each;   // each: logits of a part
+    float cold;                                // log2 e / temperature
+    double per;                                // 1 / temperature
+    float *logprob, *entropy, *stats, *top_logprob;
+    int64_t* top_index;
+    struct Sums* sums;                         // (rows, parts)
+    u64* keys;                                 // (rows, parts, top)
+};
+
+struct Sums {
+    double z, s;
+    float base, most;
+};
+
+// Logits ordered as whole numbers, above the indexes, lowest first; -0 is 0 and NaN -inf.
+__device__ __forceinline__ unsigned order_of(float v) {
+    const unsigned b = __float_as_uint(v != v ? -INFINITY : v + 0.f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ u64 key_of(float v, int j) { return static_cast<u64>(order_of(v)) << 32 | ~static_cast<unsigned>(j); }
+__device__ __forceinline__ int index_of(u64 key) { return static_cast<int>(~static_cast<unsigned>(key)); }
+
+__device__ __forceinline__ long long token_of(const LogprobArgs& A, long long row) {
+    return A.index_bits == 64 ? static_cast<const int64_t*>(A.tokens)[row] : static_cast<const int32_t*>(A.tokens)[row];
+}
+
+template <int kThreads> constexpr int kHeld = kThreads == 1024 ? 4096 : 2048;
+
+template <int kThreads>
+struct Shared {
+    double red[kThreads / 64];
+    float most[kThreads / 64], bound[kThreads / 64];
+    int count;
+    unsigned bins[256];
+    u64 prefix, answer;
+    int left;
+    u64 held[kHeld<kThreads>];
+};
+
+// The k-th largest of a wave's values, to 16 bits of their order (rounded down): at least k of them
+// are not below it.
+__device__ __forceinline__ float kth_of_wave(float v, int k) {
+    const unsigned mine = order_of(v) >> 16;
+    unsigned found = 0;
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned tried = found | 1u << bit;
+        if (__popcll(__ballot(mine >= tried)) >= k) found = tried;
+    }
+    return found <= 0x7f ? -INFINITY : value_of(found << 16);
+}
+
+// Places above the bound that is found from the histograms: exactly `top` keys (or all n) go to sh.held.
+template <class T, int kThreads>
+__device__ void select_exactly(const T* x, int first, int last, int top, Shared<kThreads>& sh) {
+    if (threadIdx.x == 0) sh.prefix = 0, sh.left = min(top, last - first), sh.answer = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        for (int b = threadIdx.x; b < 256; b += kThreads) sh.bins[b] = 0;
+        __syncthreads();
+        const u64 prefix = sh.prefix;
+        const bool done = sh.answer != 0;
+        if (!done)
+            for (int j0 = first; j0 < last; j0 += kThreads) {
+                const int j = j0 + threadIdx.x;
+                const u64 key = j < last ? key_of(to_f32(x[j]), j) : 0;
+                const bool in = j < last && (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8));
+                const int bin = static_cast<int>(key >> shift & 255);
+                const u64 live = __ballot(in);
+                if (!live) continue;
+                const int one = __shfl(bin, __ffsll(live) - 1);
+                if (__all(!in || bin == one)) {       // a wave of equal logits adds once
+                    if (threadIdx.x % 64 == 0) atomicAdd(&sh.bins[one], static_cast<unsigned>(__popcll(live)));
+                } else if (in) {
+                    atomicAdd(&sh.bins[bin], 1u);
+                }
+            }
+        __syncthreads();
+        if (threadIdx.x == 0 && !done) {
+            int left = sh.left, b = 255;
+            while (b > 0 && static_cast<int>(sh.bins[b]) < left) left -= sh.bins[b--];
+            sh.prefix = prefix | static_cast<u64>(b) << shift;
+            sh.left = left;
+            // the whole bin belongs: its first possible key is the bound
+            if (static_cast<int>(sh.bins[b]) == left || shift == 0) sh.answer = sh.prefix;
+        }
+        __syncthreads();
+    }
+    const u64 bound = sh.answer;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (int j = first + threadIdx.x; j < last; j += kThreads) {
+        const u64 key = key_of(to_f32(x[j]), j);
+        if (key >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kHeld<kThreads>) sh.held[at] = key;
+        }
+    }
+    __syncthreads();
+}
+
+// Calls put(rank, key) for the top largest of sh.held's n keys, from the largest on.
+template <int kThreads, class F>
+__device__ __forceinline__ void each_ranked(const Shared<kThreads>& sh, int n, int top, F put) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 key = sh.held[i];
+        int rank = 0;
+        for (int k = 0; k < n; ++k) rank += sh.held[k] > key;
+        if (rank < top) put(rank, key);
+    }
+}
+
+// A row's results from its sums.  Every thread has the same sums; keys go through put_top.
+struct Finish {
+    double logz;
+    float base, most;
+    bool none, broken;                        // nothing but -inf; NaN or +inf among the logits
+    __device__ __forceinline__ Finish(const Sums& S) : logz(log(S.z)), base(S.base), most(S.most) {
+        broken = !(S.z < INFINITY) || S.most == INFINITY;
+        none = !broken && S.most == -INFINITY;
+    }
+    __device__ __forceinline__ float logprob(float v, double per) const {
+        if (broken) return NAN;
+        return v == -INFINITY ? -INFINITY : static_cast<float>((static_cast<double>(v) - base) * per - logz);
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void finish_row(const LogprobArgs& A, long long row, const T* x, const Sums& S, const Finish& f) {
+    const long long token = token_of(A, row);
+    A.logprob[row] = token < 0 || token >= A.vocab ? 0.f : f.logprob(to_f32(x[token]), A.per);
+    A.entropy[row] = f.broken ? NAN : f.none ? 0.f : static_cast<float>(fmax(f.logz - kLn2 * S.s / S.z, 0.));
+    A.stats[2 * row] = f.broken ? NAN : f.most;
+    A.stats[2 * row + 1] = f.broken ? NAN : f.none ? -INFINITY
+                                                  : static_cast<float>(f.logz + (static_cast<double>(f.base) - f.most) * A.per);
+}
+
+__device__ __forceinline__ void put_top(const LogprobArgs& A, long long row, const Finish& f, int rank, u64 key) {
+    A.top_index[row * A.top + rank] = index_of(key);
+    A.top_logprob[row * A.top + rank] = f.logprob(value_of(static_cast<unsigned>(key >> 32)), A.per);
+}
+
+// One workgroup a part of a row (the whole row, where it is not cut).
+template <class T, int kThreads, bool kTop>
+__global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
+    using Vec = typename PieceOf<T>::Vec;
+    constexpr int kP = sizeof(Vec) / sizeof(T), kWaves = kThreads / 64;
+    __shared__ Shared<kThreads> sh;
+    const long long row = blockIdx.x / A.parts;
+    const int part = static_cast<int>(blockIdx.x - row * A.parts);
+    const T* x = static_cast<const T*>(A.logits) + row * A.stride;
+    const int first = part * A.each, last = min(first + A.each, A.vocab), pieces = (last - first) / kP;
+    const T* from = x + first;
+    Vec raw[kAhead];
+    auto fetch = [&](int p0) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (p0 + k * kThreads < pieces)
+                raw[k] = *reinterpret_cast<const Vec*>(from + static_cast<long long>(p0 + k * kThreads) * kP);
+    };
+    fetch(threadIdx.x);
+    // the logits that are left beside whole pieces, one a thread
+    const int odd = pieces * kP + static_cast<int>(threadIdx.x);
+    const bool has_odd = first + odd < last;
+    const float one = has_odd ? to_f32(from[odd]) : -INFINITY;
+
+    float most = has_odd ? fmaxf(one, -INFINITY) : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (static_cast<int>(threadIdx.x) + k * kThreads < pieces)
+#pragma unroll
+            for (int i = 0; i < kP; ++i) most = fmaxf(most, static_cast<float>(raw[k][i]));
+    if (threadIdx.x == 0) sh.count = 0;
+    float bound = -INFINITY;
+    {
+        const int wave = threadIdx.x / 64;
+        // waves whose every lane holds a piece share the top places among them
+        const int full = min(pieces, kThreads) / 64, quota = full ? (A.top + full - 1) / full : 65;
+        float m = most;
+        for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        float b = INFINITY;
+        if (kTop && wave < full && quota <= 64) b = kth_of_wave(most, quota);
+        if (threadIdx.x % 64 == 0) sh.most[wave] = m, sh.bound[wave] = b;
+        __syncthreads();
+        bound = INFINITY;
+        for (int v = 0; v < kWaves; ++v) {
+            most = fmaxf(most, sh.most[v]);
+            bound = fminf(bound, sh.bound[v]);
+        }
+        if (quota > 64) bound = -INFINITY;
+    }
+    float base = most == -INFINITY ? 0.f : most, limit = most == -INFINITY ? -INFINITY : base + kFar / A.cold;
+    float z = 0.f, s = 0.f;
+    auto keep = [&](float v, int j) {
+        if ((v != v ? -INFINITY : v) >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kHeld<kThreads>) sh.held[at] = key_of(v, j);
+        }
+    };
+    auto take = [&](const float* v, int n, int j) {
+        float c = v[0];
+#pragma unroll
+        for (int i = 1; i < kP; ++i)
+            if (i < n) c = fmaxf(c, v[i]);
+        most = fmaxf(most, c);
+        if (c > limit) {
+            const float less = z == 0.f ? 0.f : fmaxf((base - c) * A.cold, -1e9f);
+            const float f = __builtin_amdgcn_exp2f(less);
+            s = f * fmaf(less, z, s);
+            z *= f;
+            base = c;
+            limit = c + kFar / A.cold;
+        }
+#pragma unroll
+        for (int i = 0; i < kP; ++i)
+            if (i < n) {
+                const float y = (v[i] - base) * A.cold, w = __builtin_amdgcn_exp2f(y);
+                z += w;
+                s = fmaf(w, fmaxf(y, kNone), s);
+            }
+        if constexpr (kTop)
+            if (!(c < bound))
+#pragma unroll
+                for (int i = 0; i < kP; ++i)
+                    if (i < n) keep(v[i], j + i);
+    };
+    for (int p0 = threadIdx.x; p0 < pieces; p0 += kAhead * kThreads) {
+        if (p0 != static_cast<int>(threadIdx.x)) fetch(p0);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int p = p0 + k * kThreads;
+            if (p < pieces) {
+                float v[kP];
+#pragma unroll
+                for (int i = 0; i < kP; ++i) v[i] = static_cast<float>(raw[k][i]);
+                take(v, kP, first + p * kP);
+            }
+        }
+    }
+    if (has_odd) {
+        const float v[kP] = {one};
+        take(v, 1, first + odd);
+    }
+    // one base for the workgroup: the highest
+    const float mine = base;
+    auto up = [](float a, float b) { return fmaxf(a, b); };
+    auto add = [](double a, double b) { return a + b; };
+    Sums S;
+    S.most = block_reduce<kThreads>(most, sh.most, up);
+    S.base = block_reduce<kThreads>(z == 0.f ? -INFINITY : base, sh.bound, up);
+    if (S.base == -INFINITY) S.base = 0.f;
+    const double less = (static_cast<double>(mine) - S.base) * A.cold;
+    const double f = mine == S.base || z == 0.f ? 1. : static_cast<double>(__builtin_amdgcn_exp2f(static_cast<float>(less)));
+    S.s = block_reduce<kThreads>(f * (s + (z == 0.f ? 0. : less * z)), sh.red, add);
+    S.z = block_reduce<kThreads>(f * z, sh.red, add);
+    if constexpr (kTop) {
+        if (sh.count > kHeld<kThreads>) select_exactly<T, kThreads>(x, first, last, A.top, sh);
+    }
+    const int n = min(sh.count, kHeld<kThreads>);
+    if (A.parts == 1) {
+        const Finish done(S);
+        if (threadIdx.x == 0) finish_row(A, row, x, S, done);
+        if constexpr (kTop) each_ranked(sh, n, A.top, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
+    } else {
+        if (threadIdx.x == 0) A.sums[blockIdx.x] = S;
+        if constexpr (kTop) {
+            u64* const to = A.keys + static_cast<long long>(blockIdx.x) * A.top;
+            for (int i = n + threadIdx.x; i < A.top; i += kThreads) to[i] = 0;
+            each_ranked(sh, n, A.top, [&](int rank, u64 key) { to[rank] = key; });
+        }
+    }
+}
+
+// The parts of a row, joined.
+template <class T>
+__global__ void __launch_bounds__(256) k_logprob_join(LogprobArgs A) {
+    __shared__ Shared<256> sh;
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(A.logits) + row * A.stride;
+    Sums S{0., 0., -INFINITY, -INFINITY};
+    for (int p = 0; p < A.parts; ++p) {
+        const Sums P = A.sums[row * A.parts + p];
+        S.most = fmaxf(S.most, P.most);
+        if (P.z != 0.) S.base = fmaxf(S.base, P.base);
+    }
+    if (S.base == -INFINITY) S.base = 0.f;
+    for (int p = 0; p < A.parts; ++p) {
+        const Sums P = A.sums[row * A.parts + p];
+        const double less = P.z == 0. ? 0. : (static_cast<double>(P.base) - S.base) * A.cold, f = exp2(less);
+        S.z += f * P.z;
+        S.s += f * (P.s + less * P.z);
+    }
+    const Finish done(S);
+    if (threadIdx.x == 0) finish_row(A, row, x, S, done);
+    const int n = A.parts * A.top;
+    for (int i = threadIdx.x; i < n; i += 256) sh.held[i] = A.keys[row * n + i];
+    __syncthreads();
+    each_ranked(sh, n, A.top, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
+}
+
+struct GradArgs {
+    const void *logits, *tokens;
+    void* grad;
+    long long rows, stride, grad_stride;
+    int vocab, index_bits, blocks;
+    float cold, per;
+    const float *stats, *entropy, *pull, *turn;
+};
+
+// The gradient, kAhead pieces a thread.
+template <class T, int kThreads>
+__global__ void __launch_bounds__(kThreads) k_logprob_grad(GradArgs A) {
+    using Vec = typename PieceOf<T>::Vec;
+    constexpr int kP = sizeof(Vec) / sizeof(T);
+    for (long long id = blockIdx.x; id < A.rows * A.blocks; id += gridDim.x) {
+        const long long row = id / A.blocks;
+        const int block = static_cast<int>(id - row * A.blocks);
+        const T* x = static_cast<const T*>(A.logits) + row * A.stride;
+        T* g = static_cast<T*>(A.grad) + row * A.grad_stride;
+        const int pieces = A.vocab / kP, p0 = block * kAhead * kThreads + threadIdx.x;
+        Vec raw[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (p0 + k * kThreads < pieces)
+                raw[k] = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p0 + k * kThreads) * kP);
+        const long long named = A.index_bits == 64 ? static_cast<const int64_t*>(A.tokens)[row]
+                                                   : static_cast<const int32_t*>(A.tokens)[row];
+        const int token = named >= 0 && named < A.vocab ? static_cast<int>(named) : -1;
+        const float most = A.stats[2 * row], logz2 = A.stats[2 * row + 1] * 1.44269504088896341f;
+        const float pull = token >= 0 && A.pull ? A.pull[row] * A.per : 0.f, turn = A.turn ? A.turn[row] * A.per : 0.f;
+        const bool none = most == -INFINITY;
+        // q (a + b log2 q)
+        const float a = -(pull + turn * A.entropy[row]), b = -turn * static_cast<float>(kLn2);
+        auto slope = [&](float v) {
+            const float l = (v - most) * A.cold - logz2;
+            return none ? 0.f : __builtin_amdgcn_exp2f(l) * fmaf(b, fmaxf(l, kNone), a);
+        };
+        // at the token pull (1 - q), not a difference of nearly equal numbers
+        auto slope_at_token = [&](float v) {
+            const float l = (v - most) * A.cold - logz2;
+            const float r = __builtin_amdgcn_exp2f(l) * fmaf(b, fmaxf(l, kNone), a + pull);
+            return none ? 0.f : fmaf(-pull, expm1f(l * static_cast<float>(kLn2)), r);
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int p = p0 + k * kThreads;
+            if (p < pieces) {
+                Vec out;
+                auto put = [&](int i, float r) { out[i] = static_cast<decltype(out[0] + out[0])>(r); };
+#pragma unroll
+                for (int i = 0; i < kP; ++i) put(i, slope(static_cast<float>(raw[k][i])));
+                if (token >= 0 && token / kP == p) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kP; ++i) v = token % kP == i ? static_cast<float>(raw[k][i]) : v;
+                    const float r = slope_at_token(v);
+#pragma unroll
+                    for (int i = 0; i < kP; ++i)
+                        if (token % kP == i) put(i, r);
+                }
+                *reinterpret_cast<Vec*>(g + static_cast<long long>(p) * kP) = out;
+            }
+        }
+        const int odd = pieces * kP + threadIdx.x;
+        if (block == 0 && odd < A.vocab) {
+            const float v = to_f32(x[odd]);
+            g[odd] = from_f32<T>(odd == token ? slope_at_token(v) : slope(v));
+        }
+    }
+}
+
+// Parts of a row: one, but where rows alone leave CUs without work; of 32768 logits and more each,
+// and so few that their top places fit a workgroup's list.
+int parts_of(const hx_logprob_args& A) {
+    if (A.rows >= 256) return 1;
+    int64_t parts = std::min<int64_t>(512 / A.rows, A.vocab / 32768);
+    if (A.top) parts = std::min<int64_t>(parts, kHeld<256> / A.top);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(parts, 64)));
+}
+
+}  // namespace
+
+size_t logprob_workspace(const hx_logprob_args& A) {
+    const int parts = parts_of(A);
+    return parts > 1 ? A.rows * parts * (sizeof(Sums) + sizeof(u64) * A.top) : 0;
+}
+
+hipError_t logprob_launch(const hx_logprob_args& A) {
+    LogprobArgs L{};
+    L.logits = A.logits, L.tokens = A.tokens, L.stride = A.logits_stride;
+    L.vocab = static_cast<int>(A.vocab), L.top = static_cast<int>(A.top), L.index_bits = static_cast<int>(A.index_bits);
+    L.cold = static_cast<float>(1.4426950408889634 / A.temperature), L.per = 1.0 / A.temperature;
+    L.logprob = A.logprob, L.entropy = A.entropy, L.stats = A.stats;
+    L.top_logprob = A.top_logprob, L.top_index = A.top_index;
+    L.parts = parts_of(A);
+    L.each = ((L.vocab + L.parts - 1) / L.parts + 7) / 8 * 8;
+    L.sums = static_cast<Sums*>(A.workspace);
+    L.keys = reinterpret_cast<u64*>(L.sums + A.rows * L.parts);
+    const hipStream_t st = static_cast<hipStream_t>(A.stream);
+    return with_type(A.type, [&](auto t) -> hipError_t {
+        using T = decltype(t);
+        const unsigned grid = static_cast<unsigned>(A.rows * L.parts);
+        auto go = [&](auto threads, auto top) {
+            constexpr int kThreads = decltype(threads)::value;
+            k_logprobs<T, kThreads, decltype(top)::value><<<grid, kThreads, 0, st>>>(L);
+        };
+        using Few = std::integral_constant<int, 256>;
+        using Many = std::integral_constant<int, 1024>;
+        if (L.each <= 8192) A.top ? go(Few{}, std::true_type{}) : go(Few{}, std::false_type{});
+        else A.top ? go(Many{}, std::true_type{}) : go(Many{}, std::false_type{});
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || L.parts == 1) return e;
+        k_logprob_join<T><<<static_cast<unsigned>(A.rows), 256, 0, st>>>(L);
+        return hipGetLastError();
+    });
+}
+
+hipError_t logprob_gradient(const hx_logprob_args& A) {
+    GradArgs G{};
+    G.logits = A.logits, G.tokens = A.tokens, G.grad = A.grad;
+    G.rows = A.rows, G.stride = A.logits_stride, G.grad_stride = A.grad_stride;
+    G.vocab = static_cast<int>(A.vocab), G.index_bits = static_cast<int>(A.index_bits);
+    G.cold = static_cast<float>(1.4426950408889634 / A.temperature), G.per = static_cast<float>(1.0 / A.temperature);
+    G.stats = A.stats, G.entropy = A.entropy, G.pull = A.grad_logprob, G.turn = A.grad_entropy;
+    return with_type(A.type, [&](auto t) {
+        using T = decltype(t);
+        constexpr int kThreads = 256, kTurn = kThreads * kAhead * static_cast<int>(16 / sizeof(T));
+        G.blocks = (G.vocab + kTurn - 1) / kTurn;
+        const unsigned grid = static_cast<unsigned>(std::min<long long>(A.rows * G.blocks, 1 << 23));
+        k_logprob_grad<T, kThreads><<<grid, kThreads, 0, static_cast<hipStream_t>(A.stream)>>>(G);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace hx

@@ -13,6 +13,8 @@ a trained network, and the gradients of both.
   gated_recurrence_step                     the same for one tick
   layer_norm, layer_norm_grad               rows brought to one mean and size, for recordings and ticks alike
   distill_loss, distill_loss_grad           the loss against a teacher's top logits
+  token_logprobs, token_logprobs_grad       log probabilities of given answers, entropies and the top
+                                            alternatives, with their gradient
   sample                                    an answer drawn from logits
 
 They take and return torch tensors on one GPU (fp32, fp16 or bf16), work on torch's current
@@ -27,7 +29,7 @@ from __future__ import annotations
 import functools
 import operator
 import struct
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -38,6 +40,7 @@ _ATTENTION = struct.Struct("=9q 3Q 9q 3Q d Q 3q Q Q 3q Q 3Q Q Q Q q Q q Q")
 _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
 _NORM = struct.Struct("=4q Q q 2Q d Q q 2Q Q q Q q 2Q Q q Q")
 _RECURRENCE = struct.Struct("=4q 2Q 4q 2Q Q 2q Q Q 2q Q 2Q Q 2Q q Q q Q")
+_LOGPROB = struct.Struct("=5q Q q Q d 3Q 2Q 2Q Q q Q q Q")
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -531,6 +534,87 @@ def distill_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
           or (out.shape[-1] > 1 and out.stride(-1) != 1)):
         raise ValueError("out has to be like the logits, its last dimension contiguous")
     return _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, weight, out), out
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns of each row."""
+
+    logprob: torch.Tensor                 # (rows,) fp32
+    entropy: torch.Tensor                 # (rows,) fp32
+    top_logprob: torch.Tensor             # (rows, top) fp32, the largest first
+    top_index: torch.Tensor               # (rows, top) int64
+    stats: torch.Tensor                   # (rows, 2) fp32: the largest logit, and log of the sum beside it
+
+
+def _tokens(tokens, rows: int, device: int) -> torch.Tensor:
+    if not isinstance(tokens, torch.Tensor):
+        raise TypeError(f"tokens has to be a tensor, got {type(tokens).__name__}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens is {tokens.dtype}, expected int32 or int64")
+    return _array(tokens, "tokens", tokens.dtype, (rows,), device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprob_space(kind: int, rows: int, vocab: int, top: int) -> int:
+    need = lib().hx_token_logprobs_workspace(_LOGPROB.pack(kind, 64, rows, vocab, top, 0, 0, 0, 1.0, *[0] * 12))
+    if need < 0:
+        raise HelioxError(lib().hx_readout_error().decode())
+    return need
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,
+                   top: int = 0) -> TokenLogprobs:
+    """Of each row of logits (rows, vocab), with q = softmax(logits / temperature): log q of the row's
+    token (tokens (rows,) int32 or int64; 0 for a token outside the vocabulary, as of padding), the
+    entropy of q, and the ``top`` most likely places (at most 256; ties: the lowest index first) with
+    their log q.  NaN ranks as -inf, and a row with a NaN or +inf has NaN for all of its numbers; a row
+    of nothing but -inf has log q -inf and entropy 0.
+
+    stats holds the largest logit m and log sum exp((logits - m) / temperature), which
+    token_logprobs_grad takes; m / temperature plus the latter is the logsumexp."""
+    device, kind, logits = _logits(logits)
+    _no_graph("token_logprobs", "take it from token_logprobs_grad", logits)
+    rows, vocab = logits.shape
+    tokens = _tokens(tokens, rows, device)
+    top, temperature = _whole(top, "top"), _real(temperature, "temperature")
+    need = _logprob_space(kind, rows, vocab, top)
+    f32 = {"dtype": torch.float32, "device": logits.device}
+    got = TokenLogprobs(torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, top), **f32),
+                        torch.empty((rows, top), dtype=torch.int64, device=logits.device), torch.empty((rows, 2), **f32))
+    space = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    _call("hx_token_logprobs", device, _LOGPROB.pack(
+        kind, 32 if tokens.dtype is torch.int32 else 64, rows, vocab, top, logits.data_ptr(), logits.stride(0),
+        tokens.data_ptr(), temperature, got.logprob.data_ptr(), got.entropy.data_ptr(), got.stats.data_ptr(),
+        got.top_logprob.data_ptr(), got.top_index.data_ptr(), 0, 0, 0, 0, _ptr(space), need, _stream(device)))
+    return got
+
+
+def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, scored: TokenLogprobs,
+                        dlogprob: Optional[torch.Tensor], dentropy: Optional[torch.Tensor] = None, *,
+                        temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient by the logits, of their type, from what token_logprobs gave for them (``scored``, its
+    entropy and stats) and the loss's gradients by logprob and by entropy ((rows,) fp32, 0 where None).
+    It goes to ``out`` where that is given; it may be the logits themselves, but not overlap them
+    otherwise.  None is made for the top alternatives."""
+    device, kind, logits = _logits(logits)
+    rows, vocab = logits.shape
+    tokens = _tokens(tokens, rows, device)
+    if not isinstance(scored, TokenLogprobs):
+        raise TypeError(f"scored has to be what token_logprobs returned, got {type(scored).__name__}")
+    entropy = _array(scored.entropy, "entropy", torch.float32, (rows,), device)
+    stats = _array(scored.stats, "stats", torch.float32, (rows, 2), device)
+    dlogprob = _array(dlogprob, "dlogprob", torch.float32, (rows,), device)
+    dentropy = _array(dentropy, "dentropy", torch.float32, (rows,), device)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif (_on_gpu(out, "out") != device or out.dtype != logits.dtype or out.shape != logits.shape
+          or (out.shape[-1] > 1 and out.stride(-1) != 1)):
+        raise ValueError("out has to be like the logits, its last dimension contiguous")
+    _call("hx_token_logprobs_grad", device, _LOGPROB.pack(
+        kind, 32 if tokens.dtype is torch.int32 else 64, rows, vocab, 0, logits.data_ptr(), logits.stride(0),
+        tokens.data_ptr(), _real(temperature, "temperature"), 0, entropy.data_ptr(), stats.data_ptr(), 0, 0,
+        _ptr(dlogprob), _ptr(dentropy), out.data_ptr(), out.stride(0), 0, 0, _stream(device)))
+    return out
 
 
 Setting = Union[float, torch.Tensor]
