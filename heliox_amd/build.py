@@ -19,7 +19,7 @@ ARCH = os.environ.get("HELIOX_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["kernels.hip", "adjoint.hip", "learn.hip", "learn_runtime.cpp", "runtime.cpp", "schedule.cpp",
            "coredat.cpp", "h5out.cpp", "readout.cpp", "readout_attention.hip", "readout_distill.hip", "readout_sample.hip",
-           "readout_norm.hip", "readout_recurrence.hip", "readout_logprob.hip"]
+           "readout_norm.hip", "readout_recurrence.hip", "readout_logprob.hip", "readout_adamw.hip"]
 COMMON = ["-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 DEVICE = [f"--offload-arch={ARCH}", "-ffp-contract=off",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

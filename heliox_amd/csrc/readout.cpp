@@ -1,9 +1,13 @@
 // C entry points of the readout operators: argument checks, empty problems, error texts.
 #include "readout.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <new>
+#include <utility>
+#include <vector>
 
 namespace {
 
@@ -132,6 +136,58 @@ int logprob_sizes(const char* call, const hx_logprob_args* A) {
     return 0;
 }
 
+int adamw_tensors(const char* call, const hx_adamw_args* A) {
+    // what is written (parameters) and read (gradients): first byte, end, whether written
+    struct Range { uintptr_t from, to; bool written; };
+    std::vector<Range> ranges;
+    ranges.reserve(2 * A->count);
+    int64_t used = 0;
+    for (int64_t i = 0; i < A->count; ++i) {
+        const hx_adamw_tensor& t = A->tensors[i];
+        const long long n = i;
+        if (!known_type(t.type) || !known_type(t.grad_type)) return refuse("%s: tensor %lld: type is not known", call, n);
+        if (t.elements < 0 || t.elements > (int64_t(1) << 34))
+            return refuse("%s: tensor %lld: elements has to be in 0..2^34", call, n);
+        if (!std::isfinite(t.weight_decay)) return refuse("%s: tensor %lld: weight_decay is not finite", call, n);
+        if (t.start % 256 || t.start < used)
+            return refuse("%s: tensor %lld: moments start at multiples of 256, each after those before", call, n);
+        used = t.start + (t.elements + 255) / 256 * 256;
+        if (t.start > A->moments || used > A->moments)
+            return refuse("%s: tensor %lld: %lld moments are too few", call, n, (long long)A->moments);
+        if (!t.elements) continue;
+        if (!t.param || !t.grad) return refuse("%s: tensor %lld: param or grad is missing", call, n);
+        const uintptr_t p = reinterpret_cast<uintptr_t>(t.param), g = reinterpret_cast<uintptr_t>(t.grad);
+        ranges.push_back({p, p + t.elements * (t.type == HX_F32 ? 4 : 2), true});
+        ranges.push_back({g, g + t.elements * (t.grad_type == HX_F32 ? 4 : 2), false});
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t written = 0, any = 0;
+    for (const Range& r : ranges) {
+        if (r.from < (r.written ? any : written)) return refuse("%s: parameters overlap each other or gradients", call);
+        any = std::max(any, r.to);
+        if (r.written) written = std::max(written, r.to);
+    }
+    return 0;
+}
+
+int adamw_check(const char* call, const hx_adamw_args* A) {
+    if (!A) return refuse("%s: no arguments", call);
+    if (A->bits != 8 && A->bits != 32) return refuse("%s: bits has to be 8 or 32", call);
+    if (A->count < 0 || A->count > (1 << 20)) return refuse("%s: count has to be in 0..2^20", call);
+    if (!(A->beta1 >= 0 && A->beta1 < 1 && A->beta2 >= 0 && A->beta2 < 1))
+        return refuse("%s: beta1 and beta2 have to be in [0, 1)", call);
+    if (!(A->eps >= 0) || !std::isfinite(A->eps)) return refuse("%s: eps has to be a number, at least 0", call);
+    if (!std::isfinite(A->lr)) return refuse("%s: lr is not finite", call);
+    if (!std::isfinite(A->grad_scale)) return refuse("%s: grad_scale is not finite", call);
+    if (!A->step || (A->count && !A->tensors)) return refuse("%s: step or tensors is missing", call);
+    if (A->moments < 0 || (A->moments && (!A->m || !A->v || (A->bits == 8 && (!A->m_scale || !A->v_scale)))))
+        return refuse("%s: m, v or their scales are missing", call);
+    for (const void* p : {static_cast<const void*>(A->m), static_cast<const void*>(A->v), static_cast<const void*>(A->step)})
+        if (reinterpret_cast<uintptr_t>(p) % 16)
+            return refuse("%s: m, v and step have to start at multiples of 16 bytes", call);
+    return adamw_tensors(call, A);
+}
+
 int norm_sizes(const char* call, const hx_norm_args* A) {
     if (!A) return refuse("%s: no arguments", call);
     if (!known_type(A->type) || !known_type(A->weight_type)) return refuse("%s: type is not known", call);
@@ -227,6 +283,16 @@ int hx_sample(const hx_sample_args* A) {
     if (!A->logits || !A->u || !A->token || !A->logprob)
         return refuse("%s: logits, u, token or logprob is missing", call);
     return launched(call, hx::sample_launch(*A));
+}
+
+int hx_adamw_step(const hx_adamw_args* A) {
+    const char* call = "hx_adamw_step";
+    try {
+        if (adamw_check(call, A)) return -1;
+    } catch (const std::bad_alloc&) {
+        return refuse("%s: no host memory", call);
+    }
+    return launched(call, hx::adamw_launch(*A));
 }
 
 int64_t hx_token_logprobs_workspace(const hx_logprob_args* A) {

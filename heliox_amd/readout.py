@@ -16,6 +16,7 @@ a trained network, and the gradients of both.
   token_logprobs, token_logprobs_grad       log probabilities of given answers, entropies and the top
                                             alternatives, with their gradient
   sample                                    an answer drawn from logits
+  adamw_state, adamw_step                   an AdamW step of many parameters at once, moments in 32 bits or 8
 
 They take and return torch tensors on one GPU (fp32, fp16 or bf16), work on torch's current
 stream, wait for nothing, and may be captured into a graph.  Sums, softmax statistics and
@@ -26,10 +27,11 @@ that have one refuse inputs that require a gradient while torch records.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import operator
 import struct
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -41,6 +43,8 @@ _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
 _NORM = struct.Struct("=4q Q q 2Q d Q q 2Q Q q Q q 2Q Q q Q")
 _RECURRENCE = struct.Struct("=4q 2Q 4q 2Q Q 2q Q Q 2q Q 2Q Q 2Q q Q q Q")
 _LOGPROB = struct.Struct("=5q Q q Q d 3Q 2Q 2Q Q q Q q Q")
+_ADAMW = struct.Struct("=2q Q 2Q 2Q q 5d 2Q Q Q")
+_ADAMW_TENSOR = "2q2Q2qd"
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -656,3 +660,119 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
         kind, rows, vocab, _ptr(logits), logits.stride(0), _ptr(u), *map(_ptr, pointers), values[0], values[2],
         values[3], values[1], _ptr(token), _ptr(logprob), _stream(device)))
     return token, logprob
+
+
+class AdamWState:
+    """What adamw_step keeps for a list of parameters, made by adamw_state.  Tensor i's moments are
+    elements starts[i] to starts[i] + sizes[i] of m and v; starts are multiples of 256.
+
+    bits 32: m and v are fp32.  bits 8: m and the root of v are float8_e4m3fn, each 256 elements
+    relative to m_scale and v_scale (fp32, one for each 256).  step, int64 on the GPU, counts the
+    steps taken.  All of them may be saved, and copied into another state of the same parameters."""
+
+    def __init__(self, sizes: Sequence[int], bits: int, device: int):
+        self.bits, self.sizes, self.device, self.starts = bits, tuple(sizes), device, []
+        whole = 0
+        for n in self.sizes:
+            self.starts.append(whole)
+            whole += -(-n // 256) * 256
+        on = {"device": f"cuda:{device}"}
+        kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        self.m, self.v = (torch.zeros(whole, dtype=torch.uint8 if bits == 8 else kind, **on).view(kind) for _ in range(2))
+        self.m_scale, self.v_scale = (torch.zeros(whole // 256, **on) if bits == 8 else None for _ in range(2))
+        self._count = torch.zeros(2, dtype=torch.int64, **on)
+        self.step = self._count[:1]
+
+
+def _parameters(params) -> Tuple[list, int]:
+    params = list(params)
+    device = None
+    for i, p in enumerate(params):
+        here = _on_gpu(p, f"params[{i}]")
+        if device is None:
+            device = here
+        elif here != device:
+            raise ValueError(f"params[{i}] is on cuda:{here}, params[0] on cuda:{device}")
+        if not p.is_contiguous():
+            raise ValueError(f"params[{i}] has to be contiguous")
+        _type(p, f"params[{i}]")
+    if device is None:
+        raise ValueError("params has no tensors")
+    return params, device
+
+
+def adamw_state(params: Sequence[torch.Tensor], *, bits: int = 32) -> AdamWState:
+    """A state of zeros for these parameters (contiguous tensors on one GPU, fp32, fp16 or bf16): 8
+    bytes of moments for each of their elements with bits=32, 2 and a 32nd with bits=8."""
+    params, device = _parameters(params)
+    if bits not in (8, 32):
+        raise ValueError(f"bits has to be 8 or 32, got {bits}")
+    return AdamWState([p.numel() for p in params], bits, device)
+
+
+def _one_number(x, what: str, device: int):
+    """(a tensor's address or 0, a number): a setting that is either."""
+    if isinstance(x, torch.Tensor):
+        if x.numel() != 1:
+            raise ValueError(f"{what} has to be one number, got shape {tuple(x.shape)}")
+        return _array(x, what, torch.float32, x.shape, device).data_ptr(), 0.0
+    return 0, _real(x, what)
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], state: AdamWState, *,
+               lr: Setting, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: Union[float, Sequence[float]] = 0.01, grad_scale: Setting = 1.0) -> None:
+    """One AdamW step, in place: with t the state's step after it and g = grad_scale grad,
+
+        m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
+        p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps),
+
+    in fp32, p rounded once to its type.  grads are of the parameters' shapes and of fp32, fp16 or bf16,
+    whatever their parameter is; a parameter whose gradient is None stays as it is, with its
+    moments.  weight_decay is one number or one for each parameter.  lr and grad_scale (as of a clipped
+    norm) are numbers, or fp32 tensors of one on the GPU, which a captured step reads anew at every
+    replay, as it does the state's step.
+
+    With 8 bits the moments are rounded after the step has used them; a gradient that is not finite
+    reaches the 256 elements that share its scale.  Parameters that overlap each other or a gradient
+    are refused."""
+    if not isinstance(state, AdamWState):
+        raise TypeError(f"state has to be what adamw_state returned, got {type(state).__name__}")
+    params, device = _parameters(params)
+    grads = list(grads)
+    if device != state.device:
+        raise ValueError(f"params are on cuda:{device}, the state on cuda:{state.device}")
+    if len(grads) != len(params) or tuple(p.numel() for p in params) != state.sizes:
+        raise ValueError(f"{len(params)} params and {len(grads)} grads do not fit a state of sizes {state.sizes}")
+    if isinstance(weight_decay, (list, tuple)):
+        if len(weight_decay) != len(params):
+            raise ValueError(f"{len(weight_decay)} weight_decay for {len(params)} params")
+        decays = [_real(w, "weight_decay") for w in weight_decay]
+    else:
+        decays = [_real(weight_decay, "weight_decay")] * len(params)
+    if not isinstance(betas, (list, tuple)) or len(betas) != 2:
+        raise TypeError("betas has to be two numbers")
+    beta1, beta2 = (_real(b, "betas") for b in betas)
+    lr_ptr, lr = _one_number(lr, "lr", device)
+    scale_ptr, scale = _one_number(grad_scale, "grad_scale", device)
+    fields, kept, moved = [], [], []
+    for i, (p, g, start, decay) in enumerate(zip(params, grads, state.starts, decays)):
+        if g is None:
+            continue
+        if not isinstance(g, torch.Tensor) or g.get_device() != device:
+            if _on_gpu(g, f"grads[{i}]") != device:
+                raise ValueError(f"grads[{i}] is on {g.device}, params on cuda:{device}")
+        if g.shape != p.shape:
+            raise ValueError(f"grads[{i}] has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            kept.append(g)
+        moved.append(p)
+        fields += (_TYPES[p.dtype], _type(g, f"grads[{i}]"), p.data_ptr(), g.data_ptr(), state.sizes[i], start, decay)
+    tensors = bytearray(struct.pack("=" + _ADAMW_TENSOR * len(moved), *fields))
+    table = ctypes.addressof(ctypes.c_char.from_buffer(tensors)) if tensors else 0
+    _call("hx_adamw_step", device, _ADAMW.pack(
+        state.bits, len(moved), table, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale), _ptr(state.v_scale),
+        state.m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr, lr_ptr, state._count.data_ptr(),
+        _stream(device)))
+    torch.autograd.graph.increment_version(moved)

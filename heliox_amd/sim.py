@@ -183,6 +183,7 @@ SIGNATURES = {
     "hx_linear_attention_step": (C.c_int, [C.c_char_p]),
     "hx_distill_loss": (C.c_int, [C.c_char_p]),
     "hx_sample": (C.c_int, [C.c_char_p]),
+    "hx_adamw_step": (C.c_int, [C.c_char_p]),
     "hx_token_logprobs_workspace": (C.c_int64, [C.c_char_p]),
     "hx_token_logprobs": (C.c_int, [C.c_char_p]),
     "hx_token_logprobs_grad": (C.c_int, [C.c_char_p]),

@@ -719,9 +719,10 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * / 448 (fp32; 0, and the numbers 0, where that largest is under 2^-100), rounded to nearest even;
  * a root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
  * that is not finite reaches its block's 256 elements in 8 bits.
- * The parameters of a call do not overlap each other or the gradients (refused); arrays of moments
- * are the caller's to keep apart.  `step` (two int64: the count, and a zero that the call uses and
- * leaves zero) is device memory, so that a captured step counts on at every replay. */
+ * Tensors come in the order of their starts, each within `moments`, its last 256 filled up with
+ * elements that belong to none (kept zero).  The parameters of a call do not overlap each other or
+ * the gradients (refused).  `step` (two int64: the count, and room that the call uses; at a multiple
+ * of 16 bytes, as m and v) is device memory, so that a captured step counts on at every replay. */
 typedef struct hx_adamw_tensor {
     int64_t type, grad_type;
     void* param;                                          /* contiguous, elements of them */
