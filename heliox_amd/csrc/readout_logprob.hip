@@ -7,8 +7,9 @@
 // places come out of the same pass: every wave's lanes hold the largest logit of their first
 // pieces, and a bound that enough of these reach lets few of the row's logits through, a few
 // hundred of a hundred thousand.  They wait in LDS as whole numbers, logit above index, and each
-// counts those above it.  Where the bound lets too many through (logits that rise along the row,
-// or are all the same) the top places' own bound is found byte by byte from histograms.
+// counts those above it.  Where more than 256 come through, the top places' own bound is found
+// byte by byte from histograms, of those that came or, where a wave's list is too short for them
+// (logits that rise along the row, or are all the same), of the whole row.
 //
 // Few long rows are cut into parts, which a second launch joins.  Bound by the logits' bytes, read
 // once; the gradient reads and writes them once.
@@ -57,17 +58,16 @@ __device__ __forceinline__ long long token_of(const LogprobArgs& A, long long ro
     return A.index_bits == 64 ? static_cast<const int64_t*>(A.tokens)[row] : static_cast<const int32_t*>(A.tokens)[row];
 }
 
-template <int kThreads> constexpr int kHeld = kThreads == 1024 ? 4096 : 2048;
+constexpr int kEach = 544, kBest = 256;    // keys that a wave holds, and that are ranked
 
 template <int kThreads>
 struct Shared {
     double red[kThreads / 64];
     float most[kThreads / 64], bound[kThreads / 64];
-    int count;
+    int count[kThreads / 64], chosen, left;
     unsigned bins[256];
     u64 prefix, answer;
-    int left;
-    u64 held[kHeld<kThreads>];
+    u64 best[kBest], held[kThreads / 64][kEach];
 };
 
 // The k-th largest of a wave's values, to 16 bits of their order (rounded down): at least k of them
@@ -82,63 +82,96 @@ __device__ __forceinline__ float kth_of_wave(float v, int k) {
     return found <= 0x7f ? -INFINITY : value_of(found << 16);
 }
 
-// Places above the bound that is found from the histograms: exactly `top` keys (or all n) go to sh.held.
-template <class T, int kThreads>
-__device__ void select_exactly(const T* x, int first, int last, int top, Shared<kThreads>& sh) {
-    if (threadIdx.x == 0) sh.prefix = 0, sh.left = min(top, last - first), sh.answer = 0;
+// The top-th largest of `total` distinct keys, byte by byte from histograms.  each(f) calls f(key,
+// whether it is one) for all of them, a whole wave at a time.
+template <int kThreads, class Each>
+__device__ u64 bound_of(int top, int total, Shared<kThreads>& sh, Each each) {
+    const int lane = threadIdx.x % 64;
+    if (threadIdx.x == 0) sh.prefix = sh.answer = 0, sh.left = min(top, total);
     for (int shift = 56; shift >= 0; shift -= 8) {
         for (int b = threadIdx.x; b < 256; b += kThreads) sh.bins[b] = 0;
         __syncthreads();
-        const u64 prefix = sh.prefix;
-        const bool done = sh.answer != 0;
-        if (!done)
-            for (int j0 = first; j0 < last; j0 += kThreads) {
-                const int j = j0 + threadIdx.x;
-                const u64 key = j < last ? key_of(to_f32(x[j]), j) : 0;
-                const bool in = j < last && (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8));
-                const int bin = static_cast<int>(key >> shift & 255);
-                const u64 live = __ballot(in);
-                if (!live) continue;
-                const int one = __shfl(bin, __ffsll(live) - 1);
-                if (__all(!in || bin == one)) {       // a wave of equal logits adds once
-                    if (threadIdx.x % 64 == 0) atomicAdd(&sh.bins[one], static_cast<unsigned>(__popcll(live)));
-                } else if (in) {
-                    atomicAdd(&sh.bins[bin], 1u);
-                }
+        const u64 prefix = sh.prefix, answer = sh.answer;
+        if (answer) return answer;
+        each([&](u64 key, bool is) {
+            const bool in = is && (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8));
+            const int bin = static_cast<int>(key >> shift & 255);
+            const u64 live = __ballot(in);
+            if (!live) return;
+            const int one = __shfl(bin, __ffsll(live) - 1);
+            if (__all(!in || bin == one)) {       // a wave of equal logits adds once
+                if (lane == 0) atomicAdd(&sh.bins[one], static_cast<unsigned>(__popcll(live)));
+            } else if (in) {
+                atomicAdd(&sh.bins[bin], 1u);
             }
+        });
         __syncthreads();
-        if (threadIdx.x == 0 && !done) {
-            int left = sh.left, b = 255;
-            while (b > 0 && static_cast<int>(sh.bins[b]) < left) left -= sh.bins[b--];
-            sh.prefix = prefix | static_cast<u64>(b) << shift;
-            sh.left = left;
-            // the whole bin belongs: its first possible key is the bound
-            if (static_cast<int>(sh.bins[b]) == left || shift == 0) sh.answer = sh.prefix;
+        if (threadIdx.x < 64) {
+            // a lane for four bins, the highest first: the lane whose bins reach what is left
+            int n[4], mine = 0;
+            for (int i = 0; i < 4; ++i) mine += n[i] = sh.bins[255 - 4 * lane - i];
+            int upto = mine;
+            for (int d = 1; d < 64; d *= 2) {
+                const int below = __shfl_up(upto, d);
+                if (lane >= d) upto += below;
+            }
+            const int left = sh.left;
+            if (upto >= left && upto - mine < left) {
+                int rest = left - (upto - mine), i = 0;
+                while (n[i] < rest) rest -= n[i++];
+                sh.prefix = prefix | static_cast<u64>(255 - 4 * lane - i) << shift;
+                sh.left = rest;
+                // where the whole bin belongs its first possible key is the bound
+                if (n[i] == rest || shift == 0) sh.answer = sh.prefix;
+            }
         }
         __syncthreads();
     }
-    const u64 bound = sh.answer;
-    if (threadIdx.x == 0) sh.count = 0;
+    return sh.answer;
+}
+
+// Keys of at least `bound` to sh.best.
+template <int kThreads, class Each>
+__device__ void choose(u64 bound, Shared<kThreads>& sh, Each each) {
+    if (threadIdx.x == 0) sh.chosen = 0;
     __syncthreads();
-    for (int j = first + threadIdx.x; j < last; j += kThreads) {
-        const u64 key = key_of(to_f32(x[j]), j);
-        if (key >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kHeld<kThreads>) sh.held[at] = key;
+    each([&](u64 key, bool is) {
+        if (is && key >= bound) {
+            const int at = atomicAdd(&sh.chosen, 1);
+            if (at < kBest) sh.best[at] = key;
         }
-    }
+    });
     __syncthreads();
 }
 
-// Calls put(rank, key) for the top largest of sh.held's n keys, from the largest on.
+// Calls put(rank, key) for the top largest of sh.best's keys.
 template <int kThreads, class F>
-__device__ __forceinline__ void each_ranked(const Shared<kThreads>& sh, int n, int top, F put) {
+__device__ __forceinline__ void rank_best(int top, const Shared<kThreads>& sh, F put) {
+    const int n = min(sh.chosen, kBest);
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const u64 key = sh.held[i];
+        const u64 key = sh.best[i];
         int rank = 0;
-        for (int k = 0; k < n; ++k) rank += sh.held[k] > key;
+        for (int k = 0; k < n; ++k) rank += sh.best[k] > key;
         if (rank < top) put(rank, key);
     }
+}
+
+// Calls put(rank, key) for the top largest keys, from the largest on; all(f) as each above, over
+// every key of the part or row, for where the waves' lists do not hold those that may be among them.
+template <int kThreads, class All, class F>
+__device__ __forceinline__ void each_ranked(int top, int whole, Shared<kThreads>& sh, All all, F put) {
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    int total = 0, longest = 0;
+    for (int v = 0; v < kThreads / 64; ++v) {
+        total += sh.count[v];
+        longest = max(longest, sh.count[v]);
+    }
+    auto held = [&](auto f) {
+        for (int i = 0; i < sh.count[wave]; i += 64) f(i + lane < sh.count[wave] ? sh.held[wave][i + lane] : 0, i + lane < sh.count[wave]);
+    };
+    if (longest > kEach) choose<kThreads>(bound_of<kThreads>(top, whole, sh, all), sh, all);
+    else choose<kThreads>(total > kBest ? bound_of<kThreads>(top, total, sh, held) : 0, sh, held);
+    rank_best<kThreads>(top, sh, put);
 }
 
 // A row's results from its sums.  Every thread has the same sums; keys go through put_top.
@@ -201,32 +234,41 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
         if (static_cast<int>(threadIdx.x) + k * kThreads < pieces)
 #pragma unroll
             for (int i = 0; i < kP; ++i) most = fmaxf(most, static_cast<float>(raw[k][i]));
-    if (threadIdx.x == 0) sh.count = 0;
     float bound = -INFINITY;
     {
-        const int wave = threadIdx.x / 64;
-        // waves whose every lane holds a piece share the top places among them
-        const int full = min(pieces, kThreads) / 64, quota = full ? (A.top + full - 1) / full : 65;
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        // Waves whose every lane holds a piece share the top places among them: `quota` of a wave's
+        // lanes are not below its own bound, and the bound that `need` waves reach holds for all.
+        const int full = min(pieces, kThreads) / 64, quota = full ? max(1, (A.top + full - 1) / full) : 65;
+        const int need = (A.top + quota - 1) / quota;
         float m = most;
         for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-        float b = INFINITY;
-        if (kTop && wave < full && quota <= 64) b = kth_of_wave(most, quota);
-        if (threadIdx.x % 64 == 0) sh.most[wave] = m, sh.bound[wave] = b;
+        if (kTop && quota <= 64) bound = quota == 1 ? m : kth_of_wave(most, quota);
+        if (lane == 0) sh.most[wave] = m, sh.bound[wave] = wave < full ? bound : -INFINITY;
         __syncthreads();
-        bound = INFINITY;
+        const float mine = lane < kWaves ? sh.bound[lane] : -INFINITY;
+        int above = 0;
         for (int v = 0; v < kWaves; ++v) {
             most = fmaxf(most, sh.most[v]);
-            bound = fminf(bound, sh.bound[v]);
+            const float other = sh.bound[v];
+            above += other > mine || (other == mine && v < lane);
         }
-        if (quota > 64) bound = -INFINITY;
+        if (kTop && quota <= 64) bound = __shfl(mine, __ffsll(__ballot(lane < kWaves && above == need - 1)) - 1);
     }
     float base = most == -INFINITY ? 0.f : most, limit = most == -INFINITY ? -INFINITY : base + kFar / A.cold;
     float z = 0.f, s = 0.f;
+    // A wave's own list: no atomics, and no wait before the next logits.  The lanes that call are a
+    // wave's first ones, so that lane 0 has counted them all.
+    int kept = 0;
     auto keep = [&](float v, int j) {
-        if ((v != v ? -INFINITY : v) >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kHeld<kThreads>) sh.held[at] = key_of(v, j);
-        }
+        const bool in = (v != v ? -INFINITY : v) >= bound;
+        const u64 those = __ballot(in);
+        if (!those) return;
+        const int before = __builtin_amdgcn_readfirstlane(kept);
+        const int at = before + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(those >> 32),
+                                                        __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(those), 0));
+        if (in && at < kEach) sh.held[threadIdx.x / 64][at] = key_of(v, j);
+        kept = before + __popcll(those);
     };
     auto take = [&](const float* v, int n, int j) {
         float c = v[0];
@@ -250,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
                 s = fmaf(w, fmaxf(y, kNone), s);
             }
         if constexpr (kTop)
-            if (!(c < bound))
+            if (__any(!(c < bound)))
 #pragma unroll
                 for (int i = 0; i < kP; ++i)
                     if (i < n) keep(v[i], j + i);
@@ -285,19 +327,26 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
     S.s = block_reduce<kThreads>(f * (s + (z == 0.f ? 0. : less * z)), sh.red, add);
     S.z = block_reduce<kThreads>(f * z, sh.red, add);
     if constexpr (kTop) {
-        if (sh.count > kHeld<kThreads>) select_exactly<T, kThreads>(x, first, last, A.top, sh);
+        if (threadIdx.x % 64 == 0) sh.count[threadIdx.x / 64] = kept;
+        __syncthreads();
     }
-    const int n = min(sh.count, kHeld<kThreads>);
+    auto all = [&](auto f) {
+        for (int j0 = first; j0 < last; j0 += kThreads) {
+            const int j = j0 + static_cast<int>(threadIdx.x);
+            f(j < last ? key_of(to_f32(x[j]), j) : 0, j < last);
+        }
+    };
     if (A.parts == 1) {
         const Finish done(S);
         if (threadIdx.x == 0) finish_row(A, row, x, S, done);
-        if constexpr (kTop) each_ranked(sh, n, A.top, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
+        if constexpr (kTop)
+            each_ranked<kThreads>(A.top, last - first, sh, all, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
     } else {
         if (threadIdx.x == 0) A.sums[blockIdx.x] = S;
         if constexpr (kTop) {
             u64* const to = A.keys + static_cast<long long>(blockIdx.x) * A.top;
-            for (int i = n + threadIdx.x; i < A.top; i += kThreads) to[i] = 0;
-            each_ranked(sh, n, A.top, [&](int rank, u64 key) { to[rank] = key; });
+            for (int i = last - first + threadIdx.x; i < A.top; i += kThreads) to[i] = 0;
+            each_ranked<kThreads>(A.top, last - first, sh, all, [&](int rank, u64 key) { to[rank] = key; });
         }
     }
 }
@@ -324,9 +373,16 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobArgs A) {
     const Finish done(S);
     if (threadIdx.x == 0) finish_row(A, row, x, S, done);
     const int n = A.parts * A.top;
-    for (int i = threadIdx.x; i < n; i += 256) sh.held[i] = A.keys[row * n + i];
-    __syncthreads();
-    each_ranked(sh, n, A.top, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
+    auto all = [&](auto f) {
+        for (int i0 = 0; i0 < n; i0 += 256) {
+            const int i = i0 + static_cast<int>(threadIdx.x);
+            const u64 key = i < n ? A.keys[row * n + i] : 0;
+            f(key, key != 0);
+        }
+    };
+    if (!A.top) return;
+    choose<256>(n > kBest ? bound_of<256>(A.top, n, sh, all) : 0, sh, all);
+    rank_best<256>(A.top, sh, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
 }
 
 struct GradArgs {
@@ -400,12 +456,10 @@ __global__ void __launch_bounds__(kThreads) k_logprob_grad(GradArgs A) {
     }
 }
 
-// Parts of a row: one, but where rows alone leave CUs without work; of 32768 logits and more each,
-// and so few that their top places fit a workgroup's list.
+// Parts of a row: one, but where rows alone leave CUs without work; of 32768 logits and more each.
 int parts_of(const hx_logprob_args& A) {
     if (A.rows >= 256) return 1;
     int64_t parts = std::min<int64_t>(512 / A.rows, A.vocab / 32768);
-    if (A.top) parts = std::min<int64_t>(parts, kHeld<256> / A.top);
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(parts, 64)));
 }
 
@@ -435,10 +489,16 @@ hipError_t logprob_launch(const hx_logprob_args& A) {
             constexpr int kThreads = decltype(threads)::value;
             k_logprobs<T, kThreads, decltype(top)::value><<<grid, kThreads, 0, st>>>(L);
         };
-        using Few = std::integral_constant<int, 256>;
-        using Many = std::integral_constant<int, 1024>;
-        if (L.each <= 8192) A.top ? go(Few{}, std::true_type{}) : go(Few{}, std::false_type{});
-        else A.top ? go(Many{}, std::true_type{}) : go(Many{}, std::false_type{});
+        // Threads: 512 keep four rows on a CU, whose starts and ends lie beside the others' middles (2048 x
+        // 131072 in bf16, top 5: 118 us, with 1024 threads 127, with 256 143; top 100: 176 and 188).  More
+        // than 128 top places would pass more logits to each of eight waves than its list holds (top
+        // 256: 232 us with 1024 threads, 997 with 512).
+        auto pick = [&](auto with_top) {
+            if (L.each <= 8192) go(std::integral_constant<int, 256>{}, with_top);
+            else if (A.top <= 128) go(std::integral_constant<int, 512>{}, with_top);
+            else go(std::integral_constant<int, 1024>{}, with_top);
+        };
+        A.top ? pick(std::true_type{}) : pick(std::false_type{});
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || L.parts == 1) return e;
         k_logprob_join<T><<<static_cast<unsigned>(A.rows), 256, 0, st>>>(L);

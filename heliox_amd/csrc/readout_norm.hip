@@ -407,20 +407,24 @@ __global__ void __launch_bounds__(256) k_norm_columns(NormArgs A, long long rows
     part[A.width + j] = db;
 }
 
-// The workgroups' sums, added up: 64 columns a workgroup, sixteen runs of rows each.
+// The workgroups' sums, added up: 32 columns a workgroup, 32 runs of rows each.
 __global__ void __launch_bounds__(1024) k_norm_join(const float* part, int parts, int width, float* dw, float* db) {
-    __shared__ float sh[16][64];
-    const long long whole = 2LL * width, column = static_cast<long long>(blockIdx.x) * 64 + threadIdx.x % 64;
+    constexpr int kColumns = 32, kRuns = 32;
+    __shared__ float sh[kRuns][kColumns + 1];
+    const long long whole = 2LL * width, column = static_cast<long long>(blockIdx.x) * kColumns + threadIdx.x % kColumns;
+    const int run = threadIdx.x / kColumns;
     float s = 0.f;
-    if (column < whole)
-        for (int p = threadIdx.x / 64; p < parts; p += 16) s += part[p * whole + column];
-    sh[threadIdx.x / 64][threadIdx.x % 64] = s;
-    __syncthreads();
-    if (threadIdx.x < 64 && column < whole) {
-        s = 0.f;
-        for (int i = 0; i < 16; ++i) s += sh[i][threadIdx.x];
-        (column < width ? dw[column] : db[column - width]) = s;
+    if (column < whole) {
+#pragma unroll 8
+        for (int p = run; p < parts; p += kRuns) s += part[p * whole + column];
     }
+    sh[run][threadIdx.x % kColumns] = s;
+    __syncthreads();
+    // the 32 runs of a column lie across half a wave
+    s = sh[threadIdx.x % kRuns][threadIdx.x / kRuns];
+    for (int d = kRuns / 2; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    const long long mine = static_cast<long long>(blockIdx.x) * kColumns + threadIdx.x / kRuns;
+    if (threadIdx.x % kRuns == 0 && mine < whole) (mine < width ? dw[mine] : db[mine - width]) = s;
 }
 
 // How a row is held: kE elements a piece, kGroup lanes, kV pieces a lane.
@@ -526,7 +530,7 @@ hipError_t norm_backward(const hx_norm_args& A) {
         });
     });
     if (e != hipSuccess || !A.grad_weight) return e;
-    k_norm_join<<<static_cast<unsigned>((2 * A.width + 63) / 64), 1024, 0, st>>>(N.part, parts, N.width, A.grad_weight,
+    k_norm_join<<<static_cast<unsigned>((2 * A.width + 31) / 32), 1024, 0, st>>>(N.part, parts, N.width, A.grad_weight,
                                                                                A.grad_bias);
     return hipGetLastError();
 }
