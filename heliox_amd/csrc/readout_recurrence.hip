@@ -21,7 +21,9 @@
 namespace hx {
 namespace {
 
-constexpr int kU = 8, kW = 8, kTile = kU * kW, kThreads = 64 * kW;
+constexpr int kW = 8, kThreads = 64 * kW;
+template <int kC> constexpr int kU = 16 / kC;              // steps that a wave holds
+template <int kC> constexpr int kTile = kU<kC> * kW;
 
 struct RecurrenceArgs {
     const void *x, *gate, *grad_o;
@@ -111,12 +113,14 @@ __device__ __forceinline__ void fetch(typename Packed<T, kC>::Vec (&to)[kN], con
 // The whole walk.
 template <class T, int kC>
 __global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
     using Vec = typename Packed<T, kC>::Vec;
     using F = typename Floats<kC>::Vec;
     __shared__ float ends[2][kW][2 * kC][64];
     const int wave = wave_of(), lane = threadIdx.x % 64;
     int turn = 0;
-    for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
+    // (the segments' own launch went over the data from its start: its end is in the cache)
+    for (long long id = A.batch * A.segments * A.blocks - 1 - blockIdx.x; id >= 0; id -= gridDim.x) {
         const Where w = Where::of<kC>(A, id);
         const int first = w.segment * A.steps, last = min(first + A.steps, A.time);
         float h[kC];
@@ -195,6 +199,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
 // P, Y (and, for the gradient, R) of each segment: every wave takes a share of its steps.
 template <class T, int kC, bool kGrad>
 __global__ void __launch_bounds__(kThreads, 4) k_segments(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
     using Vec = typename Packed<T, kC>::Vec;
     constexpr int kN = kGrad ? 3 : 2;
     __shared__ float ends[kW][kN * kC][64];
@@ -298,10 +303,11 @@ __global__ void __launch_bounds__(1024) k_join(RecurrenceArgs A) {
 // The gradients of kTile steps, from what enters them on both sides.
 template <class T, int kC>
 __global__ void __launch_bounds__(kThreads, 4) k_grad(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
     using Vec = typename Packed<T, kC>::Vec;
     __shared__ float ends[kW][3 * kC][64];
     const int wave = wave_of(), lane = threadIdx.x % 64;
-    for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
+    for (long long id = A.batch * A.segments * A.blocks - 1 - blockIdx.x; id >= 0; id -= gridDim.x) {     // as above
         const Where w = Where::of<kC>(A, id);
         const int t = w.segment * kTile + wave * kU;
         Vec x[kU], g[kU], d[kU];
@@ -432,19 +438,24 @@ __global__ void __launch_bounds__(256) k_step(RecurrenceArgs A, float* states, c
     *reinterpret_cast<Few*>(o) = out;
 }
 
-int channels_a_lane(const hx_recurrence_args& A) { return A.type == HX_F32 || A.channels == 1 ? 1 : 2; }
+struct Cut { int lanes, segments, steps; };   // lanes: channels a lane
 
-struct Cut { int segments, steps; };
-
-// Segments of whole tiles.  The gradient's are one tile each.  Forward, 128 workgroups and more walk
-// along whole sequences; fewer are cut until there are 512, as far as there are tiles.
+// Segments of whole tiles.  The gradient's are one tile each.
+//
+// Forward, workgroups that walk along whole sequences read the data once, those that walk along
+// segments twice; but a walk's tiles come one after another, and a CU with one walk waits for
+// its loads.  8 x 4096 x 2048 in bf16: 128 walks of two channels a lane 123 us, 256 of one 96,
+// 670 MB in segments 137; half of the sequences: 128 walks of one channel 90, segments 76.
 Cut cut_of(const hx_recurrence_args& A, bool grad) {
-    const long long tiles = std::max<long long>(1, (A.time + kTile - 1) / kTile);
-    const long long width = 64 * channels_a_lane(A), walks = A.batch * ((A.channels + width - 1) / width);
-    long long segments = grad ? tiles : walks >= 128 ? 1 : std::min(tiles, (512 + walks - 1) / walks);
+    auto walks = [&](int lanes) { return A.batch * ((A.channels + 64 * lanes - 1) / (64 * lanes)); };
+    const int most = A.type == HX_F32 || A.channels == 1 ? 1 : 2;
+    const bool wide = most == 2 && (grad || walks(2) >= 256 || walks(1) < 160);
+    const int lanes = wide ? 2 : 1, tile = wide ? kTile<2> : kTile<1>;
+    const long long tiles = std::max<long long>(1, (A.time + tile - 1) / tile);
+    long long segments = grad ? tiles : walks(1) >= 160 ? 1 : std::min<long long>(tiles, (512 + walks(lanes) - 1) / walks(lanes));
     const long long each = (tiles + segments - 1) / segments;
     segments = (tiles + each - 1) / each;
-    return {static_cast<int>(segments), static_cast<int>(each * kTile)};
+    return {lanes, static_cast<int>(segments), static_cast<int>(each * tile)};
 }
 
 // The workspace's parts, one after another.
@@ -463,7 +474,7 @@ RecurrenceArgs recurrence_args(const hx_recurrence_args& A, const Cut& cut) {
     R.lengths = A.lengths, R.initial = A.initial_state, R.grad_end = A.grad_end;
     R.end = A.end_state, R.grad_initial = A.grad_initial;
     R.time = static_cast<int>(A.time), R.channels = static_cast<int>(A.channels), R.batch = A.batch;
-    const int width = 64 * channels_a_lane(A);
+    const int width = 64 * cut.lanes;
     R.blocks = (R.channels + width - 1) / width;
     R.segments = cut.segments, R.steps = cut.steps;
     if (cut.segments > 1) {
@@ -476,11 +487,11 @@ RecurrenceArgs recurrence_args(const hx_recurrence_args& A, const Cut& cut) {
 
 // Calls f(element type, channels a lane).
 template <class F>
-hipError_t with_lanes(const hx_recurrence_args& A, F&& f) {
+hipError_t with_lanes(const hx_recurrence_args& A, const Cut& cut, F&& f) {
     return with_type(A.type, [&](auto t) {
         using T = decltype(t);
         if constexpr (!std::is_same_v<T, float>)
-            if (channels_a_lane(A) == 2) return f(t, std::integral_constant<int, 2>{});
+            if (cut.lanes == 2) return f(t, std::integral_constant<int, 2>{});
         return f(t, std::integral_constant<int, 1>{});
     });
 }
@@ -501,10 +512,11 @@ size_t recurrence_workspace(const hx_recurrence_args& A, bool grad) {
 }
 
 hipError_t recurrence_forward(const hx_recurrence_args& A) {
-    const RecurrenceArgs R = recurrence_args(A, cut_of(A, false));
+    const Cut cut = cut_of(A, false);
+    const RecurrenceArgs R = recurrence_args(A, cut);
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
-    return with_lanes(A, [&](auto t, auto c) -> hipError_t {
+    return with_lanes(A, cut, [&](auto t, auto c) -> hipError_t {
         using T = decltype(t);
         constexpr int kC = decltype(c)::value;
         if (R.segments > 1) {
@@ -519,10 +531,11 @@ hipError_t recurrence_forward(const hx_recurrence_args& A) {
 }
 
 hipError_t recurrence_backward(const hx_recurrence_args& A) {
-    const RecurrenceArgs R = recurrence_args(A, cut_of(A, true));
+    const Cut cut = cut_of(A, true);
+    const RecurrenceArgs R = recurrence_args(A, cut);
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
-    return with_lanes(A, [&](auto t, auto c) -> hipError_t {
+    return with_lanes(A, cut, [&](auto t, auto c) -> hipError_t {
         using T = decltype(t);
         constexpr int kC = decltype(c)::value;
         if (R.segments > 1) {
@@ -537,7 +550,7 @@ hipError_t recurrence_backward(const hx_recurrence_args& A) {
 }
 
 hipError_t recurrence_step(const hx_recurrence_args& A) {
-    const RecurrenceArgs R = recurrence_args(A, Cut{1, kTile});
+    const RecurrenceArgs R = recurrence_args(A, Cut{1, 1, 1});
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const int v = A.channels % 4 == 0 ? 4 : 1;
     const unsigned grid = static_cast<unsigned>((A.batch * (A.channels / v) + 255) / 256);
