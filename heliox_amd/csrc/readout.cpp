@@ -143,22 +143,23 @@ int adamw_tensors(const char* call, const hx_adamw_args* A) {
     ranges.reserve(2 * A->count);
     int64_t used = 0;
     for (int64_t i = 0; i < A->count; ++i) {
-        const hx_adamw_tensor& t = A->tensors[i];
-        const long long n = i;
-        if (!known_type(t.type) || !known_type(t.grad_type)) return refuse("%s: tensor %lld: type is not known", call, n);
-        if (t.elements < 0 || t.elements > (int64_t(1) << 34))
-            return refuse("%s: tensor %lld: elements has to be in 0..2^34", call, n);
-        if (!std::isfinite(t.weight_decay)) return refuse("%s: tensor %lld: weight_decay is not finite", call, n);
-        if (t.start % 256 || t.start < used)
-            return refuse("%s: tensor %lld: moments start at multiples of 256, each after those before", call, n);
-        used = t.start + (t.elements + 255) / 256 * 256;
-        if (t.start > A->moments || used > A->moments)
-            return refuse("%s: tensor %lld: %lld moments are too few", call, n, (long long)A->moments);
-        if (!t.elements) continue;
-        if (!t.param || !t.grad) return refuse("%s: tensor %lld: param or grad is missing", call, n);
-        const uintptr_t p = reinterpret_cast<uintptr_t>(t.param), g = reinterpret_cast<uintptr_t>(t.grad);
-        ranges.push_back({p, p + t.elements * (t.type == HX_F32 ? 4 : 2), true});
-        ranges.push_back({g, g + t.elements * (t.grad_type == HX_F32 ? 4 : 2), false});
+        const long long at = i;
+        const int64_t n = A->elements[i], start = A->starts[i], size = A->types[i] == HX_F32 ? 4 : 2,
+                      grad_size = A->grad_types[i] == HX_F32 ? 4 : 2;
+        if (!known_type(A->types[i]) || !known_type(A->grad_types[i]))
+            return refuse("%s: tensor %lld: type is not known", call, at);
+        if (n < 0 || n > (int64_t(1) << 34)) return refuse("%s: tensor %lld: elements has to be in 0..2^34", call, at);
+        if (!std::isfinite(A->weight_decays[i])) return refuse("%s: tensor %lld: weight_decay is not finite", call, at);
+        if (start % 256 || start < used)
+            return refuse("%s: tensor %lld: moments start at multiples of 256, each after those before", call, at);
+        if (start > A->moments || (n + 255) / 256 * 256 > A->moments - start)
+            return refuse("%s: tensor %lld: %lld moments are too few", call, at, (long long)A->moments);
+        used = start + (n + 255) / 256 * 256;
+        if (!n) continue;
+        if (!A->params[i] || !A->grads[i]) return refuse("%s: tensor %lld: param or grad is missing", call, at);
+        const uintptr_t p = reinterpret_cast<uintptr_t>(A->params[i]), g = reinterpret_cast<uintptr_t>(A->grads[i]);
+        ranges.push_back({p, p + n * size, true});
+        ranges.push_back({g, g + n * grad_size, false});
     }
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
     uintptr_t written = 0, any = 0;
@@ -179,7 +180,9 @@ int adamw_check(const char* call, const hx_adamw_args* A) {
     if (!(A->eps >= 0) || !std::isfinite(A->eps)) return refuse("%s: eps has to be a number, at least 0", call);
     if (!std::isfinite(A->lr)) return refuse("%s: lr is not finite", call);
     if (!std::isfinite(A->grad_scale)) return refuse("%s: grad_scale is not finite", call);
-    if (!A->step || (A->count && !A->tensors)) return refuse("%s: step or tensors is missing", call);
+    if (!A->step) return refuse("%s: step is missing", call);
+    if (A->count && (!A->types || !A->grad_types || !A->params || !A->grads || !A->elements || !A->starts || !A->weight_decays))
+        return refuse("%s: a list of the tensors is missing", call);
     if (A->moments < 0 || (A->moments && (!A->m || !A->v || (A->bits == 8 && (!A->m_scale || !A->v_scale)))))
         return refuse("%s: m, v or their scales are missing", call);
     for (const void* p : {static_cast<const void*>(A->m), static_cast<const void*>(A->v), static_cast<const void*>(A->step)})

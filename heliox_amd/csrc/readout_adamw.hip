@@ -250,12 +250,11 @@ hipError_t adamw_launch(const hx_adamw_args& A) {
                 L.count = 0;
             };
             for (int64_t i = 0; i < A.count; ++i) {
-                const hx_adamw_tensor& t = A.tensors[i];
-                if (t.type != type || t.grad_type != grad || !t.elements) continue;
-                const long long more = (t.elements + kChunk - 1) / kChunk;
+                const long long n = A.elements[i], more = (n + kChunk - 1) / kChunk;
+                if (A.types[i] != type || A.grad_types[i] != grad || !n) continue;
                 if (L.count == kTensors || groups + more > (1 << 23)) flush();
-                L.tensor[L.count++] = {t.param, t.grad, t.elements, t.start, static_cast<unsigned>(groups),
-                                       static_cast<float>(t.weight_decay)};
+                L.tensor[L.count++] = {A.params[i], A.grads[i], n, A.starts[i], static_cast<unsigned>(groups),
+                                       static_cast<float>(A.weight_decays[i])};
                 groups += more;
             }
             flush();

@@ -27,10 +27,10 @@ that have one refuse inputs that require a gradient while torch records.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 import operator
 import struct
+from array import array
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -43,8 +43,7 @@ _DISTILL = struct.Struct("=6q Q q Q q Q q 2Q d Q Q q Q")
 _NORM = struct.Struct("=4q Q q 2Q d Q q 2Q Q q Q q 2Q Q q Q")
 _RECURRENCE = struct.Struct("=4q 2Q 4q 2Q Q 2q Q Q 2q Q 2Q Q 2Q q Q q Q")
 _LOGPROB = struct.Struct("=5q Q q Q d 3Q 2Q 2Q Q q Q q Q")
-_ADAMW = struct.Struct("=2q Q 2Q 2Q q 5d 2Q Q Q")
-_ADAMW_TENSOR = "2q2Q2qd"
+_ADAMW = struct.Struct("=2q 7Q 2Q 2Q q 5d 2Q Q Q")
 _SAMPLE = struct.Struct("=3q Q q Q Q Q 2Q 3d q 2Q Q")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -409,16 +408,15 @@ def _norm_inputs(x, weight, bias):
     kind = _type(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x has to be (..., width) with at least one value a row, got shape {tuple(x.shape)}")
-    width, weight_kind = x.shape[-1], 0
-    for w, what in ((weight, "weight"), (bias, "bias")):
-        if w is not None:
-            if not isinstance(w, torch.Tensor):
-                raise TypeError(f"{what} has to be a tensor, got {type(w).__name__}")
-            weight_kind = _type(w, what)
-    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
-        raise TypeError(f"weight is {weight.dtype}, bias is {bias.dtype}")
-    weight, bias = (None if w is None else _array(w, what, w.dtype, (width,), device)
-                    for w, what in ((weight, "weight"), (bias, "bias")))
+    size, weight_kind = x.shape[-1:], 0
+    if weight is not None:
+        weight = _array(weight, "weight", getattr(weight, "dtype", None), size, device)
+        weight_kind = _type(weight, "weight")
+    if bias is not None:
+        bias = _array(bias, "bias", getattr(bias, "dtype", None), size, device)
+        if weight is not None and bias.dtype is not weight.dtype:
+            raise TypeError(f"weight is {weight.dtype}, bias is {bias.dtype}")
+        weight_kind = _type(bias, "bias")
     return device, kind, weight_kind, _flat_rows(x), weight, bias
 
 
@@ -439,7 +437,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     device, kind, weight_kind, rows, weight, bias = _norm_inputs(x, weight, bias)
     _no_graph("layer_norm", "take it from layer_norm_grad", x, weight, bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
     n, width = rows.shape
     _call("hx_layer_norm", device, _NORM.pack(
         kind, weight_kind, n, width, rows.data_ptr(), rows.stride(0), _ptr(weight), _ptr(bias), _real(eps, "eps"),
@@ -466,7 +464,7 @@ def layer_norm_grad(x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch
     dweight = dbias = space = None
     need = 0
     if parameters:
-        dweight, dbias = (torch.empty(width, dtype=torch.float32, device=x.device) for _ in range(2))
+        dweight, dbias = torch.empty((2, width), dtype=torch.float32, device=x.device).unbind(0)
         need = _norm_space(kind, n, width)
         space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call("hx_layer_norm_grad", device, _NORM.pack(
@@ -671,43 +669,59 @@ class AdamWState:
     steps taken.  All of them may be saved, and copied into another state of the same parameters."""
 
     def __init__(self, sizes: Sequence[int], bits: int, device: int):
-        self.bits, self.sizes, self.device, self.starts = bits, tuple(sizes), device, []
+        self.bits, self.device = bits, device
+        self.sizes, self.starts = array("q", sizes), array("q")
         whole = 0
         for n in self.sizes:
             self.starts.append(whole)
             whole += -(-n // 256) * 256
         on = {"device": f"cuda:{device}"}
-        kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
-        self.m, self.v = (torch.zeros(whole, dtype=torch.uint8 if bits == 8 else kind, **on).view(kind) for _ in range(2))
+        kind, held = (torch.float32, torch.float32) if bits == 32 else (torch.float8_e4m3fn, torch.uint8)
+        self.m, self.v = (torch.zeros(whole, dtype=held, **on).view(kind) for _ in range(2))
         self.m_scale, self.v_scale = (torch.zeros(whole // 256, **on) if bits == 8 else None for _ in range(2))
         self._count = torch.zeros(2, dtype=torch.int64, **on)
         self.step = self._count[:1]
 
 
-def _parameters(params) -> Tuple[list, int]:
-    params = list(params)
-    device = None
-    for i, p in enumerate(params):
-        here = _on_gpu(p, f"params[{i}]")
-        if device is None:
-            device = here
-        elif here != device:
-            raise ValueError(f"params[{i}] is on cuda:{here}, params[0] on cuda:{device}")
-        if not p.is_contiguous():
-            raise ValueError(f"params[{i}] has to be contiguous")
-        _type(p, f"params[{i}]")
-    if device is None:
+# What is asked of hundreds of tensors in a step is asked by map, a tenth of a loop's time each.
+_device_of, _address_of, _whole_of = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_shape_of, _dtype_of, _size_of = operator.attrgetter("shape"), operator.attrgetter("dtype"), torch.Tensor.numel
+
+
+def _tensors(xs: list, what: str, device: Optional[int]) -> array:
+    """The types of tensors that are all on one GPU (`device`, or the first one's)."""
+    try:
+        places = set(map(_device_of, xs))
+        kinds = list(map(_TYPES.get, map(_dtype_of, xs)))
+    except (TypeError, AttributeError):
+        places, kinds = (), (None,)
+    if len(places) != 1 or min(places) < 0 or None in kinds or (device is not None and device not in places):
+        for i, x in enumerate(xs):
+            here = _on_gpu(x, f"{what}[{i}]")
+            _type(x, f"{what}[{i}]")
+            device = here if device is None else device
+            if here != device:
+                raise ValueError(f"{what}[{i}] is on cuda:{here}, others on cuda:{device}")
+    return array("q", kinds)
+
+
+def _parameters(params: list) -> Tuple[int, array]:
+    if not params:
         raise ValueError("params has no tensors")
-    return params, device
+    kinds = _tensors(params, "params", None)
+    if not all(map(_whole_of, params)):
+        raise ValueError("params have to be contiguous")
+    return params[0].get_device(), kinds
 
 
 def adamw_state(params: Sequence[torch.Tensor], *, bits: int = 32) -> AdamWState:
     """A state of zeros for these parameters (contiguous tensors on one GPU, fp32, fp16 or bf16): 8
     bytes of moments for each of their elements with bits=32, 2 and a 32nd with bits=8."""
-    params, device = _parameters(params)
+    params = list(params)
+    device, _ = _parameters(params)
     if bits not in (8, 32):
         raise ValueError(f"bits has to be 8 or 32, got {bits}")
-    return AdamWState([p.numel() for p in params], bits, device)
+    return AdamWState(list(map(_size_of, params)), bits, device)
 
 
 def _one_number(x, what: str, device: int):
@@ -717,6 +731,17 @@ def _one_number(x, what: str, device: int):
             raise ValueError(f"{what} has to be one number, got shape {tuple(x.shape)}")
         return _array(x, what, torch.float32, x.shape, device).data_ptr(), 0.0
     return 0, _real(x, what)
+
+
+def _decays(weight_decay, count: int) -> array:
+    if isinstance(weight_decay, (list, tuple)):
+        if len(weight_decay) != count:
+            raise ValueError(f"{len(weight_decay)} weight_decay for {count} params")
+        try:
+            return array("d", weight_decay)
+        except TypeError:
+            return array("d", [_real(w, "weight_decay") for w in weight_decay])
+    return array("d", [_real(weight_decay, "weight_decay")]) * count
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], state: AdamWState, *,
@@ -738,41 +763,33 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     are refused."""
     if not isinstance(state, AdamWState):
         raise TypeError(f"state has to be what adamw_state returned, got {type(state).__name__}")
-    params, device = _parameters(params)
-    grads = list(grads)
+    params, grads = list(params), list(grads)
+    device, kinds = _parameters(params)
     if device != state.device:
         raise ValueError(f"params are on cuda:{device}, the state on cuda:{state.device}")
-    if len(grads) != len(params) or tuple(p.numel() for p in params) != state.sizes:
-        raise ValueError(f"{len(params)} params and {len(grads)} grads do not fit a state of sizes {state.sizes}")
-    if isinstance(weight_decay, (list, tuple)):
-        if len(weight_decay) != len(params):
-            raise ValueError(f"{len(weight_decay)} weight_decay for {len(params)} params")
-        decays = [_real(w, "weight_decay") for w in weight_decay]
-    else:
-        decays = [_real(weight_decay, "weight_decay")] * len(params)
+    sizes, starts = state.sizes, state.starts
+    if len(grads) != len(params) or array("q", map(_size_of, params)) != sizes:
+        raise ValueError(f"{len(params)} params and {len(grads)} grads do not fit a state of sizes {list(sizes)}")
+    decays = _decays(weight_decay, len(params))
     if not isinstance(betas, (list, tuple)) or len(betas) != 2:
         raise TypeError("betas has to be two numbers")
     beta1, beta2 = (_real(b, "betas") for b in betas)
     lr_ptr, lr = _one_number(lr, "lr", device)
     scale_ptr, scale = _one_number(grad_scale, "grad_scale", device)
-    fields, kept, moved = [], [], []
-    for i, (p, g, start, decay) in enumerate(zip(params, grads, state.starts, decays)):
-        if g is None:
-            continue
-        if not isinstance(g, torch.Tensor) or g.get_device() != device:
-            if _on_gpu(g, f"grads[{i}]") != device:
-                raise ValueError(f"grads[{i}] is on {g.device}, params on cuda:{device}")
-        if g.shape != p.shape:
-            raise ValueError(f"grads[{i}] has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            kept.append(g)
-        moved.append(p)
-        fields += (_TYPES[p.dtype], _type(g, f"grads[{i}]"), p.data_ptr(), g.data_ptr(), state.sizes[i], start, decay)
-    tensors = bytearray(struct.pack("=" + _ADAMW_TENSOR * len(moved), *fields))
-    table = ctypes.addressof(ctypes.c_char.from_buffer(tensors)) if tensors else 0
+    if any(g is None for g in grads):
+        there = [i for i, g in enumerate(grads) if g is not None]
+        params, grads = [params[i] for i in there], [grads[i] for i in there]
+        kinds, sizes, starts = (array("q", [a[i] for i in there]) for a in (kinds, sizes, starts))
+        decays = array("d", [decays[i] for i in there])
+    grad_kinds = _tensors(grads, "grads", device)
+    if list(map(_shape_of, grads)) != list(map(_shape_of, params)):
+        raise ValueError("grads have to be of their parameters' shapes, got "
+                         + ", ".join(f"{tuple(g.shape)} for {tuple(p.shape)}" for p, g in zip(params, grads) if p.shape != g.shape))
+    if not all(map(_whole_of, grads)):
+        grads = [g.contiguous() for g in grads]
+    lists = kinds, grad_kinds, array("Q", map(_address_of, params)), array("Q", map(_address_of, grads)), sizes, starts, decays
     _call("hx_adamw_step", device, _ADAMW.pack(
-        state.bits, len(moved), table, state.m.data_ptr(), state.v.data_ptr(), _ptr(state.m_scale), _ptr(state.v_scale),
-        state.m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr, lr_ptr, state._count.data_ptr(),
-        _stream(device)))
-    torch.autograd.graph.increment_version(moved)
+        state.bits, len(params), *[a.buffer_info()[0] for a in lists], state.m.data_ptr(), state.v.data_ptr(),
+        _ptr(state.m_scale), _ptr(state.v_scale), state.m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
+        lr_ptr, state._count.data_ptr(), _stream(device)))
+    torch.autograd.graph.increment_version(params)

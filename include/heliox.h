@@ -723,16 +723,14 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * elements that belong to none (kept zero).  The parameters of a call do not overlap each other or
  * the gradients (refused).  `step` (two int64: the count, and room that the call uses; at a multiple
  * of 16 bytes, as m and v) is device memory, so that a captured step counts on at every replay. */
-typedef struct hx_adamw_tensor {
-    int64_t type, grad_type;
-    void* param;                                          /* contiguous, elements of them */
-    const void* grad;
-    int64_t elements, start;
-    double weight_decay;
-} hx_adamw_tensor;
 typedef struct hx_adamw_args {
     int64_t bits, count;
-    const hx_adamw_tensor* tensors;                       /* (count), host memory */
+    /* (count) each, host memory: */
+    const int64_t *types, *grad_types;
+    void* const* params;                                  /* contiguous */
+    const void* const* grads;
+    const int64_t *elements, *starts;
+    const double* weight_decays;
     void *m, *v;
     float *m_scale, *v_scale;
     int64_t moments;                                      /* elements of m and of v */

@@ -266,7 +266,7 @@ def test_refusals():
             (lambda: step(p[::-1], g[::-1], state, lr=0.1), ValueError, "do not fit"),
             (lambda: step(p, [g[0], g[1].cpu()], state, lr=0.1), ValueError, "GPU"),
             (lambda: step(p, [g[0], g[1].double()], state, lr=0.1), TypeError, "not float32"),
-            (lambda: step(p, [g[0], g[1].view(4, 10)], state, lr=0.1), ValueError, "grads.1. has shape"),
+            (lambda: step(p, [g[0], g[1].view(4, 10)], state, lr=0.1), ValueError, "parameters. shapes"),
             (lambda: step(p, g, state, lr=float("nan")), HelioxError, "lr"),
             (lambda: step(p, g, state, lr="0.1"), TypeError, "lr"),
             (lambda: step(p, g, state, lr=torch.ones(2).cuda()), ValueError, "lr has to be one"),
