@@ -682,7 +682,8 @@ int hx_gated_recurrence_step(const hx_recurrence_args* args);
  * largest logits, largest first (ties: the lowest index first; NaN ranks as -inf), as indexes and
  * log q.  Where fewer than top places are above -inf, -inf fills the rest, by index.  stats (rows,
  * 2) receives the largest logit m and log sum exp((logits - m) / temperature).  A row of nothing
- * but -inf has logprob -inf, entropy 0 and stats -inf, -inf; one with a NaN or +inf has NaN.
+ * but -inf has logprob -inf, entropy 0 and stats -inf, -inf; one with a NaN or +inf has NaN.  The
+ * order of a row's sums follows from the sizes and from its address within 16 bytes alone.
  * The gradient, from the same stats and entropy: grad_j =
  *   [grad_logprob (1[j = token] - q_j) - grad_entropy q_j (log q_j + entropy)] / temperature
  * (the first term 0 for a token outside the vocabulary; all 0 for a row of nothing but -inf); it may
