@@ -512,7 +512,8 @@ hipError_t logprob_launch(const hx_logprob_args& A) {
         // than 128 top places would pass more logits to each of eight waves than its list holds (top
         // 256: 232 us with 1024 threads, 997 with 512).
         auto pick = [&](auto with_top) {
-            if (L.each <= 8192) go(std::integral_constant<int, 256>{}, with_top);
+            if (L.each <= 512) go(std::integral_constant<int, 64>{}, with_top);
+            else if (L.each <= 8192) go(std::integral_constant<int, 256>{}, with_top);
             else if (A.top <= 128) go(std::integral_constant<int, 512>{}, with_top);
             else if constexpr (decltype(with_top)::value) go(std::integral_constant<int, 1024>{}, with_top);
         };
@@ -533,10 +534,14 @@ hipError_t logprob_gradient(const hx_logprob_args& A) {
     G.stats = A.stats, G.entropy = A.entropy, G.pull = A.grad_logprob, G.turn = A.grad_entropy;
     return with_type(A.type, [&](auto t) {
         using T = decltype(t);
-        constexpr int kThreads = 256, kTurn = kThreads * kAhead * static_cast<int>(16 / sizeof(T));
-        G.blocks = (G.vocab + kTurn - 1) / kTurn;
-        const unsigned grid = static_cast<unsigned>(std::min<long long>(A.rows * G.blocks, 1 << 23));
-        k_logprob_grad<T, kThreads><<<grid, kThreads, 0, static_cast<hipStream_t>(A.stream)>>>(G);
+        auto go = [&](auto threads) {
+            constexpr int kThreads = decltype(threads)::value, kTurn = kThreads * kAhead * static_cast<int>(16 / sizeof(T));
+            G.blocks = (G.vocab + kTurn - 1) / kTurn;
+            const unsigned grid = static_cast<unsigned>(std::min<long long>(A.rows * G.blocks, 1 << 23));
+            k_logprob_grad<T, kThreads><<<grid, kThreads, 0, static_cast<hipStream_t>(A.stream)>>>(G);
+        };
+        if (G.vocab <= 1024) go(std::integral_constant<int, 64>{});
+        else go(std::integral_constant<int, 256>{});
         return hipGetLastError();
     });
 }

@@ -4,8 +4,8 @@
 // 16 bytes each.  The variance is the mean square of differences from the mean (two sums over the
 // held row, not the difference of two large numbers).  Workgroups walk over the rows, so that
 // weight and bias stay in registers too, and the gradients of both are added there: each
-// workgroup writes its sums once, a second launch adds those up in a fixed order.  Both are
-// bound by the rows' bytes.
+// workgroup writes its sums once, a second launch adds those up in a fixed order.  (Few rows are
+// read a second time instead, by columns.)  Both are bound by the rows' bytes.
 #include "readout.h"
 
 #include <algorithm>
@@ -30,6 +30,8 @@ struct NormArgs {
 template <class T, int kE> struct Piece { typedef typename PieceOf<T>::Vec Vec; };
 template <> struct Piece<float, 8> { typedef float Vec __attribute__((ext_vector_type(8), aligned(4))); };
 template <class T> struct Piece<T, 1> { typedef T Vec; };
+template <> struct Piece<__half, 2> { typedef _Float16 Vec __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Piece<__hip_bfloat16, 2> { typedef __bf16 Vec __attribute__((ext_vector_type(2), aligned(2))); };
 template <> struct Piece<__half, 4> { typedef _Float16 Vec __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct Piece<__hip_bfloat16, 4> { typedef __bf16 Vec __attribute__((ext_vector_type(4), aligned(2))); };
 
@@ -389,22 +391,31 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
     }
 }
 
-// Sums of dy n and of dy over a run of rows, a column a thread.
-template <class T>
-__global__ void __launch_bounds__(256) k_norm_columns(NormArgs A, long long rows_each) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= A.width) return;
+// Sums of dy n and of dy over a run of rows, kE columns a thread.
+template <class T, int kE>
+__global__ void __launch_bounds__(256) k_norm_columns(NormArgs A, long long rows_each, float* dw, float* db) {
+    // threads past the last column do the last columns over again
+    const int j = min((static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x)) * kE, A.width - kE);
     const long long first = blockIdx.y * rows_each, end = min(first + rows_each, A.rows);
-    float dw = 0.f, db = 0.f;
+    const T* x = static_cast<const T*>(A.x) + j;
+    const T* dy = static_cast<const T*>(A.dy) + j;
+    float sum[2][kE] = {};
+#pragma unroll 8
     for (long long r = first; r < end; ++r) {
-        const float x = to_f32(static_cast<const T*>(A.x)[r * A.x_stride + j]);
-        const float dy = to_f32(static_cast<const T*>(A.dy)[r * A.dy_stride + j]);
-        dw = fmaf(dy, (x - A.mean[r]) * A.rstd[r], dw);
-        db += dy;
+        float v[kE], d[kE];
+        load<T, kE>(x + r * A.x_stride, v);
+        load<T, kE>(dy + r * A.dy_stride, d);
+        const float mean = A.mean[r], rstd = A.rstd[r];
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+            sum[0][i] = fmaf(d[i], (v[i] - mean) * rstd, sum[0][i]);
+            sum[1][i] += d[i];
+        }
     }
-    float* part = A.part + static_cast<long long>(blockIdx.y) * 2 * A.width;
-    part[j] = dw;
-    part[A.width + j] = db;
+    dw += static_cast<long long>(blockIdx.y) * 2 * A.width + j;
+    db += static_cast<long long>(blockIdx.y) * 2 * A.width + j;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) dw[i] = sum[0][i], db[i] = sum[1][i];
 }
 
 // The workgroups' sums, added up: 32 columns a workgroup, 32 runs of rows each.
@@ -464,13 +475,26 @@ NormArgs norm_args(const hx_norm_args& A) {
     return N;
 }
 
-// Workgroups that walk over rows in the gradient, each with sums of its own.
-int grad_parts(const hx_norm_args& A) {
+// How the gradients of weight and bias are summed: `held` by the workgroups that make grad_x, one
+// sum of each for each of `parts`; or by a launch over the columns that reads the rows again, in
+// `parts` runs of rows.
+//
+// A workgroup's sums are 8 bytes a column, written and read again: more than the rows, where there
+// are few.  462 x 11764 in fp16: 75 us held, 31 by columns; 5003 x 1001: 22 held.
+struct Sums { bool held; int parts; };
+
+Sums sums_of(const hx_norm_args& A) {
     return with_type(A.type, [&](auto t) {
-        return with_shape<decltype(t), true>(static_cast<int>(A.width), [&](auto shape) -> int {
+        using T = decltype(t);
+        return with_shape<T, true>(static_cast<int>(A.width), [&](auto shape) -> Sums {
             using S = decltype(shape);
-            if (!S::kE) return static_cast<int>(std::min<int64_t>(A.rows, 64));
-            return static_cast<int>(std::min<int64_t>((A.rows + S::kRows - 1) / S::kRows, 512));
+            if constexpr (S::kE != 0) {
+                const int64_t parts = std::min<int64_t>((A.rows + S::kRows - 1) / S::kRows, 512);
+                if (A.rows * static_cast<int64_t>(sizeof(T)) >= 8 * parts) return {true, static_cast<int>(parts)};
+            }
+            const int64_t blocks = (A.width + 511) / 512;
+            const int64_t most = std::max<int64_t>(1, 512 / blocks);
+            return {false, static_cast<int>(std::max<int64_t>(1, std::min({(A.rows + 15) / 16, most, int64_t(64)})))};
         });
     });
 }
@@ -479,7 +503,9 @@ int grad_parts(const hx_norm_args& A) {
 
 size_t norm_workspace(const hx_norm_args& A) {
     if (!A.grad_weight) return 0;
-    return sizeof(float) * 2 * grad_parts(A) * static_cast<size_t>(A.width);
+    const Sums sums = sums_of(A);
+    // a single run of rows writes to the gradients themselves
+    return sums.held || sums.parts > 1 ? sizeof(float) * 2 * sums.parts * static_cast<size_t>(A.width) : 0;
 }
 
 hipError_t norm_forward(const hx_norm_args& A) {
@@ -507,20 +533,22 @@ hipError_t norm_backward(const hx_norm_args& A) {
     NormArgs N = norm_args(A);
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     N.dy = A.grad_y, N.dy_stride = A.grad_y_stride, N.y = A.grad_x, N.y_stride = A.grad_x_stride;
-    N.part = A.grad_weight ? static_cast<float*>(A.workspace) : nullptr;
-    const int parts = grad_parts(A);             // none without rows: the sums are 0
-    const hipError_t e = !A.rows ? hipSuccess : with_type(A.type, [&](auto t) {
+    const Sums sums = sums_of(A);
+    const bool joined = A.grad_weight && (sums.held || sums.parts > 1);
+    float* const part = static_cast<float*>(A.workspace);
+    if (A.grad_weight && sums.held) N.part = part;
+    hipError_t e = !A.rows ? hipSuccess : with_type(A.type, [&](auto t) {
         using T = decltype(t);
         return with_shape<T, true>(N.width, [&](auto shape) {
             using S = decltype(shape);
             if constexpr (!S::kE) {
                 k_norm_grad_wide<T><<<static_cast<unsigned>(std::min<long long>(N.rows, 1 << 16)), kWide, 0, st>>>(N);
-                const long long each = (N.rows + parts - 1) / parts;
-                if (N.part) k_norm_columns<T><<<dim3((N.width + 255) / 256, parts), 256, 0, st>>>(N, each);
             } else {
-                auto go = [&](auto ragged, auto sums) {
-                    k_norm_grad<T, S::kE, S::kGroup, S::kV, decltype(ragged)::value, decltype(sums)::value>
-                        <<<parts, S::kThreads, 0, st>>>(N);
+                const long long turns = (N.rows + S::kRows - 1) / S::kRows;
+                const unsigned grid = static_cast<unsigned>(N.part ? sums.parts : std::min<long long>(turns, 256 * 1024 / S::kThreads));
+                auto go = [&](auto ragged, auto with_sums) {
+                    k_norm_grad<T, S::kE, S::kGroup, S::kV, decltype(ragged)::value, decltype(with_sums)::value>
+                        <<<grid, S::kThreads, 0, st>>>(N);
                 };
                 const bool ragged = N.width % S::kE;
                 if (N.part) ragged ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
@@ -530,8 +558,31 @@ hipError_t norm_backward(const hx_norm_args& A) {
         });
     });
     if (e != hipSuccess || !A.grad_weight) return e;
-    k_norm_join<<<static_cast<unsigned>((2 * A.width + 31) / 32), 1024, 0, st>>>(N.part, parts, N.width, A.grad_weight,
-                                                                               A.grad_bias);
+    if (!sums.held && A.rows) {
+        float* const dw = joined ? part : A.grad_weight;
+        float* const db = joined ? part + A.width : A.grad_bias;
+        e = with_type(A.type, [&](auto t) {
+            using T = decltype(t);
+            const long long each = (A.rows + sums.parts - 1) / sums.parts;
+            auto go = [&](auto columns) {
+                constexpr int kE = decltype(columns)::value;
+                const dim3 grid((N.width + 256 * kE - 1) / (256 * kE), sums.parts);
+                k_norm_columns<T, kE><<<grid, 256, 0, st>>>(N, each, dw, db);
+            };
+            if constexpr (sizeof(T) == 2)
+                if (N.width > 1) {
+                    go(std::integral_constant<int, 2>{});
+                    return hipGetLastError();
+                }
+            go(std::integral_constant<int, 1>{});
+            return hipGetLastError();
+        });
+        if (e != hipSuccess) return e;
+    }
+    // without rows the sums are 0
+    if (joined || !A.rows)
+        k_norm_join<<<static_cast<unsigned>((2 * A.width + 31) / 32), 1024, 0, st>>>(part, A.rows ? sums.parts : 0, N.width,
+                                                                                   A.grad_weight, A.grad_bias);
     return hipGetLastError();
 }
 
