@@ -7,11 +7,11 @@
 // counts a thousand times, while z keeps all of its bits.
 //
 // Lanes lie along channels, kC each, so that a step's row is read and written as it lies in
-// memory; a wave takes kU steps in registers, a workgroup's kW waves take kW kU steps in a row
-// and join in LDS.  Where sequences and channels alone fill the chip a workgroup walks along its
+// memory; a group of kL lanes (a wave; fewer, where there are few channels) takes kU steps in
+// registers, a workgroup's groups take as many more in a row and join in LDS.  Where sequences and channels alone fill the chip a workgroup walks along its
 // whole sequence, one pass over the data.  Where they do not, sequences are cut into segments:
 // one launch makes each segment's P and Y, one joins them, one walks the segments.  The gradient
-// goes that way always, a segment being kW kU steps: what the future hands back to a run,
+// goes that way always, a segment being a workgroup's steps: what the future hands back to a run,
 // G = R + P G', joins from the right as h does from the left, and both meet in the run's registers.
 #include "readout.h"
 
@@ -21,9 +21,9 @@
 namespace hx {
 namespace {
 
-constexpr int kW = 8, kThreads = 64 * kW;
-template <int kC> constexpr int kU = 16 / kC;              // steps that a wave holds
-template <int kC> constexpr int kTile = kU<kC> * kW;
+constexpr int kThreads = 512;
+template <int kC> constexpr int kU = 16 / kC;                              // steps that a lane holds
+template <int kC, int kL> constexpr int kTile = kU<kC> * (kThreads / kL);  // and a workgroup
 
 struct RecurrenceArgs {
     const void *x, *gate, *grad_o;
@@ -34,7 +34,7 @@ struct RecurrenceArgs {
     float *end, *grad_initial;
     float *p, *y, *r;                // (batch, segments, channels): P, Y and R of each segment
     float *enter, *leave;            // the same: what enters it from the left and, going back, from the right
-    int time, channels, blocks;      // blocks: of 64 kC channels
+    int time, channels, blocks;      // blocks: of kL kC channels
     int segments, steps;             // steps: of a segment
     long long batch;
 };
@@ -75,12 +75,12 @@ __device__ __forceinline__ float moved(float h, float z, float x) { return fmaf(
 struct Where {
     long long batch;
     int segment, channel, length;
-    template <int kC>
+    template <int kC, int kL>
     __device__ __forceinline__ static Where of(const RecurrenceArgs& A, long long id) {
         Where w;
         const long long row = id / A.blocks;
         // lanes past the last channel do the last channels over again, and write the same values
-        w.channel = min(static_cast<int>(id - row * A.blocks) * 64 * kC + static_cast<int>(threadIdx.x) % 64 * kC,
+        w.channel = min((static_cast<int>(id - row * A.blocks) * kL + static_cast<int>(threadIdx.x) % kL) * kC,
                         A.channels - kC);
         w.batch = row / A.segments;
         w.segment = static_cast<int>(row - w.batch * A.segments);
@@ -92,7 +92,12 @@ struct Where {
     }
 };
 
-__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+// Which of a workgroup's kThreads / kL groups of lanes this is.
+template <int kL>
+__device__ __forceinline__ int group_of() {
+    const int group = threadIdx.x / kL;
+    return kL == 64 ? __builtin_amdgcn_readfirstlane(group) : group;
+}
 
 // kU steps from t on of one array; steps past the length are not read.
 template <class T, int kC, int kN>
@@ -111,17 +116,17 @@ __device__ __forceinline__ void fetch(typename Packed<T, kC>::Vec (&to)[kN], con
 }
 
 // The whole walk.
-template <class T, int kC>
-__global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
-    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
+template <class T, int kC, int kL>
+__global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC, kL>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
     using F = typename Floats<kC>::Vec;
-    __shared__ float ends[2][kW][2 * kC][64];
-    const int wave = wave_of(), lane = threadIdx.x % 64;
+    __shared__ float ends[2][kW][2 * kC][kL];
+    const int group = group_of<kL>(), lane = threadIdx.x % kL;
     int turn = 0;
     // (the segments' own launch went over the data from its start: its end is in the cache)
     for (long long id = A.batch * A.segments * A.blocks - 1 - blockIdx.x; id >= 0; id -= gridDim.x) {
-        const Where w = Where::of<kC>(A, id);
+        const Where w = Where::of<kC, kL>(A, id);
         const int first = w.segment * A.steps, last = min(first + A.steps, A.time);
         float h[kC];
 #pragma unroll
@@ -131,10 +136,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
             else if (A.initial) h[c] = A.initial[w.batch * A.channels + w.channel + c];
         }
         Vec x[kU], g[kU];
-        fetch<T, kC>(x, A.x, A.x_stride, w, first + wave * kU);
-        fetch<T, kC>(g, A.gate, A.gate_stride, w, first + wave * kU);
+        fetch<T, kC>(x, A.x, A.x_stride, w, first + group * kU);
+        fetch<T, kC>(g, A.gate, A.gate_stride, w, first + group * kU);
         for (int tile = first; tile < last; tile += kTile, turn ^= 1) {
-            const int t = tile + wave * kU;
+            const int t = tile + group * kU;
             float p[kU][kC], y[kU][kC];
             auto run = [&](auto whole) {
                 float pp[kC], yy[kC];
@@ -160,18 +165,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
             }
 #pragma unroll
             for (int c = 0; c < kC; ++c) {
-                ends[turn][wave][c][lane] = p[kU - 1][c];
-                ends[turn][wave][kC + c][lane] = y[kU - 1][c];
+                ends[turn][group][c][lane] = p[kU - 1][c];
+                ends[turn][group][kC + c][lane] = y[kU - 1][c];
             }
             __syncthreads();
             float mine[kC];
 #pragma unroll
             for (int c = 0; c < kC; ++c) mine[c] = h[c];
-#pragma unroll
+#pragma unroll 8
             for (int v = 0; v < kW; ++v)
 #pragma unroll
                 for (int c = 0; c < kC; ++c) {
-                    if (v == wave) mine[c] = h[c];
+                    if (v == group) mine[c] = h[c];
                     h[c] = fmaf(ends[turn][v][c][lane], h[c], ends[turn][v][kC + c][lane]);
                 }
             T* o = static_cast<T*>(A.o) + w.batch * A.o_stride[0] + t * A.o_stride[1];
@@ -190,23 +195,23 @@ __global__ void __launch_bounds__(kThreads, 4) k_walk(RecurrenceArgs A) {
             if (t + kU <= w.length) write(std::true_type{});
             else write(std::false_type{});
         }
-        if (A.end && w.segment == A.segments - 1 && wave == 0)
+        if (A.end && w.segment == A.segments - 1 && group == 0)
 #pragma unroll
             for (int c = 0; c < kC; ++c) A.end[w.batch * A.channels + w.channel + c] = h[c];
     }
 }
 
 // P, Y (and, for the gradient, R) of each segment: every wave takes a share of its steps.
-template <class T, int kC, bool kGrad>
-__global__ void __launch_bounds__(kThreads, 4) k_segments(RecurrenceArgs A) {
-    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
+template <class T, int kC, int kL, bool kGrad>
+__global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_segments(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
     constexpr int kN = kGrad ? 3 : 2;
-    __shared__ float ends[kW][kN * kC][64];
-    const int wave = wave_of(), lane = threadIdx.x % 64;
+    __shared__ float ends[kW][kN * kC][kL];
+    const int group = group_of<kL>(), lane = threadIdx.x % kL;
     for (long long id = blockIdx.x; id < A.batch * A.segments * A.blocks; id += gridDim.x) {
-        const Where w = Where::of<kC>(A, id);
-        const int each = A.steps / kW, first = w.segment * A.steps + wave * each;
+        const Where w = Where::of<kC, kL>(A, id);
+        const int each = A.steps / kW, first = w.segment * A.steps + group * each;
         const int last = min(first + each, w.length);
         float p[kC], y[kC], r[kC];
 #pragma unroll
@@ -234,16 +239,16 @@ __global__ void __launch_bounds__(kThreads, 4) k_segments(RecurrenceArgs A) {
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            ends[wave][c][lane] = p[c];
-            ends[wave][kC + c][lane] = y[c];
-            if constexpr (kGrad) ends[wave][2 * kC + c][lane] = r[c];
+            ends[group][c][lane] = p[c];
+            ends[group][kC + c][lane] = y[c];
+            if constexpr (kGrad) ends[group][2 * kC + c][lane] = r[c];
         }
         __syncthreads();
-        if (wave == 0)
+        if (group == 0)
 #pragma unroll
             for (int c = 0; c < kC; ++c) {
                 float pp = p[c], yy = y[c], rr = r[c];
-#pragma unroll
+#pragma unroll 8
                 for (int v = 1; v < kW; ++v) {
                     const float q = ends[v][c][lane];
                     yy = fmaf(q, yy, ends[v][kC + c][lane]);
@@ -301,15 +306,15 @@ __global__ void __launch_bounds__(1024) k_join(RecurrenceArgs A) {
 }
 
 // The gradients of kTile steps, from what enters them on both sides.
-template <class T, int kC>
-__global__ void __launch_bounds__(kThreads, 4) k_grad(RecurrenceArgs A) {
-    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC>;
+template <class T, int kC, int kL>
+__global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceArgs A) {
+    constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC, kL>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
-    __shared__ float ends[kW][3 * kC][64];
-    const int wave = wave_of(), lane = threadIdx.x % 64;
+    __shared__ float ends[kW][3 * kC][kL];
+    const int group = group_of<kL>(), lane = threadIdx.x % kL;
     for (long long id = A.batch * A.segments * A.blocks - 1 - blockIdx.x; id >= 0; id -= gridDim.x) {     // as above
-        const Where w = Where::of<kC>(A, id);
-        const int t = w.segment * kTile + wave * kU;
+        const Where w = Where::of<kC, kL>(A, id);
+        const int t = w.segment * kTile + group * kU;
         Vec x[kU], g[kU], d[kU];
         fetch<T, kC>(x, A.x, A.x_stride, w, t);
         fetch<T, kC>(g, A.gate, A.gate_stride, w, t);
@@ -346,25 +351,25 @@ __global__ void __launch_bounds__(kThreads, 4) k_grad(RecurrenceArgs A) {
                 }
             }
         };
-        const bool whole_wave = t + kU <= w.length;
-        if (whole_wave) run(std::true_type{});
+        const bool whole_group = t + kU <= w.length;
+        if (whole_group) run(std::true_type{});
         else run(std::false_type{});
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            ends[wave][c][lane] = p[c];
-            ends[wave][kC + c][lane] = y[c];
-            ends[wave][2 * kC + c][lane] = r[c];
+            ends[group][c][lane] = p[c];
+            ends[group][kC + c][lane] = y[c];
+            ends[group][2 * kC + c][lane] = r[c];
         }
         __syncthreads();
-#pragma unroll
+#pragma unroll 8
         for (int v = 0; v < kW - 1; ++v)
-            if (v < wave)
+            if (v < group)
 #pragma unroll
                 for (int c = 0; c < kC; ++c) h[c] = fmaf(ends[v][c][lane], h[c], ends[v][kC + c][lane]);
-#pragma unroll
+#pragma unroll 8
         for (int v = kW - 1; v > 0; --v)
-            if (v > wave)
+            if (v > group)
 #pragma unroll
                 for (int c = 0; c < kC; ++c) back[c] = fmaf(ends[v][c][lane], back[c], ends[v][2 * kC + c][lane]);
         auto out = [&](auto whole) {
@@ -398,9 +403,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_grad(RecurrenceArgs A) {
                 }
             }
         };
-        if (whole_wave) out(std::true_type{});
+        if (whole_group) out(std::true_type{});
         else out(std::false_type{});
-        if (A.segments == 1 && A.grad_initial && wave == 0)
+        if (A.segments == 1 && A.grad_initial && group == 0)
 #pragma unroll
             for (int c = 0; c < kC; ++c) A.grad_initial[w.batch * A.channels + w.channel + c] = back[c];
     }
@@ -438,24 +443,39 @@ __global__ void __launch_bounds__(256) k_step(RecurrenceArgs A, float* states, c
     *reinterpret_cast<Few*>(o) = out;
 }
 
-struct Cut { int lanes, segments, steps; };   // lanes: channels a lane
+// How the work is cut: lanes a step's row (kL) and channels a lane (kC), segments of so many steps.
+struct Cut { int lanes, channels, segments, steps; };
 
-// Segments of whole tiles.  The gradient's are one tile each.
+// Calls f with kC and kL for `channels` channels a lane.
+template <class F>
+auto with_lanes(int lanes, int channels, F&& f) {
+    using One = std::integral_constant<int, 1>;
+    if (lanes == 4) return f(One{}, std::integral_constant<int, 4>{});
+    if (lanes == 16) return f(One{}, std::integral_constant<int, 16>{});
+    if (channels == 1) return f(One{}, std::integral_constant<int, 64>{});
+    return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
+}
+
+// Few channels leave lanes without one: 4 or 16 lanes then take a step's row, and a workgroup's
+// groups of them more steps (13 x 9342 x 3 in fp32, with gradient: 50 us, with 64 lanes 76), where
+// there are as many steps (2000 x 30 x 4: 156 and 40).
 //
-// Forward, workgroups that walk along whole sequences read the data once, those that walk along
-// segments twice; but a walk's tiles come one after another, and a CU with one walk waits for
-// its loads.  8 x 4096 x 2048 in bf16: 128 walks of two channels a lane 123 us, 256 of one 96,
-// 670 MB in segments 137; half of the sequences: 128 walks of one channel 90, segments 76.
+// Segments are of whole tiles, the gradient's of one tile each.  Forward, workgroups that walk along
+// whole sequences read the data once, those that walk along segments twice; but a walk's tiles come
+// one after another, and a CU with one walk waits for its loads.  8 x 4096 x 2048 in bf16: 128
+// walks of two channels a lane 123 us, 256 of one 91, 670 MB in segments 137; half of the
+// sequences: 76 either way.
 Cut cut_of(const hx_recurrence_args& A, bool grad) {
-    auto walks = [&](int lanes) { return A.batch * ((A.channels + 64 * lanes - 1) / (64 * lanes)); };
-    const int most = A.type == HX_F32 || A.channels == 1 ? 1 : 2;
-    const bool wide = most == 2 && (grad || walks(2) >= 256 || walks(1) < 160);
-    const int lanes = wide ? 2 : 1, tile = wide ? kTile<2> : kTile<1>;
+    const int lanes = A.channels <= 4 && A.time >= 1024 ? 4 : A.channels <= 16 && A.time >= 256 ? 16 : 64;
+    auto walks = [&](int channels) { return A.batch * ((A.channels + lanes * channels - 1) / (lanes * channels)); };
+    const bool wide = A.type != HX_F32 && lanes == 64 && A.channels > 1 && (grad || walks(2) >= 256 || walks(1) < 160);
+    const int channels = wide ? 2 : 1;
+    const int tile = with_lanes(lanes, channels, [](auto c, auto l) { return kTile<decltype(c)::value, decltype(l)::value>; });
     const long long tiles = std::max<long long>(1, (A.time + tile - 1) / tile);
-    long long segments = grad ? tiles : walks(1) >= 160 ? 1 : std::min<long long>(tiles, (512 + walks(lanes) - 1) / walks(lanes));
+    long long segments = grad ? tiles : walks(1) >= 160 ? 1 : std::min<long long>(tiles, (512 + walks(channels) - 1) / walks(channels));
     const long long each = (tiles + segments - 1) / segments;
     segments = (tiles + each - 1) / each;
-    return {lanes, static_cast<int>(segments), static_cast<int>(each * tile)};
+    return {lanes, channels, static_cast<int>(segments), static_cast<int>(each * tile)};
 }
 
 // The workspace's parts, one after another.
@@ -474,7 +494,7 @@ RecurrenceArgs recurrence_args(const hx_recurrence_args& A, const Cut& cut) {
     R.lengths = A.lengths, R.initial = A.initial_state, R.grad_end = A.grad_end;
     R.end = A.end_state, R.grad_initial = A.grad_initial;
     R.time = static_cast<int>(A.time), R.channels = static_cast<int>(A.channels), R.batch = A.batch;
-    const int width = 64 * cut.lanes;
+    const int width = cut.lanes * cut.channels;
     R.blocks = (R.channels + width - 1) / width;
     R.segments = cut.segments, R.steps = cut.steps;
     if (cut.segments > 1) {
@@ -485,14 +505,15 @@ RecurrenceArgs recurrence_args(const hx_recurrence_args& A, const Cut& cut) {
     return R;
 }
 
-// Calls f(element type, channels a lane).
+// Calls f(element type, kC, kL).
 template <class F>
-hipError_t with_lanes(const hx_recurrence_args& A, const Cut& cut, F&& f) {
+hipError_t with_cut(const hx_recurrence_args& A, const Cut& cut, F&& f) {
     return with_type(A.type, [&](auto t) {
-        using T = decltype(t);
-        if constexpr (!std::is_same_v<T, float>)
-            if (cut.lanes == 2) return f(t, std::integral_constant<int, 2>{});
-        return f(t, std::integral_constant<int, 1>{});
+        return with_lanes(cut.lanes, cut.channels, [&](auto c, auto l) -> hipError_t {
+            // two channels a lane are for 16 bits
+            if constexpr (std::is_same_v<decltype(t), float> && decltype(c)::value == 2) return hipErrorInvalidValue;
+            else return f(t, c, l);
+        });
     });
 }
 
@@ -516,16 +537,16 @@ hipError_t recurrence_forward(const hx_recurrence_args& A) {
     const RecurrenceArgs R = recurrence_args(A, cut);
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
-    return with_lanes(A, cut, [&](auto t, auto c) -> hipError_t {
+    return with_cut(A, cut, [&](auto t, auto c, auto l) -> hipError_t {
         using T = decltype(t);
-        constexpr int kC = decltype(c)::value;
+        constexpr int kC = decltype(c)::value, kL = decltype(l)::value;
         if (R.segments > 1) {
-            k_segments<T, kC, false><<<grid, kThreads, 0, st>>>(R);
+            k_segments<T, kC, kL, false><<<grid, kThreads, 0, st>>>(R);
             hipError_t e = hipGetLastError();
             if (e == hipSuccess) e = join<false>(R, st);
             if (e != hipSuccess) return e;
         }
-        k_walk<T, kC><<<grid, kThreads, 0, st>>>(R);
+        k_walk<T, kC, kL><<<grid, kThreads, 0, st>>>(R);
         return hipGetLastError();
     });
 }
@@ -535,22 +556,22 @@ hipError_t recurrence_backward(const hx_recurrence_args& A) {
     const RecurrenceArgs R = recurrence_args(A, cut);
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const unsigned grid = workgroups(R.batch * R.segments * R.blocks);
-    return with_lanes(A, cut, [&](auto t, auto c) -> hipError_t {
+    return with_cut(A, cut, [&](auto t, auto c, auto l) -> hipError_t {
         using T = decltype(t);
-        constexpr int kC = decltype(c)::value;
+        constexpr int kC = decltype(c)::value, kL = decltype(l)::value;
         if (R.segments > 1) {
-            k_segments<T, kC, true><<<grid, kThreads, 0, st>>>(R);
+            k_segments<T, kC, kL, true><<<grid, kThreads, 0, st>>>(R);
             hipError_t e = hipGetLastError();
             if (e == hipSuccess) e = join<true>(R, st);
             if (e != hipSuccess) return e;
         }
-        k_grad<T, kC><<<grid, kThreads, 0, st>>>(R);
+        k_grad<T, kC, kL><<<grid, kThreads, 0, st>>>(R);
         return hipGetLastError();
     });
 }
 
 hipError_t recurrence_step(const hx_recurrence_args& A) {
-    const RecurrenceArgs R = recurrence_args(A, Cut{1, 1, 1});
+    const RecurrenceArgs R = recurrence_args(A, Cut{64, 1, 1, 1});
     const hipStream_t st = static_cast<hipStream_t>(A.stream);
     const int v = A.channels % 4 == 0 ? 4 : 1;
     const unsigned grid = static_cast<unsigned>((A.batch * (A.channels / v) + 255) / 256);

@@ -17,20 +17,22 @@ def recurrence(x, gate, initial=None, lengths=None, do=None, dend=None):
     a, z = 1 / (1 + torch.exp(-gate)), 1 / (1 + torch.exp(gate))
     batch, steps, c = x.shape
     end = torch.zeros(batch, c, dtype=torch.float64) if initial is None else initial.cpu().double().clone()
-    o, dx, dgate = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x)
+    o, dx, dgate = (torch.zeros_like(x) for _ in range(3))
+    do = None if do is None else do.cpu()
     back = torch.zeros_like(end) if dend is None else dend.cpu().double().clone()
-    for i in range(batch):
-        n = steps if lengths is None else int(lengths[i])
-        before = []
-        for t in range(n):
-            before.append(end[i].clone())
-            end[i] = a[i, t] * end[i] + z[i, t] * x[i, t]
-            o[i, t] = end[i]
-        for t in reversed(range(n if do is not None else 0)):
-            l = back[i] + do[i, t].cpu().double()
-            dx[i, t] = z[i, t] * l
-            dgate[i, t] = a[i, t] * z[i, t] * l * (before[t] - x[i, t])
-            back[i] = a[i, t] * l
+    lengths = torch.full((batch,), steps) if lengths is None else lengths.cpu().long()
+    before = torch.zeros_like(x)
+    for t in range(steps):
+        live = lengths > t
+        before[live, t] = end[live]
+        end[live] = a[live, t] * end[live] + z[live, t] * x[live, t]
+        o[live, t] = end[live]
+    for t in reversed(range(steps if do is not None else 0)):
+        live = lengths > t
+        l = back[live] + do[live, t].cpu().double()
+        dx[live, t] = z[live, t] * l
+        dgate[live, t] = a[live, t] * z[live, t] * l * (before[live, t] - x[live, t])
+        back[live] = a[live, t] * l
     return o, end, dx, dgate, back
 
 
@@ -84,14 +86,15 @@ def test_lengths_of_time(time, dtype):
     check(x, gate, do, state, None, dstate)
 
 
-@pytest.mark.parametrize("channels", [1, 2, 3, 31, 63, 64, 65, 127, 128, 129, 200, 601])
+@pytest.mark.parametrize("channels", [1, 2, 3, 4, 5, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 200, 601])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_channels(channels, dtype):
     x, gate, do, state, dstate = inputs(channels, 3, 90, channels, dtype)
     check(x, gate, do, state, None, dstate)
 
 
-@pytest.mark.parametrize("batch,time,channels", [(1, 5000, 40), (2, 2500, 130), (130, 150, 3), (40, 140, 513)])
+@pytest.mark.parametrize("batch,time,channels", [(1, 5000, 40), (2, 2500, 130), (130, 150, 3), (40, 140, 513), (2, 9000, 3),
+                                                 (170, 2100, 2), (2, 2500, 14), (170, 1050, 9)])
 def test_cut_and_whole(batch, time, channels):
     """Few chains, cut into many segments, and enough for a workgroup to walk along each."""
     x, gate, do, state, dstate = inputs(0, batch, time, channels, torch.float32)
