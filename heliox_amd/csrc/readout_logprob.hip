@@ -508,12 +508,14 @@ hipError_t logprob_launch(const hx_logprob_args& A) {
             k_logprobs<T, kThreads, decltype(top)::value><<<grid, kThreads, 0, st>>>(L);
         };
         // Threads: 512 keep four rows on a CU, whose starts and ends lie beside the others' middles (2048 x
-        // 131072 in bf16, top 5: 118 us, with 1024 threads 127, with 256 143; top 100: 176 and 188).  More
+        // 131072 in bf16, top 5: 118 us, with 1024 threads 127, with 256 143; top 100: 176 and 188); of
+        // short rows 256 threads keep eight (4000 x 32000 in fp16, top 20: 83 us, with 512 threads 88; 300
+        // of them, that do not fill the chip, 25 and 19).  More
         // than 128 top places would pass more logits to each of eight waves than its list holds (top
         // 256: 232 us with 1024 threads, 997 with 512).
         auto pick = [&](auto with_top) {
             if (L.each <= 512) go(std::integral_constant<int, 64>{}, with_top);
-            else if (L.each <= 8192) go(std::integral_constant<int, 256>{}, with_top);
+            else if (L.each <= (grid >= 1024 ? 32768 : 8192)) go(std::integral_constant<int, 256>{}, with_top);
             else if (A.top <= 128) go(std::integral_constant<int, 512>{}, with_top);
             else if constexpr (decltype(with_top)::value) go(std::integral_constant<int, 1024>{}, with_top);
         };

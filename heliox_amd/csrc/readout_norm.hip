@@ -450,8 +450,6 @@ template <class T, bool kGrad, class F>
 auto with_shape(int width, F&& f) {
     constexpr int kE = sizeof(typename PieceOf<T>::Vec) / sizeof(T);
     const int pieces = (width + kE - 1) / kE;
-    // the gradient holds two rows and two sums: fewer pieces a lane
-    constexpr int kMost = kGrad ? (kE == 8 ? 2 : 4) : 4;
     if (width < kE) return f(Shape<1, 8, 1>{});
     if (pieces <= 8) return f(Shape<kE, 8, 1>{});
     if (pieces <= 16) return f(Shape<kE, 8, 2>{});
@@ -459,9 +457,18 @@ auto with_shape(int width, F&& f) {
     if (pieces <= 128) return f(Shape<kE, 64, 2>{});
     if (pieces <= 256) return f(Shape<kE, 256, 1>{});
     if (pieces <= 512) return f(Shape<kE, 256, 2>{});
-    if (pieces <= 256 * kMost) return f(Shape<kE, 256, kMost>{});
-    if (pieces <= 2048) return f(Shape<kE, 1024, 2>{});
-    if (pieces <= 1024 * kMost) return f(Shape<kE, 1024, kMost>{});
+    // The gradient holds two rows and two sums: 16 elements a lane of 1024 lanes are more than the
+    // registers hold, 12 are not (4032 x 8587 in fp16, with the forward pass: 222 us and 128).
+    if constexpr (kGrad) {
+        if (pieces <= 1024) return f(std::conditional_t<kE == 8, Shape<8, 1024, 1>, Shape<4, 256, 4>>{});
+        if (width <= 8 * 1024) return f(Shape<4, 1024, 2>{});
+        if (width <= 12 * 1024) return f(Shape<4, 1024, 3>{});
+    } else {
+        if (pieces <= 1024) return f(Shape<kE, 256, 4>{});
+        if (pieces <= 2048) return f(Shape<kE, 1024, 2>{});
+        if constexpr (kE == 4)
+            if (pieces <= 4096) return f(Shape<4, 1024, 4>{});
+    }
     return f(TooWide{});
 }
 

@@ -472,7 +472,7 @@ Cut cut_of(const hx_recurrence_args& A, bool grad) {
     const int channels = wide ? 2 : 1;
     const int tile = with_lanes(lanes, channels, [](auto c, auto l) { return kTile<decltype(c)::value, decltype(l)::value>; });
     const long long tiles = std::max<long long>(1, (A.time + tile - 1) / tile);
-    long long segments = grad ? tiles : walks(1) >= 160 ? 1 : std::min<long long>(tiles, (512 + walks(channels) - 1) / walks(channels));
+    long long segments = grad ? tiles : walks(1) >= 160 || tiles <= 4 ? 1 : std::min<long long>(tiles, (512 + walks(channels) - 1) / walks(channels));
     const long long each = (tiles + segments - 1) / segments;
     segments = (tiles + each - 1) / each;
     return {lanes, channels, static_cast<int>(segments), static_cast<int>(each * tile)};
