@@ -88,8 +88,41 @@ struct Where {
         w.length = A.lengths ? min(max(A.lengths[w.batch], 0), A.time) : A.time;
         return w;
     }
-    __device__ __forceinline__ long long at(const RecurrenceArgs& A) const {
-        return (batch * A.segments + segment) * A.channels + channel;
+    __device__ __forceinline__ long long at(const RecurrenceArgs& A) const { return at(A, segment); }
+    __device__ __forceinline__ long long at(const RecurrenceArgs& A, int s) const {
+        return (batch * A.segments + s) * A.channels + channel;
+    }
+    // What enters the segment from the left, and going back from the right: as it was joined, or, with
+    // kJoins, what enters the sequence, taken along the segments beside this one.  (Variants of their
+    // own: with both ways in one kernel its loads wait for each other, 306 us for 8 x 4096 x 2048
+    // with gradient became 309 to 317.)
+    template <bool kJoins, int kC>
+    __device__ __forceinline__ void entering(const RecurrenceArgs& A, float (&h)[kC]) const {
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            h[c] = 0.f;
+            if (!kJoins && A.segments > 1) h[c] = A.enter[at(A) + c];
+            else if (A.initial) h[c] = A.initial[batch * A.channels + channel + c];
+        }
+        if constexpr (kJoins)
+#pragma unroll 8
+            for (int s = 0; s < segment; ++s)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) h[c] = fmaf(A.p[at(A, s) + c], h[c], A.y[at(A, s) + c]);
+    }
+    template <bool kJoins, int kC>
+    __device__ __forceinline__ void leaving(const RecurrenceArgs& A, float (&g)[kC]) const {
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            g[c] = 0.f;
+            if (!kJoins && A.segments > 1) g[c] = A.leave[at(A) + c];
+            else if (A.grad_end) g[c] = A.grad_end[batch * A.channels + channel + c];
+        }
+        if constexpr (kJoins)
+#pragma unroll 8
+            for (int s = A.segments - 1; s > segment; --s)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) g[c] = fmaf(A.p[at(A, s) + c], g[c], A.r[at(A, s) + c]);
     }
 };
 
@@ -130,7 +163,7 @@ __device__ __forceinline__ void fetch(typename Packed<T, kC>::Vec (&to)[kN], con
 }
 
 // The whole walk.
-template <class T, int kC, int kL>
+template <class T, int kC, int kL, bool kJoins>
 __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceArgs A) {
     constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC, kL>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
@@ -144,12 +177,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceA
         const Where w = Where::of<kC, kL>(A, id);
         const int first = w.segment * A.steps, last = min(first + A.steps, A.time);
         float h[kC];
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            h[c] = 0.f;
-            if (A.segments > 1) h[c] = A.enter[w.at(A) + c];
-            else if (A.initial) h[c] = A.initial[w.batch * A.channels + w.channel + c];
-        }
+        w.entering<kJoins>(A, h);
         Vec x[kU], g[kU];
         fetch<T, kC>(x, A.x, A.x_stride, w, first + group * kU);
         fetch<T, kC>(g, A.gate, A.gate_stride, w, first + group * kU);
@@ -321,7 +349,7 @@ __global__ void __launch_bounds__(1024) k_join(RecurrenceArgs A) {
 }
 
 // The gradients of kTile steps, from what enters them on both sides.
-template <class T, int kC, int kL>
+template <class T, int kC, int kL, bool kJoins>
 __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceArgs A) {
     constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC, kL>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
@@ -336,17 +364,8 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
         fetch<T, kC>(g, A.gate, A.gate_stride, w, t);
         fetch<T, kC>(d, A.grad_o, A.grad_o_stride, w, t);
         float h[kC], back[kC];
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            h[c] = back[c] = 0.f;
-            if (A.segments > 1) {
-                h[c] = A.enter[w.at(A) + c];
-                back[c] = A.leave[w.at(A) + c];
-            } else {
-                if (A.initial) h[c] = A.initial[w.batch * A.channels + w.channel + c];
-                if (A.grad_end) back[c] = A.grad_end[w.batch * A.channels + w.channel + c];
-            }
-        }
+        w.entering<kJoins>(A, h);
+        w.leaving<kJoins>(A, back);
         float z[kU][kC], a[kU][kC], p[kC], y[kC], r[kC];
 #pragma unroll
         for (int c = 0; c < kC; ++c) p[c] = 1.f, y[c] = r[c] = 0.f;
@@ -421,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
         };
         if (whole_group) out(std::true_type{});
         else out(std::false_type{});
-        if (A.segments == 1 && A.grad_initial && group == 0)
+        if ((kJoins ? w.segment == 0 : A.segments == 1) && A.grad_initial && group == 0)
 #pragma unroll
             for (int c = 0; c < kC; ++c) A.grad_initial[w.batch * A.channels + w.channel + c] = back[c];
     });
@@ -493,6 +512,10 @@ Cut cut_of(const hx_recurrence_args& A, bool grad) {
     segments = (tiles + each - 1) / each;
     return {lanes, channels, static_cast<int>(segments), static_cast<int>(each * tile)};
 }
+
+// Up to so many segments join those beside them by themselves, which saves a launch (13 x 777 x 601 in
+// fp16: 21 us, with it 23; 32 segments of 2 x 2000 x 600: 40 and 38).
+constexpr int kJoined = 16;
 
 // The workspace's parts, one after another.
 size_t part_bytes(const hx_recurrence_args& A, const Cut& cut) {
@@ -567,10 +590,11 @@ hipError_t recurrence_forward(const hx_recurrence_args& A) {
         if (R.segments > 1) {
             k_segments<T, kC, kL, false><<<grid, kThreads, 0, st>>>(R);
             hipError_t e = hipGetLastError();
-            if (e == hipSuccess) e = join<false>(R, st);
+            if (e == hipSuccess && R.segments > kJoined) e = join<false>(R, st);
             if (e != hipSuccess) return e;
         }
-        k_walk<T, kC, kL><<<grid, kThreads, 0, st>>>(R);
+        if (R.segments > 1 && R.segments <= kJoined) k_walk<T, kC, kL, true><<<grid, kThreads, 0, st>>>(R);
+        else k_walk<T, kC, kL, false><<<grid, kThreads, 0, st>>>(R);
         return hipGetLastError();
     });
 }
@@ -586,10 +610,11 @@ hipError_t recurrence_backward(const hx_recurrence_args& A) {
         if (R.segments > 1) {
             k_segments<T, kC, kL, true><<<grid, kThreads, 0, st>>>(R);
             hipError_t e = hipGetLastError();
-            if (e == hipSuccess) e = join<true>(R, st);
+            if (e == hipSuccess && R.segments > kJoined) e = join<true>(R, st);
             if (e != hipSuccess) return e;
         }
-        k_grad<T, kC, kL><<<grid, kThreads, 0, st>>>(R);
+        if (R.segments > 1 && R.segments <= kJoined) k_grad<T, kC, kL, true><<<grid, kThreads, 0, st>>>(R);
+        else k_grad<T, kC, kL, false><<<grid, kThreads, 0, st>>>(R);
         return hipGetLastError();
     });
 }
