@@ -93,8 +93,8 @@ int recurrence_sizes(const char* call, const hx_recurrence_args* A) {
     if (!known_type(A->type)) return refuse("%s: type %lld is not known", call, (long long)A->type);
     if (A->batch < 0 || A->time < 0) return refuse("%s: negative batch or time", call);
     if (A->channels < 1) return refuse("%s: channels has to be at least 1", call);
-    if (checked_product(A->batch, A->channels) > INT32_MAX || A->channels > INT32_MAX || A->time > (int64_t(1) << 30))
-        return refuse("%s: batch x channels is at most 2^31 - 1 and time at most 2^30", call);
+    if (checked_product(A->batch, A->channels) > INT32_MAX || A->channels > (1 << 30) || A->time > (int64_t(1) << 30))
+        return refuse("%s: batch x channels is at most 2^31 - 1, channels and time at most 2^30", call);
     return 0;
 }
 

@@ -5,7 +5,8 @@
 // held row, not the difference of two large numbers).  Workgroups walk over the rows, so that
 // weight and bias stay in registers too, and the gradients of both are added there: each
 // workgroup writes its sums once, a second launch adds those up in a fixed order.  (Few rows are
-// read a second time instead, by columns.)  Both are bound by the rows' bytes.
+// read a second time instead, by columns.)  Both are bound by the rows' bytes: 32768 x 4096 in
+// bf16 forward 96 us, 5.6 TB/s, backward 156, 5.2, and 5 for the sums (a copy: 4.9).
 #include "readout.h"
 
 #include <algorithm>

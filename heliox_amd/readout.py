@@ -81,6 +81,11 @@ def _on_gpu(x: torch.Tensor, what: str) -> int:
     return device
 
 
+def _empty(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor like x (empty_like is the quicker call, but keeps strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x with its last dimension contiguous (a copy only where it is not)."""
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
@@ -340,7 +345,7 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, *, initial_state: Opti
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, channels), device)
     _no_graph("gated_recurrence", "take it from gated_recurrence_grad", x, gate, initial_state)
     lengths = _lengths(lengths, batch, device)
-    o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    o = _empty(x)
     end = torch.empty((batch, channels), dtype=torch.float32, device=x.device)
     need = _recurrence_space(sizes, 0)
     space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
@@ -365,7 +370,7 @@ def gated_recurrence_grad(x: torch.Tensor, gate: torch.Tensor, do: torch.Tensor,
     initial_state = _array(initial_state, "initial_state", torch.float32, (batch, channels), device)
     dstate = _array(dstate, "dstate", torch.float32, (batch, channels), device)
     lengths = _lengths(lengths, batch, device)
-    dx, dgate = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    dx, dgate = _empty(x), _empty(x)
     dinitial = None if initial_state is None else torch.empty_like(initial_state)
     need = _recurrence_space(sizes, 1)
     space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
@@ -389,7 +394,7 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         raise ValueError(f"state has shape {tuple(state.shape)}, expected (n_slots, {channels})")
     _no_graph("gated_recurrence_step", "take it from gated_recurrence_grad over the steps", x, gate, state)
     slots = _array(slots, "slots", torch.int32, (batch,), device)
-    o = torch.empty((batch, channels), dtype=x.dtype, device=x.device)
+    o = _empty(x)
     _call("hx_gated_recurrence_step", device, _RECURRENCE.pack(
         *fields, 0, 0, o.data_ptr(), channels, 0, 0, 0, 0, 0, 0, 0, 0, 0, state.data_ptr(), _ptr(slots), state.shape[0],
         0, 0, _stream(device)))
@@ -436,7 +441,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     (fp32, x's shape without the last), which layer_norm_grad takes."""
     device, kind, weight_kind, rows, weight, bias = _norm_inputs(x, weight, bias)
     _no_graph("layer_norm", "take it from layer_norm_grad", x, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
     n, width = rows.shape
     _call("hx_layer_norm", device, _NORM.pack(
@@ -460,7 +465,7 @@ def layer_norm_grad(x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch
     rstd = _array(rstd, "rstd", torch.float32, x.shape[:-1], device)
     dy = _flat_rows(dy)
     n, width = rows.shape
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _empty(x)
     dweight = dbias = space = None
     need = 0
     if parameters:
@@ -608,7 +613,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, scored: Toke
     dlogprob = _array(dlogprob, "dlogprob", torch.float32, (rows,), device)
     dentropy = _array(dentropy, "dentropy", torch.float32, (rows,), device)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = _empty(logits)
     elif (_on_gpu(out, "out") != device or out.dtype != logits.dtype or out.shape != logits.shape
           or (out.shape[-1] > 1 and out.stride(-1) != 1)):
         raise ValueError("out has to be like the logits, its last dimension contiguous")
@@ -792,4 +797,5 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         state.bits, len(params), *[a.buffer_info()[0] for a in lists], state.m.data_ptr(), state.v.data_ptr(),
         _ptr(state.m_scale), _ptr(state.v_scale), state.m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
         lr_ptr, state._count.data_ptr(), _stream(device)))
-    torch.autograd.graph.increment_version(params)
+    # what autograd kept of the old values is out of date (inference tensors are never kept)
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

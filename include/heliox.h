@@ -642,7 +642,8 @@ int hx_layer_norm_grad(const hx_norm_args* args);
  * sequence's last step; outputs past its length are zero, whatever its inputs hold there.  The
  * gradient: with l_t = grad_o_t + a_{t+1} l_{t+1} (past the end: grad_end),
  *   grad_x = (1 - a) l,  grad_gate = a (1 - a) l (h_{t-1} - x_t),  grad_initial = a_0 l_0.
- * States are (batch, channels) fp32, contiguous.  time is at most 2^30, batch x channels 2^31 - 1.
+ * States are (batch, channels) fp32, contiguous.  time and channels are at most 2^30, batch x channels
+ * 2^31 - 1.
  * What a call writes overlaps nothing that it reads (end_state and grad_initial that do are
  * refused), but for the single step's state. */
 typedef struct hx_recurrence_args {

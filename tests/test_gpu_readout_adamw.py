@@ -235,6 +235,12 @@ def test_a_graph_of_the_old_values_is_refused():
         y.backward()
 
 
+def test_inference_tensors():
+    with torch.inference_mode():
+        params, grads = tensors(0, SIZES), tensors(1, SIZES)
+        check_step(params, grads, readout.adamw_state(params), 1)
+
+
 def test_on_a_stream_of_its_own():
     a, b, grads = tensors(0, SIZES), tensors(0, SIZES), tensors(1, SIZES)
     sa, sb = readout.adamw_state(a, bits=8), readout.adamw_state(b, bits=8)

@@ -58,6 +58,7 @@ def recurrence(type=0, batch=2, time=5, channels=8, x=AT, gate=AT, initial=0, o=
 @pytest.mark.parametrize("change,text", [
     ({"type": 5}, "type"), ({"batch": -1}, "negative"), ({"time": -1}, "negative"), ({"channels": 0}, "channels"),
     ({"batch": 2 ** 28}, "2^31"), ({"batch": 2 ** 62}, "2^31"), ({"channels": 2 ** 40, "batch": 0}, "2^31"),
+    ({"channels": 2 ** 30 + 1, "batch": 1}, "2^30"),
     ({"time": 2 ** 30 + 1}, "2^30")])
 def test_recurrence_sizes_are_refused(call, change, text):
     assert getattr(lib(), call)(recurrence(**change)) == -1
