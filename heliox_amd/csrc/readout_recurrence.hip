@@ -168,7 +168,6 @@ template <class T, int kC, int kL, bool kJoins>
 __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceArgs A) {
     constexpr int kU = hx::kU<kC>, kTile = hx::kTile<kC, kL>, kW = kThreads / kL;
     using Vec = typename Packed<T, kC>::Vec;
-    using F = typename Floats<kC>::Vec;
     __shared__ float ends[2][kW][2 * kC][kL];
     const int group = group_of<kL>(), lane = threadIdx.x % kL;
     int turn = 0;
