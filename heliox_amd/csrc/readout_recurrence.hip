@@ -58,10 +58,16 @@ __device__ __forceinline__ float part(const Vec& v, int c) {
     else return static_cast<float>(v[c]);
 }
 
-template <class Vec, int kC>
-__device__ __forceinline__ void set(Vec& v, int c, float x) {
-    if constexpr (kC == 1) v = static_cast<Vec>(x);
-    else v[c] = static_cast<decltype(v[0] + v[0])>(x);
+template <class T, int kC>
+__device__ __forceinline__ typename Packed<T, kC>::Vec packed(const float* x) {
+    typename Packed<T, kC>::Vec v;
+    if constexpr (kC == 1) {
+        v = static_cast<typename Packed<T, kC>::Vec>(x[0]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < kC; ++c) v[c] = static_cast<decltype(v[0] + v[0])>(x[c]);
+    }
+    return v;
 }
 
 // e^gate; infinite over 88.
@@ -226,13 +232,14 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceA
             auto write = [&](auto whole) {
 #pragma unroll
                 for (int u = 0; u < kU; ++u, o += A.o_stride[1]) {
-                    Vec out;
+                    float out[kC];
 #pragma unroll
                     for (int c = 0; c < kC; ++c) {
                         const float v = fmaf(p[u][c], mine[c], y[u][c]);
-                        set<Vec, kC>(out, c, decltype(whole)::value || t + u < w.length ? v : 0.f);
+                        out[c] = decltype(whole)::value || t + u < w.length ? v : 0.f;
                     }
-                    if (decltype(whole)::value || t + u < A.time) *reinterpret_cast<Vec*>(o + w.channel) = out;
+                    if (decltype(whole)::value || t + u < A.time)
+                        *reinterpret_cast<Vec*>(o + w.channel) = packed<T, kC>(out);
                 }
             };
             if (t + kU <= w.length) write(std::true_type{});
@@ -424,17 +431,17 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
 #pragma unroll
             for (int u = kU - 1; u >= 0; --u) {
                 const bool live = decltype(whole)::value || t + u < w.length;
-                Vec vx, vg;
+                float vx[kC], vg[kC];
 #pragma unroll
                 for (int c = 0; c < kC; ++c) {
                     const float l = part<Vec, kC>(d[u], c) + back[c], zl = z[u][c] * l;
-                    set<Vec, kC>(vx, c, live ? zl : 0.f);
-                    set<Vec, kC>(vg, c, live ? a[u][c] * zl * off[u][c] : 0.f);
+                    vx[c] = live ? zl : 0.f;
+                    vg[c] = live ? a[u][c] * zl * off[u][c] : 0.f;
                     if (live) back[c] = left(l, z[u][c]);
                 }
                 if (decltype(whole)::value || t + u < A.time) {
-                    *reinterpret_cast<Vec*>(dx + static_cast<long long>(u) * A.channels + w.channel) = vx;
-                    *reinterpret_cast<Vec*>(dg + static_cast<long long>(u) * A.channels + w.channel) = vg;
+                    *reinterpret_cast<Vec*>(dx + static_cast<long long>(u) * A.channels + w.channel) = packed<T, kC>(vx);
+                    *reinterpret_cast<Vec*>(dg + static_cast<long long>(u) * A.channels + w.channel) = packed<T, kC>(vg);
                 }
             }
         };
