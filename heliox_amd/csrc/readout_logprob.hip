@@ -9,7 +9,7 @@
 // hundred of a hundred thousand.  They wait in LDS as whole numbers, logit above index, and each
 // counts those above it.  Where more than 256 come through, the top places' own bound is found
 // byte by byte from histograms, of those that came or, where a wave's list is too short for them
-// (logits that rise along the row, or are all the same), of the whole row.
+// (logits that rise along the row, or are all the same), of the row's values.
 //
 // Few long rows are cut into parts, which a second launch joins.  Bound by the logits' bytes, read
 // once: 2048 x 131072 in bf16 with the top 5 in 106 to 118 us, 4.6 to 5.1 TB/s; short rows by what a
@@ -97,13 +97,15 @@ __device__ __forceinline__ float kth_of_wave(float v, int k) {
     return found <= 0x7f ? -INFINITY : value_of(found << 16);
 }
 
-// The top-th largest of `total` distinct keys, byte by byte from histograms.  each(f) calls f(key,
-// whether it is one) for all of them, a whole wave at a time.
-template <int kThreads, class Each>
+// The bound that the `top` largest of `total` keys reach and no others, byte by byte from histograms.
+// each(f) calls f(key, whether it is one) for all of them, a whole wave at a time.  Where the bytes
+// from kLast bits on do not tell (equal keys) the answer is 0: sh.prefix holds those bytes of the
+// last that belong, sh.left how many of them do.
+template <int kThreads, int kLast, class Each>
 __device__ u64 bound_of(int top, int total, Shared<kThreads>& sh, Each each) {
     const int lane = threadIdx.x % 64;
     if (threadIdx.x == 0) sh.prefix = sh.answer = 0, sh.left = min(top, total);
-    for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int shift = 56; shift >= kLast; shift -= 8) {
         for (int b = threadIdx.x; b < 256; b += kThreads) sh.bins[b] = 0;
         __syncthreads();
         const u64 prefix = sh.prefix, answer = sh.answer;
@@ -171,10 +173,88 @@ __device__ __forceinline__ void rank_best(int top, const Shared<kThreads>& sh, F
     }
 }
 
-// Calls put(rank, key) for the top largest keys, from the largest on; all(f) as each above, over
-// every key of the part or row, for where the waves' lists do not hold those that may be among them.
-template <int kThreads, class All, class F>
-__device__ __forceinline__ void each_ranked(int top, int whole, Shared<kThreads>& sh, All all, F put) {
+// The top largest of a row's n logits from x on, the first of them index `first`, to sh.best: the
+// value that bounds them, then all above it and the first of those at it.
+template <class T, int kThreads>
+__device__ void choose_of_row(const T* x, int n, int first, int top, Shared<kThreads>& sh) {
+    using Vec = typename PieceOf<T>::Vec;
+    constexpr int kP = sizeof(Vec) / sizeof(T), kWaves = kThreads / 64;
+    // the bits of an order that all numbers of the type share
+    constexpr int kSame = std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 8 : 16;
+    const int pieces = n / kP, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int turns = (pieces + kThreads - 1) / kThreads;
+    // f(logits, how many, the first one's place) of this thread in a turn; the last turn is what whole pieces leave
+    auto turn = [&](int c, auto f) {
+        float v[kP];
+        const int p = c * kThreads + static_cast<int>(threadIdx.x), j = pieces * kP + static_cast<int>(threadIdx.x);
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) v[i] = 0.f;
+        if (c == turns) {
+            if (j < n) v[0] = to_f32(x[j]), count = 1;
+        } else if (p < pieces) {
+            const Vec raw = *reinterpret_cast<const Vec*>(x + static_cast<long long>(p) * kP);
+#pragma unroll
+            for (int i = 0; i < kP; ++i) v[i] = static_cast<float>(raw[i]);
+            count = kP;
+        }
+        f(v, count, c == turns ? j : p * kP);
+    };
+    const u64 answer = bound_of<kThreads, 32 + kSame>(top, n, sh, [&](auto f) {
+        for (int c = 0; c <= turns; ++c)
+            turn(c, [&](const float* v, int count, int) {
+#pragma unroll
+                for (int i = 0; i < kP; ++i) f(static_cast<u64>(order_of(v[i])) << 32, i < count);
+            });
+    });
+    // above `value` all belong, at it the first `left`
+    const unsigned value = static_cast<unsigned>((answer ? answer : sh.prefix) >> 32 >> kSame) - (answer ? 1 : 0);
+    const int left = answer ? 0 : sh.left, want = min(top, n);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.chosen = 0;
+    __syncthreads();
+    auto push = [&](float v, int j) {
+        const int at = atomicAdd(&sh.chosen, 1);
+        if (at < kBest) sh.best[at] = key_of(v, first + j);
+    };
+    int before = 0;                               // logits at the bound in earlier turns
+    for (int c = 0; c <= turns; ++c) {
+        int mine = 0, here = 0;
+        turn(c, [&](const float* v, int count, int j) {
+#pragma unroll
+            for (int i = 0; i < kP; ++i) {
+                const unsigned o = order_of(v[i]) >> kSame;
+                if (i < count && o > value) push(v[i], j + i);
+                mine += i < count && o == value;
+            }
+            int upto = mine;
+            for (int d = 1; d < 64; d *= 2) {
+                const int below = __shfl_up(upto, d);
+                if (lane >= d) upto += below;
+            }
+            if (lane == 63) sh.count[wave] = upto;
+            __syncthreads();
+            int rank = before + upto - mine;
+            for (int w = 0; w < kWaves; ++w) {
+                here += sh.count[w];
+                if (w < wave) rank += sh.count[w];
+            }
+#pragma unroll
+            for (int i = 0; i < kP; ++i)
+                if (i < count && order_of(v[i]) >> kSame == value && rank++ < left) push(v[i], j + i);
+        });
+        before += here;
+        __syncthreads();
+        const bool done = sh.chosen >= want;      // read by all before the next turn adds to it
+        __syncthreads();
+        if (done) break;
+    }
+}
+
+// Calls put(rank, key) for the top largest keys, from the largest on, of the waves' lists or, where one
+// was too short, of the n logits from x on.
+template <class T, int kThreads, class F>
+__device__ __forceinline__ void each_ranked(const T* x, int n, int first, int top, Shared<kThreads>& sh, F put) {
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     int total = 0, longest = 0;
     for (int v = 0; v < kThreads / 64; ++v) {
@@ -184,8 +264,9 @@ __device__ __forceinline__ void each_ranked(int top, int whole, Shared<kThreads>
     auto held = [&](auto f) {
         for (int i = 0; i < sh.count[wave]; i += 64) f(i + lane < sh.count[wave] ? sh.held[wave][i + lane] : 0, i + lane < sh.count[wave]);
     };
-    if (longest > kEach) choose<kThreads>(bound_of<kThreads>(top, whole, sh, all), sh, all);
-    else choose<kThreads>(total > kBest ? bound_of<kThreads>(top, total, sh, held) : 0, sh, held);
+    __syncthreads();
+    if (longest > kEach) choose_of_row<T, kThreads>(x, n, first, top, sh);
+    else choose<kThreads>(total > kBest ? bound_of<kThreads, 0>(top, total, sh, held) : 0, sh, held);
     rank_best<kThreads>(top, sh, put);
 }
 
@@ -347,23 +428,17 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
         if (threadIdx.x % 64 == 0) sh.count[threadIdx.x / 64] = kept;
         __syncthreads();
     }
-    auto all = [&](auto f) {
-        for (int j0 = first; j0 < last; j0 += kThreads) {
-            const int j = j0 + static_cast<int>(threadIdx.x);
-            f(j < last ? key_of(to_f32(x[j]), j) : 0, j < last);
-        }
-    };
     if (A.parts == 1) {
         const Finish done(S);
         if (threadIdx.x == 0) finish_row(A, row, x, S, done);
         if constexpr (kTop)
-            each_ranked<kThreads>(A.top, last - first, sh, all, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
+            each_ranked<T, kThreads>(x + first, last - first, first, A.top, sh, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
     } else {
         if (threadIdx.x == 0) A.sums[blockIdx.x] = S;
         if constexpr (kTop) {
             u64* const to = A.keys + static_cast<long long>(blockIdx.x) * A.top;
             for (int i = last - first + threadIdx.x; i < A.top; i += kThreads) to[i] = 0;
-            each_ranked<kThreads>(A.top, last - first, sh, all, [&](int rank, u64 key) { to[rank] = key; });
+            each_ranked<T, kThreads>(x + first, last - first, first, A.top, sh, [&](int rank, u64 key) { to[rank] = key; });
         }
     }
 }
@@ -398,7 +473,7 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobArgs A) {
         }
     };
     if (!A.top) return;
-    choose<256>(n > kBest ? bound_of<256>(A.top, n, sh, all) : 0, sh, all);
+    choose<256>(n > kBest ? bound_of<256, 0>(A.top, n, sh, all) : 0, sh, all);
     rank_best<256>(A.top, sh, [&](int rank, u64 key) { put_top(A, row, done, rank, key); });
 }
 
