@@ -2,7 +2,8 @@
 //
 // A workgroup takes kChunk elements of one tensor, a wave kBlocks blocks of 256 in a row, four
 // elements a lane in each, so that every array streams through as it lies in memory: bound by
-// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 308 us, 4.9 TB/s).  The tensors of a launch are listed in its arguments; a workgroup finds its own
+// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 314 us, 4.8 TB/s; with four blocks a wave
+// 327, with one 333).  The tensors of a launch are listed in its arguments; a workgroup finds its own
 // by one comparison a lane.  The count of steps, and what follows from it alone, is made by a
 // first launch of one thread, on the device, so that a captured step counts on.
 //
@@ -18,7 +19,7 @@
 namespace hx {
 namespace {
 
-constexpr int kThreads = 256, kBlocks = 4, kBlock = 256, kChunk = kThreads / 64 * kBlocks * kBlock;
+constexpr int kThreads = 256, kBlocks = 2, kBlock = 256, kChunk = kThreads / 64 * kBlocks * kBlock;
 constexpr int kTensors = 64;                       // of a launch: a lane each, 3 KB of arguments
 constexpr float kTop8 = 448.f, kLeast8 = 0x1p-9f;  // of e4m3
 constexpr float kTiny = 0x1p-100f;                 // blocks whose largest moment is below are zero
@@ -117,6 +118,12 @@ __device__ __forceinline__ int pack(Float4 x) {
 }
 
 // Codes of a block, relative to its largest; that over 448 is returned.
+//
+// A number next to the middle of two codes goes to one or the other by its last bit, and a block's
+// largest number that does so moves the scale of all by a sixteenth.  So that a state's way can be
+// followed by any other fp32 arithmetic, moments and quotients are rounded operation by operation, and
+// the quotient x / top is the correctly rounded one: from the correctly rounded 1 / top, corrected by
+// the exact remainder (Markstein's division).
 template <bool kRoot>
 __device__ __forceinline__ float quantise(Float4 x, int& code) {
     float top = 0.f;
@@ -124,10 +131,12 @@ __device__ __forceinline__ float quantise(Float4 x, int& code) {
     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[i]));
     top = wave_max(top);
     const bool live = top >= kTiny;
-    const float up = live ? kTop8 / top : 0.f;
+    const float per = live ? 1.f / top : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        x[i] *= up;
+        float q = x[i] * per;
+        q = fmaf(fmaf(-q, top, x[i]), per, q);
+        x[i] = q * kTop8;
         if (kRoot && x[i] > 0.f && x[i] < kLeast8) x[i] = kLeast8;
     }
     code = pack(x);
@@ -185,8 +194,9 @@ __global__ void __launch_bounds__(kThreads) k_adamw(AdamwArgs A) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float gg = gv[b][i] * clip;
-                mv[b][i] = fmaf(A.less1, gg, A.beta1 * mv[b][i]);
-                vv[b][i] = fmaf(A.less2 * gg, gg, A.beta2 * vv[b][i]);
+                // (each operation rounded by itself: see quantise)
+                mv[b][i] = A.beta1 * mv[b][i] + A.less1 * gg;
+                vv[b][i] = A.beta2 * vv[b][i] + A.less2 * gg * gg;
                 root[i] = sqrtf(vv[b][i]);
                 const float step = mv[b][i] * __builtin_amdgcn_rcpf(fmaf(root[i], rates.root, A.eps));
                 pv[b][i] = fmaf(-rates.size, step, pv[b][i] * keep);

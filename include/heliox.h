@@ -718,7 +718,8 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * tensors, tensor i's from element `start` (a multiple of 256) on.  bits 32: m and v as fp32.
  * bits 8: m and sqrt(v) as 8-bit floating-point numbers (4 bits of exponent, 3 of mantissa, no
  * infinity: largest 448), each 256 elements relative to m_scale and v_scale, the largest of them
- * / 448 (fp32; 0, and the numbers 0, where that largest is under 2^-100), rounded to nearest even;
+ * / 448 (fp32; 0, and the numbers 0, where that largest is under 2^-100), rounded to nearest even (m, v,
+ * their root and the quotient by the largest are fp32, rounded operation by operation, left to right);
  * a root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
  * that is not finite reaches its block's 256 elements in 8 bits.
  * Tensors come in the order of their starts, each within `moments`, its last 256 filled up with

@@ -194,6 +194,44 @@ def test_small_and_large_moments_in_8_bits():
     assert bool((state.m_scale[1:3] == 0).all()) and bool((state.v_scale[1:3] == 0).all())
 
 
+def follow(m, v, ms, vs, g, scale, betas):
+    """The 8-bit moments' way in torch's fp32, operation by operation."""
+    def held(x, floor):
+        x = torch.nn.functional.pad(x, (0, -x.numel() % 256)).view(-1, 256)
+        top = x.abs().amax(1, keepdim=True)
+        live = top >= 2.0 ** -100
+        r = torch.where(live, x / torch.where(live, top, 1.0) * 448.0, 0.0)
+        if floor:
+            r = torch.where(r > 0, r.clamp(min=2.0 ** -9), r)
+        return r.to(torch.float8_e4m3fn).flatten(), torch.where(live, top * torch.tensor(1.0 / 448.0, device=x.device), 0.0)[:, 0]
+
+    n = g.numel()
+    g = g.float() * scale
+    wide = lambda code, s: (code.float().view(-1, 256) * s[:, None]).flatten()[:n]  # noqa: E731
+    m, v = wide(m, ms), wide(v, vs)
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * (v * v) + (1 - betas[1]) * g * g
+    return *held(m, False), *held(v.sqrt(), True)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_codes_follow_fp32_arithmetic_to_the_bit(kind):
+    """Ten steps of 2 million elements: any other rounding on the way would turn some codes, and these the
+    scales of later steps."""
+    n = 2_000_001
+    params, gen = [torch.zeros(n, device="cuda")], torch.Generator(device="cuda").manual_seed(0)
+    state, scale = readout.adamw_state(params, bits=8), torch.tensor([0.7], device="cuda")
+    size = torch.exp(torch.randn(n, generator=gen, device="cuda")) * 1e-3
+    m, v, ms, vs = (x.clone() for x in (state.m, state.v, state.m_scale, state.v_scale))
+    for _ in range(10):
+        g = (size * torch.randn(n, generator=gen, device="cuda")).to(kind)
+        m, ms, v, vs = follow(m, v, ms, vs, g, scale, (0.9, 0.999))
+        readout.adamw_step(params, [g], state, lr=1e-3, grad_scale=scale)
+        assert torch.equal(state.m.view(torch.uint8), m.view(torch.uint8))
+        assert torch.equal(state.v.view(torch.uint8), v.view(torch.uint8))
+        assert torch.equal(state.m_scale, ms) and torch.equal(state.v_scale, vs)
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_what_is_not_finite(bits):
     """It reaches its element, in 8 bits no further than its 256."""
