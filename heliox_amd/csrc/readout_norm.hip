@@ -1,8 +1,8 @@
 // Layer norm of rows, and its gradient.
 //
 // A row is read once, held in registers, and written once: kGroup lanes hold it in kV pieces of
-// 16 bytes each.  The variance is the mean square of differences from the mean (two sums over the
-// held row, not the difference of two large numbers).  Workgroups walk over the rows, so that
+// 16 bytes each.  The variance is the mean square of differences from a first mean, which their own
+// sum then corrects (sums over the held row, not the difference of two large numbers).  Workgroups walk over the rows, so that
 // weight and bias stay in registers too, and the gradients of both are added there: each
 // workgroup writes its sums once, a second launch adds those up in a fixed order.  (Few rows are
 // read a second time instead, by columns.)  Both are bound by the rows' bytes: 32768 x 4096 in
@@ -107,12 +107,24 @@ struct Place {
     }
 };
 
+// From the sums of the differences from a first mean, and of their squares: what that mean was off by
+// (a sum of 500 voltages near -65 is off by their own 2^-24 many times over, their differences' is not)
+// and 1 / sqrt(variance + eps).
+struct Spread {
+    float rest, rstd;
+    __device__ __forceinline__ Spread(const float (&off)[2], const NormArgs& A) {
+        rest = off[0] * A.per_width;
+        const float variance = off[1] * A.per_width - rest * rest;
+        rstd = 1.f / sqrtf((variance < 0.f ? 0.f : variance) + A.eps);
+    }
+};
+
 template <class T, int kE, int kGroup, int kV, bool kRagged>
 __global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup) k_norm(NormArgs A) {
     constexpr int kThreads = kGroup < 256 ? 256 : kGroup, kRows = kThreads / kGroup;
     using Vec = typename Piece<T, kE>::Vec;
     using At = Place<kE, kGroup, kRagged>;
-    __shared__ float sh[2][16];
+    __shared__ float sh[2][2 * 16];
     const int lane = threadIdx.x % kGroup;
     float w[kV][kE], b[kV][kE];
 #pragma unroll
@@ -136,7 +148,7 @@ __global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup) k_norm(NormArgs A
     };
     if (row < A.rows) fetch(row);
     for (; row < A.rows; row += step) {
-        float v[kV][kE], sum[1] = {0.f}, square[1] = {0.f};
+        float v[kV][kE], sum[1] = {0.f}, off[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kV; ++k) {
             const At at(A.width, lane, k);
@@ -153,13 +165,15 @@ __global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup) k_norm(NormArgs A
 #pragma unroll
             for (int i = 0; i < kE; ++i) {
                 v[k][i] -= mean;
-                square[0] += at.here && i >= at.skip ? v[k][i] * v[k][i] : 0.f;
+                off[0] += at.here && i >= at.skip ? v[k][i] : 0.f;
+                off[1] += at.here && i >= at.skip ? v[k][i] * v[k][i] : 0.f;
             }
         }
-        group_sum<kGroup>(square, sh[1]);
-        const float rstd = 1.f / sqrtf(square[0] * A.per_width + A.eps);
+        group_sum<kGroup>(off, sh[1]);
+        const Spread spread(off, A);
+        const float rest = spread.rest, rstd = spread.rstd;
         if (lane == 0) {
-            A.mean[row] = mean;
+            A.mean[row] = mean + rest;
             A.rstd[row] = rstd;
         }
         T* y = static_cast<T*>(A.y) + row * A.y_stride;
@@ -167,7 +181,7 @@ __global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup) k_norm(NormArgs A
         for (int k = 0; k < kV; ++k) {
             const At at(A.width, lane, k);
 #pragma unroll
-            for (int i = 0; i < kE; ++i) v[k][i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
+            for (int i = 0; i < kE; ++i) v[k][i] = fmaf((v[k][i] - rest) * rstd, w[k][i], b[k][i]);
             if (at.here) store<T, kE>(y + at.at, v[k]);
         }
     }
@@ -299,16 +313,16 @@ __device__ __forceinline__ void load(const T* from, float* v) {
 
 template <class T>
 __global__ void __launch_bounds__(kWide) k_norm_wide(NormArgs A) {
-    __shared__ float sh[2][16];
+    __shared__ float sh[2][2 * 16];
     for (long long row = blockIdx.x; row < A.rows; row += gridDim.x) {
         const T* x = static_cast<const T*>(A.x) + row * A.x_stride;
         T* y = static_cast<T*>(A.y) + row * A.y_stride;
-        float sum[1] = {0.f}, square[1] = {0.f};
+        float sum[1] = {0.f}, off[2] = {0.f, 0.f};
         each_element<T>(A.width, [&](auto e, int j) {
             constexpr int kE = decltype(e)::value;
             float v[kE], s = 0.f;
             load<T, kE>(x + j, v);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) s += v[i];
             sum[0] += s;
         });
@@ -316,28 +330,33 @@ __global__ void __launch_bounds__(kWide) k_norm_wide(NormArgs A) {
         const float mean = sum[0] * A.per_width;
         each_element<T>(A.width, [&](auto e, int j) {
             constexpr int kE = decltype(e)::value;
-            float v[kE], s = 0.f;
+            float v[kE], s = 0.f, d = 0.f;
             load<T, kE>(x + j, v);
-    #pragma unroll
-            for (int i = 0; i < kE; ++i) s = fmaf(v[i] - mean, v[i] - mean, s);
-            square[0] += s;
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                d += v[i] - mean;
+                s = fmaf(v[i] - mean, v[i] - mean, s);
+            }
+            off[0] += d;
+            off[1] += s;
         });
-        group_sum<kWide>(square, sh[1]);
-        const float rstd = 1.f / sqrtf(square[0] * A.per_width + A.eps);
+        group_sum<kWide>(off, sh[1]);
+        const Spread spread(off, A);
+        const float rest = spread.rest, rstd = spread.rstd;
         if (threadIdx.x == 0) {
-            A.mean[row] = mean;
+            A.mean[row] = mean + rest;
             A.rstd[row] = rstd;
         }
         each_element<T>(A.width, [&](auto e, int j) {
             constexpr int kE = decltype(e)::value;
             float v[kE], w[kE], b[kE];
             load<T, kE>(x + j, v);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) w[i] = 1.f, b[i] = 0.f;
             if (A.weight) load_weights<kE>(A.weight, A.weight_type, j, w);
             if (A.bias) load_weights<kE>(A.bias, A.weight_type, j, b);
-    #pragma unroll
-            for (int i = 0; i < kE; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
+#pragma unroll
+            for (int i = 0; i < kE; ++i) v[i] = fmaf((v[i] - mean - rest) * rstd, w[i], b[i]);
             store<T, kE>(y + j, v);
         });
     }
@@ -358,10 +377,10 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
             float w[kE];
             load<T, kE>(x + j, n);
             load<T, kE>(dy + j, g);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) w[i] = 1.f;
             if (A.weight) load_weights<kE>(A.weight, A.weight_type, j, w);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) {
                 n[i] = (n[i] - mean) * rstd;
                 g[i] *= w[i];
@@ -371,7 +390,7 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
             constexpr int kE = decltype(e)::value;
             float n[kE], g[kE], s = 0.f, sn = 0.f;
             terms(e, j, n, g);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) {
                 s += g[i];
                 sn = fmaf(g[i], n[i], sn);
@@ -385,7 +404,7 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
             constexpr int kE = decltype(e)::value;
             float n[kE], g[kE];
             terms(e, j, n, g);
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < kE; ++i) n[i] = rstd * (g[i] - mean_g - n[i] * mean_gn);
             store<T, kE>(dx + j, n);
         });

@@ -107,6 +107,17 @@ def test_voltages_far_from_zero():
     check(x, normal(1, 500, shift=1.0), normal(2, 500), normal(3, 20, 500))
 
 
+@pytest.mark.parametrize("width", [60, 500, 3000, 40001])
+def test_a_mean_far_from_zero_keeps_its_bits(width):
+    """Rows at -65 of spread 8: the mean is off by what its own corrected sum is, not by what the sum of the
+    values is: half a step of 65 and a few of the spread, in all 8 halves of a step of either."""
+    x = normal(0, 40, width, scale=8.0, shift=-65.0)
+    y, mean, _ = readout.layer_norm(x)
+    want = formulas(x, None, None, x)
+    assert bool(((mean.cpu().double() - want["mean"]).abs() <= F32 * 65 * 1.5 + 8 * F32 * 8).all())
+    assert float((y.cpu().double() - want["y"]).norm()) <= 4 * F32 * float(want["y"].norm())
+
+
 def test_views_and_shapes():
     wide = normal(0, 5, 7, 260, dtype=torch.bfloat16)
     x = wide[..., 3:103]                                       # rows that start at odd addresses
