@@ -241,13 +241,13 @@ hipError_t adamw_launch(const hx_adamw_args& A) {
     L.rates = reinterpret_cast<const Rates*>(A.step + 1);
     k_count<<<1, 1, 0, st>>>(A.step, std::log(A.beta1), std::log(A.beta2), L.lr, L.lr_ptr);
     hipError_t e = hipGetLastError();
-    // tensors of one pair of types share launches
+    // tensors of one pair of types share launches; none follows one that failed
     for (int64_t type = HX_F32; type <= HX_BF16; ++type)
         for (int64_t grad = HX_F32; grad <= HX_BF16; ++grad) {
             long long groups = 0;
             L.count = 0;
             auto flush = [&] {
-                if (!L.count || e != hipSuccess) return;
+                if (!L.count) return;
                 e = with_type(type, [&](auto p) {
                     return with_type(grad, [&](auto g) {
                         using P = decltype(p);
@@ -259,7 +259,7 @@ hipError_t adamw_launch(const hx_adamw_args& A) {
                 groups = 0;
                 L.count = 0;
             };
-            for (int64_t i = 0; i < A.count; ++i) {
+            for (int64_t i = 0; i < A.count && e == hipSuccess; ++i) {
                 const long long n = A.elements[i], more = (n + kChunk - 1) / kChunk;
                 if (A.types[i] != type || A.grad_types[i] != grad || !n) continue;
                 if (L.count == kTensors || groups + more > (1 << 23)) flush();
@@ -267,7 +267,7 @@ hipError_t adamw_launch(const hx_adamw_args& A) {
                                        static_cast<float>(A.weight_decays[i])};
                 groups += more;
             }
-            flush();
+            if (e == hipSuccess) flush();
         }
     return e;
 }
