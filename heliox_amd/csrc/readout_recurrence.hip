@@ -4,7 +4,8 @@
 // A run of steps takes what enters it to P h + Y (P the product of the a = 1 - z, Y what the run
 // makes of nothing), and runs join: that is the scan.  What is left of P and h is h - z h in one
 // rounding, not a h: a channel that remembers for a thousand steps has a = 0.999, whose last bit
-// counts a thousand times, while z keeps all of its bits.
+// counts a thousand times, while z keeps all of its bits.  Where the gate shuts it is the other way
+// round: there z is nearly 1, and a h with a = e^gate z has the bits.
 //
 // Lanes lie along channels, kC each, so that a step's row is read and written as it lies in
 // memory; a group of kL lanes (a wave; fewer, where there are few channels) takes kU steps in
@@ -16,7 +17,7 @@
 // right as h does from the left, and both meet in the run's registers.
 //
 // Bound by memory, at 4.4 to 5.2 TB/s of what the passes move (a copy: 4.9): 8 x 4096 x 2048 in bf16
-// forward 88 us (402 MB once), backward 213 (1074 MB: inputs twice); 65536 x 512 in fp32 forward,
+// forward 89 us (402 MB once), backward 217 (1074 MB: inputs twice); 65536 x 512 in fp32 forward,
 // cut, 135 us (671 MB).
 #include "readout.h"
 
@@ -75,9 +76,48 @@ __device__ __forceinline__ float rise(float gate) { return __builtin_amdgcn_exp2
 // 1 / (1 + e^gate) from e^gate
 __device__ __forceinline__ float opening(float e) { return __builtin_amdgcn_rcpf(1.f + e); }
 
-// What an opening z leaves of h, and h moved by it towards x.
-__device__ __forceinline__ float left(float h, float z) { return fmaf(-z, h, h); }
-__device__ __forceinline__ float moved(float h, float z, float x) { return fmaf(z, x, left(h, z)); }
+// Gates up to here shut: at -2 z's own error, 3 halves of a step, is 26 of them in a = 1 - z, as much
+// as e^gate's argument is off by at -18.
+constexpr float kShut = -2.f;
+
+// A step's opening z and what it keeps, a.  Waves whose steps do not shut (kShuts false: see any_shuts)
+// go without what that takes, with the same results: 8 x 4096 x 2048 with gradient 313 us, with it
+// everywhere 321, where steps shut in every wave 322.
+template <bool kShuts>
+struct Opening {
+    float z, a;
+    bool shut;
+    __device__ __forceinline__ Opening() {}
+    __device__ __forceinline__ Opening(float gate, bool live) {
+        const float e = rise(gate);
+        z = live ? opening(e) : 0.f;
+        a = !live || gate > 80.f ? 1.f : e * z;
+        shut = kShuts && live && gate <= kShut;
+    }
+    // what is left of h, and h moved towards x
+    __device__ __forceinline__ float left(float h) const { return fmaf(shut ? a : -z, h, shut ? 0.f : h); }
+    __device__ __forceinline__ float moved(float h, float x) const { return fmaf(z, x, left(h)); }
+};
+
+// Whether some of the wave's gates are kShut or less: of the numbers' bits, as whole numbers without a
+// sign, those of negative ones are the largest, the more so the further from zero.
+template <int kC, class Vec, int kN>
+__device__ __forceinline__ bool any_shuts(const Vec (&gates)[kN]) {
+    unsigned most = 0;
+#pragma unroll
+    for (int u = 0; u < kN; ++u)
+#pragma unroll
+        for (int c = 0; c < kC; ++c) most = max(most, __float_as_uint(part<Vec, kC>(gates[u], c)));
+    return __any(most >= __float_as_uint(kShut));
+}
+
+// Calls f(whether all steps are within the length, whether some shut).
+template <class F>
+__device__ __forceinline__ void with_kind(bool whole, bool shuts, F f) {
+    if (!whole) f(std::false_type{}, std::true_type{});
+    else if (shuts) f(std::true_type{}, std::true_type{});
+    else f(std::true_type{}, std::false_type{});
+}
 
 // A workgroup's place: sequence, segment, channels.
 struct Where {
@@ -190,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceA
         for (int tile = first; tile < last; tile += kTile, turn ^= 1) {
             const int t = tile + group * kU;
             float p[kU][kC], y[kU][kC];
-            auto run = [&](auto whole) {
+            auto run = [&](auto whole, auto shuts) {
                 float pp[kC], yy[kC];
 #pragma unroll
                 for (int c = 0; c < kC; ++c) pp[c] = 1.f, yy[c] = 0.f;
@@ -199,15 +239,21 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_walk(RecurrenceA
                     const bool live = decltype(whole)::value || t + u < w.length;
 #pragma unroll
                     for (int c = 0; c < kC; ++c) {
-                        const float z = live ? opening(rise(part<Vec, kC>(g[u], c))) : 0.f;
+                        const Opening<decltype(shuts)::value> open(part<Vec, kC>(g[u], c), live);
                         const float v = live ? part<Vec, kC>(x[u], c) : 0.f;
-                        p[u][c] = pp[c] = left(pp[c], z);
-                        y[u][c] = yy[c] = moved(yy[c], z, v);
+                        p[u][c] = pp[c] = open.left(pp[c]);
+                        y[u][c] = yy[c] = open.moved(yy[c], v);
                     }
                 }
             };
-            if (t + kU <= w.length) run(std::true_type{});
-            else run(std::false_type{});
+            // With one channel a lane asking after the run, which is done over where steps shut, keeps the
+            // loads' order (8 x 4096 x 2048: 91 us, asking first 101; two channels, 13 x 777 x 601: 13.1 and 12.1).
+            if (kC == 1 && t + kU <= w.length) {
+                run(std::true_type{}, std::false_type{});
+                if (any_shuts<kC>(g)) run(std::true_type{}, std::true_type{});
+            } else {
+                with_kind(t + kU <= w.length, any_shuts<kC>(g), run);
+            }
             if (tile + kTile < last) {
                 fetch<T, kC>(x, A.x, A.x_stride, w, t + kTile);
                 fetch<T, kC>(g, A.gate, A.gate_stride, w, t + kTile);
@@ -271,20 +317,19 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_segments(Recurre
             fetch<T, kC>(x, A.x, A.x_stride, w, t);
             fetch<T, kC>(g, A.gate, A.gate_stride, w, t);
             if constexpr (kGrad) fetch<T, kC>(d, A.grad_o, A.grad_o_stride, w, t);
-            auto run = [&](auto whole) {
+            auto run = [&](auto whole, auto shuts) {
 #pragma unroll
                 for (int u = 0; u < kU; ++u)
                     if (decltype(whole)::value || t + u < last)
 #pragma unroll
                         for (int c = 0; c < kC; ++c) {
-                            const float z = opening(rise(part<Vec, kC>(g[u], c)));
-                            p[c] = left(p[c], z);
-                            y[c] = moved(y[c], z, part<Vec, kC>(x[u], c));
+                            const Opening<decltype(shuts)::value> open(part<Vec, kC>(g[u], c), true);
+                            p[c] = open.left(p[c]);
+                            y[c] = open.moved(y[c], part<Vec, kC>(x[u], c));
                             if constexpr (kGrad) r[c] = fmaf(p[c], part<Vec, kC>(d[u], c), r[c]);
                         }
             };
-            if (t + kU <= last) run(std::true_type{});
-            else run(std::false_type{});
+            with_kind(t + kU <= last, any_shuts<kC>(g), run);
         }
         __syncthreads();
 #pragma unroll
@@ -374,28 +419,33 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
         w.entering<kJoins>(A, h);
         w.leaving<kJoins>(A, back);
         float z[kU][kC], a[kU][kC], p[kC], y[kC], r[kC];
+        // an opening again, from what is held of it
+        auto held = [&](auto shuts, int u, int c, bool live) {
+            Opening<decltype(shuts)::value> open;
+            open.z = z[u][c], open.a = a[u][c];
+            open.shut = decltype(shuts)::value && live && part<Vec, kC>(g[u], c) <= kShut;
+            return open;
+        };
 #pragma unroll
         for (int c = 0; c < kC; ++c) p[c] = 1.f, y[c] = r[c] = 0.f;
-        auto run = [&](auto whole) {
+        auto run = [&](auto whole, auto shuts) {
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 const bool live = decltype(whole)::value || t + u < w.length;
 #pragma unroll
                 for (int c = 0; c < kC; ++c) {
-                    const float gate = part<Vec, kC>(g[u], c), e = rise(gate);
-                    z[u][c] = live ? opening(e) : 0.f;
-                    a[u][c] = !live || gate > 80.f ? 1.f : e * z[u][c];
-                    p[c] = left(p[c], z[u][c]);
+                    const Opening<decltype(shuts)::value> open(part<Vec, kC>(g[u], c), live);
+                    z[u][c] = open.z, a[u][c] = open.a;
+                    p[c] = open.left(p[c]);
                     if (live) {                  // what lies past the length may be no number
-                        y[c] = moved(y[c], z[u][c], part<Vec, kC>(x[u], c));
+                        y[c] = open.moved(y[c], part<Vec, kC>(x[u], c));
                         r[c] = fmaf(p[c], part<Vec, kC>(d[u], c), r[c]);
                     }
                 }
             }
         };
-        const bool whole_group = t + kU <= w.length;
-        if (whole_group) run(std::true_type{});
-        else run(std::false_type{});
+        const bool whole_group = t + kU <= w.length, some_shut = any_shuts<kC>(g);
+        with_kind(whole_group, some_shut, run);
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
@@ -414,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
             if (v > group)
 #pragma unroll
                 for (int c = 0; c < kC; ++c) back[c] = fmaf(ends[v][c][lane], back[c], ends[v][2 * kC + c][lane]);
-        auto out = [&](auto whole) {
+        auto out = [&](auto whole, auto shuts) {
             float off[kU][kC];                   // h_{t-1} - x_t
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
@@ -423,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
                 for (int c = 0; c < kC; ++c) {
                     const float v = part<Vec, kC>(x[u], c);
                     off[u][c] = h[c] - v;
-                    if (live) h[c] = moved(h[c], z[u][c], v);
+                    if (live) h[c] = held(shuts, u, c, live).moved(h[c], v);
                 }
             }
             T* dx = static_cast<T*>(A.grad_x) + (w.batch * A.time + t) * A.channels;
@@ -437,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
                     const float l = part<Vec, kC>(d[u], c) + back[c], zl = z[u][c] * l;
                     vx[c] = live ? zl : 0.f;
                     vg[c] = live ? a[u][c] * zl * off[u][c] : 0.f;
-                    if (live) back[c] = left(l, z[u][c]);
+                    if (live) back[c] = held(shuts, u, c, live).left(l);
                 }
                 if (decltype(whole)::value || t + u < A.time) {
                     *reinterpret_cast<Vec*>(dx + static_cast<long long>(u) * A.channels + w.channel) = packed<T, kC>(vx);
@@ -445,8 +495,7 @@ __global__ void __launch_bounds__(kThreads, kL == 64 ? 4 : 2) k_grad(RecurrenceA
                 }
             }
         };
-        if (whole_group) out(std::true_type{});
-        else out(std::false_type{});
+        with_kind(whole_group, some_shut, out);
         if ((kJoins ? w.segment == 0 : A.segments == 1) && A.grad_initial && group == 0)
 #pragma unroll
             for (int c = 0; c < kC; ++c) A.grad_initial[w.batch * A.channels + w.channel + c] = back[c];
@@ -475,7 +524,7 @@ __global__ void __launch_bounds__(256) k_step(RecurrenceArgs A, float* states, c
         Held h = *at;
 #pragma unroll
         for (int v = 0; v < kV; ++v) {
-            h.v[v] = moved(h.v[v], opening(rise(to_f32(gs.v[v]))), to_f32(xs.v[v]));
+            h.v[v] = Opening<true>(to_f32(gs.v[v]), true).moved(h.v[v], to_f32(xs.v[v]));
             out.v[v] = from_f32<T>(h.v[v]);
         }
         *at = h;
