@@ -2,8 +2,8 @@
 //
 // A workgroup takes kChunk elements of one tensor, a wave kBlocks blocks of 256 in a row, four
 // elements a lane in each, so that every array streams through as it lies in memory: bound by
-// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 314 us, 4.8 TB/s; with four blocks a wave
-// 327, with one 333).  The tensors of a launch are listed in its arguments; a workgroup finds its own
+// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 315 us, 4.8 TB/s, 332 where codes are rounded
+// by chance; with four blocks a wave 327, with one 333).  The tensors of a launch are listed in its arguments; a workgroup finds its own
 // by one comparison a lane.  The count of steps, and what follows from it alone, is made by a
 // first launch of one thread, on the device, so that a captured step counts on.
 //
@@ -11,6 +11,15 @@
 // block: its maximum is a reduction of the wave).  Of v the root is held: half of v's exponents, so that
 // its 3 bits of mantissa are off by 2^-4 in the step and not in its square.  A root that would
 // round to zero is held as the least number instead: a step that divides by too little has no bound.
+//
+// A moment that moves by less than half a step of its code would never move if it were rounded to
+// nearest: with beta2 = 0.999 a root falls by 0.05% a step, and codes are 6 to 12% apart (5000 steps
+// after 16384 gradients' sizes changed places a third of the steps were off by more than 2).  So
+// a code is rounded up as often as its number is near the upper one, by bits made of the
+// step's count and the element's place: the moments follow on average (of those steps 0.3% are off by more
+// than 2), and the same calls give the same state.  The first steps, as many as the longer memory
+// spans, 1 / (1 - beta), are to nearest: moments of few gradients move by whole codes, and what sticks all
+// the same is forgotten in as many steps more.
 #include "readout.h"
 
 #include <algorithm>
@@ -41,6 +50,8 @@ struct AdamwArgs {
     void *m, *v;
     float *m_scale, *v_scale;
     float beta1, beta2, less1, less2, eps, lr, grad_scale;     // less: 1 - beta
+    const int64_t* step;
+    int64_t nearest;                                           // steps that round codes to nearest
     const float *grad_scale_ptr, *lr_ptr;
     const Rates* rates;
 };
@@ -117,7 +128,33 @@ __device__ __forceinline__ int pack(Float4 x) {
     return __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], low, true);
 }
 
-// Codes of a block, relative to its largest; that over 448 is returned.
+// 32 bits for each four elements of a step: a sum of place and count times odd numbers (the first bits
+// of the fractions of the square roots of 2, 3, 11 and 17), mixed by shifts and products.  The four turn
+// them by 8 bits each and take the upper 16 for the root, the lower for m: what they share
+// does not bias either.
+constexpr unsigned kRoot2 = 0x6a09e667u, kRoot3 = 0xbb67ae85u, kRoot11 = 0x510e527fu, kRoot17 = 0x1f83d9abu;
+__device__ __forceinline__ unsigned mixed(unsigned h) {
+    h = (h ^ h >> 16) * kRoot11;
+    h = (h ^ h >> 15) * kRoot17;
+    return h ^ h >> 16;
+}
+
+// Each rounded up where the 20 bits that its code drops and 20 of chance, of which 16 are the element's
+// own, add up to 2^20.  16 tell changes of 2^-16 of a code's step, as roots' with beta2 up to 0.9999.
+template <bool kHigh>
+__device__ __forceinline__ int pack(Float4 x, unsigned bits) {
+    auto chance = [&](int i) {
+        const unsigned one = __builtin_rotateleft32(bits, 8 * i);
+        return (kHigh ? one & 0xffff0000u : one << 16) | 0x8000u;
+    };
+    int code = __builtin_amdgcn_cvt_sr_fp8_f32(x[0], chance(0), 0, 0);
+    code = __builtin_amdgcn_cvt_sr_fp8_f32(x[1], chance(1), code, 1);
+    code = __builtin_amdgcn_cvt_sr_fp8_f32(x[2], chance(2), code, 2);
+    return __builtin_amdgcn_cvt_sr_fp8_f32(x[3], chance(3), code, 3);
+}
+
+// Codes of a block, relative to its largest; that over 448 is returned.  `bits`: of these four elements, where
+// codes are not rounded to nearest.
 //
 // A number next to the middle of two codes goes to one or the other by its last bit, and a block's
 // largest number that does so moves the scale of all by a sixteenth.  So that a state's way can be
@@ -125,7 +162,7 @@ __device__ __forceinline__ int pack(Float4 x) {
 // the quotient x / top is the correctly rounded one: from the correctly rounded 1 / top, corrected by
 // the exact remainder (Markstein's division).
 template <bool kRoot>
-__device__ __forceinline__ float quantise(Float4 x, int& code) {
+__device__ __forceinline__ float quantise(Float4 x, int& code, bool dither, unsigned bits) {
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[i]));
@@ -139,7 +176,7 @@ __device__ __forceinline__ float quantise(Float4 x, int& code) {
         x[i] = q * kTop8;
         if (kRoot && x[i] > 0.f && x[i] < kLeast8) x[i] = kLeast8;
     }
-    code = pack(x);
+    code = dither ? pack<kRoot>(x, bits) : pack(x);
     return live ? top * (1.f / kTop8) : 0.f;
 }
 
@@ -156,9 +193,12 @@ __global__ void __launch_bounds__(kThreads) k_adamw(AdamwArgs A) {
     const float lr = A.lr_ptr ? *A.lr_ptr : A.lr, clip = A.grad_scale_ptr ? *A.grad_scale_ptr : A.grad_scale;
     const Rates rates = *A.rates;
     const float keep = 1.f - lr * t.decay;
+    const bool dither = kBits == 8 && *A.step > A.nearest;
     P* const p = static_cast<P*>(t.param) + base + lane * 4;
     const G* const g = static_cast<const G*>(t.grad) + base + lane * 4;
-    const long long at = t.start + base, left0 = t.elements - base;     // elements from the wave's first on
+    const long long at = t.start + base;
+    const unsigned seed = static_cast<unsigned>(at / 4 + lane) * kRoot2 + static_cast<unsigned>(*A.step) * kRoot3;
+    const long long left0 = t.elements - base;     // elements from the wave's first on
     if (left0 <= 0) return;
     auto run = [&](auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
@@ -207,7 +247,9 @@ __global__ void __launch_bounds__(kThreads) k_adamw(AdamwArgs A) {
                 *reinterpret_cast<Float4*>(static_cast<float*>(A.m) + at + b * kBlock + lane * 4) = mv[b];
                 *reinterpret_cast<Float4*>(static_cast<float*>(A.v) + at + b * kBlock + lane * 4) = vv[b];
             } else {
-                const float m_scale = quantise<false>(mv[b], mc[b]), v_scale = quantise<true>(root, vc[b]);
+                const unsigned bits = dither ? mixed(seed + b * (kBlock / 4) * kRoot2) : 0;
+                const float m_scale = quantise<false>(mv[b], mc[b], dither, bits);
+                const float v_scale = quantise<true>(root, vc[b], dither, bits);
                 *reinterpret_cast<int*>(static_cast<char*>(A.m) + at + b * kBlock + lane * 4) = mc[b];
                 *reinterpret_cast<int*>(static_cast<char*>(A.v) + at + b * kBlock + lane * 4) = vc[b];
                 if (lane == 0) {
@@ -239,6 +281,7 @@ hipError_t adamw_launch(const hx_adamw_args& A) {
     L.grad_scale = static_cast<float>(A.grad_scale);
     L.grad_scale_ptr = A.grad_scale_ptr, L.lr_ptr = A.lr_ptr;
     L.rates = reinterpret_cast<const Rates*>(A.step + 1);
+    L.step = A.step, L.nearest = std::llround(1. / (1. - std::max(A.beta1, A.beta2)));
     k_count<<<1, 1, 0, st>>>(A.step, std::log(A.beta1), std::log(A.beta2), L.lr, L.lr_ptr);
     hipError_t e = hipGetLastError();
     // tensors of one pair of types share launches; none follows one that failed

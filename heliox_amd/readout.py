@@ -763,7 +763,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     norm) are numbers, or fp32 tensors of one on the GPU, which a captured step reads anew at every
     replay, as it does the state's step.
 
-    With 8 bits the moments are rounded after the step has used them; a gradient that is not finite
+    With 8 bits the moments are rounded after the step has used them: to nearest while t is at most
+    1 / (1 - max(betas)), later up or down by a hash of t and the element, so that they follow changes
+    smaller than their codes' steps (the same calls give the same state); a gradient that is not finite
     reaches the 256 elements that share its scale.  Parameters that overlap each other or a gradient
     are refused."""
     if not isinstance(state, AdamWState):

@@ -720,8 +720,11 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * bits 8: m and sqrt(v) as 8-bit floating-point numbers (4 bits of exponent, 3 of mantissa, no
  * infinity: largest 448), each 256 elements relative to m_scale and v_scale, the largest of them
  * / 448 (fp32; 0, and the numbers 0, where that largest is under 2^-100), rounded to nearest even (m, v,
- * their root and the quotient by the largest are fp32, rounded operation by operation, left to right);
- * a root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
+ * their root and the quotient by the largest are fp32, rounded operation by operation, left to right)
+ * for the first 1 / (1 - max(beta1, beta2)) steps, which is how many the moments remember; from then on
+ * up or down, as often as they are near either side, by a hash of t and of the element's place
+ * (rounded to nearest, moments that move by less than half a step of their codes would stand still):
+ * the same calls give the same state.  A root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
  * that is not finite reaches its block's 256 elements in 8 bits.
  * Tensors come in the order of their starts, each within `moments`, its last 256 filled up with
  * elements that belong to none (kept zero).  The parameters of a call do not overlap each other or
