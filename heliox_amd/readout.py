@@ -665,13 +665,41 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
     return token, logprob
 
 
+def _held(name: str, doc: str) -> property:
+    """A tensor of a state: what is assigned is copied into it, for its address is what a step, and a captured
+    one, writes to."""
+    def get(state):
+        return getattr(state, name)
+
+    def put(state, x):
+        here = getattr(state, name)
+        if here is None and x is None:
+            return
+        if not isinstance(x, torch.Tensor) or here is None:
+            raise TypeError(f"{name[1:]} of a state in {state.bits} bits is "
+                            f"{'None' if here is None else 'a tensor'}, got {type(x).__name__}")
+        if x.dtype is not here.dtype:
+            raise TypeError(f"{name[1:]} is {here.dtype}, got {x.dtype}")
+        if x.shape != here.shape:
+            raise ValueError(f"{name[1:]} has shape {tuple(here.shape)}, got {tuple(x.shape)}")
+        here.copy_(x)
+
+    return property(get, put, doc=doc)
+
+
 class AdamWState:
     """What adamw_step keeps for a list of parameters, made by adamw_state.  Tensor i's moments are
     elements starts[i] to starts[i] + sizes[i] of m and v; starts are multiples of 256.
 
     bits 32: m and v are fp32.  bits 8: m and the root of v are float8_e4m3fn, each 256 elements
     relative to m_scale and v_scale (fp32, one for each 256).  step, int64 on the GPU, counts the
-    steps taken.  All of them may be saved, and copied into another state of the same parameters."""
+    steps taken.  All of them may be saved, and copied into another state of the same parameters;
+    a tensor that is assigned to one of them, from whichever device, is copied (step: a whole number too)."""
+
+    m = _held("_m", "first moments")
+    v = _held("_v", "second moments; with 8 bits their roots")
+    m_scale = _held("_m_scale", "what codes of m are relative to; None with 32 bits")
+    v_scale = _held("_v_scale", "the same of v")
 
     def __init__(self, sizes: Sequence[int], bits: int, device: int):
         self.bits, self.device = bits, device
@@ -682,10 +710,38 @@ class AdamWState:
             whole += -(-n // 256) * 256
         on = {"device": f"cuda:{device}"}
         kind, held = (torch.float32, torch.float32) if bits == 32 else (torch.float8_e4m3fn, torch.uint8)
-        self.m, self.v = (torch.zeros(whole, dtype=held, **on).view(kind) for _ in range(2))
-        self.m_scale, self.v_scale = (torch.zeros(whole // 256, **on) if bits == 8 else None for _ in range(2))
+        self._m, self._v = (torch.zeros(whole, dtype=held, **on).view(kind) for _ in range(2))
+        self._m_scale, self._v_scale = (torch.zeros(whole // 256, **on) if bits == 8 else None for _ in range(2))
+        # the count, and room that the library uses
         self._count = torch.zeros(2, dtype=torch.int64, **on)
-        self.step = self._count[:1]
+
+    @property
+    def step(self) -> torch.Tensor:
+        """Steps taken, (1,) int64."""
+        return self._count[:1]
+
+    @step.setter
+    def step(self, x) -> None:
+        if not isinstance(x, torch.Tensor):
+            x = _whole(x, "step")
+            if x < 0:
+                raise ValueError(f"step has to be at least 0, got {x}")
+            self._count[0] = x
+        elif x.dtype is not torch.int64 or x.numel() != 1:
+            raise TypeError(f"step has to be one int64, got {tuple(x.shape)} of {x.dtype}")
+        else:
+            self._count[:1].copy_(x.reshape(1))
+
+    def _tensors(self) -> tuple:
+        """m, v, their scales and the count, of the sizes and on the device that they were made with."""
+        whole = self.starts[-1] + -(-self.sizes[-1] // 256) * 256
+        scales = whole // 256 if self.bits == 8 else 0
+        all_ = self._m, self._v, self._m_scale, self._v_scale, self._count
+        for x, n in zip(all_, (whole, whole, scales, scales, 2)):
+            if x is not None and (x.get_device() != self.device or x.numel() != n or not x.is_contiguous()):
+                raise ValueError(f"the state's tensors were changed: {tuple(x.shape)} on {x.device} where {n} contiguous "
+                                 f"elements on cuda:{self.device} belong")
+        return all_
 
 
 # What is asked of hundreds of tensors in a step is asked by map, a tenth of a loop's time each.
@@ -794,10 +850,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
                          + ", ".join(f"{tuple(g.shape)} for {tuple(p.shape)}" for p, g in zip(params, grads) if p.shape != g.shape))
     if not all(map(_whole_of, grads)):
         grads = [g.contiguous() for g in grads]
+    m, v, m_scale, v_scale, count = state._tensors()
     lists = kinds, grad_kinds, array("Q", map(_address_of, params)), array("Q", map(_address_of, grads)), sizes, starts, decays
     _call("hx_adamw_step", device, _ADAMW.pack(
-        state.bits, len(params), *[a.buffer_info()[0] for a in lists], state.m.data_ptr(), state.v.data_ptr(),
-        _ptr(state.m_scale), _ptr(state.v_scale), state.m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
-        lr_ptr, state._count.data_ptr(), _stream(device)))
+        state.bits, len(params), *[a.buffer_info()[0] for a in lists], m.data_ptr(), v.data_ptr(),
+        _ptr(m_scale), _ptr(v_scale), m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
+        lr_ptr, count.data_ptr(), _stream(device)))
     # what autograd kept of the old values is out of date (inference tensors are never kept)
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
