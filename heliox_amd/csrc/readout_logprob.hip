@@ -354,7 +354,15 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
         if (kTop && quota <= 64) bound = __shfl(mine, __ffsll(__ballot(lane < kWaves && above == need - 1)) - 1);
     }
     float base = most == -INFINITY ? 0.f : most, limit = most == -INFINITY ? -INFINITY : base + kFar / A.cold;
+    // z and s of kAhead pieces in fp32, at most 8 terms and 4 pieces added one after another, of all in 64 bits:
+    // a thread of a long row adds thousands of terms, and where these are alike their roundings are too.
     float z = 0.f, s = 0.f;
+    double all_z = 0., all_s = 0.;
+    auto fold = [&] {
+        all_z += z;
+        all_s += s;
+        z = s = 0.f;
+    };
     // A wave's own list: no atomics, and no wait before the next logits.  The lanes that call are a
     // wave's first ones, so that lane 0 has counted them all.
     int kept = 0;
@@ -375,20 +383,24 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
             if (i < n) c = fmaxf(c, v[i]);
         most = fmaxf(most, c);
         if (c > limit) {
-            const float less = z == 0.f ? 0.f : fmaxf((base - c) * A.cold, -1e9f);
-            const float f = __builtin_amdgcn_exp2f(less);
-            s = f * fmaf(less, z, s);
-            z *= f;
+            fold();
+            const float less = all_z == 0. ? 0.f : fmaxf((base - c) * A.cold, -1e9f);
+            const double f = __builtin_amdgcn_exp2f(less);
+            all_s = f * (all_s + less * all_z);
+            all_z *= f;
             base = c;
             limit = c + kFar / A.cold;
         }
+        float piece_z = 0.f, piece_s = 0.f;
 #pragma unroll
         for (int i = 0; i < kP; ++i)
             if (i < n) {
                 const float y = (v[i] - base) * A.cold, w = __builtin_amdgcn_exp2f(y);
-                z += w;
-                s = fmaf(w, fmaxf(y, kNone), s);
+                piece_z += w;
+                piece_s = fmaf(w, fmaxf(y, kNone), piece_s);
             }
+        z += piece_z;
+        s += piece_s;
         if constexpr (kTop)
             if (__any(!(c < bound)))
 #pragma unroll
@@ -407,10 +419,12 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
                 take(v, kP, first + cut.head + p * kP);
             }
         }
+        fold();
     }
     if (has_odd) {
         const float v[kP] = {one};
         take(v, 1, odd);
+        fold();
     }
     // one base for the workgroup: the highest
     const float mine = base;
@@ -418,12 +432,12 @@ __global__ void __launch_bounds__(kThreads, 8) k_logprobs(LogprobArgs A) {
     auto add = [](double a, double b) { return a + b; };
     Sums S;
     S.most = block_reduce<kThreads>(most, sh.most, up);
-    S.base = block_reduce<kThreads>(z == 0.f ? -INFINITY : base, sh.bound, up);
+    S.base = block_reduce<kThreads>(all_z == 0. ? -INFINITY : base, sh.bound, up);
     if (S.base == -INFINITY) S.base = 0.f;
     const double less = (static_cast<double>(mine) - S.base) * A.cold;
-    const double f = mine == S.base || z == 0.f ? 1. : static_cast<double>(__builtin_amdgcn_exp2f(static_cast<float>(less)));
-    S.s = block_reduce<kThreads>(f * (s + (z == 0.f ? 0. : less * z)), sh.red, add);
-    S.z = block_reduce<kThreads>(f * z, sh.red, add);
+    const double f = mine == S.base || all_z == 0. ? 1. : static_cast<double>(__builtin_amdgcn_exp2f(static_cast<float>(less)));
+    S.s = block_reduce<kThreads>(f * (all_s + (all_z == 0. ? 0. : less * all_z)), sh.red, add);
+    S.z = block_reduce<kThreads>(f * all_z, sh.red, add);
     if constexpr (kTop) {
         if (threadIdx.x % 64 == 0) sh.count[threadIdx.x / 64] = kept;
         __syncthreads();
