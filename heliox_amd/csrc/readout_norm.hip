@@ -411,6 +411,10 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
     }
 }
 
+// Rows whose terms of a column's sum are added one after another in fp32: gradients that are alike have
+// roundings that are, too.  What follows is added in 64 bits.
+constexpr int kChain = 128;
+
 // Sums of dy n and of dy over a run of rows, kE columns a thread.
 template <class T, int kE>
 __global__ void __launch_bounds__(256) k_norm_columns(NormArgs A, long long rows_each, float* dw, float* db) {
@@ -419,32 +423,38 @@ __global__ void __launch_bounds__(256) k_norm_columns(NormArgs A, long long rows
     const long long first = blockIdx.y * rows_each, end = min(first + rows_each, A.rows);
     const T* x = static_cast<const T*>(A.x) + j;
     const T* dy = static_cast<const T*>(A.dy) + j;
-    float sum[2][kE] = {};
+    double whole[2][kE] = {};
+    for (long long r0 = first; r0 < end; r0 += kChain) {
+        const long long last = min(r0 + kChain, end);
+        float sum[2][kE] = {};
 #pragma unroll 8
-    for (long long r = first; r < end; ++r) {
-        float v[kE], d[kE];
-        load<T, kE>(x + r * A.x_stride, v);
-        load<T, kE>(dy + r * A.dy_stride, d);
-        const float mean = A.mean[r], rstd = A.rstd[r];
+        for (long long r = r0; r < last; ++r) {
+            float v[kE], d[kE];
+            load<T, kE>(x + r * A.x_stride, v);
+            load<T, kE>(dy + r * A.dy_stride, d);
+            const float mean = A.mean[r], rstd = A.rstd[r];
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-            sum[0][i] = fmaf(d[i], (v[i] - mean) * rstd, sum[0][i]);
-            sum[1][i] += d[i];
+            for (int i = 0; i < kE; ++i) {
+                sum[0][i] = fmaf(d[i], (v[i] - mean) * rstd, sum[0][i]);
+                sum[1][i] += d[i];
+            }
         }
+#pragma unroll
+        for (int i = 0; i < kE; ++i) whole[0][i] += sum[0][i], whole[1][i] += sum[1][i];
     }
     dw += static_cast<long long>(blockIdx.y) * 2 * A.width + j;
     db += static_cast<long long>(blockIdx.y) * 2 * A.width + j;
 #pragma unroll
-    for (int i = 0; i < kE; ++i) dw[i] = sum[0][i], db[i] = sum[1][i];
+    for (int i = 0; i < kE; ++i) dw[i] = static_cast<float>(whole[0][i]), db[i] = static_cast<float>(whole[1][i]);
 }
 
 // The workgroups' sums, added up: 32 columns a workgroup, 32 runs of rows each.
 __global__ void __launch_bounds__(1024) k_norm_join(const float* part, int parts, int width, float* dw, float* db) {
     constexpr int kColumns = 32, kRuns = 32;
-    __shared__ float sh[kRuns][kColumns + 1];
+    __shared__ double sh[kRuns][kColumns + 1];
     const long long whole = 2LL * width, column = static_cast<long long>(blockIdx.x) * kColumns + threadIdx.x % kColumns;
     const int run = threadIdx.x / kColumns;
-    float s = 0.f;
+    double s = 0.;
     if (column < whole) {
 #pragma unroll 8
         for (int p = run; p < parts; p += kRuns) s += part[p * whole + column];
@@ -455,7 +465,7 @@ __global__ void __launch_bounds__(1024) k_norm_join(const float* part, int parts
     s = sh[threadIdx.x % kRuns][threadIdx.x / kRuns];
     for (int d = kRuns / 2; d > 0; d >>= 1) s += __shfl_xor(s, d);
     const long long mine = static_cast<long long>(blockIdx.x) * kColumns + threadIdx.x / kRuns;
-    if (threadIdx.x % kRuns == 0 && mine < whole) (mine < width ? dw[mine] : db[mine - width]) = s;
+    if (threadIdx.x % kRuns == 0 && mine < whole) (mine < width ? dw[mine] : db[mine - width]) = static_cast<float>(s);
 }
 
 // How a row is held: kE elements a piece, kGroup lanes, kV pieces a lane.
@@ -503,7 +513,7 @@ NormArgs norm_args(const hx_norm_args& A) {
 }
 
 // How the gradients of weight and bias are summed: `held` by the workgroups that make grad_x, one
-// sum of each for each of `parts`; or by a launch over the columns that reads the rows again, in
+// sum of each for each of `parts`, of kChain turns at most; or by a launch over the columns that reads the rows again, in
 // `parts` runs of rows.
 //
 // A workgroup's sums are 8 bytes a column, written and read again: more than the rows, where there
@@ -516,7 +526,8 @@ Sums sums_of(const hx_norm_args& A) {
         return with_shape<T, true>(static_cast<int>(A.width), [&](auto shape) -> Sums {
             using S = decltype(shape);
             if constexpr (S::kE != 0) {
-                const int64_t parts = std::min<int64_t>((A.rows + S::kRows - 1) / S::kRows, 512);
+                const int64_t turns = (A.rows + S::kRows - 1) / S::kRows;
+                const int64_t parts = std::min<int64_t>({turns, std::max<int64_t>(512, (turns + kChain - 1) / kChain), 1 << 21});
                 if (A.rows * static_cast<int64_t>(sizeof(T)) >= 8 * parts) return {true, static_cast<int>(parts)};
             }
             const int64_t blocks = (A.width + 511) / 512;
