@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup) k_norm_grad(NormA
     }
 }
 
-// Rows too wide for registers: read again from the cache for each sum.
+// Rows too wide for registers: read again from the cache for each sum.  A thread adds a piece's terms in
+// fp32 and pieces, of which there may be thousands, in 64 bits.
 constexpr int kWide = 1024;
 
 template <class T, class F>
@@ -317,15 +318,16 @@ __global__ void __launch_bounds__(kWide) k_norm_wide(NormArgs A) {
     for (long long row = blockIdx.x; row < A.rows; row += gridDim.x) {
         const T* x = static_cast<const T*>(A.x) + row * A.x_stride;
         T* y = static_cast<T*>(A.y) + row * A.y_stride;
-        float sum[1] = {0.f}, off[2] = {0.f, 0.f};
+        double own = 0., own_off[2] = {0., 0.};
         each_element<T>(A.width, [&](auto e, int j) {
             constexpr int kE = decltype(e)::value;
             float v[kE], s = 0.f;
             load<T, kE>(x + j, v);
 #pragma unroll
             for (int i = 0; i < kE; ++i) s += v[i];
-            sum[0] += s;
+            own += s;
         });
+        float sum[1] = {static_cast<float>(own)};
         group_sum<kWide>(sum, sh[0]);
         const float mean = sum[0] * A.per_width;
         each_element<T>(A.width, [&](auto e, int j) {
@@ -337,9 +339,10 @@ __global__ void __launch_bounds__(kWide) k_norm_wide(NormArgs A) {
                 d += v[i] - mean;
                 s = fmaf(v[i] - mean, v[i] - mean, s);
             }
-            off[0] += d;
-            off[1] += s;
+            own_off[0] += d;
+            own_off[1] += s;
         });
+        float off[2] = {static_cast<float>(own_off[0]), static_cast<float>(own_off[1])};
         group_sum<kWide>(off, sh[1]);
         const Spread spread(off, A);
         const float rest = spread.rest, rstd = spread.rstd;
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
         const T* dy = static_cast<const T*>(A.dy) + row * A.dy_stride;
         T* dx = static_cast<T*>(A.y) + row * A.y_stride;
         const float mean = A.mean[row], rstd = A.rstd[row];
-        float sum[2] = {0.f, 0.f};
+        double own[2] = {0., 0.};
         auto terms = [&](auto e, int j, float* n, float* g) {
             constexpr int kE = decltype(e)::value;
             float w[kE];
@@ -395,9 +398,10 @@ __global__ void __launch_bounds__(kWide) k_norm_grad_wide(NormArgs A) {
                 s += g[i];
                 sn = fmaf(g[i], n[i], sn);
             }
-            sum[0] += s;
-            sum[1] += sn;
+            own[0] += s;
+            own[1] += sn;
         });
+        float sum[2] = {static_cast<float>(own[0]), static_cast<float>(own[1])};
         group_sum<kWide>(sum, sh[turn]);
         const float mean_g = sum[0] * A.per_width, mean_gn = sum[1] * A.per_width;
         each_element<T>(A.width, [&](auto e, int j) {
