@@ -23,7 +23,8 @@ stream, wait for nothing, and may be captured into a graph.  Sums, softmax stati
 states are fp32 or wider whatever the inputs are.  Arguments that do not fit raise ValueError
 or TypeError; sizes, values and overlaps that the library refuses, and launches that fail, raise
 HelioxError.  Results carry no graph for autograd: gradients are calls of their own, and the calls
-that have one refuse inputs that require a gradient while torch records.
+that have one refuse inputs that require a gradient while torch records.  What a call writes in
+place counts as changed: a backward pass that kept its old values is refused by torch.
 """
 from __future__ import annotations
 
@@ -141,6 +142,19 @@ def _ptr(x: Optional[torch.Tensor]) -> int:
 # object for it takes 2 us to make).
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+# A tensor that a call writes in place counts it, so that a backward pass that kept the old values says so (the
+# public call takes twice as long for one tensor).
+_count_writes = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+
+
+def _written(x: torch.Tensor) -> None:
+    try:
+        _count_writes([x])
+    except RuntimeError:
+        if not x.is_inference():              # those are never kept
+            raise
+
 
 _entries: dict = {}
 
@@ -294,6 +308,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     _call("hx_linear_attention_step", device, _ATTENTION.pack(
         *fields, 0, 0, _scale(scale, dk), o.data_ptr(), heads * dv, 0, dv, 0, 0, 0, 0, 0, 0, 0, 0,
         0, 0, state.data_ptr(), _ptr(slots), state.shape[0], 0, 0, _stream(device)))
+    _written(state)
     return o
 
 
@@ -398,6 +413,7 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
     _call("hx_gated_recurrence_step", device, _RECURRENCE.pack(
         *fields, 0, 0, o.data_ptr(), channels, 0, 0, 0, 0, 0, 0, 0, 0, 0, state.data_ptr(), _ptr(slots), state.shape[0],
         0, 0, _stream(device)))
+    _written(state)
     return o
 
 
@@ -540,7 +556,9 @@ def distill_loss_grad(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     elif (_on_gpu(out, "out") != _on_gpu(logits, "logits") or out.dtype != logits.dtype or out.shape != logits.shape
           or (out.shape[-1] > 1 and out.stride(-1) != 1)):
         raise ValueError("out has to be like the logits, its last dimension contiguous")
-    return _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, weight, out), out
+    loss = _distill(logits, teacher_index, teacher_logits, temperature, teacher_lse, weight, out)
+    _written(out)
+    return loss, out
 
 
 class TokenLogprobs(NamedTuple):
@@ -621,6 +639,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, scored: Toke
         kind, 32 if tokens.dtype is torch.int32 else 64, rows, vocab, 0, logits.data_ptr(), logits.stride(0),
         tokens.data_ptr(), _real(temperature, "temperature"), 0, entropy.data_ptr(), stats.data_ptr(), 0, 0,
         _ptr(dlogprob), _ptr(dentropy), out.data_ptr(), out.stride(0), 0, 0, _stream(device)))
+    _written(out)
     return out
 
 
@@ -856,5 +875,4 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         state.bits, len(params), *[a.buffer_info()[0] for a in lists], m.data_ptr(), v.data_ptr(),
         _ptr(m_scale), _ptr(v_scale), m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
         lr_ptr, count.data_ptr(), _stream(device)))
-    # what autograd kept of the old values is out of date (inference tensors are never kept)
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    _count_writes([p for p in params if not p.is_inference()])
