@@ -2,6 +2,7 @@
 #include "readout.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -24,6 +25,11 @@ int refuse(const char* fmt, ...) {
 int launched(const char* call, hipError_t e) {
     return e == hipSuccess ? 0 : refuse("%s: %s", call, hipGetErrorString(e));
 }
+
+// Settings that are fp32 numbers in a kernel; an epsilon keeps zero from being divided by, which it does
+// from the least number on whose reciprocal is one.
+bool fits_f32(double x) { return std::fabs(x) <= FLT_MAX; }
+bool epsilon(double x) { return x == 0 || (x >= FLT_MIN && fits_f32(x)); }
 
 bool known_type(int64_t t) { return t == HX_F32 || t == HX_F16 || t == HX_BF16; }
 
@@ -149,7 +155,7 @@ int adamw_tensors(const char* call, const hx_adamw_args* A) {
         if (!known_type(A->types[i]) || !known_type(A->grad_types[i]))
             return refuse("%s: tensor %lld: type is not known", call, at);
         if (n < 0 || n > (int64_t(1) << 34)) return refuse("%s: tensor %lld: elements has to be in 0..2^34", call, at);
-        if (!std::isfinite(A->weight_decays[i])) return refuse("%s: tensor %lld: weight_decay is not finite", call, at);
+        if (!fits_f32(A->weight_decays[i])) return refuse("%s: tensor %lld: weight_decay is not finite in fp32", call, at);
         if (start % 256 || start < used)
             return refuse("%s: tensor %lld: moments start at multiples of 256, each after those before", call, at);
         if (start > A->moments || (n + 255) / 256 * 256 > A->moments - start)
@@ -177,9 +183,9 @@ int adamw_check(const char* call, const hx_adamw_args* A) {
     if (A->count < 0 || A->count > (1 << 20)) return refuse("%s: count has to be in 0..2^20", call);
     if (!(A->beta1 >= 0 && A->beta1 < 1 && A->beta2 >= 0 && A->beta2 < 1))
         return refuse("%s: beta1 and beta2 have to be in [0, 1)", call);
-    if (!(A->eps >= 0) || !std::isfinite(A->eps)) return refuse("%s: eps has to be a number, at least 0", call);
-    if (!std::isfinite(A->lr)) return refuse("%s: lr is not finite", call);
-    if (!std::isfinite(A->grad_scale)) return refuse("%s: grad_scale is not finite", call);
+    if (!epsilon(A->eps)) return refuse("%s: eps has to be 0, or a number of fp32 from 2^-126 on", call);
+    if (!fits_f32(A->lr)) return refuse("%s: lr is not finite in fp32", call);
+    if (!fits_f32(A->grad_scale)) return refuse("%s: grad_scale is not finite in fp32", call);
     if (!A->step) return refuse("%s: step is missing", call);
     if (A->count && (!A->types || !A->grad_types || !A->params || !A->grads || !A->elements || !A->starts || !A->weight_decays))
         return refuse("%s: a list of the tensors is missing", call);
@@ -197,7 +203,7 @@ int norm_sizes(const char* call, const hx_norm_args* A) {
     if (A->rows < 0 || A->rows > INT32_MAX) return refuse("%s: rows has to be in 0..2^31 - 1", call);
     if (A->width < 1 || A->width > (1 << 24))
         return refuse("%s: width (%lld) has to be in 1..2^24", call, (long long)A->width);
-    if (!(A->eps >= 0) || !std::isfinite(A->eps)) return refuse("%s: eps has to be a number, at least 0", call);
+    if (!epsilon(A->eps)) return refuse("%s: eps has to be 0, or a number of fp32 from 2^-126 on", call);
     if (!A->grad_weight != !A->grad_bias) return refuse("%s: grad_weight and grad_bias come together", call);
     return 0;
 }

@@ -453,7 +453,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension of x (..., width);
     weight and bias (width,) are of one type, fp32, fp16 or bf16, whatever x's is (1 and 0 unless
-    given).  Returns y of x's shape and type, and each row's mean and 1 / sqrt(variance + eps)
+    given); eps is 0 or at least 2^-126.  Returns y of x's shape and type, and each row's mean and 1 / sqrt(variance + eps)
     (fp32, x's shape without the last), which layer_norm_grad takes."""
     device, kind, weight_kind, rows, weight, bias = _norm_inputs(x, weight, bias)
     _no_graph("layer_norm", "take it from layer_norm_grad", x, weight, bias)

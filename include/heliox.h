@@ -618,7 +618,7 @@ typedef struct hx_norm_args {
     const void* x;
     int64_t x_stride;                                     /* of rows, as the others */
     const void *weight, *bias;                            /* (width) each, or NULL: 1 and 0 */
-    double eps;                                           /* at least 0 */
+    double eps;                                           /* 0, or 2^-126 and more, finite in fp32 */
     void* y;
     int64_t y_stride;
     float *mean, *rstd;                                   /* (rows) each: written, read by the gradient */
@@ -726,6 +726,7 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * (rounded to nearest, moments that move by less than half a step of their codes would stand still):
  * the same calls give the same state.  A root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
  * that is not finite reaches its block's 256 elements in 8 bits.
+ * lr, grad_scale and weight decays are finite in fp32, eps is 0 or, finite there, at least 2^-126.
  * Tensors come in the order of their starts, each within `moments`, its last 256 filled up with
  * elements that belong to none (kept zero).  The parameters of a call do not overlap each other or
  * the gradients (refused).  `step` (two int64: the count, and room that the call uses; at a multiple
