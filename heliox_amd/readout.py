@@ -799,6 +799,7 @@ def adamw_state(params: Sequence[torch.Tensor], *, bits: int = 32) -> AdamWState
     bytes of moments for each of their elements with bits=32, 2 and a 32nd with bits=8."""
     params = list(params)
     device, _ = _parameters(params)
+    bits = _whole(bits, "bits")
     if bits not in (8, 32):
         raise ValueError(f"bits has to be 8 or 32, got {bits}")
     return AdamWState(list(map(_size_of, params)), bits, device)
@@ -819,7 +820,7 @@ def _decays(weight_decay, count: int) -> array:
             raise ValueError(f"{len(weight_decay)} weight_decay for {count} params")
         try:
             return array("d", weight_decay)
-        except TypeError:
+        except (TypeError, ValueError, OverflowError):
             return array("d", [_real(w, "weight_decay") for w in weight_decay])
     return array("d", [_real(weight_decay, "weight_decay")]) * count
 

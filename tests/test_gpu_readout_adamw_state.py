@@ -85,3 +85,9 @@ def test_a_state_whose_tensors_were_changed_is_refused(name, change):
     with pytest.raises(ValueError, match="were changed"):
         readout.adamw_step(params, grads, state, lr=0.1)
     assert all(torch.equal(a, b) for a, b in zip(params, kept)) and int(state.step) == 0
+
+
+@pytest.mark.parametrize("bits,error", [(8.0, TypeError), ("8", TypeError), (None, TypeError), (16, ValueError), (2 ** 70, ValueError)])
+def test_bits_are_whole_numbers(bits, error):
+    with pytest.raises(error, match="bits"):
+        readout.adamw_state(tensors(0), bits=bits)

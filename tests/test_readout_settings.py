@@ -1,7 +1,8 @@
 """Settings of layer norm and the AdamW step that fp32 cannot hold are refused (no GPU)."""
 import pytest
+import torch
 
-from heliox_amd import lib
+from heliox_amd import lib, readout
 from test_readout_training import Tensors, error, norm
 
 # over fp32's largest; an epsilon that is zero in fp32, and ones whose reciprocal is infinite there
@@ -36,3 +37,10 @@ def test_what_fits_goes_on(eps):
     assert lib().hx_layer_norm_workspace(norm(eps=eps)) > 0
     # (no room for moments: refused after the settings)
     assert step(eps=eps, lr=3e38, scale=-3e38) == -1 and "too few" in error()
+
+
+@pytest.mark.parametrize("decay,error_type", [([0.1, 10 ** 400], ValueError), (10 ** 400, ValueError), ([0.1, "0.1"], TypeError),
+                                              ([0.1, None], TypeError), ([0.1, torch.zeros(2)], TypeError), ((0.1,), ValueError)])
+def test_decays_that_are_no_numbers(decay, error_type):
+    with pytest.raises(error_type, match="weight_decay"):
+        readout._decays(decay, 2)
