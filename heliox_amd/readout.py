@@ -143,17 +143,16 @@ def _ptr(x: Optional[torch.Tensor]) -> int:
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 
-# A tensor that a call writes in place counts it, so that a backward pass that kept the old values says so (the
-# public call takes twice as long for one tensor).
+# (the public call takes twice as long for one tensor)
 _count_writes = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
-def _written(x: torch.Tensor) -> None:
+def _written(*xs: torch.Tensor) -> None:
+    """Counts a write in place, so that a backward pass that kept the old values says so."""
     try:
-        _count_writes([x])
+        _count_writes(xs)
     except RuntimeError:
-        if not x.is_inference():              # those are never kept
-            raise
+        _count_writes([x for x in xs if not x.is_inference()])      # inference tensors are never kept
 
 
 _entries: dict = {}
@@ -733,6 +732,8 @@ class AdamWState:
         self._m_scale, self._v_scale = (torch.zeros(whole // 256, **on) if bits == 8 else None for _ in range(2))
         # the count, and room that the library uses
         self._count = torch.zeros(2, dtype=torch.int64, **on)
+        self._held = [x for x in (self._m, self._v, self._m_scale, self._v_scale, self._count) if x is not None]
+        self._elements = [x.numel() for x in self._held]
 
     @property
     def step(self) -> torch.Tensor:
@@ -751,16 +752,13 @@ class AdamWState:
         else:
             self._count[:1].copy_(x.reshape(1))
 
-    def _tensors(self) -> tuple:
-        """m, v, their scales and the count, of the sizes and on the device that they were made with."""
-        whole = self.starts[-1] + -(-self.sizes[-1] // 256) * 256
-        scales = whole // 256 if self.bits == 8 else 0
-        all_ = self._m, self._v, self._m_scale, self._v_scale, self._count
-        for x, n in zip(all_, (whole, whole, scales, scales, 2)):
-            if x is not None and (x.get_device() != self.device or x.numel() != n or not x.is_contiguous()):
-                raise ValueError(f"the state's tensors were changed: {tuple(x.shape)} on {x.device} where {n} contiguous "
-                                 f"elements on cuda:{self.device} belong")
-        return all_
+    def _check(self) -> None:
+        """Its tensors are of the sizes and on the device that they were made with."""
+        held = self._held
+        if (list(map(_size_of, held)) != self._elements or set(map(_device_of, held)) != {self.device}
+                or not all(map(_whole_of, held))):
+            raise ValueError(f"the state's tensors were changed: {[tuple(x.shape) for x in held]} on {[str(x.device) for x in held]} "
+                             f"where {self._elements} contiguous elements on cuda:{self.device} belong")
 
 
 # What is asked of hundreds of tensors in a step is asked by map, a tenth of a loop's time each.
@@ -870,10 +868,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
                          + ", ".join(f"{tuple(g.shape)} for {tuple(p.shape)}" for p, g in zip(params, grads) if p.shape != g.shape))
     if not all(map(_whole_of, grads)):
         grads = [g.contiguous() for g in grads]
-    m, v, m_scale, v_scale, count = state._tensors()
+    state._check()
     lists = kinds, grad_kinds, array("Q", map(_address_of, params)), array("Q", map(_address_of, grads)), sizes, starts, decays
     _call("hx_adamw_step", device, _ADAMW.pack(
-        state.bits, len(params), *[a.buffer_info()[0] for a in lists], m.data_ptr(), v.data_ptr(),
-        _ptr(m_scale), _ptr(v_scale), m.numel(), lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
-        lr_ptr, count.data_ptr(), _stream(device)))
-    _count_writes([p for p in params if not p.is_inference()])
+        state.bits, len(params), *[a.buffer_info()[0] for a in lists], state._m.data_ptr(), state._v.data_ptr(),
+        _ptr(state._m_scale), _ptr(state._v_scale), state._elements[0], lr, beta1, beta2, _real(eps, "eps"), scale, scale_ptr,
+        lr_ptr, state._count.data_ptr(), _stream(device)))
+    _written(*params)
