@@ -14,9 +14,9 @@
 //
 // A moment that moves by less than half a step of its code would never move if it were rounded to
 // nearest: with beta2 = 0.999 a root falls by 0.05% a step, and codes are 6 to 12% apart (5000 steps
-// after 16384 gradients' sizes changed places a third of the steps were off by more than 2).  So
+// after 16384 gradients' sizes changed places a third of the roots were off by more than 2).  So
 // a code is rounded up as often as its number is near the upper one, by bits made of the
-// step's count and the element's place: the moments follow on average (of those steps 0.3% are off by more
+// step's count and the element's place: the moments follow on average (of those roots 0.3% are off by more
 // than 2), and the same calls give the same state.  The first steps, as many as the longer memory
 // spans, 1 / (1 - beta), are to nearest: moments of few gradients move by whole codes, and what sticks all
 // the same is forgotten in as many steps more.

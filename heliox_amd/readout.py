@@ -591,8 +591,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     """Of each row of logits (rows, vocab), with q = softmax(logits / temperature): log q of the row's
     token (tokens (rows,) int32 or int64; 0 for a token outside the vocabulary, as of padding), the
     entropy of q, and the ``top`` most likely places (at most 256; ties: the lowest index first) with
-    their log q.  NaN ranks as -inf, and a row with a NaN or +inf has NaN for all of its numbers; a row
-    of nothing but -inf has log q -inf and entropy 0.
+    their log q.  NaN ranks as -inf, and a row with a NaN or +inf has NaN for all of its numbers (but 0 for
+    a token outside the vocabulary); a row of nothing but -inf has log q -inf and entropy 0.
 
     stats holds the largest logit m and log sum exp((logits - m) / temperature), which
     token_logprobs_grad takes; m / temperature plus the latter is the logsumexp."""
@@ -839,9 +839,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
 
     With 8 bits the moments are rounded after the step has used them: to nearest while t is at most
     1 / (1 - max(betas)), later up or down by a hash of t and the element, so that they follow changes
-    smaller than their codes' steps (the same calls give the same state); a gradient that is not finite
-    reaches the 256 elements that share its scale.  Parameters that overlap each other or a gradient
-    are refused."""
+    smaller than their codes' steps (the same calls give the same state).  An infinite gradient makes
+    the moments of the 256 elements that share its scale NaN, a NaN only its own.  Parameters in 16
+    bits lose updates under half a step of their own: keep them in fp32 where that matters.
+    Parameters that overlap each other or a gradient are refused."""
     if not isinstance(state, AdamWState):
         raise TypeError(f"state has to be what adamw_state returned, got {type(state).__name__}")
     params, grads = list(params), list(grads)

@@ -610,7 +610,8 @@ int hx_sample(const hx_sample_args* args);
  * same mean and rstd: with n = (x - mean) rstd and g = grad_y weight,
  *   grad_x = rstd (g - mean(g) - n mean(g n)),  grad_weight = sum over rows of grad_y n,
  *   grad_bias = sum over rows of grad_y
- * (fp32, added in an order of the sizes alone).  grad_weight and grad_bias are both made or both NULL.
+ * (fp32, added in an order of the sizes alone).  Squares of differences are fp32 numbers: rows with values
+ * over some 1e19 have an rstd of 0 or NaN.  grad_weight and grad_bias are both made or both NULL.
  * rows is at most 2^31 - 1, width at most 2^24.  What a call writes overlaps nothing that it reads. */
 typedef struct hx_norm_args {
     int64_t type, weight_type;                            /* weight and bias are of weight_type */
@@ -638,8 +639,8 @@ int hx_layer_norm_grad(const hx_norm_args* args);
 
 /* h_t = a_t h_{t-1} + (1 - a_t) x_t for each channel, a = 1 / (1 + e^-gate) (1 - a taken as
  * 1 / (1 + e^gate); where the gate is over -2 a h is h less (1 - a) h, so that long memories keep
- * their bits, and a times h where it shuts), o_t = h_t: the exponential step of a membrane towards x whose conductance
- * is the gate's.  h_{-1} is the initial state (NULL: zero), end_state the state after a
+ * their bits, and a times h where it shuts), o_t = h_t: the exponential step of a membrane towards x
+ * whose conductance is the gate's.  h_{-1} is the initial state (NULL: zero), end_state the state after a
  * sequence's last step; outputs past its length are zero, whatever its inputs hold there.  The
  * gradient: with l_t = grad_o_t + a_{t+1} l_{t+1} (past the end: grad_end),
  *   grad_x = (1 - a) l,  grad_gate = a (1 - a) l (h_{t-1} - x_t),  grad_initial = a_0 l_0.
@@ -684,8 +685,8 @@ int hx_gated_recurrence_step(const hx_recurrence_args* args);
  * largest logits, largest first (ties: the lowest index first; NaN ranks as -inf), as indexes and
  * log q.  Where fewer than top places are above -inf, -inf fills the rest, by index.  stats (rows,
  * 2) receives the largest logit m and log sum exp((logits - m) / temperature).  A row of nothing
- * but -inf has logprob -inf, entropy 0 and stats -inf, -inf; one with a NaN or +inf has NaN.  The
- * order of a row's sums follows from the sizes and from its address within 16 bytes alone.
+ * but -inf has logprob -inf, entropy 0 and stats -inf, -inf; one with a NaN or +inf has NaN (and still 0
+ * for a token outside).  The order of a row's sums follows from the sizes and from its address within 16 bytes alone.
  * The gradient, from the same stats and entropy: grad_j =
  *   [grad_logprob (1[j = token] - q_j) - grad_entropy q_j (log q_j + entropy)] / temperature
  * (the first term 0 for a token outside the vocabulary; all 0 for a row of nothing but -inf); it may
@@ -724,8 +725,9 @@ int hx_token_logprobs_grad(const hx_logprob_args* args);
  * for the first 1 / (1 - max(beta1, beta2)) steps, which is how many the moments remember; from then on
  * up or down, as often as they are near either side, by a hash of t and of the element's place
  * (rounded to nearest, moments that move by less than half a step of their codes would stand still):
- * the same calls give the same state.  A root that is not zero is held as 2^-9 at least, so that its step stays bounded.  A gradient
- * that is not finite reaches its block's 256 elements in 8 bits.
+ * the same calls give the same state.  A root that is not zero is held as 2^-9 at least, so that its
+ * step stays bounded.  In 8 bits a gradient that is infinite, or whose (1 - beta2) g^2 is in fp32, makes
+ * its block's 256 moments NaN; a NaN stays with its element, as both do in 32 bits.
  * lr, grad_scale and weight decays are finite in fp32, eps is 0 or, finite there, at least 2^-126.
  * Tensors come in the order of their starts, each within `moments`, its last 256 filled up with
  * elements that belong to none (kept zero).  The parameters of a call do not overlap each other or
