@@ -76,13 +76,13 @@ __device__ __forceinline__ float rise(float gate) { return __builtin_amdgcn_exp2
 // 1 / (1 + e^gate) from e^gate
 __device__ __forceinline__ float opening(float e) { return __builtin_amdgcn_rcpf(1.f + e); }
 
-// Gates up to here shut: at -2 z's own error, 3 halves of a step, is 26 of them in a = 1 - z, as much
-// as e^gate's argument is off by at -18.
-constexpr float kShut = -2.f;
+// Gates up to here shut: at -1 z = 0.73 is off by at most 4 halves of a step, a = 1 - z by 10 of its own, as
+// e^gate z is there.  (Of e^gate the exponent's rounding is the most, 22 halves at -25.)
+constexpr float kShut = -1.f;
 
 // A step's opening z and what it keeps, a.  Waves whose steps do not shut (kShuts false: see any_shuts)
 // go without what that takes, with the same results: 8 x 4096 x 2048 with gradient 313 us, with it
-// everywhere 321, where steps shut in every wave 322.
+// everywhere 321, where steps shut in every wave 317.
 template <bool kShuts>
 struct Opening {
     float z, a;

@@ -638,7 +638,7 @@ int hx_layer_norm(const hx_norm_args* args);
 int hx_layer_norm_grad(const hx_norm_args* args);
 
 /* h_t = a_t h_{t-1} + (1 - a_t) x_t for each channel, a = 1 / (1 + e^-gate) (1 - a taken as
- * 1 / (1 + e^gate); where the gate is over -2 a h is h less (1 - a) h, so that long memories keep
+ * 1 / (1 + e^gate); where the gate is over -1 a h is h less (1 - a) h, so that long memories keep
  * their bits, and a times h where it shuts), o_t = h_t: the exponential step of a membrane towards x
  * whose conductance is the gate's.  h_{-1} is the initial state (NULL: zero), end_state the state after a
  * sequence's last step; outputs past its length are zero, whatever its inputs hold there.  The

@@ -1,5 +1,6 @@
 """What an AdamW state does with tensors that are assigned to it, and when its own were changed."""
 import copy
+import io
 
 import pytest
 import torch
@@ -51,6 +52,20 @@ def test_a_copy_counts_by_itself():
     state.step = 7
     readout.adamw_step(params, grads, state, lr=0.1)
     assert int(state.step) == 8
+
+
+def test_a_saved_state_goes_on():
+    params, grads = tensors(0), tensors(1)
+    state, file = readout.adamw_state(params, bits=8), io.BytesIO()
+    readout.adamw_step(params, grads, state, lr=0.1)
+    torch.save(state, file)
+    again = [p.clone() for p in params]
+    other, host = (torch.load(io.BytesIO(file.getvalue()), weights_only=False, map_location=at) for at in (None, "cpu"))
+    readout.adamw_step(params, grads, state, lr=0.1)
+    readout.adamw_step(again, grads, other, lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(params, again)) and int(other.step) == 2
+    with pytest.raises(ValueError, match="were changed"):       # on the CPU
+        readout.adamw_step(again, grads, host, lr=0.1)
 
 
 def test_assignments_are_refused():

@@ -39,8 +39,7 @@ def resets(batch, time, channels, dtype):
 def test_what_a_reset_leaves(batch, time, channels, dtype):
     """Without inputs every value is a product.  An open step rounds once; z's own error counts 1e-4 times there.
     A shut step's a takes e^gate (its argument, up to 37, is off by half a step of 32 and by the constant's own error:
-    28 halves in all, the instruction's unit 2), 1 + e, its reciprocal (2) and two products: 36.  Above -2 it is 1 - z,
-    z (3 halves) being at most 0.88 and a at least 0.12: 28.  Runs join in at most 64 products.  dgate is a value of
+    28 halves in all, the instruction's unit 2), 1 + e, its reciprocal (2) and two products: 36.  Runs join in at most 64 products.  dgate is a value of
     the way there times one of the way back, and three more products."""
     gate, state, last, at = resets(batch, time, channels, dtype)
     x, do = torch.zeros_like(gate), torch.zeros_like(gate)
@@ -70,6 +69,20 @@ def test_a_single_step(channels, dtype):
     torch.cuda.synchronize()
     near(o, want, dtype, 40, "o")
     near(state, want, None, 40, "state")
+
+
+def test_around_where_gates_shut():
+    """From -3 to 3: a of e^gate (its argument 3 halves, the constant's error 1, the instruction's unit 2), 1 + e, its
+    reciprocal (2) and a product is off by 10 halves of itself; 1 - z, z being at most 0.73 and off by 4 halves,
+    by 4 * 0.73 / 0.27 = 11.  One product more."""
+    gate = torch.linspace(-3, 3, 100_001)[None].cuda()
+    state = torch.full_like(gate, 1000.0)
+    want = 1000 / (1 + torch.exp(-gate.cpu().double()))
+    o, end = readout.gated_recurrence(torch.zeros_like(gate)[None], gate[None], initial_state=state)
+    readout.gated_recurrence_step(torch.zeros_like(gate), gate, state)
+    torch.cuda.synchronize()
+    for got in (o[0], end, state):
+        near(got, want, None, 12, "a step")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
