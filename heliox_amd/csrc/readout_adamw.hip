@@ -2,10 +2,11 @@
 //
 // A workgroup takes kChunk elements of one tensor, a wave kBlocks blocks of 256 in a row, four
 // elements a lane in each, so that every array streams through as it lies in memory: bound by
-// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 315 us, 4.8 TB/s, 332 where codes are rounded
-// by chance; with four blocks a wave 327, with one 333).  The tensors of a launch are listed in its arguments; a workgroup finds its own
-// by one comparison a lane.  The count of steps, and what follows from it alone, is made by a
-// first launch of one thread, on the device, so that a captured step counts on.
+// their bytes (300 tensors of 150 million bf16 elements, 8 bits: 315 us, 4.8 TB/s, 332 where codes are
+// rounded by chance; with four blocks a wave 327, with one 333).  The tensors of a launch are listed in
+// its arguments; a workgroup finds its own by one comparison a lane.  The count of steps, and what
+// follows from it alone, is made by a first launch of one thread, on the device, so that a captured
+// step counts on.
 //
 // In 8 bits a block's moments are e4m3 numbers relative to the block's largest (a wave holds a
 // block: its maximum is a reduction of the wave).  Of v the root is held: half of v's exponents, so that
